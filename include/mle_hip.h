@@ -490,6 +490,76 @@ int mle_softmax_xent_keys_fwd_rowstats_read(mle_stream stream, const float* logi
                                             float* loss_host);
 
 /* ------------------------------------------------------------------------- */
+/* The vocabulary's projection with its cross entropy, no logits kept        */
+/* ------------------------------------------------------------------------- */
+
+/* Cross entropy of a Linear's outputs l = X W + bias against token ids, without
+ * a rows x vocab tensor: for large vocabularies, where the logits and their
+ * gradient (mle_gemm_rowstats, mle_softmax_xent_keys_*) would be most of a step's
+ * memory.  X [rows, d] (row stride ldx), W [d, vocab] (ldw), bias [vocab] or NULL.
+ * Row r = b*clen + s has the id keys[b*max_clen + s]; a row whose id is outside
+ * [0, vocab) takes no part: its loss is 0, its gradient 0, and what X holds there
+ * (NaN included) reaches neither the loss nor dW.
+ *   forward:   lse[r] = log sum_v exp l[r, v], for every row;
+ *              row_loss[r] = lse[r] - l[r, id] (row_loss may be NULL);
+ *              loss[0] = loss_scale * sum of the row losses (1 / the number of
+ *              rows that take part gives their mean).
+ *   backward:  P = grad_scale * (upstream ? upstream[0] : 1) * (exp(l - lse) - onehot),
+ *              dX (+)= P W^T (lddx), dW (+)= X^T P (lddw), db (+)= column sums of P;
+ *              dX may be NULL, and dW with db (or db alone).  lse is the forward's.
+ * A bias of -infinity takes an entry out of the vocabulary (probability and
+ * gradient 0); a row with no finite logit has no finite loss.  The logits are
+ * formed in pieces of the vocabulary in ws, in the forward and again in the
+ * backward; ws carries nothing from one call to the next.  fp32 accuracy; sums in
+ * a fixed order.  X, W, dX and dW are buffers of their own.
+ * The reference forms and keeps them (SoftMaxCrossEntropy, Engine/engine.cu:2064-2124). */
+size_t mle_vocab_xent_ws_bytes(int rows, int d, int vocab);
+int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W,
+                       int64_t ldw, const float* bias, const int32_t* keys, int clen, int max_clen, float loss_scale,
+                       float* lse, float* row_loss, float* loss, void* ws, size_t ws_bytes);
+int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W,
+                       int64_t ldw, const float* bias, const int32_t* keys, int clen, int max_clen, const float* lse,
+                       const float* upstream, float grad_scale, float* dX, int64_t lddx, int accumulate_dx, float* dW,
+                       int64_t lddw, float* db, int accumulate_dw, void* ws, size_t ws_bytes);
+
+/* ------------------------------------------------------------------------- */
+/* Activations kept in 8 bits for the backward pass                          */
+/* ------------------------------------------------------------------------- */
+
+/* The 8 bits of x [rows, cols] (row stride ldx): codes q [rows, cols] (ldq) and
+ * one exponent byte e [rows, ceil(cols/32)] (lde) per 32 consecutive columns.
+ * A group's step is 2^(e - 127), the smallest power of two in [2^-126, 2^121]
+ * for which its largest magnitude is below 127.5 steps; a value is kept as the
+ * nearest whole number of steps, ties to even, at most 127, so |x - value| <=
+ * half a step (a step above 127.5 * 2^121, some 0.4 % below fp32's largest).  A group
+ * with an infinity or a NaN has e = 255: its infinities come back, its other
+ * values as NaN.  1.03 bytes a value.  No reference counterpart: it keeps every
+ * activation in fp32.
+ *   mle_q8_quantize:    q, e from x
+ *   mle_q8_dequantize:  y = the values of q, e
+ *   mle_q8_act_fwd:     y = act(x) (mle_act_fwd's function), and x's q, e from the same read
+ *   mle_q8_act_bwd:     dx (+)= act'(kept x) * dy (mle_act_bwd's, on the kept values)
+ *   mle_q8_linear_wgrad: a Linear's weight gradient from its kept input:
+ *                       dW [in, out] (+)= X^T dY, and (db non-null) db (+)= column
+ *                       sums of dY; X the values of q, e [rows, in], which enter the
+ *                       products exactly.  fp32 accuracy, sums in a fixed order.
+ *                       rows 0 assigns zeros.
+ * Rows of 16-byte (floats) and 8-byte (codes) alignment are read and written
+ * whole; any others element by element.  dx may be dy's buffer, y may be x's. */
+int mle_q8_quantize(mle_stream stream, int rows, int cols, const float* x, int64_t ldx, int8_t* q, int64_t ldq,
+                    uint8_t* e, int64_t lde);
+int mle_q8_dequantize(mle_stream stream, int rows, int cols, const int8_t* q, int64_t ldq, const uint8_t* e,
+                      int64_t lde, float* y, int64_t ldy);
+int mle_q8_act_fwd(mle_stream stream, int kind, int rows, int cols, const float* x, int64_t ldx, float* y, int64_t ldy,
+                   int8_t* q, int64_t ldq, uint8_t* e, int64_t lde);
+int mle_q8_act_bwd(mle_stream stream, int kind, int rows, int cols, const int8_t* q, int64_t ldq, const uint8_t* e,
+                   int64_t lde, const float* dy, int64_t lddy, float* dx, int64_t lddx, int accumulate);
+size_t mle_q8_linear_wgrad_ws_bytes(int rows, int in, int out);
+int mle_q8_linear_wgrad(mle_stream stream, int rows, int in, int out, const int8_t* q, int64_t ldq, const uint8_t* e,
+                        int64_t lde, const float* dY, int64_t lddy, float* dW, int64_t lddw, float* db, int accumulate,
+                        void* ws, size_t ws_bytes);
+
+/* ------------------------------------------------------------------------- */
 /* Normalisation (gamma = 1, beta = 0, as the reference)                     */
 /* ------------------------------------------------------------------------- */
 
@@ -597,6 +667,27 @@ int mle_rmsnorm_fwd(mle_stream stream, const float* x, float* y, float* norms, i
  * Accumulate_rmsnorm_kernel (Engine/kernels.cu:2073-2105). */
 int mle_rmsnorm_bwd(mle_stream stream, const float* y, const float* dy, const float* norms, float* dx,
                     int bc, int rows, int cols, int type, int accumulate);
+
+/* The residual Add and a root-mean-square norm with a learned weight that reads
+ * it, along rows of [rows, cols] (the reference's RMSNorm above is an L2
+ * normalisation without a weight):
+ *   forward:   h = x + r (r NULL: h = x), rstd[row] = 1 / sqrt(mean(h^2) + eps),
+ *              y = h * rstd * w (w NULL: 1), formed in 64 bits and rounded once;
+ *              q, e = the 8 bits of y (mle_q8_quantize's format and bits).  h, y,
+ *              and q with e may be NULL.
+ *   backward:  with u = h * rstd and g = dy * w,
+ *              dh (+)= (dres ? dres : 0) + rstd * (g - u * mean(g u)), and (dw non-null)
+ *              dw (+)= sum over rows of dy * u.  h is the forward's (x where r was
+ *              NULL); dres is the gradient that reaches h past the norm; dh is the
+ *              gradient of x and of r.  ws is needed for dw only.
+ * h may be x's or r's buffer, y any buffer of its own; dh may be dy's or dres's. */
+int mle_add_rmsnorm_q8_fwd(mle_stream stream, int rows, int cols, const float* x, const float* r, const float* w,
+                           float eps, float* h, float* y, float* rstd, int8_t* q, int64_t ldq, uint8_t* e,
+                           int64_t lde);
+size_t mle_add_rmsnorm_ws_bytes(int rows, int cols);
+int mle_add_rmsnorm_bwd(mle_stream stream, int rows, int cols, const float* h, const float* w, const float* rstd,
+                        const float* dy, const float* dres, float* dh, int accumulate_dh, float* dw, int accumulate_dw,
+                        void* ws, size_t ws_bytes);
 
 /* ------------------------------------------------------------------------- */
 /* Layout (U-Net skip concatenation, transposed-convolution weights)         */
@@ -753,6 +844,27 @@ int mle_embed_gather_indexed(mle_stream stream, float* out, const float* table, 
  * Engine/kernels.cu:1536-1549). */
 int mle_embed_grad_indexed(mle_stream stream, float* dtable, const float* grad, const void* index,
                            int batch, int clen, int dim, int vocab, int accumulate);
+/* Embedding lookup with scaling, and the table's gradient by sorted tokens, for
+ * any vocabulary:
+ *   mle_embed_scaled_fwd:   out[b, s, :] = scale * table[keys[b*max_clen + s], :];
+ *     ids outside [0, vocab) give zero rows.  With index non-null (16-byte
+ *     aligned, mle_embed_sorted_index_bytes long) the same launch lists the
+ *     tokens by id, in token order within an id.
+ *   mle_embed_sorted_grad:  dtable[v, :] (+)= scale * sum of dy[t, :] over the
+ *     tokens t listed under v (accumulate 0 assigns: rows of no token become 0;
+ *     1 leaves them as they were).  index is the forward's, for the same batch,
+ *     clen and vocab; it is only read, and may serve several gradients.
+ * Tokens of an id are summed in token order, in runs of 16 where there are more,
+ * so results do not depend on timing.  GatherEmbeddings and KeyUpdate (Engine/
+ * kernels.cu:2279-2296, 1536-1549) with a scale; mle_embed_gather_indexed and
+ * mle_embed_grad_indexed have none and end at 16384 rows. */
+size_t mle_embed_sorted_index_bytes(int batch, int clen, int vocab);
+int mle_embed_scaled_fwd(mle_stream stream, float* out, const float* table, const int32_t* keys, int batch, int clen,
+                         int max_clen, int dim, int vocab, float scale, void* index, size_t index_bytes);
+size_t mle_embed_sorted_grad_ws_bytes(int batch, int clen, int dim);
+int mle_embed_sorted_grad(mle_stream stream, float* dtable, const float* dy, const void* index, size_t index_bytes,
+                          int batch, int clen, int dim, int vocab, float scale, int accumulate, void* ws,
+                          size_t ws_bytes);
 /* out[(b*clen + s)*vocab + key] = 1 for valid keys (out must be zeroed).
  * OneHotEmbeddings (Engine/kernels.cu:1551-1560). */
 int mle_onehot(mle_stream stream, float* out, const int32_t* keys, int batch, int clen, int max_clen, int vocab);

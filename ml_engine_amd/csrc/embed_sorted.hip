@@ -1,0 +1,439 @@
+// Embedding lookup with scaling, and the table's gradient by sorted tokens.
+//
+//   out[t] = scale table[key t],   dtable[v] = scale * sum of dy[t] over the tokens t with key v
+//
+// The forward also lists the tokens by key, in token order within a key: the
+// index that the gradient sums from, so that no two threads add to one element
+// and every sum has a fixed order, whatever the vocabulary's size.  Both
+// directions are bound by memory (rows of the table and of dy); the index is
+// latency that hides behind the lookup's stream, in the same launch.
+//
+// Index, in ints: head[64] (head[0]: tokens listed), rinfo[vocab] = {start,
+// count} of each table row's tokens, list[tokens], skey[tokens] (the row of
+// each place in the list).
+#include "common.hpp"
+
+#include <algorithm>
+
+using namespace mle;
+
+namespace {
+
+constexpr int IX_NT = 1024;
+constexpr int IX_RMAX = 1024;   // table rows of an index workgroup
+constexpr int IX_CHUNK = 8192;  // tokens that it sorts at a time
+constexpr int IX_HOT = 32;      // tokens of a row in a chunk above which a wave lists them by a scan
+constexpr int HEAD = 64;
+constexpr int PART = 16;        // places of the list that one partial sum covers
+
+struct IndexArgs {
+  const int32_t* keys;
+  int clen, max_clen, ntok, vocab, rows_per_wg, nix;
+  int32_t* head;
+  int2* rinfo;
+  int32_t* list;
+  int32_t* skey;
+};
+
+__device__ __forceinline__ int key_of(const IndexArgs& a, int t) {
+  return a.clen == a.max_clen ? a.keys[t] : a.keys[(int64_t)(t / a.clen) * a.max_clen + t % a.clen];
+}
+
+struct IndexLds {
+  int total[IX_RMAX];          // tokens of each row
+  int next[IX_RMAX];           // the row's next place in the list
+  int count[IX_RMAX];          // tokens of each row in this chunk
+  int end[IX_RMAX];            // places in `perm`, counted down while filling
+  int perm[IX_CHUNK];          // (row << 16) | token of the chunk, by row, in arrival order
+  unsigned short rel[IX_CHUNK];  // the row of each token of the chunk, 0xffff: none of this workgroup's
+  int hot[IX_CHUNK / (IX_HOT + 1) + 1];  // rows of the chunk that are listed by a scan
+  int wave[IX_NT / 64];
+  int smaller;
+};
+
+// Exclusive prefix sums of one value per thread over the workgroup; total in `sum`.
+__device__ __forceinline__ int exclusive_scan(int v, int* wave, int& sum) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int incl = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += x;
+  }
+  __syncthreads();
+  if (lane == 63) wave[w] = incl;
+  __syncthreads();
+  int before = 0;
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < IX_NT / 64; ++i) {
+    if (i < w) before += wave[i];
+    sum += wave[i];
+  }
+  return before + incl - v;
+}
+
+// Lists the tokens of table rows [v0, v0 + nrows): every workgroup reads all
+// the keys, and counts how many lie below its rows, which is where its part of
+// the list starts.
+__device__ void index_rows(const IndexArgs& a, int wg, IndexLds& s) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int v0 = wg * a.rows_per_wg, nrows = min(a.rows_per_wg, a.vocab - v0);
+  if (tid < IX_RMAX) s.total[tid] = 0;
+  if (tid == 0) s.smaller = 0;
+  __syncthreads();
+  int below = 0;
+  for (int t0 = tid; t0 < a.ntok; t0 += 8 * IX_NT) {
+    int key[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) key[k] = t0 + k * IX_NT < a.ntok ? key_of(a, t0 + k * IX_NT) : -1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      below += key[k] >= 0 && key[k] < v0;
+      if (key[k] >= v0 && key[k] < v0 + nrows) atomicAdd(&s.total[key[k] - v0], 1);
+    }
+  }
+  below = wave_sum(below);
+  if (lane == 0) atomicAdd(&s.smaller, below);
+  __syncthreads();
+  const int mine = tid < nrows ? s.total[tid] : 0;
+  int kept;
+  const int start = s.smaller + exclusive_scan(mine, s.wave, kept);
+  if (tid < nrows) {
+    s.next[tid] = start;
+    a.rinfo[v0 + tid] = make_int2(start, mine);
+  }
+  if (wg == a.nix - 1 && tid == 0) a.head[0] = s.smaller + kept;
+  if (kept == 0) return;
+  for (int c0 = 0; c0 < a.ntok; c0 += IX_CHUNK) {
+    const int count = min(IX_CHUNK, a.ntok - c0);
+    __syncthreads();
+    if (tid < IX_RMAX) s.count[tid] = 0;
+    __syncthreads();
+    constexpr int PER = IX_CHUNK / IX_NT;
+    int rel[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = tid + k * IX_NT;
+      const unsigned r = i < count ? (unsigned)key_of(a, c0 + i) - (unsigned)v0 : 0xffffffffu;
+      rel[k] = r < (unsigned)nrows ? (int)r : -1;
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      s.rel[tid + k * IX_NT] = (unsigned short)(rel[k] < 0 ? 0xffff : rel[k]);
+      if (rel[k] >= 0) atomicAdd(&s.count[rel[k]], 1);
+    }
+    __syncthreads();
+    // places in `perm` for the rows that are ordered by rank
+    const int here = tid < nrows ? s.count[tid] : 0;
+    const int cold = here <= IX_HOT ? here : 0;
+    int placed;
+    const int first = exclusive_scan(cold, s.wave, placed);
+    if (tid < IX_RMAX) s.end[tid] = first + cold;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (rel[k] >= 0 && s.count[rel[k]] <= IX_HOT)
+        s.perm[atomicSub(&s.end[rel[k]], 1) - 1] = (rel[k] << 16) | (tid + k * IX_NT);
+    __syncthreads();
+    // s.end is now each row's start; an entry's rank is the number of the row's
+    // entries with a smaller token
+    for (int p = tid; p < placed; p += IX_NT) {
+      const int r = s.perm[p] >> 16, i = s.perm[p] & 0xffff;
+      const int b = s.end[r], n = s.count[r];
+      int rank = 0;
+      for (int q = 0; q < n; ++q) rank += (s.perm[b + q] & 0xffff) < i;
+      const int to = s.next[r] + rank;
+      a.list[to] = c0 + i;
+      a.skey[to] = v0 + r;
+    }
+    // frequent rows: a wave walks the chunk and lists one of them in order
+    int nhot;
+    const int h = exclusive_scan(here > IX_HOT, s.wave, nhot);
+    if (here > IX_HOT) s.hot[h] = tid;
+    __syncthreads();
+    for (int k = w; k < nhot; k += IX_NT / 64) {
+      const int r = s.hot[k];
+      int to = s.next[r];
+      for (int i0 = 0; i0 < count; i0 += 256) {
+        bool hit[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) hit[u] = s.rel[i0 + 64 * u + lane] == r;  // (0xffff past the chunk's end)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const unsigned long long m = __ballot(hit[u]);
+          if (hit[u]) {
+            const int at = to + __popcll(m & ((1ull << lane) - 1));
+            a.list[at] = c0 + i0 + 64 * u + lane;
+            a.skey[at] = v0 + r;
+          }
+          to += __popcll(m);
+        }
+      }
+    }
+    __syncthreads();
+    if (tid < nrows) s.next[tid] += s.count[tid];
+  }
+}
+
+// Workgroups [0, nix) build the index, the rest look rows up.
+template <bool VEC, typename U>
+__global__ __launch_bounds__(IX_NT, 8) void embed_fwd_kernel(IndexArgs a, float* __restrict__ out,
+                                                          const float* __restrict__ table, int dim, float scale,
+                                                          U units) {
+  __shared__ IndexLds lds;
+  if ((int)blockIdx.x < a.nix) {
+    index_rows(a, blockIdx.x, lds);
+    return;
+  }
+  typedef float vec __attribute__((ext_vector_type(VEC ? 4 : 1)));
+  constexpr int W = VEC ? 4 : 1, UN = 4;
+  const U stride = (U)(gridDim.x - a.nix) * IX_NT, per = (U)(dim / W);
+  for (U u0 = (U)(blockIdx.x - a.nix) * IX_NT + threadIdx.x; u0 < units; u0 += UN * stride) {
+    vec v[UN];
+#pragma unroll
+    for (int k = 0; k < UN; ++k) {
+      const U u = u0 + k * stride;
+      v[k] = vec(0.f);
+      if (u < units) {
+        const U t = u / per;
+        const int key = key_of(a, (int)t);
+        if (key >= 0 && key < a.vocab)
+          v[k] = scale * *reinterpret_cast<const vec*>(table + (int64_t)key * dim + (int64_t)(u - t * per) * W);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < UN; ++k) {
+      const U u = u0 + k * stride;
+      if (u < units) *reinterpret_cast<vec*>(out + (int64_t)u * W) = v[k];
+    }
+  }
+}
+
+struct GradArgs {
+  float* dtable;
+  const float* dy;
+  const int32_t* head;
+  const int2* rinfo;
+  const int32_t* list;
+  const int32_t* skey;
+  float* part;  // [blocks][2][dim]
+  int dim, vocab, accumulate, blocks;
+  float scale;
+};
+
+// The sum of dy's rows list[at .. at + n), column group c, in order.
+template <typename vec>
+__device__ __forceinline__ vec sum_rows(const GradArgs& a, int at, int n, int c) {
+  constexpr int W = sizeof(vec) / 4;
+  vec s = vec(0.f);
+  const float* dy = a.dy + (int64_t)c * W;
+  int j = 0;
+  for (; j + 4 <= n; j += 4) {
+    vec v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const vec*>(dy + (int64_t)a.list[at + j + k] * a.dim);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += v[k];
+  }
+  for (; j < n; ++j) s += *reinterpret_cast<const vec*>(dy + (int64_t)a.list[at + j] * a.dim);
+  return s;
+}
+template <typename vec>
+__device__ __forceinline__ void put_row(const GradArgs& a, int row, int c, vec s) {
+  vec* p = reinterpret_cast<vec*>(a.dtable + (int64_t)row * a.dim + (int64_t)c * (sizeof(vec) / 4));
+  *p = a.accumulate ? *p + a.scale * s : a.scale * s;
+}
+
+// A token that occurs often would keep one wave busy for long, so a row with
+// more than PART tokens is summed in blocks of PART places of the list: waves
+// [0, blocks) write each block's sum of such a row (at most two rows reach
+// into a block: one that began before it or at its start, slot 0, and one
+// that begins within it, slot 1), and embed_join_kernel adds a row's blocks in
+// order.  The other waves take 2^(6 - lw) table rows each, one after another
+// by all their lanes' columns.
+template <bool VEC>
+__global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, int lw) {
+  typedef float vec __attribute__((ext_vector_type(VEC ? 4 : 1)));
+  const int lane = threadIdx.x & 63;
+  const int cols = a.dim / (VEC ? 4 : 1);
+  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if (w < a.blocks) {
+    const int total = a.head[0], p0 = (int)w * PART, n = min(PART, total - p0);
+    if (n <= 0) return;
+    const int key = lane < n ? a.skey[p0 + lane] : -1;
+    const int2 info = lane < n ? a.rinfo[key] : make_int2(0, 0);
+    const unsigned long long hot = __ballot(lane < n && info.y > PART);
+    if (!hot) return;
+#pragma unroll
+    for (int slot = 0; slot < 2; ++slot) {
+      // slot 0: the row of place p0; slot 1: the first hot row that begins later
+      const unsigned long long begins = __ballot(lane < n && info.y > PART && info.x == p0 + lane && lane > 0);
+      int b;
+      if (slot == 0) {
+        if (!(hot & 1)) continue;
+        b = 0;
+      } else {
+        if (!begins) continue;
+        b = __ffsll((long long)begins) - 1;
+      }
+      const int row = __shfl(key, b, 64);
+      const int len = __popcll(__ballot(lane < n && key == row));
+      for (int c = lane; c < cols; c += 64)
+        *reinterpret_cast<vec*>(a.part + (w * 2 + slot) * a.dim + (int64_t)c * (VEC ? 4 : 1)) = sum_rows<vec>(a, p0 + b, len, c);
+    }
+    return;
+  }
+  const int64_t row = (w - a.blocks) * (64 >> lw) + (lane >> lw);
+  if (row >= a.vocab) return;
+  const int2 info = a.rinfo[row];
+  if (info.y > PART || (a.accumulate && info.y == 0)) return;
+  for (int c = lane & ((1 << lw) - 1); c < cols; c += 1 << lw) put_row<vec>(a, (int)row, c, sum_rows<vec>(a, info.x, info.y, c));
+}
+
+// One workgroup per block of the list: joins the row that begins in it, if it
+// is one of more than PART tokens.  CW threads cover CW column groups, 1024 / CW
+// of them take the row's blocks in turn, and their sums are added in order.
+template <bool VEC>
+__global__ __launch_bounds__(1024) void embed_join_kernel(GradArgs a, int cw) {
+  typedef float vec __attribute__((ext_vector_type(VEC ? 4 : 1)));
+  constexpr int W = VEC ? 4 : 1;
+  __shared__ vec red[1024];
+  const int total = a.head[0], p0 = (int)blockIdx.x * PART, n = min(PART, total - p0);
+  if (n <= 0) return;
+  const int lane = threadIdx.x & 63;
+  const int2 info = lane < n ? a.rinfo[a.skey[p0 + lane]] : make_int2(0, 0);
+  const unsigned long long begins = __ballot(lane < n && info.y > PART && info.x == p0 + lane);
+  if (!begins) return;  // (the same in every wave)
+  const int b = __ffsll((long long)begins) - 1;
+  const int row = a.skey[p0 + b], count = __shfl(info.y, b, 64);
+  const int nblk = (b + count + PART - 1) / PART;
+  const int cols = a.dim / W, groups = 1024 / cw, g = threadIdx.x / cw, t = threadIdx.x % cw;
+  const int per = (nblk + groups - 1) / groups;  // each group a run of blocks
+  for (int c0 = 0; c0 < cols; c0 += cw) {
+    const int c = c0 + t;
+    vec s = vec(0.f);
+    if (c < cols) {
+      const int k1 = min(nblk, (g + 1) * per);
+      int k = g * per;
+      auto at = [&](int i) {
+        return reinterpret_cast<const vec*>(a.part + (((int64_t)blockIdx.x + i) * 2 + (i == 0 && b > 0 ? 1 : 0)) * a.dim +
+                                            (int64_t)c * W);
+      };
+      for (; k + 4 <= k1; k += 4) {
+        vec v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *at(k + i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += v[i];
+      }
+      for (; k < k1; ++k) s += *at(k);
+    }
+    __syncthreads();
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (g == 0 && c < cols) {
+      for (int i = 1; i < groups; ++i) s += red[i * cw + t];
+      put_row<vec>(a, row, c, s);
+    }
+  }
+}
+
+int check(const char* who, int batch, int clen, int dim, int vocab) {
+  MLE_CHECK_ARG(batch >= 0 && clen > 0 && dim > 0 && vocab > 0, "%s: bad shape (batch %d, clen %d, dim %d, vocab %d)", who,
+                batch, clen, dim, vocab);
+  MLE_CHECK_ARG((long long)batch * clen < 2147483647LL - IX_CHUNK, "%s: too many tokens", who);
+  return MLE_OK;
+}
+
+size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// The smallest power of two >= n, at most most.
+int pow2_at_least(int n, int most) {
+  int p = 1;
+  while (p < n && p < most) p *= 2;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mle_embed_sorted_index_bytes(int batch, int clen, int vocab) {
+  if (batch < 0 || clen <= 0 || vocab <= 0) return 0;
+  return round256((HEAD + 2 * (size_t)vocab + 2 * (size_t)batch * clen) * sizeof(int32_t));
+}
+
+int mle_embed_scaled_fwd(mle_stream stream, float* out, const float* table, const int32_t* keys, int batch, int clen,
+                         int max_clen, int dim, int vocab, float scale, void* index, size_t index_bytes) {
+  const int rc = check("mle_embed_scaled_fwd", batch, clen, dim, vocab);
+  if (rc) return rc;
+  MLE_CHECK_ARG(table && max_clen >= clen && (batch == 0 || (out && keys)), "mle_embed_scaled_fwd: bad argument");
+  if (index && (!aligned16(index) || index_bytes < mle_embed_sorted_index_bytes(batch, clen, vocab)))
+    return set_error(MLE_ERR_WORKSPACE, "mle_embed_scaled_fwd: index of %zu bytes, 16-byte aligned, needed",
+                     mle_embed_sorted_index_bytes(batch, clen, vocab));
+  const int ntok = batch * clen;
+  if (ntok == 0 && !index) return MLE_OK;
+  IndexArgs a{keys, clen, max_clen, ntok, vocab, 0, 0, nullptr, nullptr, nullptr, nullptr};
+  if (index) {
+    a.rows_per_wg = std::min(IX_RMAX, std::max(32, (vocab + 255) / 256));
+    a.nix = (vocab + a.rows_per_wg - 1) / a.rows_per_wg;
+    a.head = static_cast<int32_t*>(index);
+    a.rinfo = reinterpret_cast<int2*>(a.head + HEAD);
+    a.list = reinterpret_cast<int32_t*>(a.rinfo + vocab);
+    a.skey = a.list + ntok;
+  }
+  const bool vec = dim % 4 == 0 && aligned16(out) && aligned16(table);
+  const size_t units = (size_t)ntok * (dim / (vec ? 4 : 1));
+  const unsigned grid = (unsigned)a.nix + (ntok ? stream_grid((units + 3) / 4, IX_NT, 2048) : 0u);
+  hipStream_t s = as_stream(stream);
+  // 32-bit numbering where the unrolled walk stays below 2^32
+  const bool small = units < 4000000000u;
+  if (vec && small) mle::launch(embed_fwd_kernel<true, uint32_t>, grid, IX_NT, 0, s, a, out, table, dim, scale, (uint32_t)units);
+  else if (vec) mle::launch(embed_fwd_kernel<true, uint64_t>, grid, IX_NT, 0, s, a, out, table, dim, scale, (uint64_t)units);
+  else if (small) mle::launch(embed_fwd_kernel<false, uint32_t>, grid, IX_NT, 0, s, a, out, table, dim, scale, (uint32_t)units);
+  else mle::launch(embed_fwd_kernel<false, uint64_t>, grid, IX_NT, 0, s, a, out, table, dim, scale, (uint64_t)units);
+  return check_launch("mle_embed_scaled_fwd");
+}
+
+size_t mle_embed_sorted_grad_ws_bytes(int batch, int clen, int dim) {
+  if (batch <= 0 || clen <= 0 || dim <= 0) return 0;
+  return round256(((size_t)batch * clen + PART - 1) / PART * 2 * dim * sizeof(float));
+}
+
+int mle_embed_sorted_grad(mle_stream stream, float* dtable, const float* dy, const void* index, size_t index_bytes,
+                          int batch, int clen, int dim, int vocab, float scale, int accumulate, void* ws,
+                          size_t ws_bytes) {
+  const int rc = check("mle_embed_sorted_grad", batch, clen, dim, vocab);
+  if (rc) return rc;
+  MLE_CHECK_ARG(dtable && index && (batch == 0 || dy), "mle_embed_sorted_grad: null pointer");
+  if (!aligned16(index) || index_bytes < mle_embed_sorted_index_bytes(batch, clen, vocab))
+    return set_error(MLE_ERR_WORKSPACE, "mle_embed_sorted_grad: index of %zu bytes, 16-byte aligned, needed",
+                     mle_embed_sorted_index_bytes(batch, clen, vocab));
+  const size_t need = mle_embed_sorted_grad_ws_bytes(batch, clen, dim);
+  if (need && (!ws || !aligned16(ws) || ws_bytes < need))
+    return set_error(MLE_ERR_WORKSPACE, "mle_embed_sorted_grad: workspace of %zu bytes, 16-byte aligned, needed", need);
+  const int ntok = batch * clen;
+  const int32_t* head = static_cast<const int32_t*>(index);
+  const int2* rinfo = reinterpret_cast<const int2*>(head + HEAD);
+  const int32_t* list = reinterpret_cast<const int32_t*>(rinfo + vocab);
+  GradArgs a{dtable, dy, head, rinfo, list, list + ntok, static_cast<float*>(ws), dim, vocab, accumulate,
+             (ntok + PART - 1) / PART, scale};
+  const bool vec = dim % 4 == 0 && aligned16(dtable) && aligned16(dy);
+  const int cols = dim / (vec ? 4 : 1);
+  int lw = 4;  // lanes of a table row: 16, 32 or 64
+  while (lw < 6 && (1 << lw) < cols) ++lw;
+  const int64_t waves = a.blocks + ((int64_t)vocab + (64 >> lw) - 1) / (64 >> lw);
+  hipStream_t s = as_stream(stream);
+  const unsigned grid = (unsigned)((waves + 3) / 4);
+  if (vec) mle::launch(embed_grad_kernel<true>, grid, 256, 0, s, a, lw);
+  else mle::launch(embed_grad_kernel<false>, grid, 256, 0, s, a, lw);
+  if (ntok > PART) {
+    const int cw = pow2_at_least(cols, 256);
+    if (vec) mle::launch(embed_join_kernel<true>, (unsigned)a.blocks, 1024, 0, s, a, cw);
+    else mle::launch(embed_join_kernel<false>, (unsigned)a.blocks, 1024, 0, s, a, cw);
+  }
+  return check_launch("mle_embed_sorted_grad");
+}
+
+}  // extern "C"

@@ -1,0 +1,207 @@
+// Activations kept in 8 bits for the backward pass (q8.hpp has the format):
+// quantising, reading back, the activation functions around it, and a Linear's
+// weight gradient from a kept input.
+#include "activation.hpp"
+#include "q8.hpp"
+
+#include <algorithm>
+
+using namespace mle;
+using namespace q8;
+
+namespace {
+
+constexpr int NT = 256;
+
+// The elementwise kernels walk units of eight values of a row, four lanes to a
+// group of 32: units of a row are numbered to whole groups, so a group's lanes
+// always run together.
+struct Q8Args {
+  int rows, cols, units;  // units of a row: 4 per group
+  const float* x;
+  int64_t ldx;
+  float* y;
+  int64_t ldy;
+  int8_t* q;
+  int64_t ldq;
+  uint8_t* e;
+  int64_t lde;
+  float* dx;
+  int64_t lddx;
+  int accumulate;
+  int vx, vy, vq, vdx;  // rows of x, y, q, dx eight values at a time
+};
+
+// Calls f(row, column, values left of the row (0 .. 8), lane's place in the
+// group) for every unit.
+template <class F>
+__device__ __forceinline__ void each_unit(const Q8Args& a, F f) {
+  const int64_t total = (int64_t)a.rows * a.units;
+  const int64_t stride = (int64_t)gridDim.x * NT;
+  for (int64_t u = (int64_t)blockIdx.x * NT + threadIdx.x; u < total; u += stride) {
+    const int64_t row = total <= 0xffffffffLL ? (int64_t)((uint32_t)u / (uint32_t)a.units) : u / a.units;
+    const int col = (int)(u - row * a.units) * 8;
+    f(row, col, min(max(a.cols - col, 0), 8));
+  }
+}
+
+// q, e = the 8 bits of x; with KIND >= 0 also y = act(x) from the same read.
+template <int KIND>
+__global__ __launch_bounds__(NT) void q8_quantize_kernel(Q8Args a) {
+  each_unit(a, [&](int64_t row, int col, int n) {
+    float x[8];
+    load_row8(a.x + row * a.ldx + col, n, a.vx, x);
+    uint2 code;
+    const unsigned e = quantize8(x, code);
+    if (n > 0) store_codes(a.q + row * a.ldq + col, code, n, a.vq);
+    if ((threadIdx.x & 3) == 0) a.e[row * a.lde + col / q8::kGroup] = (uint8_t)e;
+    if (KIND >= 0) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = act_f<KIND < 0 ? 0 : KIND>(x[j]);
+      if (n > 0) store_row8(a.y + row * a.ldy + col, y, n, a.vy);
+    }
+  });
+}
+
+// y = the values of q, e.
+__global__ __launch_bounds__(NT) void q8_dequantize_kernel(Q8Args a) {
+  each_unit(a, [&](int64_t row, int col, int n) {
+    if (n == 0) return;
+    float y[8];
+    values8(load_codes(a.q + row * a.ldq + col, n, a.vq), q8::step_of(a.e[row * a.lde + col / q8::kGroup]), y);
+    store_row8(a.y + row * a.ldy + col, y, n, a.vy);
+  });
+}
+
+// dx (+)= act'(the kept x) * dy (a.x), as the elementwise activation backward forms it.
+template <int KIND>
+__global__ __launch_bounds__(NT) void q8_act_bwd_kernel(Q8Args a) {
+  each_unit(a, [&](int64_t row, int col, int n) {
+    if (n == 0) return;
+    float v[8], dy[8], old[8] = {};
+    values8(load_codes(a.q + row * a.ldq + col, n, a.vq), q8::step_of(a.e[row * a.lde + col / q8::kGroup]), v);
+    load_row8(a.x + row * a.ldx + col, n, a.vx, dy);
+    float* p = a.dx + row * a.lddx + col;
+    if (a.accumulate) load_row8(p, n, a.vdx, old);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act_bwd_k<KIND>(v[j], dy[j], old[j], a.accumulate != 0);
+    store_row8(p, v, n, a.vdx);
+  });
+}
+
+unsigned grid_of(const Q8Args& a) { return stream_grid((size_t)a.rows * a.units, NT, 16384); }
+
+int check_shape(const char* who, int rows, int cols, const void* q, int64_t ldq, const void* e, int64_t lde) {
+  MLE_CHECK_ARG(rows >= 0 && cols > 0, "%s: bad shape %d x %d", who, rows, cols);
+  MLE_CHECK_ARG(rows == 0 || (q && e), "%s: null pointer", who);
+  MLE_CHECK_ARG(ldq >= cols && lde >= q8::groups(cols), "%s: ldq %lld < %d or lde %lld < %d", who, (long long)ldq, cols,
+                (long long)lde, q8::groups(cols));
+  return MLE_OK;
+}
+
+#define Q8_LAUNCH_ACT(kernel, kind, a, s)                                                    \
+  switch (kind) {                                                                            \
+    case MLE_RELU: mle::launch(kernel<MLE_RELU>, grid_of(a), NT, 0, s, a); break;            \
+    case MLE_GELU: mle::launch(kernel<MLE_GELU>, grid_of(a), NT, 0, s, a); break;            \
+    case MLE_SILU: mle::launch(kernel<MLE_SILU>, grid_of(a), NT, 0, s, a); break;            \
+    case MLE_TANH: mle::launch(kernel<MLE_TANH>, grid_of(a), NT, 0, s, a); break;            \
+    case MLE_SIGMOID: mle::launch(kernel<MLE_SIGMOID>, grid_of(a), NT, 0, s, a); break;      \
+    default: mle::launch(kernel<MLE_LEAKY_RELU>, grid_of(a), NT, 0, s, a); break;            \
+  }
+
+}  // namespace
+
+extern "C" {
+
+int mle_q8_quantize(mle_stream stream, int rows, int cols, const float* x, int64_t ldx, int8_t* q, int64_t ldq,
+                    uint8_t* e, int64_t lde) {
+  const int rc = check_shape("mle_q8_quantize", rows, cols, q, ldq, e, lde);
+  if (rc) return rc;
+  MLE_CHECK_ARG((x || rows == 0) && ldx >= cols, "mle_q8_quantize: null pointer or ldx %lld < %d", (long long)ldx, cols);
+  if (rows == 0) return MLE_OK;
+  Q8Args a{rows, cols, 4 * q8::groups(cols), x, ldx, nullptr, 0, q, ldq, e, lde, nullptr, 0, 0, 0, 0, 0, 0};
+  a.vx = q8::rows_vec(x, ldx);
+  a.vq = q8::codes_vec(q, ldq);
+  mle::launch(q8_quantize_kernel<-1>, grid_of(a), NT, 0, as_stream(stream), a);
+  return check_launch("mle_q8_quantize");
+}
+
+int mle_q8_dequantize(mle_stream stream, int rows, int cols, const int8_t* q, int64_t ldq, const uint8_t* e,
+                      int64_t lde, float* y, int64_t ldy) {
+  const int rc = check_shape("mle_q8_dequantize", rows, cols, q, ldq, e, lde);
+  if (rc) return rc;
+  MLE_CHECK_ARG((y || rows == 0) && ldy >= cols, "mle_q8_dequantize: null pointer or ldy %lld < %d", (long long)ldy, cols);
+  if (rows == 0) return MLE_OK;
+  Q8Args a{rows, cols, 4 * q8::groups(cols), nullptr, 0, y, ldy, const_cast<int8_t*>(q), ldq, const_cast<uint8_t*>(e),
+           lde, nullptr, 0, 0, 0, 0, 0, 0};
+  a.vy = q8::rows_vec(y, ldy);
+  a.vq = q8::codes_vec(q, ldq);
+  mle::launch(q8_dequantize_kernel, grid_of(a), NT, 0, as_stream(stream), a);
+  return check_launch("mle_q8_dequantize");
+}
+
+int mle_q8_act_fwd(mle_stream stream, int kind, int rows, int cols, const float* x, int64_t ldx, float* y, int64_t ldy,
+                   int8_t* q, int64_t ldq, uint8_t* e, int64_t lde) {
+  const int rc = check_shape("mle_q8_act_fwd", rows, cols, q, ldq, e, lde);
+  if (rc) return rc;
+  MLE_CHECK_ARG(kind >= MLE_RELU && kind <= MLE_LEAKY_RELU, "mle_q8_act_fwd: activation %d", kind);
+  MLE_CHECK_ARG(((x && y) || rows == 0) && ldx >= cols && ldy >= cols,
+                "mle_q8_act_fwd: null pointer or a leading dimension below %d", cols);
+  if (rows == 0) return MLE_OK;
+  Q8Args a{rows, cols, 4 * q8::groups(cols), x, ldx, y, ldy, q, ldq, e, lde, nullptr, 0, 0, 0, 0, 0, 0};
+  a.vx = q8::rows_vec(x, ldx);
+  a.vy = q8::rows_vec(y, ldy);
+  a.vq = q8::codes_vec(q, ldq);
+  Q8_LAUNCH_ACT(q8_quantize_kernel, kind, a, as_stream(stream));
+  return check_launch("mle_q8_act_fwd");
+}
+
+int mle_q8_act_bwd(mle_stream stream, int kind, int rows, int cols, const int8_t* q, int64_t ldq, const uint8_t* e,
+                   int64_t lde, const float* dy, int64_t lddy, float* dx, int64_t lddx, int accumulate) {
+  const int rc = check_shape("mle_q8_act_bwd", rows, cols, q, ldq, e, lde);
+  if (rc) return rc;
+  MLE_CHECK_ARG(kind >= MLE_RELU && kind <= MLE_LEAKY_RELU, "mle_q8_act_bwd: activation %d", kind);
+  MLE_CHECK_ARG(((dy && dx) || rows == 0) && lddy >= cols && lddx >= cols,
+                "mle_q8_act_bwd: null pointer or a leading dimension below %d", cols);
+  if (rows == 0) return MLE_OK;
+  Q8Args a{rows, cols, 4 * q8::groups(cols), dy, lddy, nullptr, 0, const_cast<int8_t*>(q), ldq, const_cast<uint8_t*>(e),
+           lde, dx, lddx, accumulate, 0, 0, 0, 0};
+  a.vx = q8::rows_vec(dy, lddy);
+  a.vdx = q8::rows_vec(dx, lddx);
+  a.vq = q8::codes_vec(q, ldq);
+  Q8_LAUNCH_ACT(q8_act_bwd_kernel, kind, a, as_stream(stream));
+  return check_launch("mle_q8_act_bwd");
+}
+
+// The weight gradient: the kept values written out as floats into the
+// workspace, then the library's product.
+static size_t values_bytes(int rows, int in) { return ((size_t)rows * in * sizeof(float) + 255) & ~(size_t)255; }
+
+size_t mle_q8_linear_wgrad_ws_bytes(int rows, int in, int out) {
+  if (rows <= 0 || in <= 0 || out <= 0) return 0;
+  return values_bytes(rows, in) + mle_gemm_ws_bytes(in, out, rows, 1);
+}
+
+int mle_q8_linear_wgrad(mle_stream stream, int rows, int in, int out, const int8_t* q, int64_t ldq, const uint8_t* e,
+                        int64_t lde, const float* dY, int64_t lddy, float* dW, int64_t lddw, float* db, int accumulate,
+                        void* ws, size_t ws_bytes) {
+  int rc = check_shape("mle_q8_linear_wgrad", rows, in, q, ldq, e, lde);
+  if (rc) return rc;
+  MLE_CHECK_ARG(out > 0 && dW && (dY || rows == 0) && lddy >= out && lddw >= out,
+                "mle_q8_linear_wgrad: bad argument (out %d, lddy %lld, lddw %lld)", out, (long long)lddy, (long long)lddw);
+  if (ws_bytes < mle_q8_linear_wgrad_ws_bytes(rows, in, out) || (rows > 0 && (!ws || !aligned16(ws))))
+    return set_error(MLE_ERR_WORKSPACE, "mle_q8_linear_wgrad: workspace of %zu bytes, 16-byte aligned, needed",
+                     mle_q8_linear_wgrad_ws_bytes(rows, in, out));
+  float* x = static_cast<float*>(ws);
+  rc = mle_q8_dequantize(stream, rows, in, q, ldq, e, lde, x, in);
+  if (rc) return rc;
+  if (db && !accumulate) {
+    rc = mle_fill(stream, db, 0.f, (size_t)out);
+    if (rc) return rc;
+  }
+  return mle_gemm_ex(stream, 1, 0, in, out, rows, 1.f, x, in, 0, dY, lddy, 0, accumulate ? 1.f : 0.f, dW, lddw, 0, 1, db,
+                     nullptr, static_cast<char*>(ws) + values_bytes(rows, in), ws_bytes - values_bytes(rows, in));
+}
+
+}  // extern "C"

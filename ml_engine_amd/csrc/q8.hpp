@@ -1,0 +1,128 @@
+// Activations in 8 bits: one power-of-two step per 32 consecutive values of a
+// row.  A group's step is 2^k, k the smallest exponent in [-126, 121] for which
+// its largest magnitude is below 127.5 steps; a value is kept as the nearest
+// whole number of steps (ties to even), q in [-127, 127], and the step as the
+// byte e = k + 127.  q 2^k is off by at most half a step (magnitudes above
+// 127.5 * 2^121, whose nearest multiple would be 2^128, by less than one); every
+// operation is exact, so the same tensor always gives the same codes.
+//
+// A power of two costs up to one bit against a free scale, and buys that q 2^k
+// is a bf16 number: the matrix cores read a kept activation as it is, in one
+// bf16 plane.
+//
+// A group with an infinity or a NaN has e = 255 and the codes +1 for +inf, -1
+// for -inf, 0 for the rest: the byte as a float's exponent is infinity, so its
+// infinities come back as they were and all other values of the group as NaN.
+#pragma once
+#include "common.hpp"
+
+namespace q8 {
+
+constexpr int kGroup = 32;
+
+inline int groups(int cols) { return (cols + kGroup - 1) / kGroup; }
+
+// The value of a group's step.
+__device__ __forceinline__ float step_of(unsigned e) { return __builtin_bit_cast(float, e << 23); }
+
+// e of a group whose largest magnitude has the bits `top` (NaN above infinity).
+__device__ __forceinline__ unsigned exponent_of(unsigned top) {
+  if (top >= 0x7f800000u) return 255u;
+  const unsigned e = (top >> 23) + ((top & 0x7fffffu) >= 0x7f0000u ? 1u : 0u);
+  return e > 7u ? (e < 254u ? e - 6u : 248u) : 1u;
+}
+
+// The code of x under e, from inv = inverse_of(e).
+__device__ __forceinline__ float inverse_of(unsigned e) { return __builtin_bit_cast(float, (254u - e) << 23); }
+__device__ __forceinline__ int code_of(float x, unsigned e, float inv) {
+  if (e == 255u) return __builtin_isinf(x) ? (x > 0.f ? 1 : -1) : 0;
+  return (int)fminf(fmaxf(rintf(x * inv), -127.f), 127.f);
+}
+
+__device__ __forceinline__ unsigned magnitude(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
+
+// The larger of a value over the four lanes 4 i .. 4 i + 3.
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+  const unsigned a = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false);  // lanes 1 0 3 2
+  v = v > a ? v : a;
+  const unsigned b = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false);  // lanes 2 3 0 1
+  return v > b ? v : b;
+}
+
+// Eight values of a row, four lanes to a group: their codes in two words, and
+// the group's e.  All four lanes of a group run this together (values past
+// the row's end given as 0).
+__device__ __forceinline__ unsigned quantize8(const float (&x)[8], uint2& code) {
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned m = magnitude(x[j]);
+    top = top > m ? top : m;
+  }
+  const unsigned e = exponent_of(quad_max(top));
+  const float inv = inverse_of(e);
+  unsigned w[2] = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j >> 2] |= ((unsigned)code_of(x[j], e, inv) & 0xffu) << (8 * (j & 3));
+  code = make_uint2(w[0], w[1]);
+  return e;
+}
+
+// The values of eight codes under a step.
+__device__ __forceinline__ void values8(uint2 code, float step, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const unsigned w = j < 4 ? code.x : code.y;
+    x[j] = (float)(int)(signed char)(w >> (8 * (j & 3))) * step;
+  }
+}
+
+// n <= 8 codes at p (vec: eight of them, 8-byte aligned).
+__device__ __forceinline__ uint2 load_codes(const int8_t* __restrict__ p, int n, bool vec) {
+  if (vec && n == 8) return *reinterpret_cast<const uint2*>(p);
+  unsigned w[2] = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) w[j >> 2] |= (unsigned)(unsigned char)p[j] << (8 * (j & 3));
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ void store_codes(int8_t* __restrict__ p, uint2 c, int n, bool vec) {
+  if (vec && n == 8) {
+    *reinterpret_cast<uint2*>(p) = c;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < n) p[j] = (int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+}
+
+// n <= 8 floats at p (vec: eight of them, 16-byte aligned), the rest 0.
+__device__ __forceinline__ void load_row8(const float* __restrict__ p, int n, bool vec, float (&x)[8]) {
+  if (vec && n == 8) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = a[j];
+      x[4 + j] = b[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
+  }
+}
+__device__ __forceinline__ void store_row8(float* __restrict__ p, const float (&x)[8], int n, bool vec) {
+  if (vec && n == 8) {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = x[j];
+  }
+}
+
+// Whether rows of a tensor can be read and written eight values at a time.
+inline bool rows_vec(const float* p, int64_t ld) { return mle::aligned16(p) && ld % 4 == 0; }
+inline bool codes_vec(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0 && ld % 8 == 0; }
+
+}  // namespace q8

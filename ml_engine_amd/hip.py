@@ -104,6 +104,15 @@ SIGNATURES: dict[str, tuple] = {
     "mle_softmax_xent_keys_bwd": (I, [P, P, P, P, I, I, P, P, I, I, I]),
     "mle_softmax_xent_fwd": (I, [P, P, P, P, I, I, P, P, SZ]),
     "mle_softmax_xent_bwd": (I, [P, P, P, P, P, SZ, I]),
+    "mle_vocab_xent_ws_bytes": (SZ, [I, I, I]),
+    "mle_vocab_xent_fwd": (I, [P, I, I, I, P, I64, P, I64, P, P, I, I, F, P, P, P, P, SZ]),
+    "mle_vocab_xent_bwd": (I, [P, I, I, I, P, I64, P, I64, P, P, I, I, P, P, F, P, I64, I, P, I64, P, I, P, SZ]),
+    "mle_q8_quantize": (I, [P, I, I, P, I64, P, I64, P, I64]),
+    "mle_q8_dequantize": (I, [P, I, I, P, I64, P, I64, P, I64]),
+    "mle_q8_act_fwd": (I, [P, I, I, I, P, I64, P, I64, P, I64, P, I64]),
+    "mle_q8_act_bwd": (I, [P, I, I, I, P, I64, P, I64, P, I64, P, I64, I]),
+    "mle_q8_linear_wgrad_ws_bytes": (SZ, [I, I, I]),
+    "mle_q8_linear_wgrad": (I, [P, I, I, I, P, I64, P, I64, P, I64, P, I64, P, I, P, SZ]),
     "mle_norm_ws_bytes": (SZ, [I, I, SZ, I]),
     "mle_norm_fwd": (I, [P, P, P, P, I, I, SZ, I, F, P, SZ]),
     "mle_norm_fwd_ex": (I, [P, P, P, P, I, I, SZ, I, F, P, SZ, I]),
@@ -119,6 +128,9 @@ SIGNATURES: dict[str, tuple] = {
     "mle_batchnorm_bwd": (I, [P, P, P, P, P, I, I, SZ, F, P, SZ, I]),
     "mle_rmsnorm_fwd": (I, [P, P, P, P, I, I, I, I]),
     "mle_rmsnorm_bwd": (I, [P, P, P, P, P, I, I, I, I, I]),
+    "mle_add_rmsnorm_q8_fwd": (I, [P, I, I, P, P, P, F, P, P, P, P, I64, P, I64]),
+    "mle_add_rmsnorm_ws_bytes": (SZ, [I, I]),
+    "mle_add_rmsnorm_bwd": (I, [P, I, I, P, P, P, P, P, P, I, P, I, P, SZ]),
     "mle_copy_crop_fwd": (I, [P, P, P, P, I, I, I, I, I, I, I]),
     "mle_copy_crop_bwd": (I, [P, P, P, P, I, I, I, I, I, I, I, I, I]),
     "mle_weight_swap": (I, [P, P, P, I, I, I, I]),
@@ -145,6 +157,10 @@ SIGNATURES: dict[str, tuple] = {
     "mle_embed_index_bytes": (SZ, [I, I, I]),
     "mle_embed_gather_indexed": (I, [P, P, P, P, I, I, I, I, I, P, SZ]),
     "mle_embed_grad_indexed": (I, [P, P, P, P, I, I, I, I, I]),
+    "mle_embed_sorted_index_bytes": (SZ, [I, I, I]),
+    "mle_embed_scaled_fwd": (I, [P, P, P, P, I, I, I, I, I, F, P, SZ]),
+    "mle_embed_sorted_grad_ws_bytes": (SZ, [I, I, I]),
+    "mle_embed_sorted_grad": (I, [P, P, P, P, SZ, I, I, I, I, F, I, P, SZ]),
     "mle_onehot": (I, [P, P, P, I, I, I, I]),
     "mle_onehot_update": (I, [P, P, P, P, I, I, I, I]),
     "mle_argmax": (I, [P, P, I, I, P]),

@@ -1,0 +1,297 @@
+"""The vocabulary's cross entropy without stored logits, against 64 bits."""
+import numpy as np
+import pytest
+
+from conftest import rng
+
+pytestmark = pytest.mark.gpu
+STEP = 2.0 ** -23  # a step of fp32: a sum that is truncated loses at most one per term
+
+
+class Case:
+    """Inputs on the device, strided, with what lies past the rows filled."""
+
+    def __init__(self, hip, rows, d, vocab, bias=True, ignored=0.2, pad=0, clen=None, max_clen=None, seed=0, scale=1.0):
+        r = rng(seed + rows + d + vocab)
+        self.hip, self.rows, self.d, self.vocab = hip, rows, d, vocab
+        self.clen = clen or rows
+        self.max_clen = max_clen or self.clen
+        self.x = (scale * r.standard_normal((rows, d))).astype(np.float32)
+        self.w = (r.uniform(-1, 1, (d, vocab)) * np.sqrt(3.0 / d)).astype(np.float32)
+        self.b = r.uniform(-1, 1, vocab).astype(np.float32) if bias else None
+        self.keys = r.integers(0, vocab, rows).astype(np.int32)
+        self.keys[r.random(rows) < ignored] = r.choice(np.array([-1, -2 ** 31, vocab, 2 ** 31 - 1]))
+        self.pad = pad
+        self.scale = 1.0 / max(1, int(self.valid().sum()))
+
+    def valid(self):
+        return (self.keys >= 0) & (self.keys < self.vocab)
+
+    def put(self):
+        wide = lambda a, n: np.concatenate([a, np.full((a.shape[0], n), np.nan, np.float32)], axis=1)  # noqa: E731
+        full = np.full((self.rows // self.clen, self.max_clen), 1, np.int32)
+        full[:, : self.clen] = self.keys.reshape(-1, self.clen)
+        B = self.hip.Buffer
+        self.gx, self.gw = B.from_array(wide(self.x, self.pad)), B.from_array(wide(self.w, self.pad))
+        self.gb = B.from_array(self.b) if self.b is not None else None
+        self.gk = B.from_array(full)
+        self.ws = B(self.hip.lib().mle_vocab_xent_ws_bytes(self.rows, self.d, self.vocab))
+        self.lse, self.row_loss, self.loss = B.empty(self.rows), B.empty(self.rows), B.empty(1)
+
+    def shape(self):
+        return (self.rows, self.d, self.vocab, self.gx.ptr, self.d + self.pad, self.gw.ptr, self.vocab + self.pad,
+                self.gb.ptr if self.gb else None, self.gk.ptr, self.clen, self.max_clen)
+
+    def forward(self, stream=None):
+        self.hip.call("mle_vocab_xent_fwd", stream, *self.shape(), self.scale, self.lse.ptr, self.row_loss.ptr, self.loss.ptr,
+                      self.ws.ptr, self.ws.nbytes)
+        return self.lse.numpy(), self.row_loss.numpy(), float(self.loss.numpy()[0])
+
+    def backward(self, acc=0, upstream=None, want=("dx", "dw", "db"), old=0.0, stream=None):
+        B = self.hip.Buffer
+        full = lambda *s: B.from_array(np.full(s, old, np.float32))  # noqa: E731
+        self.gdx, self.gdw, self.gdb = full(self.rows, self.d + self.pad), full(self.d, self.vocab + self.pad), full(self.vocab)
+        up = B.from_array(np.array([upstream], np.float32)) if upstream is not None else None
+        self.hip.call("mle_vocab_xent_bwd", stream, *self.shape(), self.lse.ptr, up.ptr if up else None, self.scale,
+                      self.gdx.ptr if "dx" in want else None, self.d + self.pad, acc, self.gdw.ptr if "dw" in want else None,
+                      self.vocab + self.pad, self.gdb.ptr if "db" in want else None, acc, self.ws.ptr, self.ws.nbytes)
+        dx, dw, db = self.gdx.numpy(), self.gdw.numpy(), self.gdb.numpy()
+        assert (dx[:, self.d:] == np.float32(old)).all() and (dw[:, self.vocab:] == np.float32(old)).all()
+        return dx[:, : self.d], dw[:, : self.vocab], db
+
+    def exact(self, upstream=1.0):
+        """Values in 64 bits, and how far fp32 sums may be from them."""
+        x, w = self.x.astype(np.float64), self.w.astype(np.float64)
+        b = self.b.astype(np.float64) if self.b is not None else np.zeros(self.vocab)
+        ok, at = self.valid(), np.arange(self.rows)
+        l = x @ w + b
+        top = l.max(1, keepdims=True)
+        e = np.exp(l - top)
+        lse = (top + np.log(e.sum(1, keepdims=True)))[:, 0]
+        k = np.where(ok, self.keys, 0)
+        row_loss = np.where(ok, lse - l[at, k], 0)
+        p = np.exp(l - lse[:, None])
+        # a logit: a step per product and for the bias; lse: the largest logit's
+        # error, the sum's relative one, and the final operations'
+        dl = STEP * ((self.d + 4) * (np.abs(x) @ np.abs(w)) + 2 * np.abs(b))
+        dlse = (p * dl).sum(1) + STEP * (8 + np.log2(self.vocab) + 2 * np.abs(lse) + 2 * np.abs(top[:, 0]))
+        # (a probability below 2^-126 is no normal number: it may come out as 0)
+        dp = p * (dl + dlse[:, None] + STEP * (8 + np.abs(l) + np.abs(lse)[:, None])) + 2.0 ** -126
+        p[at, k] -= ok
+        dp[at, k] += STEP
+        g = ok[:, None] * self.scale * upstream
+        p, dp = p * g, (dp + 4 * STEP * np.abs(p)) * np.abs(g)
+        x0 = np.where(ok[:, None], x, 0)
+        out = dict(lse=lse, row_loss=row_loss, loss=row_loss.sum() * self.scale, dx=p @ w.T, dw=x0.T @ p, db=p.sum(0))
+        tol = dict(lse=dlse, row_loss=ok * (dlse + dl[at, k] + 2 * STEP * np.abs(row_loss)),
+                   dx=dp @ np.abs(w.T) + (self.vocab + 4) * STEP * (np.abs(p) @ np.abs(w.T)),
+                   dw=np.abs(x0.T) @ dp + (self.rows + 4) * STEP * (np.abs(x0.T) @ np.abs(p)),
+                   db=dp.sum(0) + (self.rows + 4) * STEP * np.abs(p).sum(0))
+        tol["loss"] = self.scale * tol["row_loss"].sum() + 4 * STEP * abs(out["loss"])
+        return out, tol
+
+
+def close(got, ref, tol, what):
+    err = np.abs(np.asarray(got, np.float64) - ref)
+    assert (err <= tol).all(), f"{what}: {np.max(err / np.maximum(tol, 1e-300)):.3g} times the bound"
+
+
+SHAPES = [(1, 1, 1), (1, 8, 100), (3, 33, 70), (64, 64, 1000), (64, 256, 4096), (100, 31, 257), (130, 96, 129), (255, 40, 513),
+          (256, 128, 1024), (300, 330, 1007), (513, 64, 640), (1030, 65, 777), (2048, 64, 300), (5, 512, 20011)]
+
+
+@pytest.mark.parametrize("rows,d,vocab", SHAPES)
+@pytest.mark.parametrize("bias,pad,acc", [(True, 0, 0), (False, 3, 1), (True, 4, 1)])
+def test_against_64_bits(hip, rows, d, vocab, bias, pad, acc):
+    c = Case(hip, rows, d, vocab, bias, pad=pad)
+    c.put()
+    ref, tol = c.exact(upstream=0.75)
+    lse, row_loss, loss = c.forward()
+    close(lse, ref["lse"], tol["lse"], "lse")
+    close(row_loss, ref["row_loss"], tol["row_loss"], "row_loss")
+    close(loss, ref["loss"], tol["loss"], "loss")
+    old = 0.25
+    dx, dw, db = c.backward(acc=acc, upstream=0.75, old=old)
+    for name, got in (("dx", dx), ("dw", dw), ("db", db)):
+        base = old if acc else 0.0
+        close(got, ref[name] + base, tol[name] + 2 * STEP * (base + np.abs(ref[name])), name)
+    assert acc or (dx[~c.valid()] == 0).all()
+
+
+@pytest.mark.parametrize("clen,max_clen", [(20, 20), (20, 27)])
+def test_padded_sequences(hip, clen, max_clen):
+    c = Case(hip, 120, 48, 333, clen=clen, max_clen=max_clen)
+    c.put()
+    ref, tol = c.exact()
+    _, row_loss, _ = c.forward()
+    close(row_loss, ref["row_loss"], tol["row_loss"], "row_loss")
+    close(c.backward()[1], ref["dw"], tol["dw"], "dw")
+
+
+@pytest.mark.parametrize("rows", [40, 700])
+def test_what_rows_outside_hold_stays_there(hip, rows):
+    """NaN and infinity in rows that take no part: the loss, dW, db and the other rows' dX as without them."""
+    c = Case(hip, rows, 64, 500, ignored=0.3)
+    bad = np.flatnonzero(~c.valid())
+    c.x[bad] = 0
+    c.put()
+    ref, tol = c.exact()
+    c.x[bad[::2]] = np.nan
+    c.x[bad[1::2], 3] = -np.inf
+    c.put()
+    _, row_loss, loss = c.forward()
+    dx, dw, db = c.backward()
+    # (not the same bits: a tile of products that meets a NaN is multiplied
+    # again in fp32, whose sums round elsewhere within the same bounds)
+    for name, got in (("row_loss", row_loss), ("loss", loss), ("dx", dx), ("dw", dw), ("db", db)):
+        close(got, ref[name], tol[name], name)
+
+
+def test_no_row_takes_part(hip):
+    c = Case(hip, 70, 32, 200, ignored=1.1)
+    c.put()
+    _, row_loss, loss = c.forward()
+    dx, dw, db = c.backward()
+    assert loss == 0 and not row_loss.any() and not dx.any() and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("rows", [33, 600])
+def test_masked_entries(hip, rows):
+    """A bias of -infinity: as if the entry were not in the vocabulary."""
+    c = Case(hip, rows, 64, 400)
+    out = np.arange(0, 400, 3)
+    c.keys[np.isin(c.keys, out)] += 1
+    keep = np.setdiff1d(np.arange(400), out)
+    c.b[out] = -np.inf
+    c.put()
+    lse, row_loss, _ = c.forward()
+    dx, dw, db = c.backward()
+    small = Case(hip, rows, 64, keep.size)
+    small.x, small.w, small.b, small.scale = c.x, np.ascontiguousarray(c.w[:, keep]), c.b[keep], c.scale
+    small.keys = np.where(c.valid(), np.searchsorted(keep, np.where(c.valid(), c.keys, keep[0])), -1).astype(np.int32)
+    ref, tol = small.exact()
+    close(lse, ref["lse"], tol["lse"], "lse")
+    close(row_loss, ref["row_loss"], tol["row_loss"], "row_loss")
+    close(dx, ref["dx"], tol["dx"], "dx")
+    close(dw[:, keep], ref["dw"], tol["dw"], "dw")
+    assert not dw[:, out].any() and not db[out].any()
+
+
+@pytest.mark.parametrize("rows", [20, 520])
+def test_not_finite_rows(hip, rows):
+    """A NaN in a row that takes part: its lse and the loss are NaN, other rows' values stay."""
+    c = Case(hip, rows, 64, 300, ignored=0.0)
+    c.put()
+    ref, tol = c.exact()
+    c.x[7, 5] = np.nan
+    c.put()
+    lse, row_loss, loss = c.forward()
+    assert np.isnan(lse[7]) and np.isnan(row_loss[7]) and np.isnan(loss)
+    close(np.delete(lse, 7), np.delete(ref["lse"], 7), np.delete(tol["lse"], 7), "lse")
+    dx, dw, _ = c.backward()
+    assert np.isnan(dx[7]).all() and np.isfinite(np.delete(dx, 7, 0)).all() and np.isnan(dw).all()
+
+
+@pytest.mark.parametrize("rows", [50, 640])
+def test_parts_of_the_gradient(hip, rows):
+    """dX alone, dW alone, dW without db, and no row losses: the same bits."""
+    c = Case(hip, rows, 96, 700)
+    c.put()
+    c.forward()
+    dx, dw, db = c.backward()
+    assert np.array_equal(c.backward(want=("dx",))[0], dx)
+    one = c.backward(want=("dw", "db"))
+    assert np.array_equal(one[1], dw) and np.array_equal(one[2], db)
+    assert np.array_equal(c.backward(want=("dw",))[1], dw)
+    lse, loss = c.lse.numpy(), c.loss.numpy()
+    c.hip.call("mle_vocab_xent_fwd", None, *c.shape(), c.scale, c.lse.ptr, None, c.loss.ptr, c.ws.ptr, c.ws.nbytes)
+    assert np.array_equal(c.lse.numpy(), lse) and np.array_equal(c.loss.numpy(), loss)
+
+
+@pytest.mark.parametrize("rows,scale", [(48, 2.0 ** -40), (48, 60.0), (600, 2.0 ** -40), (600, 60.0)])
+def test_small_and_confident_rows(hip, rows, scale):
+    """Rows of tiny values (a flat softmax), and logits up to some hundreds."""
+    c = Case(hip, rows, 64, 600, scale=scale)
+    c.put()
+    ref, tol = c.exact()
+    lse, row_loss, _ = c.forward()
+    close(lse, ref["lse"], tol["lse"], "lse")
+    close(row_loss, ref["row_loss"], tol["row_loss"], "row_loss")
+    dx, dw, db = c.backward()
+    close(dx, ref["dx"], tol["dx"], "dx")
+    close(dw, ref["dw"], tol["dw"], "dw")
+    close(db, ref["db"], tol["db"], "db")
+
+
+@pytest.mark.parametrize("rows", [64, 900])
+def test_values_of_very_different_size(hip, rows):
+    """Columns of X and rows of W from 2^-30 to 2^30 of each other."""
+    c = Case(hip, rows, 64, 500)
+    f = np.exp2(rng(1).integers(-30, 31, 64)).astype(np.float32)
+    c.x = (c.x * f).astype(np.float32)
+    c.w = (c.w / f[:, None]).astype(np.float32)
+    c.put()
+    ref, tol = c.exact()
+    close(c.forward()[0], ref["lse"], tol["lse"], "lse")
+    dx, dw, _ = c.backward()
+    close(dx, ref["dx"], tol["dx"], "dx")
+    close(dw, ref["dw"], tol["dw"], "dw")
+
+
+@pytest.mark.parametrize("rows,d,vocab", [(64, 256, 4096), (1024, 256, 2000), (2048, 512, 1000)])
+def test_two_norm(hip, rows, d, vocab):
+    """The error of a typical case in the 2-norm: that of fp32 products, well
+    under the worst-case bounds above (24 bits each, random in sign)."""
+    c = Case(hip, rows, d, vocab, ignored=0.0)
+    c.put()
+    ref, _ = c.exact()
+    lse, _, _ = c.forward()
+    dx, dw, db = c.backward()
+    for got, want in ((lse, ref["lse"]), (dx, ref["dx"]), (dw, ref["dw"]), (db, ref["db"])):
+        assert np.linalg.norm(got - want) <= 2e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("rows", [60, 800])
+def test_repeats(hip, rows):
+    c = Case(hip, rows, 80, 900)
+    c.put()
+    a = (*c.forward(), *c.backward())
+    b = (*c.forward(), *c.backward())
+    for u, v in zip(a, b):
+        assert np.array_equal(u, v)
+
+
+def test_gradient_against_differences(hip):
+    c = Case(hip, 6, 10, 30, ignored=0.3)
+    c.put()
+    c.forward()
+    dx, dw, db = c.backward()
+
+    def f(x, w, b):
+        l = x @ w + b
+        m = l.max(1)
+        z = m + np.log(np.exp(l - m[:, None]).sum(1))
+        ok = c.valid()
+        return float((z - l[np.arange(6), np.where(ok, c.keys, 0)])[ok].sum() * c.scale)
+
+    args, h = [a.astype(np.float64) for a in (c.x, c.w, c.b)], 1e-5
+    for n, grad in enumerate((dx, dw, db)):
+        for i in np.ndindex(*args[n].shape):
+            d = [a.copy() for a in args]
+            d[n][i] += h
+            up = f(*d)
+            d[n][i] -= 2 * h
+            # the difference's own error is about h^2 and 1e-16 / h
+            assert abs((up - f(*d)) / (2 * h) - grad[i]) <= 1e-6
+
+
+def test_no_rows(hip):
+    w, loss = hip.Buffer.from_array(np.ones((8, 20), np.float32)), hip.Buffer.from_array(np.ones(1, np.float32))
+    dw, db = hip.Buffer.from_array(np.ones((8, 20), np.float32)), hip.Buffer.from_array(np.ones(20, np.float32))
+    shape = (0, 8, 20, None, 8, w.ptr, 20, None, None, 1, 1)
+    hip.call("mle_vocab_xent_fwd", None, *shape, 1.0, None, None, loss.ptr, None, 0)
+    assert loss.numpy()[0] == 0
+    hip.call("mle_vocab_xent_bwd", None, *shape, None, None, 1.0, None, 8, 0, dw.ptr, 20, db.ptr, 1, None, 0)
+    assert (dw.numpy() == 1).all() and (db.numpy() == 1).all()
+    hip.call("mle_vocab_xent_bwd", None, *shape, None, None, 1.0, None, 8, 0, dw.ptr, 20, db.ptr, 0, None, 0)
+    assert not dw.numpy().any() and not db.numpy().any()
