@@ -149,4 +149,133 @@ __device__ __forceinline__ void multiply(const Operand& A, const Operand& B, int
   }
 }
 
+// The same with one accumulator, cleared every `run` stages: end(first stage of
+// the run) then adds it to sums that the caller keeps.  For operands whose later
+// planes are not scaled against the first, so that all products are of one scale.
+template <class S, class F>
+__device__ __forceinline__ void multiply_runs(const Operand& A, const Operand& B, int tm, int tn, int k0, int k1, int run,
+                                              char* lds, const Lane<S>& w, f32x4 (&acc)[4][4], F end) {
+  if (k0 < k1) stage_load<S>(A, B, tm, tn, k0, lds);
+  for (int kr = k0; kr < k1; kr += run) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) acc[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int ke = min(k1, kr + run);
+    for (int k = kr; k < ke; ++k) {
+      char* cur = lds + ((k - k0) & 1) * S::STAGE;
+      char* nxt = lds + (((k - k0) & 1) ^ 1) * S::STAGE;
+      __syncthreads();
+      if (k + 1 < k1) stage_load<S>(A, B, tm, tn, k + 1, nxt);
+      stage_mma<S>(cur, w, acc, acc);
+    }
+    end(kr);
+  }
+}
+
+// ------------------------------------------------------------- fp16 operands
+// x 2^e in two fp16 planes, h + 2^-LO l: with |x 2^e| < 2^15 the pair holds 22 bits
+// of every value down to 2^(LO - 14) and 2^-(24 + LO) of the smaller ones.  What is
+// not finite stays in the first plane.
+template <int LO>
+__device__ __forceinline__ void split16(float x, int e, _Float16& h, _Float16& l) {
+  const float v = __builtin_ldexpf(x, e);
+  h = (_Float16)v;
+  const float rest = v - (float)h;
+  l = __builtin_isfinite(v) ? (_Float16)__builtin_ldexpf(rest, LO) : (_Float16)0.f;
+}
+template <int LO>
+__device__ __forceinline__ void put16(char* p, const float (&x)[8], const int (&e)[8]) {
+  f16x8 h, l;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    _Float16 a, b;
+    split16<LO>(x[j], e[j], a, b);
+    h[j] = a;
+    l[j] = b;
+  }
+  *reinterpret_cast<f16x8*>(p) = h;
+  *reinterpret_cast<f16x8*>(p + kUnit) = l;
+}
+
+struct PackArgs {
+  const float* src;
+  int64_t ld;
+  int rows, k;          // of the operand; rest zeros
+  int blocks, kblocks;  // of the packed operand
+  const int* ex;        // exponents by k or by row
+  const int* keys;      // nullable, by k: < 0 leaves that k out (zeros, whatever it holds)
+  char* out;
+  int vec;              // 16-byte loads
+};
+
+// Operands whose k runs along the source's rows (element (row, k) at row * ld + k): a
+// wave per unit, 128 contiguous bytes of 16 rows.
+template <bool EX_BY_K, int LO>
+__global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
+  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (u >= (int64_t)a.blocks * a.kblocks) return;
+  const int lane = threadIdx.x & 63;
+  const int kb = (int)(u / a.blocks), blk = (int)(u - (int64_t)kb * a.blocks);
+  const int row = (blk >> 2) * 64 + 4 * (lane & 15) + (blk & 3), k = kb * 32 + 8 * (lane >> 4);
+  float x[8];
+  int e[8];
+  const int n = row < a.rows ? min(max(a.k - k, 0), 8) : 0;
+  const float* p = a.src + (int64_t)row * a.ld + k;
+  if (a.vec && n == 8) {
+    const f32x4 v0 = reinterpret_cast<const f32x4*>(p)[0], v1 = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = v0[j];
+      x[4 + j] = v1[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = EX_BY_K ? a.ex[min(k + j, a.k - 1)] : a.ex[min(row, a.rows - 1)];
+  put16<LO>(a.out + u * 2 * kUnit + lane * 16, x, e);
+}
+
+// Operands whose rows run along the source's (element (row, k) at k * ld + row): a
+// wave per 64-row group and k block, 256 contiguous bytes of 32 source rows; the
+// 4 x 8 values of a lane are transposed in its registers.
+template <bool EX_BY_K, int LO>
+__global__ __launch_bounds__(256) void pack_cols_kernel(PackArgs a) {
+  const int groups = a.blocks >> 2;
+  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (u >= (int64_t)groups * a.kblocks) return;
+  const int lane = threadIdx.x & 63;
+  const int kb = (int)(u / groups), g = (int)(u - (int64_t)kb * groups);
+  const int row = g * 64 + 4 * (lane & 15), k = kb * 32 + 8 * (lane >> 4);
+  f32x4 x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool live = k + j < a.k && (!a.keys || a.keys[k + j] >= 0);
+    const float* p = a.src + (int64_t)(k + j) * a.ld + row;
+    x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (live && a.vec && row + 3 < a.rows) {
+      x[j] = *reinterpret_cast<const f32x4*>(p);
+    } else if (live) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row + i < a.rows) x[j][i] = p[i];
+    }
+  }
+  int e[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = EX_BY_K ? a.ex[min(k + j, a.k - 1)] : 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = x[j][i];
+      if (!EX_BY_K) e[j] = a.ex[min(row + i, a.rows - 1)];
+    }
+    put16<LO>(a.out + ((int64_t)kb * a.blocks + g * 4 + i) * 2 * kUnit + lane * 16, v, e);
+  }
+}
+
 }  // namespace planes

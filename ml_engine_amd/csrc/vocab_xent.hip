@@ -9,7 +9,28 @@
 // The logits are formed piece by piece of the vocabulary, once in the forward
 // and once more in the backward: 8 rows d vocab operations where keeping
 // rows x vocab logits would take 6.
-#include "common.hpp"
+//
+// Few rows: the library's product writes a piece's logits to the workspace and
+// small kernels walk them.  More rows: products of fp16 planes (planes.hpp), in which
+// no logit is ever stored.
+//
+//   An fp32 value scaled into fp16's range is the sum of two fp16 values to 22
+//   bits, and three MFMAs (h h, h l, l h) make a product where three bf16 planes
+//   (split_core.hpp) need six.  The error per product, 2^-22 and random, is that
+//   of fp32 products summed over a long k.  Scales are powers of two, one per index
+//   wherever the sum allows it:
+//     logits  X by feature (its largest magnitude to 2^15), W by the same feature
+//             inversely and one factor per piece: a feature's share of a logit
+//             keeps its bits however the two sides divide it
+//     dX      W by feature; P as it is, |P| <= 1
+//     dW      X by feature; P by column and 64 rows, whose partial sums are
+//             scaled back one by one
+//   so that a small gradient of a column or feature is as exact as a large one.
+//
+//   P leaves the tile that forms it in both orders, packed for the two products
+//   that read it; db's column sums are taken from the same registers.
+#include "gemm_args.hpp"
+#include "planes.hpp"
 
 #include <float.h>
 
@@ -24,7 +45,9 @@ constexpr int NT = 256;
 struct Rows {
   const int32_t* keys;
   int clen, max_clen, vocab;
+  int r0;  // the call's row that is row 0 here
   __device__ __forceinline__ int key(int64_t r) const {
+    r += r0;
     const int k = keys[clen == max_clen ? r : r / clen * max_clen + r % clen];
     return k >= 0 && k < vocab ? k : -1;
   }
@@ -63,7 +86,7 @@ __global__ __launch_bounds__(NT) void xent_stats_kernel(const float* __restrict_
 // lse, the row losses and their scaled sum; one workgroup.
 __global__ __launch_bounds__(1024) void xent_finish_kernel(const RowState* __restrict__ state, int nrows, Rows rows,
                                                            float scale, float* __restrict__ lse,
-                                                           float* __restrict__ row_loss, float* __restrict__ loss) {
+                                                           float* __restrict__ row_loss, float* __restrict__ loss, int add) {
   __shared__ double red[16];
   double sum = 0.0;
   for (int64_t r = threadIdx.x; r < nrows; r += 1024) {
@@ -75,7 +98,7 @@ __global__ __launch_bounds__(1024) void xent_finish_kernel(const RowState* __res
     sum += (double)one;
   }
   sum = block_sum<1024>(sum, red);
-  if (threadIdx.x == 0) loss[0] = (float)(sum * (double)scale);
+  if (threadIdx.x == 0) loss[0] = (float)(sum * (double)scale) + (add ? loss[0] : 0.f);
 }
 
 // The rows of X that take part, the others as zeros: what a row that takes no
@@ -98,17 +121,417 @@ __global__ __launch_bounds__(NT) void xent_grad_kernel(float* __restrict__ l, in
   for (int c = threadIdx.x; c < cols; c += NT) x[c] = k >= 0 ? g * (expf(x[c] - z) - (c + v0 == k ? 1.f : 0.f)) : 0.f;
 }
 
+// ---------------------------------------------------------------- fp16 planes
+using planes::Operand;
+using S = planes::Shape<planes::Fp16, 2, 2, 2, 2>;  // 128 x 128 of C, two workgroups to a CU
+constexpr int kTile = 128;
+constexpr int kLo = 11;      // the second plane's scale against the first, where it has one
+constexpr int kTop = 15;     // scaled magnitudes are below 2^kTop
+constexpr int kNone = -400;  // exponent of a feature that is zero everywhere
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// ceil(log2) of the finite magnitudes seen: every one of them is below 2^this.
+__device__ __forceinline__ int exponent_above(unsigned bits) {
+  return bits == 0 ? kNone : max((int)(bits >> 23), 1) - 126;
+}
+__device__ __forceinline__ unsigned finite_bits(float x) {
+  const unsigned b = __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+struct AmaxArgs {
+  const float* X;
+  int64_t ldx;
+  const float* W;
+  int64_t ldw;
+  int rows, d, vocab, piece, chunks;  // chunks: of 4096 columns, per piece
+  int slabs, slab_rows, xblocks;      // X: blocks of 256 columns x slabs
+  unsigned* xpart;                    // [slabs][d]
+  unsigned* wpart;                    // [pieces][chunks][d]
+};
+
+// The largest finite magnitude of each feature: of X over slabs of rows, of W over
+// chunks of a piece's columns.
+__global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a) {
+  __shared__ unsigned red[NT / 64];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < a.xblocks) {
+    const int tiles = (a.d + NT - 1) / NT;
+    const int slab = blockIdx.x / tiles, k = (blockIdx.x % tiles) * NT + tid;
+    if (k >= a.d) return;
+    const int r1 = min(a.rows, (slab + 1) * a.slab_rows);
+    unsigned m = 0;
+#pragma unroll 8
+    for (int r = slab * a.slab_rows; r < r1; ++r) m = max(m, finite_bits(a.X[(int64_t)r * a.ldx + k]));
+    a.xpart[(int64_t)slab * a.d + k] = m;
+    return;
+  }
+  const int64_t b = blockIdx.x - a.xblocks;
+  const int k = (int)(b % a.d), c = (int)(b / a.d);
+  const int v0 = c / a.chunks * a.piece + c % a.chunks * 4096;
+  const int v1 = min(min(v0 + 4096, (c / a.chunks + 1) * a.piece), a.vocab);
+  unsigned m = 0;
+  const float* w = a.W + (int64_t)k * a.ldw;
+#pragma unroll 4
+  for (int v = v0 + tid; v < v1; v += NT) m = max(m, finite_bits(w[v]));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = m;
+  __syncthreads();
+  if (tid == 0) a.wpart[(int64_t)c * a.d + k] = max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+// Exponents: ex[k] of X; for piece p, el[p][k] of W in the logits, en[p][k] of W in dX,
+// scale[p]: a logit is its sum times 2^scale.  A workgroup per piece.
+__global__ __launch_bounds__(NT) void xent_scales_kernel(AmaxArgs a, int* __restrict__ ex, int* __restrict__ el,
+                                                         int* __restrict__ en, int* __restrict__ scale) {
+  __shared__ int red[NT / 64];
+  const int p = blockIdx.x, tid = threadIdx.x;
+  int top = 2 * kNone;
+  for (int k = tid; k < a.d; k += NT) {
+    unsigned x = 0, w = 0;
+#pragma unroll 8
+    for (int s = 0; s < a.slabs; ++s) x = max(x, a.xpart[(int64_t)s * a.d + k]);
+    for (int c = 0; c < a.chunks; ++c) w = max(w, a.wpart[((int64_t)p * a.chunks + c) * a.d + k]);
+    const int lx = exponent_above(x), lw = exponent_above(w);
+    if (p == 0) ex[k] = kTop - lx;
+    en[(int64_t)p * a.d + k] = kTop - lw;
+    el[(int64_t)p * a.d + k] = lx;  // completed below
+    top = max(top, lx + lw);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = top;
+  __syncthreads();
+  top = max(max(red[0], red[1]), max(red[2], red[3]));
+  for (int k = tid; k < a.d; k += NT) el[(int64_t)p * a.d + k] += kTop - top;
+  if (tid == 0) scale[p] = top - 2 * kTop;
+}
+
+// Each row's id (-1: takes no part) and, for the backward, its log-sum; padded rows take no part.
+__global__ __launch_bounds__(NT) void xent_keys_kernel(Rows rows, int nrows, int padded, const float* __restrict__ lse,
+                                                       int* __restrict__ key, float* __restrict__ z) {
+  const int r = blockIdx.x * NT + threadIdx.x;
+  if (r >= padded) return;
+  key[r] = r < nrows ? rows.key(r) : -1;
+  if (z) z[r] = r < nrows ? lse[r] : 0.f;
+}
+
+struct TileArgs {
+  Operand A, B;
+  int nk, gx, gy;
+  int cols, v0;         // columns of the piece, its first id
+  const float* bias;    // the piece's, or null
+  const int* scale;
+  const int* key;
+  int64_t padded;       // rows
+  int64_t pcols;        // padded columns of the piece
+  float2* part;         // forward: [64-column block][padded rows] maximum, sum of exp
+  float* target;
+  const float* lse;     // backward
+  char* prow;           // P packed for dX (rows, k = columns)
+  char* pcol;           // and for dW (columns, k = rows)
+  float* cfac;          // [64-row block][pcols] what a column's sum over the block is scaled back by
+  float* csum;          // [64-row block][pcols] column sums of P
+};
+
+// The sum or maximum over the 16 lanes of a row.
+template <int CTRL>
+__device__ __forceinline__ float rotated(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float row_max(float x) {
+  x = fmaxf(x, rotated<0x128>(x));
+  x = fmaxf(x, rotated<0x124>(x));
+  x = fmaxf(x, rotated<0x122>(x));
+  return fmaxf(x, rotated<0x121>(x));
+}
+__device__ __forceinline__ float row_add(float x) {
+  x += rotated<0x128>(x);
+  x += rotated<0x124>(x);
+  x += rotated<0x122>(x);
+  return x + rotated<0x121>(x);
+}
+
+// A tile of logits, and from them the rows' statistics or P.
+template <bool GRAD>
+__global__ __launch_bounds__(S::NTH, 2) void xent_tile_kernel(TileArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+  const planes::Lane<S> w;
+  int tm, tn, z;
+  gemm::item_tile(blockIdx.x, a.gx * a.gy, a.gx, a.gy, tm, tn, z);
+  f32x4 l[4][4], lo[4][4];
+  planes::multiply<S>(a.A, a.B, tm, tn, 0, a.nk, lds, w, l, lo);
+
+  const int64_t row0 = (int64_t)tm * kTile + 64 * w.wm + 16 * w.q;  // this lane's rows row0 + 4 r + i
+  const int c0 = tn * kTile + w.col();                              // and columns c0 + n
+  const int sc = a.scale[0];
+  float bias[4];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) bias[n] = a.bias && c0 + n < a.cols ? a.bias[c0 + n] : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        l[i][n][r] = __builtin_ldexpf(fmaf(lo[i][n][r], 1.f / (1 << kLo), l[i][n][r]), sc) + bias[n];
+  int key[4][4];  // [r][i]: this lane's column of the row's id, if 0 .. 3
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int4 k = *reinterpret_cast<const int4*>(a.key + row0 + 4 * r);
+    key[r][0] = k.x;
+    key[r][1] = k.y;
+    key[r][2] = k.z;
+    key[r][3] = k.w;
+  }
+  const int v = a.v0 + c0;
+
+  if (!GRAD) {
+    float m_mine = 0.f, s_mine = 0.f;  // of row row0 + lr
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = key[r][i] - v;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if (c == n && key[r][i] >= 0) a.target[row0 + 4 * r + i] = l[i][n][r];
+        float x[4], m = -FLT_MAX, s = 0.f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          x[n] = c0 + n < a.cols ? l[i][n][r] : -INFINITY;
+          m = fmaxf(m, x[n]);
+        }
+        m = row_max(m);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s += __builtin_amdgcn_exp2f((x[n] - m) * kLog2e);
+        s = row_add(s);
+        if (w.lr == 4 * r + i) {
+          m_mine = m;
+          s_mine = s;
+        }
+      }
+    a.part[(int64_t)(tn * 2 + w.wn) * a.padded + row0 + w.lr] = make_float2(m_mine, s_mine);
+    return;
+  }
+
+  float cmax[4] = {0.f, 0.f, 0.f, 0.f}, csum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const f32x4 z4 = *reinterpret_cast<const f32x4*>(a.lse + row0 + 4 * r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = key[r][i] - v;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        float p = __builtin_amdgcn_exp2f((l[i][n][r] - z4[i]) * kLog2e);
+        if (c == n) p -= 1.f;
+        p = key[r][i] >= 0 && c0 + n < a.cols ? p : 0.f;
+        l[i][n][r] = p;
+        cmax[n] = fmaxf(cmax[n], fabsf(p));
+        csum[n] += p;
+      }
+    }
+  }
+  int ec[4];  // exponents of the columns over these 64 rows
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    cmax[n] = fmaxf(cmax[n], __shfl_xor(cmax[n], 16, 64));
+    cmax[n] = fmaxf(cmax[n], __shfl_xor(cmax[n], 32, 64));
+    csum[n] += __shfl_xor(csum[n], 16, 64);
+    csum[n] += __shfl_xor(csum[n], 32, 64);
+    ec[n] = min(kTop - exponent_above(__builtin_bit_cast(unsigned, cmax[n])), 126);
+  }
+  if (w.q == 0) {
+    const int64_t at = ((int64_t)tm * 2 + w.wm) * a.pcols + c0;
+    f32x4 f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) f[n] = __builtin_bit_cast(float, (unsigned)(127 - ec[n]) << 23);
+    *reinterpret_cast<f32x4*>(a.cfac + at) = f;
+    *reinterpret_cast<f32x4*>(a.csum + at) = f32x4{csum[0], csum[1], csum[2], csum[3]};
+  }
+  // by column: this lane has 16 consecutive rows of each of its columns
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x[8];
+      int e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = l[j & 3][n][2 * h + (j >> 2)];
+        e[j] = ec[n];
+      }
+      planes::put16<0>(a.pcol + planes::chunk_at<2>(a.pcols / 16, c0 + n, row0 + 8 * h), x, e);
+    }
+  // by row: lanes 2 j and 2 j + 1 have 8 consecutive columns together; the even one
+  // takes rows i = 0, 1, the odd one 2, 3
+  const bool odd = w.lr & 1;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float x[8];
+      int e[8];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float own = odd ? l[2 + j][n][r] : l[j][n][r], give = odd ? l[j][n][r] : l[2 + j][n][r];
+        const float got = rotated<0xB1>(give);  // the other lane of the pair
+        x[n] = odd ? got : own;
+        x[4 + n] = odd ? own : got;
+        e[n] = e[4 + n] = kTop;
+      }
+      const int64_t row = row0 + 4 * r + (odd ? 2 + j : j);
+      planes::put16<kLo>(a.prow + planes::chunk_at<2>(a.padded / 16, row, c0 & ~7), x, e);
+    }
+}
+
+// A piece's statistics join the rows'.
+__global__ __launch_bounds__(NT) void xent_join_kernel(const float2* __restrict__ part, int blocks, int64_t padded, int nrows,
+                                                       const float* __restrict__ target, RowState* __restrict__ state,
+                                                       int first) {
+  const int r = blockIdx.x * NT + threadIdx.x;
+  if (r >= nrows) return;
+  RowState t{-FLT_MAX, 0.f, 0.f, 0.f};
+  if (!first) t = state[r];
+  for (int b0 = 0; b0 < blocks; b0 += 8) {
+    float2 x[8];
+    float m = t.max;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = b0 + j < blocks ? part[(int64_t)(b0 + j) * padded + r] : make_float2(-FLT_MAX, 0.f);
+      m = fmaxf(m, x[j].x);
+    }
+    t.sum *= expf(t.max - m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t.sum += x[j].y * expf(x[j].x - m);
+    t.max = m;
+  }
+  t.target = target[r];
+  state[r] = t;
+}
+
+// What finishes a product: C (+)= 2^(exponent of its row or column) g sum.
+struct OutArgs {
+  float* C;
+  int64_t ldc;
+  int rows, cols, accumulate;
+  const int* ex;
+  int ex_by_row, add;  // the exponent is add - ex[row or column]
+  float scale;
+  const float* upstream;
+  __device__ __forceinline__ float g() const { return upstream ? upstream[0] * scale : scale; }
+  __device__ __forceinline__ void put(int64_t row, int col, float sum, float gg) const {
+    float* p = C + row * ldc + col;
+    const float v = __builtin_ldexpf(sum, add - ex[ex_by_row ? row : col]) * gg;
+    *p = accumulate ? *p + v : v;
+  }
+};
+
+struct ProductArgs {
+  Operand A, B;
+  int nk, gx, gy, splits, per;  // stages; per split
+  const float* cfac;            // dW: [64-row block][pcols]
+  int64_t pcols;
+  OutArgs out;
+  float* part;                  // [split][padded rows][padded cols] where splits > 1
+};
+
+// COLS false: dX = P W^T.  true: dW = X^T P, whose sums over each 64 rows (two
+// stages) are scaled back column by column.
+template <bool COLS>
+__global__ __launch_bounds__(S::NTH, 2) void xent_product_kernel(ProductArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+  const planes::Lane<S> w;
+  int tm, tn, z;
+  gemm::item_tile(blockIdx.x, a.gx * a.gy * a.splits, a.gx, a.gy, tm, tn, z);
+  const int k0 = z * a.per, k1 = min(a.nk, k0 + a.per);
+  f32x4 sum[4][4], acc[4][4];
+  if (COLS) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) sum[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* fac = a.cfac + (int64_t)tn * kTile + w.col();
+    planes::multiply_runs<S>(a.A, a.B, tm, tn, k0, k1, 2, lds, w, acc, [&](int k) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(fac + (int64_t)(k >> 1) * a.pcols);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) sum[i][n] += f[n] * acc[i][n];
+    });
+  } else {
+    planes::multiply<S>(a.A, a.B, tm, tn, k0, k1, lds, w, sum, acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) sum[i][n] += acc[i][n] * (1.f / (1 << kLo));
+  }
+  const int64_t row0 = (int64_t)tm * kTile + 64 * w.wm + 16 * w.q;
+  const int c0 = tn * kTile + w.col();
+  if (a.splits > 1) {
+    const int64_t ld = (int64_t)a.gx * kTile;
+    float* p = a.part + (int64_t)z * a.gy * kTile * ld + row0 * ld + c0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(p + (4 * r + i) * ld) = f32x4{sum[i][0][r], sum[i][1][r], sum[i][2][r], sum[i][3][r]};
+    return;
+  }
+  const float g = a.out.g();
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (row0 + 4 * r + i < a.out.rows && c0 + n < a.out.cols) a.out.put(row0 + 4 * r + i, c0 + n, sum[i][n][r], g);
+}
+
+// The splits' sums in order.
+__global__ __launch_bounds__(NT) void xent_reduce_kernel(ProductArgs a) {
+  const int64_t ld = (int64_t)a.gx * kTile, total = (int64_t)a.out.rows * (ld / 4), step = (int64_t)a.gy * kTile * ld;
+  const float g = a.out.g();
+  for (int64_t u = (int64_t)blockIdx.x * NT + threadIdx.x; u < total; u += (int64_t)gridDim.x * NT) {
+    const int64_t row = u / (ld / 4);
+    const int col = (int)(u - row * (ld / 4)) * 4;
+    if (col >= a.out.cols) continue;
+    const float* p = a.part + row * ld + col;
+    f32x4 s = *reinterpret_cast<const f32x4*>(p);
+    for (int z = 1; z < a.splits; ++z) s += *reinterpret_cast<const f32x4*>(p + z * step);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (col + n < a.out.cols) a.out.put(row, col + n, s[n], g);
+  }
+}
+
+// db of a piece (+)= g times the 64-row blocks' column sums, in order.
+__global__ __launch_bounds__(NT) void xent_db_kernel(const float* __restrict__ csum, int blocks, int64_t pcols, int cols,
+                                                     float* __restrict__ db, int accumulate, float scale,
+                                                     const float* __restrict__ upstream) {
+  const int c = blockIdx.x * NT + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int b = 0; b < blocks; ++b) s += csum[(int64_t)b * pcols + c];
+  s *= upstream ? upstream[0] * scale : scale;
+  db[c] = accumulate ? db[c] + s : s;
+}
+
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// Columns of a piece, and the workspace's parts.
-struct Plan {
+// ----------------------------------------------------------------------- plans
+// Few rows: columns of a piece, and the workspace's parts.
+struct SmallPlan {
   int piece;
   size_t logits, rows, state, gemm;  // bytes
   size_t total() const { return logits + rows + state + gemm; }
 };
 constexpr size_t kPieceBytes = (size_t)128 << 20;
-Plan plan_of(int rows, int d, int vocab) {
-  Plan p;
+SmallPlan small_plan(int rows, int d, int vocab) {
+  SmallPlan p;
   const size_t cols = kPieceBytes / sizeof(float) / (size_t)rows / 256 * 256;
   p.piece = (int)std::min<size_t>((size_t)vocab, std::max<size_t>(cols, 256));
   p.logits = round256((size_t)rows * p.piece * sizeof(float));
@@ -120,6 +543,85 @@ Plan plan_of(int rows, int d, int vocab) {
     p.gemm = std::max(p.gemm, std::max(mle_gemm_ws_bytes(rows, v, d, 1),
                                        std::max(mle_gemm_ws_bytes(rows, d, v, 1), mle_gemm_ws_bytes(d, v, rows, 1))));
   p.gemm = round256(p.gemm);
+  return p;
+}
+
+// Where the products of fp16 planes run.
+constexpr int kPlaneRows = 256;
+bool use_planes(int rows, int d, int vocab) { return rows >= kPlaneRows && vocab <= (1 << 30); }
+
+// Splits of a product's K: enough workgroups for two to a CU, and at least 16 stages each.
+int splits_of(int64_t tiles, int stages) {
+  const int64_t want = 2 * gemm::kChipCus / std::max<int64_t>(tiles, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, stages / 16));
+}
+// Stages of a split, even (the column factors cover two).
+int per_split(int stages, int splits) { return ((stages + splits - 1) / splits + 1) / 2 * 2; }
+
+// The planes' plan: rows are taken kRowsAtOnce at a time (rows of a chunk, padded to
+// whole tiles), the vocabulary in pieces that keep both packed P below
+// kPlaneBytes.
+constexpr int kRowsAtOnce = 32768;
+constexpr size_t kPlaneBytes = (size_t)192 << 20;
+struct PlanePlan {
+  int rows, d, vocab;
+  int padded, dk, dp, piece, pieces, chunks, slabs, slab_rows;
+  // offsets into the workspace
+  size_t xpart, wpart, ex, el, en, scale, key, z, state, target, part, xl, xt, wl, wn, prow, pcol, cfac, csum, split, total;
+};
+PlanePlan plane_plan(int all_rows, int d, int vocab) {
+  PlanePlan p;
+  p.rows = std::min(all_rows, kRowsAtOnce);
+  p.d = d;
+  p.vocab = vocab;
+  p.padded = (p.rows + kTile - 1) / kTile * kTile;
+  p.dk = (d + 31) / 32;
+  p.dp = (d + kTile - 1) / kTile * kTile;
+  const int64_t most = std::max<int64_t>(kTile, (int64_t)(kPlaneBytes / 8 / p.padded) / kTile * kTile);
+  p.pieces = (int)((vocab + most - 1) / most);
+  p.piece = ((vocab + p.pieces - 1) / p.pieces + kTile - 1) / kTile * kTile;
+  p.pieces = (vocab + p.piece - 1) / p.piece;
+  p.chunks = (p.piece + 4095) / 4096;
+  p.slabs = std::min(64, (p.rows + 31) / 32);
+  p.slab_rows = (p.rows + p.slabs - 1) / p.slabs;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += round256(bytes);
+    return o;
+  };
+  const size_t padded = p.padded, piece = p.piece;
+  p.xpart = take((size_t)p.slabs * d * 4);
+  p.wpart = take((size_t)p.pieces * p.chunks * d * 4);
+  p.ex = take((size_t)d * 4);
+  p.el = take((size_t)p.pieces * d * 4);
+  p.en = take((size_t)p.pieces * d * 4);
+  p.scale = take((size_t)p.pieces * 4);
+  p.key = take(padded * 4);
+  p.z = take(padded * 4);
+  p.state = take(padded * sizeof(RowState));
+  p.target = take(padded * 4);
+  p.xl = take(padded * p.dk * 32 * 4);
+  p.wl = take(piece * p.dk * 32 * 4);
+  // the forward's statistics lie where the backward's planes do
+  p.part = p.xt = take(std::max(padded * p.dp * 4, padded * (piece / 64) * sizeof(float2)));
+  p.wn = take(piece * p.dp * 4);
+  p.prow = take(padded * piece * 4);
+  p.pcol = take(padded * piece * 4);
+  p.cfac = take(padded / 64 * piece * 4);
+  p.csum = take(padded / 64 * piece * 4);
+  size_t split = 0;
+  const int last = (vocab - (p.pieces - 1) * p.piece + kTile - 1) / kTile * kTile;
+  for (int cols : {p.piece, last}) {
+    const int sx = splits_of((int64_t)(p.padded / kTile) * (p.dp / kTile), cols / 32);
+    const int sw = splits_of((int64_t)(p.dp / kTile) * (cols / kTile), p.padded / 32);
+    if (sx > 1) split = std::max(split, (size_t)sx * padded * p.dp * 4);
+    if (sw > 1) split = std::max(split, (size_t)sw * p.dp * cols * 4);
+  }
+  // (a last chunk of fewer rows may have more splits, of at most two tiles to a CU in all)
+  if (all_rows > kRowsAtOnce) split = std::max(split, (size_t)2 * gemm::kChipCus * kTile * kTile * 4);
+  p.split = take(split);
+  p.total = at;
   return p;
 }
 
@@ -138,18 +640,175 @@ int check_ws(const char* who, size_t need, const void* ws, size_t ws_bytes) {
   return MLE_OK;
 }
 
+size_t ws_need(int rows, int d, int vocab) {
+  return use_planes(rows, d, vocab) ? plane_plan(rows, d, vocab).total : small_plan(rows, d, vocab).total();
+}
+
 #define TRY(call)                  \
   do {                             \
     const int rc_ = (call);        \
     if (rc_ != MLE_OK) return rc_; \
   } while (0)
 
+// The part of a call that the planes' forward and backward share: exponents, ids and
+// X for the logits, over one chunk of rows.
+struct Chunk {
+  PlanePlan p;
+  char* ws;
+  hipStream_t s;
+  const float* X;
+  int64_t ldx;
+  const float* W;
+  int64_t ldw;
+  const float* bias;
+  int rows, padded;
+  template <class T = char>
+  T* at(size_t o) const {
+    return reinterpret_cast<T*>(ws + o);
+  }
+
+  void begin(const Rows& rw, const float* lse) const {
+    const unsigned xtiles = (unsigned)((p.d + NT - 1) / NT);
+    const AmaxArgs a{X,       ldx,     W,           ldw,           rows,
+                     p.d,     p.vocab, p.piece,     p.chunks,      p.slabs,
+                     p.slab_rows, (int)(xtiles * p.slabs), at<unsigned>(p.xpart), at<unsigned>(p.wpart)};
+    const int64_t wblocks = (int64_t)p.pieces * p.chunks * p.d;
+    mle::launch(xent_amax_kernel, (unsigned)(xtiles * p.slabs + wblocks), NT, 0, s, a);
+    mle::launch(xent_scales_kernel, (unsigned)p.pieces, NT, 0, s, a, at<int>(p.ex), at<int>(p.el), at<int>(p.en), at<int>(p.scale));
+    mle::launch(xent_keys_kernel, (unsigned)((padded + NT - 1) / NT), NT, 0, s, rw, rows, padded, lse, at<int>(p.key),
+                lse ? at<float>(p.z) : nullptr);
+    planes::PackArgs pa{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, at(p.xl), 0};
+    pa.vec = aligned16(X) && ldx % 4 == 0;
+    mle::launch(planes::pack_rows_kernel<true, kLo>, (unsigned)((pa.blocks * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
+  }
+  int cols(int i) const { return std::min(p.piece, p.vocab - i * p.piece); }
+  int pcols(int i) const { return (cols(i) + kTile - 1) / kTile * kTile; }
+  // Piece i of W as the logits' second operand.
+  void pack_piece(int i) const {
+    planes::PackArgs pa{W + (int64_t)i * p.piece, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d,
+                        nullptr, at(p.wl), 0};
+    pa.vec = aligned16(W) && ldw % 4 == 0;  // (pieces begin at multiples of 128)
+    mle::launch(planes::pack_cols_kernel<true, kLo>, (unsigned)((pa.blocks / 4 * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
+  }
+  TileArgs tile(int i) const {
+    TileArgs a{};
+    a.A = Operand{at(p.xl), (int64_t)padded / 16 * 2 * planes::kUnit};
+    a.B = Operand{at(p.wl), (int64_t)pcols(i) / 16 * 2 * planes::kUnit};
+    a.nk = p.dk;
+    a.gx = pcols(i) / kTile;
+    a.gy = padded / kTile;
+    a.cols = cols(i);
+    a.v0 = i * p.piece;
+    a.bias = bias ? bias + (int64_t)i * p.piece : nullptr;
+    a.scale = at<int>(p.scale) + i;
+    a.key = at<int>(p.key);
+    a.padded = padded;
+    a.pcols = pcols(i);
+    return a;
+  }
+  template <bool COLS>
+  void product(const char* A, int m, const char* B, int n, int stages, const OutArgs& out) const {
+    ProductArgs a{};
+    a.A = Operand{A, (int64_t)m / 16 * 2 * planes::kUnit};
+    a.B = Operand{B, (int64_t)n / 16 * 2 * planes::kUnit};
+    a.nk = stages;
+    a.gx = n / kTile;
+    a.gy = m / kTile;
+    a.per = per_split(stages, splits_of((int64_t)a.gx * a.gy, stages));
+    a.splits = (stages + a.per - 1) / a.per;
+    a.cfac = at<float>(p.cfac);
+    a.pcols = n;
+    a.out = out;
+    a.part = at<float>(p.split);
+    mle::launch(xent_product_kernel<COLS>, (unsigned)((int64_t)a.gx * a.gy * a.splits), S::NTH, 0, s, a);
+    if (a.splits > 1)
+      mle::launch(xent_reduce_kernel, stream_grid((size_t)out.rows * n / 4, NT, 8192), NT, 0, s, a);
+  }
+};
+
+// Rows [r0, ..) of a call.
+Chunk chunk_of(const PlanePlan& p, void* ws, hipStream_t s, int r0, int all_rows, const float* X, int64_t ldx,
+               const float* W, int64_t ldw, const float* bias) {
+  const int rows = std::min(p.rows, all_rows - r0);
+  return Chunk{p, static_cast<char*>(ws), s, X + (int64_t)r0 * ldx, ldx, W, ldw, bias, rows, (rows + kTile - 1) / kTile * kTile};
+}
+
+int planes_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W, int64_t ldw,
+               const float* bias, Rows rw, float loss_scale, float* lse, float* row_loss, float* loss, void* ws) {
+  const PlanePlan p = plane_plan(rows, d, vocab);
+  hipStream_t s = as_stream(stream);
+  for (int r0 = 0; r0 < rows; r0 += p.rows) {
+    const Chunk c = chunk_of(p, ws, s, r0, rows, X, ldx, W, ldw, bias);
+    rw.r0 = r0;
+    c.begin(rw, nullptr);
+    for (int i = 0; i < p.pieces; ++i) {
+      c.pack_piece(i);
+      TileArgs a = c.tile(i);
+      a.part = c.at<float2>(p.part);
+      a.target = c.at<float>(p.target);
+      mle::launch(xent_tile_kernel<false>, (unsigned)(a.gx * a.gy), S::NTH, 0, s, a);
+      mle::launch(xent_join_kernel, (unsigned)((c.rows + NT - 1) / NT), NT, 0, s, a.part, 2 * a.gx, a.padded, c.rows, a.target,
+                  c.at<RowState>(p.state), i == 0 ? 1 : 0);
+    }
+    mle::launch(xent_finish_kernel, 1u, 1024, 0, s, c.at<RowState>(p.state), c.rows, rw, loss_scale, lse + r0,
+                row_loss ? row_loss + r0 : nullptr, loss, r0 > 0 ? 1 : 0);
+  }
+  return check_launch("mle_vocab_xent_fwd");
+}
+
+int planes_bwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W, int64_t ldw,
+               const float* bias, Rows rw, const float* lse, const float* upstream, float grad_scale, float* dX,
+               int64_t lddx, int accumulate_dx, float* dW, int64_t lddw, float* db, int accumulate_dw, void* ws) {
+  const PlanePlan p = plane_plan(rows, d, vocab);
+  hipStream_t s = as_stream(stream);
+  for (int r0 = 0; r0 < rows; r0 += p.rows) {
+    const Chunk c = chunk_of(p, ws, s, r0, rows, X, ldx, W, ldw, bias);
+    rw.r0 = r0;
+    c.begin(rw, lse + r0);
+    if (dW) {
+      planes::PackArgs pa{X + (int64_t)r0 * ldx, ldx, d, c.rows, p.dp / 16, c.padded / 32, c.at<int>(p.ex), c.at<int>(p.key),
+                          c.at(p.xt), 0};
+      pa.vec = aligned16(X) && ldx % 4 == 0;
+      mle::launch(planes::pack_cols_kernel<false, 0>, (unsigned)((pa.blocks / 4 * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
+    }
+    for (int i = 0; i < p.pieces; ++i) {
+      const int64_t v0 = (int64_t)i * p.piece;
+      c.pack_piece(i);
+      TileArgs a = c.tile(i);
+      a.lse = c.at<float>(p.z);
+      a.prow = c.at(p.prow);
+      a.pcol = c.at(p.pcol);
+      a.cfac = c.at<float>(p.cfac);
+      a.csum = c.at<float>(p.csum);
+      mle::launch(xent_tile_kernel<true>, (unsigned)(a.gx * a.gy), S::NTH, 0, s, a);
+      if (dX) {
+        planes::PackArgs pa{W + v0, ldw, d, c.cols(i), p.dp / 16, c.pcols(i) / 32, c.at<int>(p.en) + (int64_t)i * d, nullptr,
+                            c.at(p.wn), 0};
+        pa.vec = aligned16(W) && ldw % 4 == 0;
+        mle::launch(planes::pack_rows_kernel<false, kLo>, (unsigned)((pa.blocks * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
+        const OutArgs out{dX + (int64_t)r0 * lddx, lddx, c.rows, d, accumulate_dx || i > 0, c.at<int>(p.en) + (int64_t)i * d, 0,
+                          -kTop, grad_scale, upstream};
+        c.product<false>(c.at(p.prow), c.padded, c.at(p.wn), p.dp, c.pcols(i) / 32, out);
+      }
+      const int add = accumulate_dw || r0 > 0;
+      if (dW) {
+        const OutArgs out{dW + v0, lddw, d, c.cols(i), add, c.at<int>(p.ex), 1, 0, grad_scale, upstream};
+        c.product<true>(c.at(p.xt), p.dp, c.at(p.pcol), c.pcols(i), c.padded / 32, out);
+      }
+      if (db)
+        mle::launch(xent_db_kernel, (unsigned)((c.cols(i) + NT - 1) / NT), NT, 0, s, c.at<float>(p.csum), c.padded / 64,
+                    (int64_t)c.pcols(i), c.cols(i), db + v0, add, grad_scale, upstream);
+    }
+  }
+  return check_launch("mle_vocab_xent_bwd");
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t mle_vocab_xent_ws_bytes(int rows, int d, int vocab) {
-  return rows <= 0 || d <= 0 || vocab <= 0 ? 0 : plan_of(rows, d, vocab).total();
+  return rows <= 0 || d <= 0 || vocab <= 0 ? 0 : ws_need(rows, d, vocab);
 }
 
 int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W,
@@ -158,10 +817,13 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
   TRY(check("mle_vocab_xent_fwd", rows, d, vocab, X, ldx, W, ldw, keys, clen, max_clen));
   MLE_CHECK_ARG(loss && (lse || rows == 0), "mle_vocab_xent_fwd: null pointer");
   if (rows == 0) return mle_fill(stream, loss, 0.f, 1);
-  const Plan p = plan_of(rows, d, vocab);
-  TRY(check_ws("mle_vocab_xent_fwd", p.total(), ws, ws_bytes));
+  TRY(check_ws("mle_vocab_xent_fwd", ws_need(rows, d, vocab), ws, ws_bytes));
+  if (use_planes(rows, d, vocab))
+    return planes_fwd(stream, rows, d, vocab, X, ldx, W, ldw, bias, Rows{keys, clen, max_clen, vocab, 0}, loss_scale, lse,
+                      row_loss, loss, ws);
+  const SmallPlan p = small_plan(rows, d, vocab);
   hipStream_t s = as_stream(stream);
-  const Rows rw{keys, clen, max_clen, vocab};
+  const Rows rw{keys, clen, max_clen, vocab, 0};
   float* l = static_cast<float*>(ws);
   RowState* state = reinterpret_cast<RowState*>(static_cast<char*>(ws) + p.logits + p.rows);
   void* gws = reinterpret_cast<char*>(state) + p.state;
@@ -171,7 +833,7 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
                     bias ? bias + v0 : nullptr, gws, p.gemm));
     mle::launch(xent_stats_kernel, (unsigned)rows, NT, 0, s, l, n, v0, rw, state, v0 == 0 ? 1 : 0);
   }
-  mle::launch(xent_finish_kernel, 1u, 1024, 0, s, state, rows, rw, loss_scale, lse, row_loss, loss);
+  mle::launch(xent_finish_kernel, 1u, 1024, 0, s, state, rows, rw, loss_scale, lse, row_loss, loss, 0);
   return check_launch("mle_vocab_xent_fwd");
 }
 
@@ -184,8 +846,11 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
                 "mle_vocab_xent_bwd: null pointer, or lddx %lld < %d or lddw %lld < %d", (long long)lddx, d,
                 (long long)lddw, vocab);
   MLE_CHECK_ARG(dW || !db, "mle_vocab_xent_bwd: db without dW");
-  const Plan p = rows > 0 ? plan_of(rows, d, vocab) : Plan{};
-  if (rows > 0) TRY(check_ws("mle_vocab_xent_bwd", p.total(), ws, ws_bytes));
+  if (rows > 0) TRY(check_ws("mle_vocab_xent_bwd", ws_need(rows, d, vocab), ws, ws_bytes));
+  if (rows > 0 && use_planes(rows, d, vocab))
+    return !dX && !dW ? MLE_OK
+                      : planes_bwd(stream, rows, d, vocab, X, ldx, W, ldw, bias, Rows{keys, clen, max_clen, vocab, 0}, lse,
+                                   upstream, grad_scale, dX, lddx, accumulate_dx, dW, lddw, db, accumulate_dw, ws);
   if (db && !accumulate_dw) TRY(mle_fill(stream, db, 0.f, (size_t)vocab));
   if (rows == 0) {
     if (dW && !accumulate_dw)
@@ -194,8 +859,9 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
     return MLE_OK;
   }
   if (!dX && !dW) return MLE_OK;
+  const SmallPlan p = small_plan(rows, d, vocab);
   hipStream_t s = as_stream(stream);
-  const Rows rw{keys, clen, max_clen, vocab};
+  const Rows rw{keys, clen, max_clen, vocab, 0};
   float* l = static_cast<float*>(ws);
   float* xs = reinterpret_cast<float*>(static_cast<char*>(ws) + p.logits);
   void* gws = static_cast<char*>(ws) + p.logits + p.rows + p.state;
