@@ -174,25 +174,28 @@ __device__ __forceinline__ void multiply_runs(const Operand& A, const Operand& B
 }
 
 // ------------------------------------------------------------- fp16 operands
-// x 2^e in two fp16 planes, h + 2^-LO l: with |x 2^e| < 2^15 the pair holds 22 bits
-// of every value down to 2^(LO - 14) and 2^-(24 + LO) of the smaller ones.  What is
-// not finite stays in the first plane.
+// A scaled value v in two fp16 planes, h + 2^-LO l: with |v| < 2^15 the pair holds 22
+// bits of every value down to 2^-(LO + 3) and 2^-(24 + LO) of the smaller ones.
 template <int LO>
-__device__ __forceinline__ void split16(float x, int e, _Float16& h, _Float16& l) {
-  const float v = __builtin_ldexpf(x, e);
-  h = (_Float16)v;
-  const float rest = v - (float)h;
-  l = __builtin_isfinite(v) ? (_Float16)__builtin_ldexpf(rest, LO) : (_Float16)0.f;
+__device__ __forceinline__ void put16(char* p, const float (&v)[8]) {
+  f16x8 h, l;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    h[j] = (_Float16)v[j];
+    l[j] = (_Float16)((v[j] - (float)h[j]) * (float)(1 << LO));
+  }
+  *reinterpret_cast<f16x8*>(p) = h;
+  *reinterpret_cast<f16x8*>(p + kUnit) = l;
 }
+// The same of x 2^e; what is not finite stays in the first plane.
 template <int LO>
 __device__ __forceinline__ void put16(char* p, const float (&x)[8], const int (&e)[8]) {
   f16x8 h, l;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    _Float16 a, b;
-    split16<LO>(x[j], e[j], a, b);
-    h[j] = a;
-    l[j] = b;
+    const float v = __builtin_ldexpf(x[j], e[j]);
+    h[j] = (_Float16)v;
+    l[j] = __builtin_isfinite(v) ? (_Float16)((v - (float)h[j]) * (float)(1 << LO)) : (_Float16)0.f;
   }
   *reinterpret_cast<f16x8*>(p) = h;
   *reinterpret_cast<f16x8*>(p + kUnit) = l;
@@ -207,13 +210,16 @@ struct PackArgs {
   const int* keys;      // nullable, by k: < 0 leaves that k out (zeros, whatever it holds)
   char* out;
   int vec;              // 16-byte loads
+  // Blocks of 256 threads that pack it.
+  __host__ __device__ int64_t rows_blocks() const { return ((int64_t)blocks * kblocks + 3) / 4; }
+  __host__ __device__ int64_t cols_blocks() const { return ((int64_t)(blocks / 4) * kblocks + 3) / 4; }
 };
 
 // Operands whose k runs along the source's rows (element (row, k) at row * ld + k): a
-// wave per unit, 128 contiguous bytes of 16 rows.
+// wave per unit, 128 contiguous bytes of 16 rows; 256 threads to a block.
 template <bool EX_BY_K, int LO>
-__global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
-  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+__device__ __forceinline__ void pack_rows(const PackArgs& a, int64_t block) {
+  const int64_t u = block * 4 + (threadIdx.x >> 6);
   if (u >= (int64_t)a.blocks * a.kblocks) return;
   const int lane = threadIdx.x & 63;
   const int kb = (int)(u / a.blocks), blk = (int)(u - (int64_t)kb * a.blocks);
@@ -242,9 +248,9 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(PackArgs a) {
 // wave per 64-row group and k block, 256 contiguous bytes of 32 source rows; the
 // 4 x 8 values of a lane are transposed in its registers.
 template <bool EX_BY_K, int LO>
-__global__ __launch_bounds__(256) void pack_cols_kernel(PackArgs a) {
+__device__ __forceinline__ void pack_cols(const PackArgs& a, int64_t block) {
   const int groups = a.blocks >> 2;
-  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t u = block * 4 + (threadIdx.x >> 6);
   if (u >= (int64_t)groups * a.kblocks) return;
   const int lane = threadIdx.x & 63;
   const int kb = (int)(u / groups), g = (int)(u - (int64_t)kb * groups);

@@ -148,16 +148,29 @@ struct AmaxArgs {
   int slabs, slab_rows, xblocks;      // X: blocks of 256 columns x slabs
   unsigned* xpart;                    // [slabs][d]
   unsigned* wpart;                    // [pieces][chunks][d]
+  int padded, kblocks;                // rows: blocks of 256
+  const float* lse;                   // backward
+  int* key;
+  float* z;
 };
 
 // The largest finite magnitude of each feature: of X over slabs of rows, of W over
-// chunks of a piece's columns.
-__global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a) {
+// chunks of a piece's columns.  And each row's id (-1: takes no part) with, for the
+// backward, its log-sum; padded rows take no part.
+__global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a, Rows rows) {
   __shared__ unsigned red[NT / 64];
   const int tid = threadIdx.x;
-  if ((int)blockIdx.x < a.xblocks) {
+  if ((int)blockIdx.x < a.kblocks) {
+    const int r = blockIdx.x * NT + tid;
+    if (r >= a.padded) return;
+    a.key[r] = r < a.rows ? rows.key(r) : -1;
+    if (a.lse) a.z[r] = r < a.rows ? a.lse[r] : 0.f;
+    return;
+  }
+  const int bx = blockIdx.x - a.kblocks;
+  if (bx < a.xblocks) {
     const int tiles = (a.d + NT - 1) / NT;
-    const int slab = blockIdx.x / tiles, k = (blockIdx.x % tiles) * NT + tid;
+    const int slab = bx / tiles, k = (bx % tiles) * NT + tid;
     if (k >= a.d) return;
     const int r1 = min(a.rows, (slab + 1) * a.slab_rows);
     unsigned m = 0;
@@ -166,8 +179,8 @@ __global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a) {
     a.xpart[(int64_t)slab * a.d + k] = m;
     return;
   }
-  const int64_t b = blockIdx.x - a.xblocks;
-  const int k = (int)(b % a.d), c = (int)(b / a.d);
+  const int b = bx - a.xblocks;
+  const int k = b % a.d, c = b / a.d;
   const int v0 = c / a.chunks * a.piece + c % a.chunks * 4096;
   const int v1 = min(min(v0 + 4096, (c / a.chunks + 1) * a.piece), a.vocab);
   unsigned m = 0;
@@ -183,12 +196,12 @@ __global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a) {
 
 // Exponents: ex[k] of X; for piece p, el[p][k] of W in the logits, en[p][k] of W in dX,
 // scale[p]: a logit is its sum times 2^scale.  A workgroup per piece.
-__global__ __launch_bounds__(NT) void xent_scales_kernel(AmaxArgs a, int* __restrict__ ex, int* __restrict__ el,
+__global__ __launch_bounds__(1024) void xent_scales_kernel(AmaxArgs a, int* __restrict__ ex, int* __restrict__ el,
                                                          int* __restrict__ en, int* __restrict__ scale) {
-  __shared__ int red[NT / 64];
+  __shared__ int red[1024 / 64];
   const int p = blockIdx.x, tid = threadIdx.x;
   int top = 2 * kNone;
-  for (int k = tid; k < a.d; k += NT) {
+  for (int k = tid; k < a.d; k += 1024) {
     unsigned x = 0, w = 0;
 #pragma unroll 8
     for (int s = 0; s < a.slabs; ++s) x = max(x, a.xpart[(int64_t)s * a.d + k]);
@@ -203,18 +216,23 @@ __global__ __launch_bounds__(NT) void xent_scales_kernel(AmaxArgs a, int* __rest
   for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
   if ((tid & 63) == 0) red[tid >> 6] = top;
   __syncthreads();
-  top = max(max(red[0], red[1]), max(red[2], red[3]));
-  for (int k = tid; k < a.d; k += NT) el[(int64_t)p * a.d + k] += kTop - top;
+#pragma unroll
+  for (int i = 0; i < 1024 / 64; ++i) top = max(top, red[i]);
+  for (int k = tid; k < a.d; k += 1024) el[(int64_t)p * a.d + k] += kTop - top;
   if (tid == 0) scale[p] = top - 2 * kTop;
 }
 
-// Each row's id (-1: takes no part) and, for the backward, its log-sum; padded rows take no part.
-__global__ __launch_bounds__(NT) void xent_keys_kernel(Rows rows, int nrows, int padded, const float* __restrict__ lse,
-                                                       int* __restrict__ key, float* __restrict__ z) {
-  const int r = blockIdx.x * NT + threadIdx.x;
-  if (r >= padded) return;
-  key[r] = r < nrows ? rows.key(r) : -1;
-  if (z) z[r] = r < nrows ? lse[r] : 0.f;
+// X as the logits' first operand and, in the backward, as dW's; a piece of W as the
+// logits' second and dX's.
+__global__ __launch_bounds__(256) void xent_pack_x_kernel(planes::PackArgs l, planes::PackArgs w) {
+  const int64_t b = blockIdx.x, n = l.rows_blocks();
+  if (b < n) planes::pack_rows<true, kLo>(l, b);
+  else planes::pack_cols<false, 0>(w, b - n);
+}
+__global__ __launch_bounds__(256) void xent_pack_w_kernel(planes::PackArgs l, planes::PackArgs x) {
+  const int64_t b = blockIdx.x, n = l.cols_blocks();
+  if (b < n) planes::pack_cols<true, kLo>(l, b);
+  else planes::pack_rows<false, kLo>(x, b - n);
 }
 
 struct TileArgs {
@@ -232,7 +250,8 @@ struct TileArgs {
   char* prow;           // P packed for dX (rows, k = columns)
   char* pcol;           // and for dW (columns, k = rows)
   float* cfac;          // [64-row block][pcols] what a column's sum over the block is scaled back by
-  float* csum;          // [64-row block][pcols] column sums of P
+  float* csum;          // [64-row block][all columns] column sums of P, the piece's first
+  int64_t all;
 };
 
 // The sum or maximum over the 16 lanes of a row.
@@ -344,12 +363,12 @@ __global__ __launch_bounds__(S::NTH, 2) void xent_tile_kernel(TileArgs a) {
     ec[n] = min(kTop - exponent_above(__builtin_bit_cast(unsigned, cmax[n])), 126);
   }
   if (w.q == 0) {
-    const int64_t at = ((int64_t)tm * 2 + w.wm) * a.pcols + c0;
+    const int64_t blk = (int64_t)tm * 2 + w.wm;
     f32x4 f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) f[n] = __builtin_bit_cast(float, (unsigned)(127 - ec[n]) << 23);
-    *reinterpret_cast<f32x4*>(a.cfac + at) = f;
-    *reinterpret_cast<f32x4*>(a.csum + at) = f32x4{csum[0], csum[1], csum[2], csum[3]};
+    *reinterpret_cast<f32x4*>(a.cfac + blk * a.pcols + c0) = f;
+    *reinterpret_cast<f32x4*>(a.csum + blk * a.all + c0) = f32x4{csum[0], csum[1], csum[2], csum[3]};
   }
   // by column: this lane has 16 consecutive rows of each of its columns
 #pragma unroll
@@ -357,59 +376,81 @@ __global__ __launch_bounds__(S::NTH, 2) void xent_tile_kernel(TileArgs a) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float x[8];
-      int e[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = l[j & 3][n][2 * h + (j >> 2)];
-        e[j] = ec[n];
-      }
-      planes::put16<0>(a.pcol + planes::chunk_at<2>(a.pcols / 16, c0 + n, row0 + 8 * h), x, e);
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_ldexpf(l[j & 3][n][2 * h + (j >> 2)], ec[n]);
+      planes::put16<0>(a.pcol + planes::chunk_at<2>(a.pcols / 16, c0 + n, row0 + 8 * h), x);
     }
   // by row: lanes 2 j and 2 j + 1 have 8 consecutive columns together; the even one
-  // takes rows i = 0, 1, the odd one 2, 3
+  // takes rows i = 0, 1, the odd one 2, 3.  Rows lie in a block by 4 r + q here (q + 4 r
+  // elsewhere), so that the four lane groups write 64 contiguous bytes; dX's rows
+  // come out accordingly.
   const bool odd = w.lr & 1;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       float x[8];
-      int e[8];
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const float own = odd ? l[2 + j][n][r] : l[j][n][r], give = odd ? l[j][n][r] : l[2 + j][n][r];
         const float got = rotated<0xB1>(give);  // the other lane of the pair
-        x[n] = odd ? got : own;
-        x[4 + n] = odd ? own : got;
-        e[n] = e[4 + n] = kTop;
+        x[n] = (odd ? got : own) * (float)(1 << kTop);
+        x[4 + n] = (odd ? own : got) * (float)(1 << kTop);
       }
-      const int64_t row = row0 + 4 * r + (odd ? 2 + j : j);
-      planes::put16<kLo>(a.prow + planes::chunk_at<2>(a.padded / 16, row, c0 & ~7), x, e);
+      const int64_t row = (int64_t)tm * kTile + 64 * w.wm + 16 * r + 4 * w.q + (odd ? 2 + j : j);
+      planes::put16<kLo>(a.prow + planes::chunk_at<2>(a.padded / 16, row, c0 & ~7), x);
     }
 }
 
-// A piece's statistics join the rows'.
-__global__ __launch_bounds__(NT) void xent_join_kernel(const float2* __restrict__ part, int blocks, int64_t padded, int nrows,
-                                                       const float* __restrict__ target, RowState* __restrict__ state,
-                                                       int first) {
-  const int r = blockIdx.x * NT + threadIdx.x;
-  if (r >= nrows) return;
-  RowState t{-FLT_MAX, 0.f, 0.f, 0.f};
-  if (!first) t = state[r];
-  for (int b0 = 0; b0 < blocks; b0 += 8) {
+// lse and the row losses from the blocks' statistics, 64 rows to a workgroup whose
+// waves take every 16th block, and the sum of the workgroup's row losses.
+__global__ __launch_bounds__(1024) void xent_join_kernel(const float2* __restrict__ part, int blocks, int64_t padded, int nrows,
+                                                         const float* __restrict__ target, const int* __restrict__ key,
+                                                         float* __restrict__ lse, float* __restrict__ row_loss,
+                                                         double* __restrict__ sums) {
+  __shared__ float2 red[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int r = blockIdx.x * 64 + lane;  // (< padded)
+  float m = -FLT_MAX, s = 0.f;
+  for (int b0 = w; b0 < blocks; b0 += 128) {
     float2 x[8];
-    float m = t.max;
+    float top = m;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[j] = b0 + j < blocks ? part[(int64_t)(b0 + j) * padded + r] : make_float2(-FLT_MAX, 0.f);
-      m = fmaxf(m, x[j].x);
+      x[j] = b0 + 16 * j < blocks ? part[(int64_t)(b0 + 16 * j) * padded + r] : make_float2(-FLT_MAX, 0.f);
+      top = fmaxf(top, x[j].x);
     }
-    t.sum *= expf(t.max - m);
+    s *= expf(m - top);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t.sum += x[j].y * expf(x[j].x - m);
-    t.max = m;
+    for (int j = 0; j < 8; ++j) s += x[j].y * expf(x[j].x - top);
+    m = top;
   }
-  t.target = target[r];
-  state[r] = t;
+  red[w][lane] = make_float2(m, s);
+  __syncthreads();
+  if (w != 0) return;
+#pragma unroll
+  for (int j = 1; j < 16; ++j) m = fmaxf(m, red[j][lane].x);
+  s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) s += red[j][lane].y * expf(red[j][lane].x - m);
+  const float z = m + logf(s);
+  double one = 0.0;
+  if (r < nrows) {
+    const float v = key[r] >= 0 ? z - target[r] : 0.f;
+    lse[r] = z;
+    if (row_loss) row_loss[r] = v;
+    one = (double)v;
+  }
+  one = wave_sum(one);
+  if (lane == 0) sums[blockIdx.x] = one;
+}
+__global__ __launch_bounds__(NT) void xent_loss_kernel(const double* __restrict__ sums, int n, float scale,
+                                                       float* __restrict__ loss, int add) {
+  __shared__ double red[NT / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += NT) s += sums[i];
+  s = block_sum<NT>(s, red);
+  if (threadIdx.x == 0) loss[0] = (float)(s * (double)scale) + (add ? loss[0] : 0.f);
 }
 
 // What finishes a product: C (+)= 2^(exponent of its row or column) g sum.
@@ -421,31 +462,43 @@ struct OutArgs {
   int ex_by_row, add;  // the exponent is add - ex[row or column]
   float scale;
   const float* upstream;
+  int vec;  // four columns at a time
   __device__ __forceinline__ float g() const { return upstream ? upstream[0] * scale : scale; }
-  __device__ __forceinline__ void put(int64_t row, int col, float sum, float gg) const {
+  // Columns col .. col + 3 of a row (those of the matrix).
+  __device__ __forceinline__ void put(int64_t row, int col, f32x4 v, float gg) const {
+    if (row >= rows || col >= cols) return;
     float* p = C + row * ldc + col;
-    const float v = __builtin_ldexpf(sum, add - ex[ex_by_row ? row : col]) * gg;
-    *p = accumulate ? *p + v : v;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) v[n] = __builtin_ldexpf(v[n], add - ex[ex_by_row ? row : min(col + n, cols - 1)]) * gg;
+    if (vec) {
+      if (accumulate) v += *reinterpret_cast<const f32x4*>(p);
+      *reinterpret_cast<f32x4*>(p) = v;
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if (col + n < cols) p[n] = accumulate ? p[n] + v[n] : v[n];
+    }
   }
 };
 
 struct ProductArgs {
   Operand A, B;
   int nk, gx, gy, splits, per;  // stages; per split
+  int items;                    // workgroups
   const float* cfac;            // dW: [64-row block][pcols]
   int64_t pcols;
   OutArgs out;
   float* part;                  // [split][padded rows][padded cols] where splits > 1
 };
 
-// COLS false: dX = P W^T.  true: dW = X^T P, whose sums over each 64 rows (two
-// stages) are scaled back column by column.
+// COLS false: dX = P W^T, whose rows lie in their blocks as the tile kernel left
+// them.  true: dW = X^T P, whose sums over each 64 rows (two stages) are scaled back
+// column by column.
 template <bool COLS>
-__global__ __launch_bounds__(S::NTH, 2) void xent_product_kernel(ProductArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+__device__ __forceinline__ void xent_product(const ProductArgs& a, int item, char* lds) {
   const planes::Lane<S> w;
   int tm, tn, z;
-  gemm::item_tile(blockIdx.x, a.gx * a.gy * a.splits, a.gx, a.gy, tm, tn, z);
+  gemm::item_tile(item, a.items, a.gx, a.gy, tm, tn, z);
   const int k0 = z * a.per, k1 = min(a.nk, k0 + a.per);
   f32x4 sum[4][4], acc[4][4];
   if (COLS) {
@@ -468,26 +521,29 @@ __global__ __launch_bounds__(S::NTH, 2) void xent_product_kernel(ProductArgs a) 
 #pragma unroll
       for (int n = 0; n < 4; ++n) sum[i][n] += acc[i][n] * (1.f / (1 << kLo));
   }
-  const int64_t row0 = (int64_t)tm * kTile + 64 * w.wm + 16 * w.q;
+  const int64_t row0 = (int64_t)tm * kTile + 64 * w.wm + (COLS ? 16 : 4) * w.q;
   const int c0 = tn * kTile + w.col();
-  if (a.splits > 1) {
-    const int64_t ld = (int64_t)a.gx * kTile;
-    float* p = a.part + (int64_t)z * a.gy * kTile * ld + row0 * ld + c0;
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<f32x4*>(p + (4 * r + i) * ld) = f32x4{sum[i][0][r], sum[i][1][r], sum[i][2][r], sum[i][3][r]};
-    return;
-  }
-  const float g = a.out.g();
+  const float g = a.splits > 1 ? 0.f : a.out.g();
+  const int64_t ld = (int64_t)a.gx * kTile;
+  float* p = a.part + (int64_t)z * a.gy * kTile * ld + c0;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-        if (row0 + 4 * r + i < a.out.rows && c0 + n < a.out.cols) a.out.put(row0 + 4 * r + i, c0 + n, sum[i][n][r], g);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = row0 + (COLS ? 4 : 16) * r + i;
+      const f32x4 v = f32x4{sum[i][0][r], sum[i][1][r], sum[i][2][r], sum[i][3][r]};
+      if (a.splits > 1) *reinterpret_cast<f32x4*>(p + row * ld) = v;
+      else a.out.put(row, c0, v, g);
+    }
+}
+
+// Both products of a piece in one launch, dW's items first (they are the longer
+// ones, or equal), so that the chip stays full to the end of the second.
+__global__ __launch_bounds__(S::NTH, 2) void xent_products_kernel(ProductArgs w, ProductArgs x, int start) {
+  __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+  const int b = blockIdx.x;
+  if (b < w.items) xent_product<true>(w, b, lds);
+  else if (b >= start) xent_product<false>(x, b - start, lds);
 }
 
 // The splits' sums in order.
@@ -501,21 +557,27 @@ __global__ __launch_bounds__(NT) void xent_reduce_kernel(ProductArgs a) {
     const float* p = a.part + row * ld + col;
     f32x4 s = *reinterpret_cast<const f32x4*>(p);
     for (int z = 1; z < a.splits; ++z) s += *reinterpret_cast<const f32x4*>(p + z * step);
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (col + n < a.out.cols) a.out.put(row, col + n, s[n], g);
+    a.out.put(row, col, s, g);
   }
 }
 
-// db of a piece (+)= g times the 64-row blocks' column sums, in order.
-__global__ __launch_bounds__(NT) void xent_db_kernel(const float* __restrict__ csum, int blocks, int64_t pcols, int cols,
+// db (+)= g times the 64-row blocks' column sums: 64 columns to a workgroup, whose
+// waves take every fourth block; their sums in order.
+__global__ __launch_bounds__(NT) void xent_db_kernel(const float* __restrict__ csum, int blocks, int64_t all, int vocab,
                                                      float* __restrict__ db, int accumulate, float scale,
                                                      const float* __restrict__ upstream) {
-  const int c = blockIdx.x * NT + threadIdx.x;
-  if (c >= cols) return;
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
   float s = 0.f;
+  if (c < vocab) {
 #pragma unroll 8
-  for (int b = 0; b < blocks; ++b) s += csum[(int64_t)b * pcols + c];
+    for (int b = w; b < blocks; b += 4) s += csum[(int64_t)b * all + c];
+  }
+  red[w][lane] = s;
+  __syncthreads();
+  if (w != 0 || c >= vocab) return;
+  s = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
   s *= upstream ? upstream[0] * scale : scale;
   db[c] = accumulate ? db[c] + s : s;
 }
@@ -550,24 +612,45 @@ SmallPlan small_plan(int rows, int d, int vocab) {
 constexpr int kPlaneRows = 256;
 bool use_planes(int rows, int d, int vocab) { return rows >= kPlaneRows && vocab <= (1 << 30); }
 
-// Splits of a product's K: enough workgroups for two to a CU, and at least 16 stages each.
-int splits_of(int64_t tiles, int stages) {
-  const int64_t want = 2 * gemm::kChipCus / std::max<int64_t>(tiles, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(want, stages / 16));
+// The two products of a piece share a grid of two workgroups to a CU.  A product
+// whose workgroups would each take more than 5/4 of a CU slot's share of the
+// stages has its K split, into at least 16 stages each (an even number: the column
+// factors cover two).
+struct Split {
+  int splits, per;
+};
+Split split_of(int stages, int64_t share) {
+  int n = (int)std::max<int64_t>(1, std::min<int64_t>((stages + share * 5 / 4 - 1) / std::max<int64_t>(share * 5 / 4, 1), stages / 16));
+  const int per = ((stages + n - 1) / n + 1) / 2 * 2;
+  return Split{(stages + per - 1) / per, per};
 }
-// Stages of a split, even (the column factors cover two).
-int per_split(int stages, int splits) { return ((stages + splits - 1) / splits + 1) / 2 * 2; }
+struct PairSplit {
+  Split w, x;
+  size_t wbytes, xbytes;  // of partial sums
+};
+PairSplit pair_split(int padded, int dp, int pcols, bool has_w, bool has_x) {
+  const int64_t tw = has_w ? (int64_t)(dp / kTile) * (pcols / kTile) : 0, tx = has_x ? (int64_t)(padded / kTile) * (dp / kTile) : 0;
+  const int sw = padded / 32, sx = pcols / 32;
+  const int64_t share = (tw * sw + tx * sx + 2 * gemm::kChipCus - 1) / (2 * gemm::kChipCus);
+  PairSplit p{split_of(sw, share), split_of(sx, share), 0, 0};
+  if (has_w && p.w.splits > 1) p.wbytes = (size_t)p.w.splits * dp * pcols * 4;
+  if (has_x && p.x.splits > 1) p.xbytes = (size_t)p.x.splits * padded * dp * 4;
+  return p;
+}
 
 // The planes' plan: rows are taken kRowsAtOnce at a time (rows of a chunk, padded to
-// whole tiles), the vocabulary in pieces that keep both packed P below
+// whole tiles), the vocabulary in pieces that keep both packed P within
 // kPlaneBytes.
 constexpr int kRowsAtOnce = 32768;
-constexpr size_t kPlaneBytes = (size_t)192 << 20;
+constexpr size_t kPlaneBytes = (size_t)256 << 20;
 struct PlanePlan {
   int rows, d, vocab;
   int padded, dk, dp, piece, pieces, chunks, slabs, slab_rows;
   // offsets into the workspace
-  size_t xpart, wpart, ex, el, en, scale, key, z, state, target, part, xl, xt, wl, wn, prow, pcol, cfac, csum, split, total;
+  size_t xpart, wpart, ex, el, en, scale, key, z, target, sums, xl, wl;
+  size_t part;                                         // forward
+  size_t xt, wn, prow, pcol, cfac, csum, wsplit, xsplit;  // backward, at the same place
+  size_t total;
 };
 PlanePlan plane_plan(int all_rows, int d, int vocab) {
   PlanePlan p;
@@ -590,7 +673,7 @@ PlanePlan plane_plan(int all_rows, int d, int vocab) {
     at += round256(bytes);
     return o;
   };
-  const size_t padded = p.padded, piece = p.piece;
+  const size_t padded = p.padded, piece = p.piece, all = (size_t)p.pieces * p.piece;
   p.xpart = take((size_t)p.slabs * d * 4);
   p.wpart = take((size_t)p.pieces * p.chunks * d * 4);
   p.ex = take((size_t)d * 4);
@@ -599,29 +682,34 @@ PlanePlan plane_plan(int all_rows, int d, int vocab) {
   p.scale = take((size_t)p.pieces * 4);
   p.key = take(padded * 4);
   p.z = take(padded * 4);
-  p.state = take(padded * sizeof(RowState));
   p.target = take(padded * 4);
+  p.sums = take(padded / 64 * 8);
   p.xl = take(padded * p.dk * 32 * 4);
   p.wl = take(piece * p.dk * 32 * 4);
-  // the forward's statistics lie where the backward's planes do
-  p.part = p.xt = take(std::max(padded * p.dp * 4, padded * (piece / 64) * sizeof(float2)));
+  const size_t both = at;
+  p.part = take(padded * (all / 64) * sizeof(float2));
+  const size_t fwd = at;
+  at = both;
+  p.xt = take(padded * p.dp * 4);
   p.wn = take(piece * p.dp * 4);
   p.prow = take(padded * piece * 4);
   p.pcol = take(padded * piece * 4);
   p.cfac = take(padded / 64 * piece * 4);
-  p.csum = take(padded / 64 * piece * 4);
-  size_t split = 0;
-  const int last = (vocab - (p.pieces - 1) * p.piece + kTile - 1) / kTile * kTile;
-  for (int cols : {p.piece, last}) {
-    const int sx = splits_of((int64_t)(p.padded / kTile) * (p.dp / kTile), cols / 32);
-    const int sw = splits_of((int64_t)(p.dp / kTile) * (cols / kTile), p.padded / 32);
-    if (sx > 1) split = std::max(split, (size_t)sx * padded * p.dp * 4);
-    if (sw > 1) split = std::max(split, (size_t)sw * p.dp * cols * 4);
-  }
-  // (a last chunk of fewer rows may have more splits, of at most two tiles to a CU in all)
-  if (all_rows > kRowsAtOnce) split = std::max(split, (size_t)2 * gemm::kChipCus * kTile * kTile * 4);
-  p.split = take(split);
-  p.total = at;
+  p.csum = take(padded / 64 * all * 4);
+  // partial sums, whichever products a call has and of whichever piece and chunk
+  const int last_cols = (int)(vocab - (size_t)(p.pieces - 1) * piece + kTile - 1) / kTile * kTile;
+  const int last_rows = ((all_rows - 1) % p.rows + kTile) / kTile * kTile;
+  size_t wbytes = 0, xbytes = 0;
+  for (int cols : {p.piece, last_cols})
+    for (int rows : {p.padded, last_rows})
+      for (int has : {1, 2, 3}) {
+        const PairSplit s = pair_split(rows, p.dp, cols, has & 1, has & 2);
+        wbytes = std::max(wbytes, s.wbytes);
+        xbytes = std::max(xbytes, s.xbytes);
+      }
+  p.wsplit = take(wbytes);
+  p.xsplit = take(xbytes);
+  p.total = std::max(at, fwd);
   return p;
 }
 
@@ -667,62 +755,91 @@ struct Chunk {
     return reinterpret_cast<T*>(ws + o);
   }
 
-  void begin(const Rows& rw, const float* lse) const {
-    const unsigned xtiles = (unsigned)((p.d + NT - 1) / NT);
-    const AmaxArgs a{X,       ldx,     W,           ldw,           rows,
-                     p.d,     p.vocab, p.piece,     p.chunks,      p.slabs,
-                     p.slab_rows, (int)(xtiles * p.slabs), at<unsigned>(p.xpart), at<unsigned>(p.wpart)};
-    const int64_t wblocks = (int64_t)p.pieces * p.chunks * p.d;
-    mle::launch(xent_amax_kernel, (unsigned)(xtiles * p.slabs + wblocks), NT, 0, s, a);
-    mle::launch(xent_scales_kernel, (unsigned)p.pieces, NT, 0, s, a, at<int>(p.ex), at<int>(p.el), at<int>(p.en), at<int>(p.scale));
-    mle::launch(xent_keys_kernel, (unsigned)((padded + NT - 1) / NT), NT, 0, s, rw, rows, padded, lse, at<int>(p.key),
-                lse ? at<float>(p.z) : nullptr);
-    planes::PackArgs pa{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, at(p.xl), 0};
-    pa.vec = aligned16(X) && ldx % 4 == 0;
-    mle::launch(planes::pack_rows_kernel<true, kLo>, (unsigned)((pa.blocks * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
+  // Exponents, ids, and X packed (for dW too where `weights`).
+  void begin(const Rows& rw, const float* lse, bool weights) const {
+    AmaxArgs a{};
+    a.X = X;
+    a.ldx = ldx;
+    a.W = W;
+    a.ldw = ldw;
+    a.rows = rows;
+    a.d = p.d;
+    a.vocab = p.vocab;
+    a.piece = p.piece;
+    a.chunks = p.chunks;
+    a.slabs = p.slabs;
+    a.slab_rows = p.slab_rows;
+    a.xblocks = (p.d + NT - 1) / NT * p.slabs;
+    a.xpart = at<unsigned>(p.xpart);
+    a.wpart = at<unsigned>(p.wpart);
+    a.padded = padded;
+    a.kblocks = (padded + NT - 1) / NT;
+    a.lse = lse;
+    a.key = at<int>(p.key);
+    a.z = at<float>(p.z);
+    mle::launch(xent_amax_kernel, (unsigned)(a.kblocks + a.xblocks + p.pieces * p.chunks * p.d), NT, 0, s, a, rw);
+    mle::launch(xent_scales_kernel, (unsigned)p.pieces, 1024, 0, s, a, at<int>(p.ex), at<int>(p.el), at<int>(p.en), at<int>(p.scale));
+    const int vec = aligned16(X) && ldx % 4 == 0;
+    const planes::PackArgs l{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, at(p.xl), vec};
+    const planes::PackArgs w{X, ldx, p.d, rows, p.dp / 16, padded / 32, at<int>(p.ex), at<int>(p.key), at(p.xt), vec};
+    mle::launch(xent_pack_x_kernel, (unsigned)(l.rows_blocks() + (weights ? w.cols_blocks() : 0)), 256, 0, s, l, w);
   }
   int cols(int i) const { return std::min(p.piece, p.vocab - i * p.piece); }
   int pcols(int i) const { return (cols(i) + kTile - 1) / kTile * kTile; }
-  // Piece i of W as the logits' second operand.
-  void pack_piece(int i) const {
-    planes::PackArgs pa{W + (int64_t)i * p.piece, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d,
-                        nullptr, at(p.wl), 0};
-    pa.vec = aligned16(W) && ldw % 4 == 0;  // (pieces begin at multiples of 128)
-    mle::launch(planes::pack_cols_kernel<true, kLo>, (unsigned)((pa.blocks / 4 * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
+  // Piece i of W for the logits, and for dX where `inputs`.
+  void pack_piece(int i, bool inputs) const {
+    const float* w = W + (int64_t)i * p.piece;
+    const int vec = aligned16(W) && ldw % 4 == 0;  // (pieces begin at multiples of 128)
+    const planes::PackArgs l{w, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d, nullptr, at(p.wl), vec};
+    const planes::PackArgs x{w, ldw, p.d, cols(i), p.dp / 16, pcols(i) / 32, at<int>(p.en) + (int64_t)i * p.d, nullptr, at(p.wn), vec};
+    mle::launch(xent_pack_w_kernel, (unsigned)(l.cols_blocks() + (inputs ? x.rows_blocks() : 0)), 256, 0, s, l, x);
   }
+  Operand operand(size_t o, int padded_rows) const { return Operand{at(o), (int64_t)padded_rows / 16 * 2 * planes::kUnit}; }
   TileArgs tile(int i) const {
     TileArgs a{};
-    a.A = Operand{at(p.xl), (int64_t)padded / 16 * 2 * planes::kUnit};
-    a.B = Operand{at(p.wl), (int64_t)pcols(i) / 16 * 2 * planes::kUnit};
+    a.A = operand(p.xl, padded);
+    a.B = operand(p.wl, pcols(i));
     a.nk = p.dk;
     a.gx = pcols(i) / kTile;
     a.gy = padded / kTile;
     a.cols = cols(i);
     a.v0 = i * p.piece;
-    a.bias = bias ? bias + (int64_t)i * p.piece : nullptr;
+    a.bias = bias ? bias + a.v0 : nullptr;
     a.scale = at<int>(p.scale) + i;
     a.key = at<int>(p.key);
     a.padded = padded;
     a.pcols = pcols(i);
     return a;
   }
-  template <bool COLS>
-  void product(const char* A, int m, const char* B, int n, int stages, const OutArgs& out) const {
-    ProductArgs a{};
-    a.A = Operand{A, (int64_t)m / 16 * 2 * planes::kUnit};
-    a.B = Operand{B, (int64_t)n / 16 * 2 * planes::kUnit};
-    a.nk = stages;
-    a.gx = n / kTile;
-    a.gy = m / kTile;
-    a.per = per_split(stages, splits_of((int64_t)a.gx * a.gy, stages));
-    a.splits = (stages + a.per - 1) / a.per;
-    a.cfac = at<float>(p.cfac);
-    a.pcols = n;
-    a.out = out;
-    a.part = at<float>(p.split);
-    mle::launch(xent_product_kernel<COLS>, (unsigned)((int64_t)a.gx * a.gy * a.splits), S::NTH, 0, s, a);
-    if (a.splits > 1)
-      mle::launch(xent_reduce_kernel, stream_grid((size_t)out.rows * n / 4, NT, 8192), NT, 0, s, a);
+  // The products of piece i; a null matrix leaves its product out.
+  void products(int i, OutArgs ow, OutArgs ox) const {
+    const PairSplit ps = pair_split(padded, p.dp, pcols(i), ow.C != nullptr, ox.C != nullptr);
+    auto product = [&](Operand A, Operand B, int stages, int gx, int gy, Split sp, const OutArgs& out, size_t part) {
+      ProductArgs a{};
+      a.A = A;
+      a.B = B;
+      a.nk = stages;
+      a.gx = gx;
+      a.gy = gy;
+      a.splits = sp.splits;
+      a.per = sp.per;
+      a.items = out.C ? gx * gy * sp.splits : 0;
+      a.cfac = at<float>(p.cfac);
+      a.pcols = pcols(i);
+      a.out = out;
+      a.out.vec = aligned16(out.C) && out.ldc % 4 == 0 && out.cols % 4 == 0;
+      a.part = at<float>(part);
+      return a;
+    };
+    const ProductArgs w = product(operand(p.xt, p.dp), operand(p.pcol, pcols(i)), padded / 32, pcols(i) / kTile, p.dp / kTile,
+                                  ps.w, ow, p.wsplit);
+    const ProductArgs x = product(operand(p.prow, padded), operand(p.wn, p.dp), pcols(i) / 32, p.dp / kTile, padded / kTile,
+                                  ps.x, ox, p.xsplit);
+    const int start = (w.items + gemm::kXcds - 1) / gemm::kXcds * gemm::kXcds;  // (item 0 of dX on XCD 0 again)
+    mle::launch(xent_products_kernel, (unsigned)(start + x.items), S::NTH, 0, s, w, x, start);
+    for (const ProductArgs& a : {w, x})
+      if (a.items && a.splits > 1)
+        mle::launch(xent_reduce_kernel, stream_grid((size_t)a.out.rows * a.gx * (kTile / 4), NT, 8192), NT, 0, s, a);
   }
 };
 
@@ -740,18 +857,20 @@ int planes_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
   for (int r0 = 0; r0 < rows; r0 += p.rows) {
     const Chunk c = chunk_of(p, ws, s, r0, rows, X, ldx, W, ldw, bias);
     rw.r0 = r0;
-    c.begin(rw, nullptr);
+    c.begin(rw, nullptr, false);
+    int blocks = 0;
     for (int i = 0; i < p.pieces; ++i) {
-      c.pack_piece(i);
+      c.pack_piece(i, false);
       TileArgs a = c.tile(i);
-      a.part = c.at<float2>(p.part);
+      a.part = c.at<float2>(p.part) + (int64_t)blocks * c.padded;
       a.target = c.at<float>(p.target);
       mle::launch(xent_tile_kernel<false>, (unsigned)(a.gx * a.gy), S::NTH, 0, s, a);
-      mle::launch(xent_join_kernel, (unsigned)((c.rows + NT - 1) / NT), NT, 0, s, a.part, 2 * a.gx, a.padded, c.rows, a.target,
-                  c.at<RowState>(p.state), i == 0 ? 1 : 0);
+      blocks += 2 * a.gx;
     }
-    mle::launch(xent_finish_kernel, 1u, 1024, 0, s, c.at<RowState>(p.state), c.rows, rw, loss_scale, lse + r0,
-                row_loss ? row_loss + r0 : nullptr, loss, r0 > 0 ? 1 : 0);
+    const int groups = c.padded / 64;
+    mle::launch(xent_join_kernel, (unsigned)groups, 1024, 0, s, c.at<float2>(p.part), blocks, (int64_t)c.padded, c.rows,
+                c.at<float>(p.target), c.at<int>(p.key), lse + r0, row_loss ? row_loss + r0 : nullptr, c.at<double>(p.sums));
+    mle::launch(xent_loss_kernel, 1u, NT, 0, s, c.at<double>(p.sums), groups, loss_scale, loss, r0 > 0 ? 1 : 0);
   }
   return check_launch("mle_vocab_xent_fwd");
 }
@@ -764,41 +883,30 @@ int planes_bwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
   for (int r0 = 0; r0 < rows; r0 += p.rows) {
     const Chunk c = chunk_of(p, ws, s, r0, rows, X, ldx, W, ldw, bias);
     rw.r0 = r0;
-    c.begin(rw, lse + r0);
-    if (dW) {
-      planes::PackArgs pa{X + (int64_t)r0 * ldx, ldx, d, c.rows, p.dp / 16, c.padded / 32, c.at<int>(p.ex), c.at<int>(p.key),
-                          c.at(p.xt), 0};
-      pa.vec = aligned16(X) && ldx % 4 == 0;
-      mle::launch(planes::pack_cols_kernel<false, 0>, (unsigned)((pa.blocks / 4 * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
-    }
+    c.begin(rw, lse + r0, dW != nullptr);
+    const int add = accumulate_dw || r0 > 0;
+    const int64_t all = (int64_t)p.pieces * p.piece;
     for (int i = 0; i < p.pieces; ++i) {
       const int64_t v0 = (int64_t)i * p.piece;
-      c.pack_piece(i);
+      c.pack_piece(i, dX != nullptr);
       TileArgs a = c.tile(i);
       a.lse = c.at<float>(p.z);
       a.prow = c.at(p.prow);
       a.pcol = c.at(p.pcol);
       a.cfac = c.at<float>(p.cfac);
-      a.csum = c.at<float>(p.csum);
+      a.csum = c.at<float>(p.csum) + v0;
+      a.all = all;
       mle::launch(xent_tile_kernel<true>, (unsigned)(a.gx * a.gy), S::NTH, 0, s, a);
-      if (dX) {
-        planes::PackArgs pa{W + v0, ldw, d, c.cols(i), p.dp / 16, c.pcols(i) / 32, c.at<int>(p.en) + (int64_t)i * d, nullptr,
-                            c.at(p.wn), 0};
-        pa.vec = aligned16(W) && ldw % 4 == 0;
-        mle::launch(planes::pack_rows_kernel<false, kLo>, (unsigned)((pa.blocks * (int64_t)pa.kblocks + 3) / 4), 256, 0, s, pa);
-        const OutArgs out{dX + (int64_t)r0 * lddx, lddx, c.rows, d, accumulate_dx || i > 0, c.at<int>(p.en) + (int64_t)i * d, 0,
-                          -kTop, grad_scale, upstream};
-        c.product<false>(c.at(p.prow), c.padded, c.at(p.wn), p.dp, c.pcols(i) / 32, out);
-      }
-      const int add = accumulate_dw || r0 > 0;
-      if (dW) {
-        const OutArgs out{dW + v0, lddw, d, c.cols(i), add, c.at<int>(p.ex), 1, 0, grad_scale, upstream};
-        c.product<true>(c.at(p.xt), p.dp, c.at(p.pcol), c.pcols(i), c.padded / 32, out);
-      }
-      if (db)
-        mle::launch(xent_db_kernel, (unsigned)((c.cols(i) + NT - 1) / NT), NT, 0, s, c.at<float>(p.csum), c.padded / 64,
-                    (int64_t)c.pcols(i), c.cols(i), db + v0, add, grad_scale, upstream);
+      OutArgs ow{}, ox{};
+      if (dW) ow = OutArgs{dW + v0, lddw, d, c.cols(i), add, c.at<int>(p.ex), 1, 0, grad_scale, upstream, 0};
+      if (dX)
+        ox = OutArgs{dX + (int64_t)r0 * lddx, lddx, c.rows, d, accumulate_dx || i > 0, c.at<int>(p.en) + (int64_t)i * d, 0, -kTop,
+                     grad_scale, upstream, 0};
+      c.products(i, ow, ox);
     }
+    if (db)
+      mle::launch(xent_db_kernel, (unsigned)((vocab + 63) / 64), NT, 0, s, c.at<float>(p.csum), c.padded / 64, all, vocab, db,
+                  add, grad_scale, upstream);
   }
   return check_launch("mle_vocab_xent_bwd");
 }
