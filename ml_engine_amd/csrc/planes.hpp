@@ -149,14 +149,16 @@ __device__ __forceinline__ void multiply(const Operand& A, const Operand& B, int
   }
 }
 
-// The same with one accumulator, cleared every `run` stages: end(first stage of
-// the run) then adds it to sums that the caller keeps.  For operands whose later
+// The same with one accumulator, cleared every `run` stages: begin(first stage of
+// the run) is called before the run, whose loads are then there at its end, and end()
+// after it, to add the sums to what the caller keeps.  For operands whose later
 // planes are not scaled against the first, so that all products are of one scale.
-template <class S, class F>
+template <class S, class F, class G>
 __device__ __forceinline__ void multiply_runs(const Operand& A, const Operand& B, int tm, int tn, int k0, int k1, int run,
-                                              char* lds, const Lane<S>& w, f32x4 (&acc)[4][4], F end) {
+                                              char* lds, const Lane<S>& w, f32x4 (&acc)[4][4], F begin, G end) {
   if (k0 < k1) stage_load<S>(A, B, tm, tn, k0, lds);
   for (int kr = k0; kr < k1; kr += run) {
+    begin(kr);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -169,7 +171,7 @@ __device__ __forceinline__ void multiply_runs(const Operand& A, const Operand& B
       if (k + 1 < k1) stage_load<S>(A, B, tm, tn, k + 1, nxt);
       stage_mma<S>(cur, w, acc, acc);
     }
-    end(kr);
+    end();
   }
 }
 

@@ -507,13 +507,16 @@ __device__ __forceinline__ void xent_product(const ProductArgs& a, int item, cha
 #pragma unroll
       for (int n = 0; n < 4; ++n) sum[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float* fac = a.cfac + (int64_t)tn * kTile + w.col();
-    planes::multiply_runs<S>(a.A, a.B, tm, tn, k0, k1, 2, lds, w, acc, [&](int k) {
-      const f32x4 f = *reinterpret_cast<const f32x4*>(fac + (int64_t)(k >> 1) * a.pcols);
+    f32x4 f;
+    planes::multiply_runs<S>(
+        a.A, a.B, tm, tn, k0, k1, 2, lds, w, acc,
+        [&](int k) { f = *reinterpret_cast<const f32x4*>(fac + (int64_t)(k >> 1) * a.pcols); },
+        [&]() {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) sum[i][n] += f[n] * acc[i][n];
-    });
+            for (int n = 0; n < 4; ++n) sum[i][n] += f[n] * acc[i][n];
+        });
   } else {
     planes::multiply<S>(a.A, a.B, tm, tn, k0, k1, lds, w, sum, acc);
 #pragma unroll
