@@ -542,8 +542,9 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
  *   mle_q8_linear_wgrad: a Linear's weight gradient from its kept input:
  *                       dW [in, out] (+)= X^T dY, and (db non-null) db (+)= column
  *                       sums of dY; X the values of q, e [rows, in], which enter the
- *                       products exactly.  fp32 accuracy, sums in a fixed order.
- *                       rows 0 assigns zeros.
+ *                       products exactly.  fp32 accuracy, sums in a fixed order;
+ *                       an infinity or NaN in dY makes its column of dW NaN, one
+ *                       among the kept values its group's rows.  rows 0 assigns zeros.
  * Rows of 16-byte (floats) and 8-byte (codes) alignment are read and written
  * whole; any others element by element.  dx may be dy's buffer, y may be x's. */
 int mle_q8_quantize(mle_stream stream, int rows, int cols, const float* x, int64_t ldx, int8_t* q, int64_t ldq,

@@ -1,6 +1,6 @@
 // Activations kept in 8 bits for the backward pass (q8.hpp has the format):
-// quantising, reading back, the activation functions around it, and a Linear's
-// weight gradient from a kept input.
+// quantising, reading back, and the activation functions around it.  A Linear's weight
+// gradient from a kept input is in q8_wgrad.hip.
 #include "activation.hpp"
 #include "q8.hpp"
 
@@ -92,14 +92,6 @@ __global__ __launch_bounds__(NT) void q8_act_bwd_kernel(Q8Args a) {
 
 unsigned grid_of(const Q8Args& a) { return stream_grid((size_t)a.rows * a.units, NT, 16384); }
 
-int check_shape(const char* who, int rows, int cols, const void* q, int64_t ldq, const void* e, int64_t lde) {
-  MLE_CHECK_ARG(rows >= 0 && cols > 0, "%s: bad shape %d x %d", who, rows, cols);
-  MLE_CHECK_ARG(rows == 0 || (q && e), "%s: null pointer", who);
-  MLE_CHECK_ARG(ldq >= cols && lde >= q8::groups(cols), "%s: ldq %lld < %d or lde %lld < %d", who, (long long)ldq, cols,
-                (long long)lde, q8::groups(cols));
-  return MLE_OK;
-}
-
 #define Q8_LAUNCH_ACT(kernel, kind, a, s)                                                    \
   switch (kind) {                                                                            \
     case MLE_RELU: mle::launch(kernel<MLE_RELU>, grid_of(a), NT, 0, s, a); break;            \
@@ -172,36 +164,6 @@ int mle_q8_act_bwd(mle_stream stream, int kind, int rows, int cols, const int8_t
   a.vq = q8::codes_vec(q, ldq);
   Q8_LAUNCH_ACT(q8_act_bwd_kernel, kind, a, as_stream(stream));
   return check_launch("mle_q8_act_bwd");
-}
-
-// The weight gradient: the kept values written out as floats into the
-// workspace, then the library's product.
-static size_t values_bytes(int rows, int in) { return ((size_t)rows * in * sizeof(float) + 255) & ~(size_t)255; }
-
-size_t mle_q8_linear_wgrad_ws_bytes(int rows, int in, int out) {
-  if (rows <= 0 || in <= 0 || out <= 0) return 0;
-  return values_bytes(rows, in) + mle_gemm_ws_bytes(in, out, rows, 1);
-}
-
-int mle_q8_linear_wgrad(mle_stream stream, int rows, int in, int out, const int8_t* q, int64_t ldq, const uint8_t* e,
-                        int64_t lde, const float* dY, int64_t lddy, float* dW, int64_t lddw, float* db, int accumulate,
-                        void* ws, size_t ws_bytes) {
-  int rc = check_shape("mle_q8_linear_wgrad", rows, in, q, ldq, e, lde);
-  if (rc) return rc;
-  MLE_CHECK_ARG(out > 0 && dW && (dY || rows == 0) && lddy >= out && lddw >= out,
-                "mle_q8_linear_wgrad: bad argument (out %d, lddy %lld, lddw %lld)", out, (long long)lddy, (long long)lddw);
-  if (ws_bytes < mle_q8_linear_wgrad_ws_bytes(rows, in, out) || (rows > 0 && (!ws || !aligned16(ws))))
-    return set_error(MLE_ERR_WORKSPACE, "mle_q8_linear_wgrad: workspace of %zu bytes, 16-byte aligned, needed",
-                     mle_q8_linear_wgrad_ws_bytes(rows, in, out));
-  float* x = static_cast<float*>(ws);
-  rc = mle_q8_dequantize(stream, rows, in, q, ldq, e, lde, x, in);
-  if (rc) return rc;
-  if (db && !accumulate) {
-    rc = mle_fill(stream, db, 0.f, (size_t)out);
-    if (rc) return rc;
-  }
-  return mle_gemm_ex(stream, 1, 0, in, out, rows, 1.f, x, in, 0, dY, lddy, 0, accumulate ? 1.f : 0.f, dW, lddw, 0, 1, db,
-                     nullptr, static_cast<char*>(ws) + values_bytes(rows, in), ws_bytes - values_bytes(rows, in));
 }
 
 }  // extern "C"

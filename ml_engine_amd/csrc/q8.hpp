@@ -121,6 +121,14 @@ __device__ __forceinline__ void store_row8(float* __restrict__ p, const float (&
   }
 }
 
+inline int check_shape(const char* who, int rows, int cols, const void* q, int64_t ldq, const void* e, int64_t lde) {
+  MLE_CHECK_ARG(rows >= 0 && cols > 0, "%s: bad shape %d x %d", who, rows, cols);
+  MLE_CHECK_ARG(rows == 0 || (q && e), "%s: null pointer", who);
+  MLE_CHECK_ARG(ldq >= cols && lde >= groups(cols), "%s: ldq %lld < %d or lde %lld < %d", who, (long long)ldq, cols,
+                (long long)lde, groups(cols));
+  return MLE_OK;
+}
+
 // Whether rows of a tensor can be read and written eight values at a time.
 inline bool rows_vec(const float* p, int64_t ld) { return mle::aligned16(p) && ld % 4 == 0; }
 inline bool codes_vec(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0 && ld % 8 == 0; }

@@ -27,7 +27,7 @@ QUANT = dict(stream=None, rows=8, cols=40, x=A, ldx=40, q=A, ldq=40, e=A, lde=2)
 DEQUANT = dict(stream=None, rows=8, cols=40, q=A, ldq=40, e=A, lde=2, y=A, ldy=40)
 ACT_FWD = dict(stream=None, kind=1, rows=8, cols=40, x=A, ldx=40, y=A, ldy=40, q=A, ldq=40, e=A, lde=2)
 ACT_BWD = dict(stream=None, kind=1, rows=8, cols=40, q=A, ldq=40, e=A, lde=2, dy=A, lddy=40, dx=A, lddx=40, acc=0)
-WGRAD = dict(stream=None, rows=8, inp=40, out=24, q=A, ldq=40, e=A, lde=2, dY=A, lddy=24, dW=A, lddw=24, db=A, acc=0, ws=A,
+WGRAD = dict(stream=None, rows=4096, inp=40, out=24, q=A, ldq=40, e=A, lde=2, dY=A, lddy=24, dW=A, lddw=24, db=A, acc=0, ws=A,
              ws_bytes=1 << 40)
 NORM_FWD = dict(stream=None, rows=8, cols=40, x=A, r=A, w=A, eps=1e-5, h=A, y=A, rstd=A, q=A, ldq=40, e=A, lde=2)
 NORM_BWD = dict(stream=None, rows=8, cols=40, h=A, w=A, rstd=A, dy=A, dres=A, dh=A, acc_dh=0, dw=A, acc_dw=0, ws=A,

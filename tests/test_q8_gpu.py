@@ -151,7 +151,9 @@ def wgrad(hip, x, dy, ldq, lde, lddy, lddw, old_dw, old_db, acc, bias=True):
 
 @pytest.mark.parametrize("rows,inp,out,pad,acc", [(1, 1, 1, 0, 0), (1, 40, 24, 1, 1), (31, 33, 65, 3, 0), (64, 64, 64, 0, 1),
                                                   (200, 96, 130, 0, 0), (1000, 330, 516, 0, 0), (257, 128, 256, 8, 1),
-                                                  (2048, 256, 384, 0, 0), (4096, 48, 52, 0, 0), (333, 1024, 64, 0, 0)])
+                                                  (2048, 256, 384, 0, 0), (4096, 48, 52, 0, 0), (333, 1024, 64, 0, 0),
+                                                  (500, 3, 130, 0, 1), (70, 5, 9, 2, 0), (1500, 700, 2100, 0, 0),
+                                                  (8200, 257, 1030, 1, 1)])
 def test_linear_wgrad(hip, rows, inp, out, pad, acc):
     r = rng(rows + inp + out)
     x = (r.standard_normal((rows, inp)) * np.exp2(r.integers(-6, 6, (rows, 1)))).astype(np.float32)
