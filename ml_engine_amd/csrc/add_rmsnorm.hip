@@ -226,22 +226,29 @@ __global__ __launch_bounds__(NT) void rmsnorm_dw_kernel(NormBwdArgs a) {
   a.part[(int64_t)blockIdx.y * a.cols + col] = s;
 }
 
-// dw (+)= the partial sums: 16 columns to a workgroup, 16 threads to a column,
-// each adding every 16th part, and the threads' sums in order.
-__global__ __launch_bounds__(NT) void rmsnorm_join_kernel(const float* __restrict__ part, int parts, int cols,
-                                                          float* __restrict__ dw, int accumulate) {
-  __shared__ float red[16][17];
+// dw (+)= the partial sums: 16 columns to a workgroup, 64 threads to a column, each
+// adding every 64th part, and the threads' sums in order.
+__global__ __launch_bounds__(1024) void rmsnorm_join_kernel(const float* __restrict__ part, int parts, int cols,
+                                                            float* __restrict__ dw, int accumulate) {
+  __shared__ float red[64][17];
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
   const int col = blockIdx.x * 16 + c;
   float s = 0.f;
-  if (col < cols)
-    for (int p = g; p < parts; p += 16) s += part[(int64_t)p * cols + col];
+  if (col < cols) {
+#pragma unroll 8
+    for (int p = g; p < parts; p += 64) s += part[(int64_t)p * cols + col];
+  }
   red[g][c] = s;
   __syncthreads();
-  if (g != 0 || col >= cols) return;
-  float v = red[0][c];
+  if (threadIdx.x >= 64) return;
+  // a quarter of the threads' sums to each of four lanes, then the quarters
+  s = 0.f;
+  const int q = threadIdx.x >> 4;
 #pragma unroll
-  for (int i = 1; i < 16; ++i) v += red[i][c];
+  for (int i = 0; i < 16; ++i) s += red[16 * q + i][c];
+  const float a = __shfl(s, c, 64), b = __shfl(s, 16 + c, 64), d = __shfl(s, 32 + c, 64), e = __shfl(s, 48 + c, 64);
+  if (q != 0 || col >= cols) return;
+  const float v = ((a + b) + d) + e;
   dw[col] = accumulate ? dw[col] + v : v;
 }
 
@@ -315,7 +322,7 @@ int mle_add_rmsnorm_bwd(mle_stream stream, int rows, int cols, const float* h, c
     mle::launch(rmsnorm_bwd_wide_kernel, (unsigned)rows, 1024, 0, s, a);
   }
   if (dw)
-    mle::launch(rmsnorm_join_kernel, (unsigned)((cols + 15) / 16), NT, 0, s, static_cast<const float*>(ws), parts, cols, dw,
+    mle::launch(rmsnorm_join_kernel, (unsigned)((cols + 15) / 16), 1024, 0, s, static_cast<const float*>(ws), parts, cols, dw,
                 accumulate_dw);
   return check_launch("mle_add_rmsnorm_bwd");
 }
