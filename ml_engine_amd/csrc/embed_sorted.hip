@@ -22,7 +22,6 @@ namespace {
 constexpr int IX_NT = 1024;
 constexpr int IX_RMAX = 1024;   // table rows of an index workgroup
 constexpr int IX_CHUNK = 8192;  // tokens that it sorts at a time
-constexpr int IX_HOT = 32;      // tokens of a row in a chunk above which a wave lists them by a scan
 constexpr int HEAD = 64;
 constexpr int PART = 16;        // places of the list that one partial sum covers
 
@@ -39,15 +38,13 @@ __device__ __forceinline__ int key_of(const IndexArgs& a, int t) {
   return a.clen == a.max_clen ? a.keys[t] : a.keys[(int64_t)(t / a.clen) * a.max_clen + t % a.clen];
 }
 
+constexpr int IX_WAVES = IX_NT / 64;
+constexpr int IX_PER = IX_CHUNK / IX_NT;  // tokens of a lane in a chunk
+
 struct IndexLds {
-  int total[IX_RMAX];          // tokens of each row
-  int next[IX_RMAX];           // the row's next place in the list
-  int count[IX_RMAX];          // tokens of each row in this chunk
-  int end[IX_RMAX];            // places in `perm`, counted down while filling
-  int perm[IX_CHUNK];          // (row << 16) | token of the chunk, by row, in arrival order
-  unsigned short rel[IX_CHUNK];  // the row of each token of the chunk, 0xffff: none of this workgroup's
-  int hot[IX_CHUNK / (IX_HOT + 1) + 1];  // rows of the chunk that are listed by a scan
-  int wave[IX_NT / 64];
+  int count[IX_WAVES][IX_RMAX];  // tokens of each row among a wave's, then where they go
+  int next[IX_RMAX];             // the row's next place in the list
+  int wave[IX_WAVES];
   int smaller;
 };
 
@@ -75,28 +72,75 @@ __device__ __forceinline__ int exclusive_scan(int v, int* wave, int& sum) {
 
 // Lists the tokens of table rows [v0, v0 + nrows): every workgroup reads all
 // the keys, and counts how many lie below its rows, which is where its part of
-// the list starts.
+// the list starts.  A chunk's tokens are taken in order by the waves (512
+// consecutive ones each), 64 at a time.  Lanes with equal rows find each other by a
+// ballot per bit of the row, so that a token knows its place among the wave's; the
+// waves' counts in order give the rest.
 __device__ void index_rows(const IndexArgs& a, int wg, IndexLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int v0 = wg * a.rows_per_wg, nrows = min(a.rows_per_wg, a.vocab - v0);
-  if (tid < IX_RMAX) s.total[tid] = 0;
+  const int rbits = 32 - __clz(max(nrows - 1, 1));
+  // this lane's keys of a chunk, in token order by (wave, k, lane); -1 past the end
+  auto load = [&](int c0, int (&key)[IX_PER]) {
+#pragma unroll
+    for (int k = 0; k < IX_PER; ++k) {
+      const int t = c0 + w * (IX_CHUNK / IX_WAVES) + k * 64 + lane;
+      key[k] = t < a.ntok ? key_of(a, t) : -1;
+    }
+  };
+  auto clear = [&]() {
+    for (int i = tid; i < IX_WAVES * nrows; i += IX_NT) s.count[i / nrows][i % nrows] = 0;
+  };
+  // rank: the token's place among the wave's of its row (row: -1 for others')
+  auto rank_wave = [&](const int (&key)[IX_PER], int (&row)[IX_PER], int (&rank)[IX_PER]) {
+#pragma unroll
+    for (int k = 0; k < IX_PER; ++k) {
+      const unsigned r = (unsigned)key[k] - (unsigned)v0;
+      const bool mine = key[k] >= 0 && r < (unsigned)nrows;
+      row[k] = mine ? (int)r : -1;
+      unsigned long long same = __ballot(mine);
+      if (same == 0) continue;
+      for (int b = 0; b < rbits; ++b) {
+        const bool bit = (r >> b) & 1;
+        const unsigned long long m = __ballot(bit);
+        same &= bit ? m : ~m;
+      }
+      if (mine) {
+        const int before = __popcll(same & ((1ull << lane) - 1));
+        const int base = s.count[w][r];
+        rank[k] = base + before;
+        if (before == 0) s.count[w][r] = base + __popcll(same);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's next 64 read what these wrote
+    }
+  };
+  const bool single = a.ntok <= IX_CHUNK;
+  int key[IX_PER], row[IX_PER], rank[IX_PER];
   if (tid == 0) s.smaller = 0;
+  clear();
   __syncthreads();
-  int below = 0;
-  for (int t0 = tid; t0 < a.ntok; t0 += 8 * IX_NT) {
-    int key[8];
+  int below = 0, mine = 0;
+  if (single) {
+    load(0, key);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) key[k] = t0 + k * IX_NT < a.ntok ? key_of(a, t0 + k * IX_NT) : -1;
+    for (int k = 0; k < IX_PER; ++k) below += key[k] >= 0 && key[k] < v0;
+    rank_wave(key, row, rank);
+  } else {
+    for (int c0 = 0; c0 < a.ntok; c0 += IX_CHUNK) {
+      load(c0, key);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      below += key[k] >= 0 && key[k] < v0;
-      if (key[k] >= v0 && key[k] < v0 + nrows) atomicAdd(&s.total[key[k] - v0], 1);
+      for (int k = 0; k < IX_PER; ++k) {
+        below += key[k] >= 0 && key[k] < v0;
+        if (key[k] >= v0 && key[k] < v0 + nrows) atomicAdd(&s.count[w][key[k] - v0], 1);
+      }
     }
   }
   below = wave_sum(below);
   if (lane == 0) atomicAdd(&s.smaller, below);
   __syncthreads();
-  const int mine = tid < nrows ? s.total[tid] : 0;
+  if (tid < nrows)
+#pragma unroll
+    for (int i = 0; i < IX_WAVES; ++i) mine += s.count[i][tid];
   int kept;
   const int start = s.smaller + exclusive_scan(mine, s.wave, kept);
   if (tid < nrows) {
@@ -106,73 +150,32 @@ __device__ void index_rows(const IndexArgs& a, int wg, IndexLds& s) {
   if (wg == a.nix - 1 && tid == 0) a.head[0] = s.smaller + kept;
   if (kept == 0) return;
   for (int c0 = 0; c0 < a.ntok; c0 += IX_CHUNK) {
-    const int count = min(IX_CHUNK, a.ntok - c0);
-    __syncthreads();
-    if (tid < IX_RMAX) s.count[tid] = 0;
-    __syncthreads();
-    constexpr int PER = IX_CHUNK / IX_NT;
-    int rel[PER];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int i = tid + k * IX_NT;
-      const unsigned r = i < count ? (unsigned)key_of(a, c0 + i) - (unsigned)v0 : 0xffffffffu;
-      rel[k] = r < (unsigned)nrows ? (int)r : -1;
-    }
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      s.rel[tid + k * IX_NT] = (unsigned short)(rel[k] < 0 ? 0xffff : rel[k]);
-      if (rel[k] >= 0) atomicAdd(&s.count[rel[k]], 1);
+    if (!single) {
+      __syncthreads();
+      clear();
+      __syncthreads();
+      load(c0, key);
+      rank_wave(key, row, rank);
     }
     __syncthreads();
-    // places in `perm` for the rows that are ordered by rank
-    const int here = tid < nrows ? s.count[tid] : 0;
-    const int cold = here <= IX_HOT ? here : 0;
-    int placed;
-    const int first = exclusive_scan(cold, s.wave, placed);
-    if (tid < IX_RMAX) s.end[tid] = first + cold;
-    __syncthreads();
+    if (tid < nrows) {
+      int at = s.next[tid];
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
-      if (rel[k] >= 0 && s.count[rel[k]] <= IX_HOT)
-        s.perm[atomicSub(&s.end[rel[k]], 1) - 1] = (rel[k] << 16) | (tid + k * IX_NT);
-    __syncthreads();
-    // s.end is now each row's start; an entry's rank is the number of the row's
-    // entries with a smaller token
-    for (int p = tid; p < placed; p += IX_NT) {
-      const int r = s.perm[p] >> 16, i = s.perm[p] & 0xffff;
-      const int b = s.end[r], n = s.count[r];
-      int rank = 0;
-      for (int q = 0; q < n; ++q) rank += (s.perm[b + q] & 0xffff) < i;
-      const int to = s.next[r] + rank;
-      a.list[to] = c0 + i;
-      a.skey[to] = v0 + r;
-    }
-    // frequent rows: a wave walks the chunk and lists one of them in order
-    int nhot;
-    const int h = exclusive_scan(here > IX_HOT, s.wave, nhot);
-    if (here > IX_HOT) s.hot[h] = tid;
-    __syncthreads();
-    for (int k = w; k < nhot; k += IX_NT / 64) {
-      const int r = s.hot[k];
-      int to = s.next[r];
-      for (int i0 = 0; i0 < count; i0 += 256) {
-        bool hit[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) hit[u] = s.rel[i0 + 64 * u + lane] == r;  // (0xffff past the chunk's end)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const unsigned long long m = __ballot(hit[u]);
-          if (hit[u]) {
-            const int at = to + __popcll(m & ((1ull << lane) - 1));
-            a.list[at] = c0 + i0 + 64 * u + lane;
-            a.skey[at] = v0 + r;
-          }
-          to += __popcll(m);
-        }
+      for (int i = 0; i < IX_WAVES; ++i) {
+        const int n = s.count[i][tid];
+        s.count[i][tid] = at;
+        at += n;
       }
+      s.next[tid] = at;
     }
     __syncthreads();
-    if (tid < nrows) s.next[tid] += s.count[tid];
+#pragma unroll
+    for (int k = 0; k < IX_PER; ++k)
+      if (row[k] >= 0) {
+        const int to = s.count[w][row[k]] + rank[k];
+        a.list[to] = c0 + w * (IX_CHUNK / IX_WAVES) + k * 64 + lane;
+        a.skey[to] = v0 + row[k];
+      }
   }
 }
 
