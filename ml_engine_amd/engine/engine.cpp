@@ -1054,6 +1054,76 @@ graph Linear::forward(const graph& X) {
   return node;
 }
 
+graph Linear::cross_entropy(const graph& X, const int32_t* keys, int clen, int max_clen, const bool last) {
+  if (X->dim[3] != in || X->dim[1] != 1 || X->dim[2] != clen || max_clen < clen) {
+    std::cout << "Shape Mismatch in cross entropy of " << op_name << ": \n";
+    Dimension(X);
+    std::cout << "Expected (batch, 1, " << clen << ", " << in << ") and ids for at most " << max_clen << " positions \n";
+    std::exit(1);
+  }
+  auto node = std::make_shared<NodeBackProp>(op_name + " cross entropy", 1, 1, 1, 1, 1);
+  node->lazy_grad_writer = true;
+  node->inputs = {X};
+  const int batch = X->dim[0], rows = batch * clen, n = in, p = out;
+  AdamParameter* W = &W1;
+  AdamParameter* Bb = bias ? &B1 : nullptr;
+  NodeBackProp *nd = node.get(), *x = X.get();
+  const str name = op_name;
+  node->params = Bb ? std::vector<AdamParameter*>{W, Bb} : std::vector<AdamParameter*>{W};
+  const size_t ws_bytes = mle_vocab_xent_ws_bytes(rows, n, p);
+  void* ws = mle::gemm_workspace(ws_bytes);  // carries nothing from one call to the next
+  float* lse = mle::alloc_output(rows);
+  // The loss is divided by the logits' count and its gradient by the batch, as
+  // SoftMaxCrossEntropy does.
+  const float loss_scale = (float)(1.0 / ((double)rows * p)), grad_scale = 1.0f / batch;
+  auto run = [=]() {
+    check(mle_vocab_xent_fwd(mle::stream(), rows, n, p, x->output, n, W->output, p, Bb ? Bb->output : nullptr, keys, clen,
+                             max_clen, loss_scale, lse, nullptr, nd->output, ws, ws_bytes),
+          "cross entropy of " + name);
+    nd->output_pending_zero = false;  // written whole
+  };
+  auto ready = std::make_shared<bool>(false);  // lse is of the last forward
+  node->forward = [=]() {
+    *ready = GraphOperations::calculate_loss || !last;
+    if (!*ready) return;
+    run();
+    if (last) check(mle_read_scalar(mle::stream(), nd->output, &GraphOperations::loss), "CE loss");
+  };
+  node->backward = [=]() {
+    if (!*ready) run();  // a forward that was asked for no loss
+    *ready = true;
+    check(mle_vocab_xent_bwd(mle::stream(), rows, n, p, x->output, n, W->output, p, Bb ? Bb->output : nullptr, keys, clen,
+                             max_clen, lse, last ? nullptr : nd->grad, grad_scale, x->grad, n, mle::accumulate_flag(x),
+                             W->grad, p, Bb ? Bb->grad : nullptr, mle::params_write_flag({W, Bb}), ws, ws_bytes),
+          "derivative of cross entropy of " + name);
+  };
+  node->zero_grad = [=]() {
+    mle::defer_zero_output(nd);
+    if (!last) mle::defer_zero(nd);
+    mle::defer_zero(W);
+    if (Bb) mle::defer_zero(Bb);
+  };
+  node->free = [=]() {
+    nd->clear();
+    mle::release(lse, rows, false);
+  };
+  node->serious_free = [=]() {};
+  node->accumulate = [=](double* s) {
+    W->accumulate_grad(s);
+    if (Bb) Bb->accumulate_grad(s);
+  };
+  node->clipnorm = [=](const double* s) {
+    W->gradnorm(s);
+    if (Bb) Bb->gradnorm(s);
+  };
+  node->updateParams = [=](const float lr, const bool adamw) {
+    W->update(lr, adamw);
+    if (Bb) Bb->update(lr, adamw);
+  };
+  node->printparams = [=](const bool) {};
+  return node;
+}
+
 // ---------------------------------------------------------------------------
 // Sibling Linear fusion (see engine.h).
 namespace mle {
@@ -1444,6 +1514,43 @@ graph Embedding::forward(const int32_t* keys, int batch, int clen, int max_clen)
       check(mle_embed_grad(mle::stream(), T->grad, nd->grad, keys, batch, clen, max_clen, D, V,
                            mle::params_write_flag({T}), ws, wsb),
             "Embedding gradient");
+  };
+  node->zero_grad = [=]() {
+    mle::defer_zero(nd);
+    mle::defer_zero(T);
+  };
+  node->free = [=]() { nd->clear(); };
+  node->accumulate = [=](double* s) { T->accumulate_grad(s); };
+  node->clipnorm = [=](const double* s) { T->gradnorm(s); };
+  node->updateParams = [=](const float lr, const bool adamw) { T->update(lr, adamw); };
+  return node;
+}
+
+graph Embedding::forward(const int32_t* keys, int batch, int clen, int max_clen, float scale) {
+  auto node = std::make_shared<NodeBackProp>(E.op_name + " scaled lookup", batch, 1, clen, dim, 1);
+  node->lazy_grad_writer = true;
+  keys_ = keys;
+  batch_ = batch;
+  clen_ = clen;
+  max_clen_ = max_clen;
+  ws_bytes_ = mle_embed_scatter_ws_bytes(batch, clen);  // UpdateSGD's
+  ws_ = mle::alloc_scratch(ws_bytes_);
+  AdamParameter* T = &E;
+  NodeBackProp* nd = node.get();
+  const int V = vocab, D = dim;
+  // This node's own index: the keys do not change before its backward.
+  const size_t ixb = mle_embed_sorted_index_bytes(batch, clen, V), wsb = mle_embed_sorted_grad_ws_bytes(batch, clen, D);
+  void* index = mle::alloc_scratch(ixb);
+  void* ws = mle::gemm_workspace(wsb);
+  node->params = {T};
+  node->forward = [=]() {
+    check(mle_embed_scaled_fwd(mle::stream(), nd->output, T->output, keys, batch, clen, max_clen, D, V, scale, index, ixb),
+          "scaled embedding lookup");
+  };
+  node->backward = [=]() {
+    check(mle_embed_sorted_grad(mle::stream(), T->grad, nd->grad, index, ixb, batch, clen, D, V, scale,
+                                mle::params_write_flag({T}), ws, wsb),
+          "Embedding gradient");
   };
   node->zero_grad = [=]() {
     mle::defer_zero(nd);

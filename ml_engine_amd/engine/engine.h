@@ -356,6 +356,7 @@ graph_tree topological_sort(const graph& root);
 class GraphOperations {
  private:
   static bool calculate_loss;
+  friend class Linear;  // (its cross entropy node reads calculate_loss)
 
  public:
   graph_tree nodes;
@@ -436,6 +437,13 @@ class Linear {
   str op_name = "Linear Layer";
   Linear(const int input, const int output, const str name = "", const bool bias = true);
   graph forward(const graph& X);
+  // SoftMaxCrossEntropy(forward(X), OneHot(keys, batch, clen, max_clen, out_features()), last)
+  // in one node that keeps no logits and no gradient of them (mle_vocab_xent_*):
+  // the same loss, and the same gradients of X, W1 and B1, for ids in the
+  // vocabulary.  A position whose id is outside it (INT_MIN past a sequence's
+  // end) has no loss and no gradient.  X is [batch, 1, clen, in_features()];
+  // keys are device ids [batch][max_clen].
+  graph cross_entropy(const graph& X, const int32_t* keys, int clen, int max_clen, const bool last = true);
   bool has_bias() const { return bias; }
   int in_features() const { return in; }
   int out_features() const { return out; }
@@ -519,6 +527,10 @@ class Embedding {
   AdamParameter E;
   Embedding(int vocab, int dim, const str name = "Embedding");
   graph forward(const int32_t* keys, int batch, int clen, int max_clen);
+  // The lookup times `scale` (sqrt(dim) in a transformer whose table is also its
+  // output projection), any vocabulary; the table gradient by sorted tokens
+  // (mle_embed_scaled_fwd, mle_embed_sorted_grad).
+  graph forward(const int32_t* keys, int batch, int clen, int max_clen, float scale);
   void UpdateSGD(const graph& X, float lr = LEARNING_RATE);
   // AdamParameter checkpoint record of the table (with its Adam moments).
   void save(std::ofstream& f) const;

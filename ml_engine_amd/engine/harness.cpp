@@ -3,6 +3,7 @@
 // It drives the engine exactly as a reference application does
 // (use_cases/mnist.cu:284-293: zero_grad, forward(calc_loss), backward,
 // ParameterUpdate) and adds host access to parameters and gradients.
+#include <math.h>
 #include <string.h>
 
 #include <fstream>
@@ -142,6 +143,25 @@ void build_c6(Model* m, const long long* d) {
   m->params = {&m->up->W1, &m->up->B1};
 }
 
+// A language model's ends around one feed-forward: scaled embedding, x + FFN(x),
+// the vocabulary's cross entropy.  whole 1 takes the loss in one node without
+// logits, 0 through the Linear and SoftMaxCrossEntropy.
+// dims {B, S, D, F, V, whole, max_clen}
+void build_c8(Model* m, const long long* d) {
+  const int B = (int)d[0], S = (int)d[1], D = (int)d[2], F = (int)d[3], V = (int)d[4], mx = (int)d[6];
+  auto* ids = static_cast<int32_t*>(input_buffer(m, sizeof(int32_t) * B * mx));
+  auto* tgt = static_cast<int32_t*>(input_buffer(m, sizeof(int32_t) * B * mx));
+  m->emb.reset(new Embedding(V, D, "Token Embedding"));
+  m->ffn1.reset(new Linear(D, F, "FFN1"));
+  m->ffn2.reset(new Linear(F, D, "FFN2"));
+  m->lm.reset(new Linear(D, V, "Projection"));
+  auto x = m->emb->forward(ids, B, S, mx, sqrtf((float)D));
+  auto h = GraphOperations::Add(x, m->ffn2->forward(GraphOperations::GELU(m->ffn1->forward(x))));
+  if (d[5]) m->root = m->lm->cross_entropy(h, tgt, S, mx);
+  else m->root = GraphOperations::SoftMaxCrossEntropy(m->lm->forward(h), GraphOperations::OneHot(tgt, B, S, mx, V), true);
+  m->params = {&m->emb->E, &m->ffn1->W1, &m->ffn1->B1, &m->ffn2->W1, &m->ffn2->B1, &m->lm->W1, &m->lm->B1};
+}
+
 // C2: a flat set of parameters; each parameter is carried by a hook node (as
 // Linear's output node carries W1/B1) under one track() root.
 void build_c2(Model* m, const long long* d, int nd) {
@@ -206,6 +226,7 @@ void* mle_model_create(int kind, const long long* dims, int ndims) {
     case 5: build_c5(m, dims); break;
     case 6: build_c6(m, dims); break;
     case 7: build_c7(m, dims); break;
+    case 8: build_c8(m, dims); break;
     default:
       delete m;
       return nullptr;

@@ -21,7 +21,10 @@ enum { MLE_STEP_CLOBBER_SCALE = 16 };
  *         (Convolute2DT, CopyCrop, BatchNorm, RMSNorm, InstanceNorm, MSE)
  *                                                             inputs: x, skip, target f32
  * kind 7: 1x1 Convolute2D -> LayerNorm over [C, H, W] -> MSE  dims {N, Cin, C, H, W}
- *                                                             inputs: x, target f32 */
+ *                                                             inputs: x, target f32
+ * kind 8: scaled embedding -> x + FFN(x) -> vocabulary cross entropy, in one node
+ *         without logits (whole 1) or through them  dims {B, S, D, F, V, whole, max_clen}
+ *                                                             inputs: ids i32, targets i32 [B][max_clen] */
 void* mle_model_create(int kind, const long long* dims, int ndims);
 void mle_model_destroy(void* h);
 /* Reference bugs reproduced (1, default) or fixed (0); see mle::Quirks. */
