@@ -59,17 +59,19 @@ struct RowState {
 };
 
 // One row of a piece to a workgroup: its maximum and sum join the row's.
-__global__ __launch_bounds__(NT) void xent_stats_kernel(const float* __restrict__ l, int cols, int v0, Rows rows,
-                                                        RowState* __restrict__ state, int first) {
-  __shared__ float red[NT / 64];
+__global__ __launch_bounds__(1024) void xent_stats_kernel(const float* __restrict__ l, int cols, int v0, Rows rows,
+                                                          RowState* __restrict__ state, int first) {
+  __shared__ float red[1024 / 64];
   const int64_t r = blockIdx.x;
   const float* x = l + r * cols;
   float m = -FLT_MAX;
-  for (int c = threadIdx.x; c < cols; c += NT) m = fmaxf(m, x[c]);
-  m = block_max<NT>(m, red);
+#pragma unroll 4
+  for (int c = threadIdx.x; c < cols; c += 1024) m = fmaxf(m, x[c]);
+  m = block_max<1024>(m, red);
   float s = 0.f;
-  for (int c = threadIdx.x; c < cols; c += NT) s += expf(x[c] - m);
-  s = block_sum<NT>(s, red);
+#pragma unroll 4
+  for (int c = threadIdx.x; c < cols; c += 1024) s += expf(x[c] - m);
+  s = block_sum<1024>(s, red);
   if (threadIdx.x != 0) return;
   RowState t{m, s, 0.f, 0.f};
   if (!first) {
@@ -101,24 +103,26 @@ __global__ __launch_bounds__(1024) void xent_finish_kernel(const RowState* __res
   if (threadIdx.x == 0) loss[0] = (float)(sum * (double)scale) + (add ? loss[0] : 0.f);
 }
 
-// The rows of X that take part, the others as zeros: what a row that takes no
-// part holds, NaN included, must not reach dW.
-__global__ __launch_bounds__(NT) void xent_rows_kernel(const float* __restrict__ X, int64_t ldx, int d, Rows rows,
-                                                       float* __restrict__ out) {
-  const int64_t r = blockIdx.x;
-  const bool live = rows.key(r) >= 0;
-  for (int c = threadIdx.x; c < d; c += NT) out[r * d + c] = live ? X[r * ldx + c] : 0.f;
-}
-
-// A piece's logits to P, in place.
+// A piece's logits to P, in place: 1024 columns of a row to a workgroup.  Those past
+// the columns' take the rows of X that take part, the others as zeros, for dW: what
+// a row that takes no part holds, NaN included, must not reach it.
 __global__ __launch_bounds__(NT) void xent_grad_kernel(float* __restrict__ l, int cols, int v0, Rows rows,
                                                        const float* __restrict__ lse, const float* __restrict__ upstream,
-                                                       float scale) {
+                                                       float scale, int blocks, const float* __restrict__ X, int64_t ldx,
+                                                       int d, float* __restrict__ out) {
   const int64_t r = blockIdx.x;
-  float* x = l + r * cols;
   const int k = rows.key(r);
+  if ((int)blockIdx.y >= blocks) {
+    for (int c = threadIdx.x; c < d; c += NT) out[r * d + c] = k >= 0 ? X[r * ldx + c] : 0.f;
+    return;
+  }
+  float* x = l + r * cols;
   const float z = lse[r], g = upstream ? upstream[0] * scale : scale;
-  for (int c = threadIdx.x; c < cols; c += NT) x[c] = k >= 0 ? g * (expf(x[c] - z) - (c + v0 == k ? 1.f : 0.f)) : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = (int)blockIdx.y * 4 * NT + i * NT + threadIdx.x;
+    if (c < cols) x[c] = k >= 0 ? g * (expf(x[c] - z) - (c + v0 == k ? 1.f : 0.f)) : 0.f;
+  }
 }
 
 // ---------------------------------------------------------------- fp16 planes
@@ -607,13 +611,18 @@ SmallPlan small_plan(int rows, int d, int vocab) {
   for (int v : {p.piece, last})
     p.gemm = std::max(p.gemm, std::max(mle_gemm_ws_bytes(rows, v, d, 1),
                                        std::max(mle_gemm_ws_bytes(rows, d, v, 1), mle_gemm_ws_bytes(d, v, rows, 1))));
+  if (p.piece == vocab) p.gemm = std::max(p.gemm, mle_linear_bwd_ws_bytes(rows, d, vocab, 1));
   p.gemm = round256(p.gemm);
   return p;
 }
 
-// Where the products of fp16 planes run.
-constexpr int kPlaneRows = 256;
-bool use_planes(int rows, int d, int vocab) { return rows >= kPlaneRows && vocab <= (1 << 30); }
+// Where the products of fp16 planes run: from 128 rows (a whole tile) and 3 M logits
+// up.  Below, their eight launches more cost what the faster products save (forward
+// and backward, planes against stored pieces, us: 512 x 256 -> 4096 96 / 98, 256 x
+// 1024 -> 8000 175 / 180, 1000 x 128 -> 1000 86 / 62, 64 x 1024 -> 32000 406 / 306;
+// above: 128 x 512 -> 32000 224 / 243, 512 x 1024 -> 8000 204 / 250, 8192 x 96 ->
+// 4000 251 / 375).
+bool use_planes(int rows, int vocab) { return rows >= kTile && (double)rows * vocab >= 3e6 && vocab <= (1 << 30); }
 
 // The two products of a piece share a grid of two workgroups to a CU.  A product
 // whose workgroups would each take more than 5/4 of a CU slot's share of the
@@ -732,7 +741,7 @@ int check_ws(const char* who, size_t need, const void* ws, size_t ws_bytes) {
 }
 
 size_t ws_need(int rows, int d, int vocab) {
-  return use_planes(rows, d, vocab) ? plane_plan(rows, d, vocab).total : small_plan(rows, d, vocab).total();
+  return use_planes(rows, vocab) ? plane_plan(rows, d, vocab).total : small_plan(rows, d, vocab).total();
 }
 
 #define TRY(call)                  \
@@ -929,7 +938,7 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
   MLE_CHECK_ARG(loss && (lse || rows == 0), "mle_vocab_xent_fwd: null pointer");
   if (rows == 0) return mle_fill(stream, loss, 0.f, 1);
   TRY(check_ws("mle_vocab_xent_fwd", ws_need(rows, d, vocab), ws, ws_bytes));
-  if (use_planes(rows, d, vocab))
+  if (use_planes(rows, vocab))
     return planes_fwd(stream, rows, d, vocab, X, ldx, W, ldw, bias, Rows{keys, clen, max_clen, vocab, 0}, loss_scale, lse,
                       row_loss, loss, ws);
   const SmallPlan p = small_plan(rows, d, vocab);
@@ -942,7 +951,7 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
     const int n = std::min(p.piece, vocab - v0);
     TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr,
                     bias ? bias + v0 : nullptr, gws, p.gemm));
-    mle::launch(xent_stats_kernel, (unsigned)rows, NT, 0, s, l, n, v0, rw, state, v0 == 0 ? 1 : 0);
+    mle::launch(xent_stats_kernel, (unsigned)rows, 1024, 0, s, l, n, v0, rw, state, v0 == 0 ? 1 : 0);
   }
   mle::launch(xent_finish_kernel, 1u, 1024, 0, s, state, rows, rw, loss_scale, lse, row_loss, loss, 0);
   return check_launch("mle_vocab_xent_fwd");
@@ -958,12 +967,12 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
                 (long long)lddw, vocab);
   MLE_CHECK_ARG(dW || !db, "mle_vocab_xent_bwd: db without dW");
   if (rows > 0) TRY(check_ws("mle_vocab_xent_bwd", ws_need(rows, d, vocab), ws, ws_bytes));
-  if (rows > 0 && use_planes(rows, d, vocab))
+  if (rows > 0 && use_planes(rows, vocab))
     return !dX && !dW ? MLE_OK
                       : planes_bwd(stream, rows, d, vocab, X, ldx, W, ldw, bias, Rows{keys, clen, max_clen, vocab, 0}, lse,
                                    upstream, grad_scale, dX, lddx, accumulate_dx, dW, lddw, db, accumulate_dw, ws);
-  if (db && !accumulate_dw) TRY(mle_fill(stream, db, 0.f, (size_t)vocab));
   if (rows == 0) {
+    if (db && !accumulate_dw) TRY(mle_fill(stream, db, 0.f, (size_t)vocab));
     if (dW && !accumulate_dw)
       TRY(mle_gemm_ex(stream, 1, 0, d, vocab, 0, 1.f, nullptr, d, 0, nullptr, vocab, 0, 0.f, dW, lddw, 0, 1, nullptr, nullptr,
                       nullptr, 0));
@@ -976,12 +985,19 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
   float* l = static_cast<float*>(ws);
   float* xs = reinterpret_cast<float*>(static_cast<char*>(ws) + p.logits);
   void* gws = static_cast<char*>(ws) + p.logits + p.rows + p.state;
-  if (dW) mle::launch(xent_rows_kernel, (unsigned)rows, NT, 0, s, X, ldx, d, rw, xs);
+  // The Linear backward's own launches where its matrices are dense.
+  const bool dense = dX && dW && p.piece == vocab && ldw == vocab && lddw == vocab && lddx == d;
+  if (db && !accumulate_dw && !dense) TRY(mle_fill(stream, db, 0.f, (size_t)vocab));
   for (int v0 = 0; v0 < vocab; v0 += p.piece) {
-    const int n = std::min(p.piece, vocab - v0);
+    const int n = std::min(p.piece, vocab - v0), blocks = (n + 4 * NT - 1) / (4 * NT);
     TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr,
                     bias ? bias + v0 : nullptr, gws, p.gemm));
-    mle::launch(xent_grad_kernel, (unsigned)rows, NT, 0, s, l, n, v0, rw, lse, upstream, grad_scale);
+    mle::launch(xent_grad_kernel, dim3((unsigned)rows, (unsigned)(blocks + (dW && v0 == 0 ? 1 : 0))), NT, 0, s, l, n, v0, rw, lse,
+                upstream, grad_scale, blocks, X, ldx, d, xs);
+    if (dense) {
+      TRY(mle_linear_bwd_ex(stream, rows, d, vocab, 1, xs, l, 0, W, 0, dX, accumulate_dx, dW, db, 0, accumulate_dw, gws, p.gemm));
+      break;
+    }
     if (dX)
       TRY(mle_gemm_ex(stream, 0, 1, rows, d, n, 1.f, l, n, 0, W + v0, ldw, 0, accumulate_dx || v0 > 0 ? 1.f : 0.f, dX,
                       lddx, 0, 1, nullptr, nullptr, gws, p.gemm));

@@ -66,7 +66,7 @@ def exact(dims, params, ids, tgt):
 
 # one of few rows (pieces of stored logits), one of many (fp16 planes), one with a
 # table above the indexed lookup's limit
-SHAPES = [(2, 20, 32, 48, 101, 20), (4, 100, 64, 96, 500, 104), (3, 130, 48, 32, 20000, 130)]
+SHAPES = [(2, 20, 32, 48, 101, 20), (4, 100, 64, 96, 8000, 104), (3, 130, 48, 32, 20000, 130)]
 
 
 @pytest.mark.parametrize("dims", SHAPES)
