@@ -500,7 +500,8 @@ int mle_softmax_xent_keys_fwd_rowstats_read(mle_stream stream, const float* logi
  * Row r = b*clen + s has the id keys[b*max_clen + s]; a row whose id is outside
  * [0, vocab) takes no part: its loss is 0, its gradient 0, and what X holds there
  * (NaN included) reaches neither the loss nor dW.
- *   forward:   lse[r] = log sum_v exp l[r, v], for every row;
+ *   forward:   lse[r] = log sum_v exp l[r, v], for every row (of no meaning where a
+ *              row that takes no part holds what no row would);
  *              row_loss[r] = lse[r] - l[r, id] (row_loss may be NULL);
  *              loss[0] = loss_scale * sum of the row losses (1 / the number of
  *              rows that take part gives their mean).
@@ -508,7 +509,8 @@ int mle_softmax_xent_keys_fwd_rowstats_read(mle_stream stream, const float* logi
  *              dX (+)= P W^T (lddx), dW (+)= X^T P (lddw), db (+)= column sums of P;
  *              dX may be NULL, and dW with db (or db alone).  lse is the forward's.
  * A bias of -infinity takes an entry out of the vocabulary (probability and
- * gradient 0); a row with no finite logit has no finite loss.  The logits are
+ * gradient 0; its weights are finite, of any size); a row with no finite logit
+ * has no finite loss.  The logits are
  * formed in pieces of the vocabulary in ws, in the forward and again in the
  * backward; ws carries nothing from one call to the next.  fp32 accuracy; sums in
  * a fixed order.  X, W, dX and dW are buffers of their own.

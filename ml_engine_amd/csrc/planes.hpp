@@ -209,7 +209,10 @@ struct PackArgs {
   int rows, k;          // of the operand; rest zeros
   int blocks, kblocks;  // of the packed operand
   const int* ex;        // exponents by k or by row
-  const int* keys;      // nullable, by k: < 0 leaves that k out (zeros, whatever it holds)
+  // What is left out, zeros whatever it holds (nullable): pack_cols: k with keys < 0;
+  // rows (pack_cols) or k (pack_rows) with a bias of -infinity.
+  const int* keys;
+  const float* bias;
   char* out;
   int vec;              // 16-byte loads
   // Blocks of 256 threads that pack it.
@@ -240,6 +243,11 @@ __device__ __forceinline__ void pack_rows(const PackArgs& a, int64_t block) {
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
+  }
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (a.bias[min(k + j, a.k - 1)] == -INFINITY) x[j] = 0.f;
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) e[j] = EX_BY_K ? a.ex[min(k + j, a.k - 1)] : a.ex[min(row, a.rows - 1)];
@@ -277,9 +285,10 @@ __device__ __forceinline__ void pack_cols(const PackArgs& a, int64_t block) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float v[8];
+    const bool out = a.bias && a.bias[min(row + i, a.rows - 1)] == -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      v[j] = x[j][i];
+      v[j] = out ? 0.f : x[j][i];
       if (!EX_BY_K) e[j] = a.ex[min(row + i, a.rows - 1)];
     }
     put16<LO>(a.out + ((int64_t)kb * a.blocks + g * 4 + i) * 2 * kUnit + lane * 16, v, e);

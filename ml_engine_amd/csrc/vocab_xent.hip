@@ -143,14 +143,20 @@ __device__ __forceinline__ unsigned finite_bits(float x) {
   return b < 0x7f800000u ? b : 0u;
 }
 
+constexpr int kRowsAtOnce = 32768;  // rows of a chunk
+constexpr int kSlabs = 64;          // of them, at most
+constexpr int kFeatures = 4;        // of W to a workgroup,
+constexpr int kChunk = 4 * NT;      // and columns
+
 struct AmaxArgs {
   const float* X;
   int64_t ldx;
   const float* W;
   int64_t ldw;
-  int rows, d, vocab, piece, chunks;  // chunks: of 4096 columns, per piece
+  int rows, d, vocab, piece, chunks;  // chunks: of kChunk columns, per piece
   int slabs, slab_rows, xblocks;      // X: blocks of 256 columns x slabs
-  unsigned* xpart;                    // [slabs][d]
+  const float* bias;
+  unsigned* xpart;                    // [2][slabs][d]: of rows that take part, of the others
   unsigned* wpart;                    // [pieces][chunks][d]
   int padded, kblocks;                // rows: blocks of 256
   const float* lse;                   // backward
@@ -159,10 +165,11 @@ struct AmaxArgs {
 };
 
 // The largest finite magnitude of each feature: of X over slabs of rows, of W over
-// chunks of a piece's columns.  And each row's id (-1: takes no part) with, for the
+// chunks of a piece's columns (those that a bias of -infinity takes out left out:
+// their weights may be anything).  And each row's id (-1: takes no part) with, for the
 // backward, its log-sum; padded rows take no part.
 __global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a, Rows rows) {
-  __shared__ unsigned red[NT / 64];
+  __shared__ unsigned red[kFeatures][NT / 64];
   const int tid = threadIdx.x;
   if ((int)blockIdx.x < a.kblocks) {
     const int r = blockIdx.x * NT + tid;
@@ -175,54 +182,99 @@ __global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a, Rows rows) {
   if (bx < a.xblocks) {
     const int tiles = (a.d + NT - 1) / NT;
     const int slab = bx / tiles, k = (bx % tiles) * NT + tid;
+    const int r0 = slab * a.slab_rows, n = min(a.rows - r0, a.slab_rows);
+    unsigned m = 0, other = 0;
+    const float* x = a.X + (int64_t)r0 * a.ldx + min(k, a.d - 1);
+    for (int b0 = 0; b0 < n; b0 += 64) {
+      const int lane = tid & 63;
+      const unsigned long long live = __ballot(b0 + lane < n && rows.key(r0 + min(b0 + lane, n - 1)) >= 0);
+      const int nb = min(n - b0, 64);
+#pragma unroll 16
+      for (int r = 0; r < nb; ++r) {
+        const unsigned b = finite_bits(x[(int64_t)(b0 + r) * a.ldx]), keep = (live >> r) & 1 ? 0xffffffffu : 0u;
+        m = max(m, b & keep);
+        other = max(other, b & ~keep);
+      }
+    }
     if (k >= a.d) return;
-    const int r1 = min(a.rows, (slab + 1) * a.slab_rows);
-    unsigned m = 0;
-#pragma unroll 8
-    for (int r = slab * a.slab_rows; r < r1; ++r) m = max(m, finite_bits(a.X[(int64_t)r * a.ldx + k]));
     a.xpart[(int64_t)slab * a.d + k] = m;
+    a.xpart[(int64_t)(a.slabs + slab) * a.d + k] = other;
     return;
   }
-  const int b = bx - a.xblocks;
-  const int k = b % a.d, c = b / a.d;
-  const int v0 = c / a.chunks * a.piece + c % a.chunks * 4096;
-  const int v1 = min(min(v0 + 4096, (c / a.chunks + 1) * a.piece), a.vocab);
-  unsigned m = 0;
-  const float* w = a.W + (int64_t)k * a.ldw;
-#pragma unroll 4
-  for (int v = v0 + tid; v < v1; v += NT) m = max(m, finite_bits(w[v]));
+  const int fblocks = (a.d + kFeatures - 1) / kFeatures, b = bx - a.xblocks;
+  const int k0 = b % fblocks * kFeatures, c = b / fblocks;
+  const int v0 = c / a.chunks * a.piece + c % a.chunks * kChunk;
+  const int v1 = min(min(v0 + kChunk, (c / a.chunks + 1) * a.piece), a.vocab);
+  unsigned m[kFeatures] = {};
+  const float* w = a.W + (int64_t)k0 * a.ldw;
+  const float* bias = a.bias ? a.bias : w;  // (loaded either way: a branch would part the loads)
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = m;
+  for (int i = 0; i < kChunk / NT; ++i) {
+    const int v = min(v0 + i * NT + tid, v1 - 1);  // (the last column again past the end)
+    const unsigned keep = ((bias[v] == -INFINITY) & (a.bias != nullptr)) ? 0u : 0xffffffffu;
+#pragma unroll
+    for (int f = 0; f < kFeatures; ++f)
+      m[f] = max(m[f], finite_bits(w[(int64_t)min(f, a.d - 1 - k0) * a.ldw + v]) & keep);
+  }
+#pragma unroll
+  for (int f = 0; f < kFeatures; ++f) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m[f] = max(m[f], (unsigned)__shfl_xor((int)m[f], o, 64));
+    if ((tid & 63) == 0) red[f][tid >> 6] = m[f];
+  }
   __syncthreads();
-  if (tid == 0) a.wpart[(int64_t)c * a.d + k] = max(max(red[0], red[1]), max(red[2], red[3]));
+  if (tid < kFeatures && k0 + tid < a.d)
+    a.wpart[(int64_t)c * a.d + k0 + tid] = max(max(red[tid][0], red[tid][1]), max(red[tid][2], red[tid][3]));
 }
 
 // Exponents: ex[k] of X; for piece p, el[p][k] of W in the logits, en[p][k] of W in dX,
 // scale[p]: a logit is its sum times 2^scale.  A workgroup per piece.
+//
+// Rows that take no part have a log-sum too, but what they hold must not cost the
+// others their bits: their values raise a feature's scale, and the piece's, by
+// 2^kRoom at most.  (A row beyond that overflows, by itself.)
+constexpr int kRoom = 12;
 __global__ __launch_bounds__(1024) void xent_scales_kernel(AmaxArgs a, int* __restrict__ ex, int* __restrict__ el,
-                                                         int* __restrict__ en, int* __restrict__ scale) {
-  __shared__ int red[1024 / 64];
+                                                           int* __restrict__ en, int* __restrict__ scale) {
+  __shared__ int red[2][1024 / 64];
   const int p = blockIdx.x, tid = threadIdx.x;
-  int top = 2 * kNone;
+  int top = 2 * kNone, all = 2 * kNone;
   for (int k = tid; k < a.d; k += 1024) {
-    unsigned x = 0, w = 0;
+    unsigned x = 0, o = 0, w = 0;
 #pragma unroll 8
-    for (int s = 0; s < a.slabs; ++s) x = max(x, a.xpart[(int64_t)s * a.d + k]);
+    for (int s = 0; s < a.slabs; ++s) {
+      x = max(x, a.xpart[(int64_t)s * a.d + k]);
+      o = max(o, a.xpart[(int64_t)(a.slabs + s) * a.d + k]);
+    }
+#pragma unroll 4
     for (int c = 0; c < a.chunks; ++c) w = max(w, a.wpart[((int64_t)p * a.chunks + c) * a.d + k]);
-    const int lx = exponent_above(x), lw = exponent_above(w);
+    const int live = exponent_above(x), other = exponent_above(o), lw = exponent_above(w);
+    const int lx = live == kNone ? other : max(live, min(other, live + kRoom));
     if (p == 0) ex[k] = kTop - lx;
     en[(int64_t)p * a.d + k] = kTop - lw;
     el[(int64_t)p * a.d + k] = lx;  // completed below
-    top = max(top, lx + lw);
+    top = max(top, live == kNone ? 2 * kNone : live + lw);
+    all = max(all, lx + lw);
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = top;
+  for (int o = 32; o > 0; o >>= 1) {
+    top = max(top, __shfl_xor(top, o, 64));
+    all = max(all, __shfl_xor(all, o, 64));
+  }
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = top;
+    red[1][tid >> 6] = all;
+  }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 1024 / 64; ++i) top = max(top, red[i]);
-  for (int k = tid; k < a.d; k += 1024) el[(int64_t)p * a.d + k] += kTop - top;
+  for (int i = 0; i < 1024 / 64; ++i) {
+    top = max(top, red[0][i]);
+    all = max(all, red[1][i]);
+  }
+  top = top == 2 * kNone ? all : max(top, min(all, top + kRoom));
+  // (a feature that only those rows have stays below 2^kTop on W's side too)
+  for (int k = tid; k < a.d; k += 1024)
+    el[(int64_t)p * a.d + k] = min(el[(int64_t)p * a.d + k] + kTop - top, en[(int64_t)p * a.d + k]);
   if (tid == 0) scale[p] = top - 2 * kTop;
 }
 
@@ -653,7 +705,6 @@ PairSplit pair_split(int padded, int dp, int pcols, bool has_w, bool has_x) {
 // The planes' plan: rows are taken kRowsAtOnce at a time (rows of a chunk, padded to
 // whole tiles), the vocabulary in pieces that keep both packed P within
 // kPlaneBytes.
-constexpr int kRowsAtOnce = 32768;
 constexpr size_t kPlaneBytes = (size_t)256 << 20;
 struct PlanePlan {
   int rows, d, vocab;
@@ -676,8 +727,8 @@ PlanePlan plane_plan(int all_rows, int d, int vocab) {
   p.pieces = (int)((vocab + most - 1) / most);
   p.piece = ((vocab + p.pieces - 1) / p.pieces + kTile - 1) / kTile * kTile;
   p.pieces = (vocab + p.piece - 1) / p.piece;
-  p.chunks = (p.piece + 4095) / 4096;
-  p.slabs = std::min(64, (p.rows + 31) / 32);
+  p.chunks = (p.piece + kChunk - 1) / kChunk;
+  p.slabs = std::min(kSlabs, (p.rows + 31) / 32);
   p.slab_rows = (p.rows + p.slabs - 1) / p.slabs;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -686,7 +737,7 @@ PlanePlan plane_plan(int all_rows, int d, int vocab) {
     return o;
   };
   const size_t padded = p.padded, piece = p.piece, all = (size_t)p.pieces * p.piece;
-  p.xpart = take((size_t)p.slabs * d * 4);
+  p.xpart = take((size_t)2 * p.slabs * d * 4);
   p.wpart = take((size_t)p.pieces * p.chunks * d * 4);
   p.ex = take((size_t)d * 4);
   p.el = take((size_t)p.pieces * d * 4);
@@ -732,6 +783,14 @@ int check(const char* who, int rows, int d, int vocab, const float* X, int64_t l
   MLE_CHECK_ARG(ldx >= d && ldw >= vocab, "%s: ldx %lld < %d or ldw %lld < %d", who, (long long)ldx, d, (long long)ldw,
                 vocab);
   MLE_CHECK_ARG(clen > 0 && max_clen >= clen, "%s: clen %d, max_clen %d", who, clen, max_clen);
+  return MLE_OK;
+}
+// The planes' launches number (feature, chunk of columns) pairs in 31 bits.
+int check_planes(const char* who, int rows, int d, int vocab) {
+  if (rows <= 0 || !use_planes(rows, vocab)) return MLE_OK;
+  const PlanePlan p = plane_plan(rows, d, vocab);
+  if ((double)p.pieces * p.chunks * d >= 1073741824.0 || p.dk > (1 << 26))
+    return set_error(MLE_ERR_UNSUPPORTED, "%s: d %d with a vocabulary of %d is too large", who, d, vocab);
   return MLE_OK;
 }
 int check_ws(const char* who, size_t need, const void* ws, size_t ws_bytes) {
@@ -786,14 +845,15 @@ struct Chunk {
     a.wpart = at<unsigned>(p.wpart);
     a.padded = padded;
     a.kblocks = (padded + NT - 1) / NT;
+    a.bias = bias;
     a.lse = lse;
     a.key = at<int>(p.key);
     a.z = at<float>(p.z);
-    mle::launch(xent_amax_kernel, (unsigned)(a.kblocks + a.xblocks + p.pieces * p.chunks * p.d), NT, 0, s, a, rw);
+    mle::launch(xent_amax_kernel, (unsigned)(a.kblocks + a.xblocks + p.pieces * p.chunks * ((p.d + kFeatures - 1) / kFeatures)), NT, 0, s, a, rw);
     mle::launch(xent_scales_kernel, (unsigned)p.pieces, 1024, 0, s, a, at<int>(p.ex), at<int>(p.el), at<int>(p.en), at<int>(p.scale));
     const int vec = aligned16(X) && ldx % 4 == 0;
-    const planes::PackArgs l{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, at(p.xl), vec};
-    const planes::PackArgs w{X, ldx, p.d, rows, p.dp / 16, padded / 32, at<int>(p.ex), at<int>(p.key), at(p.xt), vec};
+    const planes::PackArgs l{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, nullptr, at(p.xl), vec};
+    const planes::PackArgs w{X, ldx, p.d, rows, p.dp / 16, padded / 32, at<int>(p.ex), at<int>(p.key), nullptr, at(p.xt), vec};
     mle::launch(xent_pack_x_kernel, (unsigned)(l.rows_blocks() + (weights ? w.cols_blocks() : 0)), 256, 0, s, l, w);
   }
   int cols(int i) const { return std::min(p.piece, p.vocab - i * p.piece); }
@@ -802,8 +862,8 @@ struct Chunk {
   void pack_piece(int i, bool inputs) const {
     const float* w = W + (int64_t)i * p.piece;
     const int vec = aligned16(W) && ldw % 4 == 0;  // (pieces begin at multiples of 128)
-    const planes::PackArgs l{w, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d, nullptr, at(p.wl), vec};
-    const planes::PackArgs x{w, ldw, p.d, cols(i), p.dp / 16, pcols(i) / 32, at<int>(p.en) + (int64_t)i * p.d, nullptr, at(p.wn), vec};
+    const planes::PackArgs l{w, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d, nullptr, bias ? bias + (int64_t)i * p.piece : nullptr, at(p.wl), vec};
+    const planes::PackArgs x{w, ldw, p.d, cols(i), p.dp / 16, pcols(i) / 32, at<int>(p.en) + (int64_t)i * p.d, nullptr, bias ? bias + (int64_t)i * p.piece : nullptr, at(p.wn), vec};
     mle::launch(xent_pack_w_kernel, (unsigned)(l.cols_blocks() + (inputs ? x.rows_blocks() : 0)), 256, 0, s, l, x);
   }
   Operand operand(size_t o, int padded_rows) const { return Operand{at(o), (int64_t)padded_rows / 16 * 2 * planes::kUnit}; }
@@ -937,6 +997,7 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
   TRY(check("mle_vocab_xent_fwd", rows, d, vocab, X, ldx, W, ldw, keys, clen, max_clen));
   MLE_CHECK_ARG(loss && (lse || rows == 0), "mle_vocab_xent_fwd: null pointer");
   if (rows == 0) return mle_fill(stream, loss, 0.f, 1);
+  TRY(check_planes("mle_vocab_xent_fwd", rows, d, vocab));
   TRY(check_ws("mle_vocab_xent_fwd", ws_need(rows, d, vocab), ws, ws_bytes));
   if (use_planes(rows, vocab))
     return planes_fwd(stream, rows, d, vocab, X, ldx, W, ldw, bias, Rows{keys, clen, max_clen, vocab, 0}, loss_scale, lse,
@@ -966,6 +1027,7 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
                 "mle_vocab_xent_bwd: null pointer, or lddx %lld < %d or lddw %lld < %d", (long long)lddx, d,
                 (long long)lddw, vocab);
   MLE_CHECK_ARG(dW || !db, "mle_vocab_xent_bwd: db without dW");
+  TRY(check_planes("mle_vocab_xent_bwd", rows, d, vocab));
   if (rows > 0) TRY(check_ws("mle_vocab_xent_bwd", ws_need(rows, d, vocab), ws, ws_bytes));
   if (rows > 0 && use_planes(rows, vocab))
     return !dX && !dW ? MLE_OK

@@ -135,14 +135,15 @@ def test_padded_sequences(hip, clen, max_clen):
 
 @pytest.mark.parametrize("rows,vocab", [(40, 500), (1000, 3100)])
 def test_what_rows_outside_hold_stays_there(hip, rows, vocab):
-    """NaN and infinity in rows that take no part: the loss, dW, db and the other rows' dX as without them."""
+    """NaN, infinity and huge values in rows that take no part: the loss, dW, db and the other rows' dX as without them."""
     c = Case(hip, rows, 64, vocab, ignored=0.3)
     bad = np.flatnonzero(~c.valid())
     c.x[bad] = 0
     c.put()
     ref, tol = c.exact()
-    c.x[bad[::2]] = np.nan
-    c.x[bad[1::2], 3] = -np.inf
+    c.x[bad[::3]] = np.nan
+    c.x[bad[1::3], 3] = -np.inf
+    c.x[bad[2::3]] = 3e38
     c.put()
     _, row_loss, loss = c.forward()
     dx, dw, db = c.backward()
@@ -170,6 +171,7 @@ def test_masked_entries(hip, rows, vocab):
     c.keys[c.keys == -1] = 1
     keep = np.setdiff1d(np.arange(vocab), out)
     c.b[out] = -np.inf
+    c.w[:, out[::2]] *= 1e30  # what no entry holds
     c.put()
     lse, row_loss, _ = c.forward()
     dx, dw, db = c.backward()
@@ -182,6 +184,42 @@ def test_masked_entries(hip, rows, vocab):
     close(dx, ref["dx"], tol["dx"], "dx")
     close(dw[:, keep], ref["dw"], tol["dw"], "dw")
     assert not dw[:, out].any() and not db[out].any()
+
+
+@pytest.mark.parametrize("rows,vocab", [(40, 300), (1030, 3000)])
+@pytest.mark.parametrize("size", [1.0, 60.0, 2.0 ** -30])
+def test_rows_outside_have_their_log_sum(hip, rows, vocab, size):
+    """Ordinary values there, other than the rest's: lse is theirs.  Some features are
+    zero in every row that takes part."""
+    c = Case(hip, rows, 64, vocab, ignored=0.4)
+    c.x[~c.valid()] *= np.float32(size)
+    c.x[np.ix_(c.valid(), np.arange(5))] = 0
+    c.put()
+    ref, tol = c.exact()
+    close(c.forward()[0], ref["lse"], tol["lse"], "lse")
+    dx, dw, db = c.backward()
+    for name, got in (("dx", dx), ("dw", dw), ("db", db)):
+        close(got, ref[name], tol[name], name)
+
+
+@pytest.mark.parametrize("rows,vocab", [(30, 200), (1000, 3100)])
+def test_unaligned_buffers(hip, rows, vocab):
+    """Every float buffer begins 4 bytes past an aligned address."""
+    c = Case(hip, rows, 36, vocab)
+    c.put()
+    ref, tol = c.exact()
+    B = hip.Buffer
+    off = lambda a: B.from_array(np.concatenate([np.zeros(1, np.float32), a.reshape(-1).astype(np.float32)]))  # noqa: E731
+    gx, gw, gb = off(c.x), off(c.w), off(c.b)
+    out = {k: off(np.zeros(n)) for k, n in (("lse", rows), ("row_loss", rows), ("loss", 1), ("dx", rows * 36),
+                                            ("dw", 36 * vocab), ("db", vocab))}
+    p = {k: v.ptr + 4 for k, v in out.items()}
+    shape = (rows, 36, vocab, gx.ptr + 4, 36, gw.ptr + 4, vocab, gb.ptr + 4, c.gk.ptr, rows, rows)
+    hip.call("mle_vocab_xent_fwd", None, *shape, c.scale, p["lse"], p["row_loss"], p["loss"], c.ws.ptr, c.ws.nbytes)
+    hip.call("mle_vocab_xent_bwd", None, *shape, p["lse"], None, c.scale, p["dx"], 36, 0, p["dw"], vocab, p["db"], 0, c.ws.ptr,
+             c.ws.nbytes)
+    for k, v in out.items():
+        close(v.numpy()[1:], np.asarray(ref[k]).reshape(-1), np.asarray(tol[k]).reshape(-1), k)
 
 
 @pytest.mark.parametrize("rows,vocab", [(20, 300), (1030, 3000)])
