@@ -159,6 +159,8 @@ struct AmaxArgs {
   unsigned* xpart;                    // [2][slabs][d]: of rows that take part, of the others
   unsigned* wpart;                    // [pieces][chunks][d]
   int padded, kblocks;                // rows: blocks of 256
+  int xvec;                           // rows of X four at a time
+  unsigned* done;                     // workgroups that have finished a later sum: 0
   const float* lse;                   // backward
   int* key;
   float* z;
@@ -170,9 +172,11 @@ struct AmaxArgs {
 // backward, its log-sum; padded rows take no part.
 __global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a, Rows rows) {
   __shared__ unsigned red[kFeatures][NT / 64];
+  __shared__ __attribute__((aligned(16))) unsigned part[2 * 4 * NT];
   const int tid = threadIdx.x;
   if ((int)blockIdx.x < a.kblocks) {
     const int r = blockIdx.x * NT + tid;
+    if (r == 0) *a.done = 0;
     if (r >= a.padded) return;
     a.key[r] = r < a.rows ? rows.key(r) : -1;
     if (a.lse) a.z[r] = r < a.rows ? a.lse[r] : 0.f;
@@ -180,25 +184,47 @@ __global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a, Rows rows) {
   }
   const int bx = blockIdx.x - a.kblocks;
   if (bx < a.xblocks) {
-    const int tiles = (a.d + NT - 1) / NT;
-    const int slab = bx / tiles, k = (bx % tiles) * NT + tid;
+    // 256 features of a slab: four to a lane, a quarter of the rows to a wave
+    const int tiles = (a.d + NT - 1) / NT, lane = tid & 63, wave = tid >> 6;
+    const int slab = bx / tiles, k = (bx % tiles) * NT + 4 * lane;
     const int r0 = slab * a.slab_rows, n = min(a.rows - r0, a.slab_rows);
-    unsigned m = 0, other = 0;
-    const float* x = a.X + (int64_t)r0 * a.ldx + min(k, a.d - 1);
-    for (int b0 = 0; b0 < n; b0 += 64) {
-      const int lane = tid & 63;
-      const unsigned long long live = __ballot(b0 + lane < n && rows.key(r0 + min(b0 + lane, n - 1)) >= 0);
-      const int nb = min(n - b0, 64);
-#pragma unroll 16
+    const int at = min(k, max(a.d - 4, 0)), per = (n + 3) / 4, b1 = min(n, (wave + 1) * per);
+    unsigned m[4] = {}, other[4] = {};
+    for (int b0 = wave * per; b0 < b1; b0 += 64) {
+      const unsigned long long live = __ballot(b0 + lane < b1 && rows.key(r0 + min(b0 + lane, n - 1)) >= 0);
+      const float* x = a.X + (int64_t)(r0 + b0) * a.ldx + at;
+      const int nb = min(b1 - b0, 64);
+#pragma unroll 8
       for (int r = 0; r < nb; ++r) {
-        const unsigned b = finite_bits(x[(int64_t)(b0 + r) * a.ldx]), keep = (live >> r) & 1 ? 0xffffffffu : 0u;
-        m = max(m, b & keep);
-        other = max(other, b & ~keep);
+        f32x4 v;
+        if (a.xvec) v = *reinterpret_cast<const f32x4*>(x + (int64_t)r * a.ldx);
+        else v = f32x4{x[(int64_t)r * a.ldx], x[(int64_t)r * a.ldx + min(1, a.d - 1)], x[(int64_t)r * a.ldx + min(2, a.d - 1)],
+                       x[(int64_t)r * a.ldx + min(3, a.d - 1)]};
+        const unsigned keep = (live >> r) & 1 ? 0xffffffffu : 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m[j] = max(m[j], finite_bits(v[j]) & keep);
+          other[j] = max(other[j], finite_bits(v[j]) & ~keep);
+        }
       }
     }
-    if (k >= a.d) return;
-    a.xpart[(int64_t)slab * a.d + k] = m;
-    a.xpart[(int64_t)(a.slabs + slab) * a.d + k] = other;
+    uint4* mine = reinterpret_cast<uint4*>(part) + tid;
+    mine[0] = make_uint4(m[0], m[1], m[2], m[3]);
+    mine[NT] = make_uint4(other[0], other[1], other[2], other[3]);
+    __syncthreads();
+    // thread c: feature c of the 256, its maxima over the waves
+    const int f = (bx % tiles) * NT + tid;
+    if (f >= a.d) return;
+    // (at the matrix's end a lane holds the last four features)
+    const int home = (tid >> 2) * 4 + (bx % tiles) * NT, shift = home - min(home, max(a.d - 4, 0)), j = (tid & 3) + shift;
+    unsigned w = 0, o = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w = max(w, part[(64 * i + (tid >> 2)) * 4 + j]);
+      o = max(o, part[4 * NT + (64 * i + (tid >> 2)) * 4 + j]);
+    }
+    a.xpart[(int64_t)slab * a.d + f] = w;
+    a.xpart[(int64_t)(a.slabs + slab) * a.d + f] = o;
     return;
   }
   const int fblocks = (a.d + kFeatures - 1) / kFeatures, b = bx - a.xblocks;
@@ -279,16 +305,19 @@ __global__ __launch_bounds__(1024) void xent_scales_kernel(AmaxArgs a, int* __re
 }
 
 // X as the logits' first operand and, in the backward, as dW's; a piece of W as the
-// logits' second and dX's.
-__global__ __launch_bounds__(256) void xent_pack_x_kernel(planes::PackArgs l, planes::PackArgs w) {
-  const int64_t b = blockIdx.x, n = l.rows_blocks();
-  if (b < n) planes::pack_rows<true, kLo>(l, b);
-  else planes::pack_cols<false, 0>(w, b - n);
-}
-__global__ __launch_bounds__(256) void xent_pack_w_kernel(planes::PackArgs l, planes::PackArgs x) {
-  const int64_t b = blockIdx.x, n = l.cols_blocks();
-  if (b < n) planes::pack_cols<true, kLo>(l, b);
-  else planes::pack_rows<false, kLo>(x, b - n);
+// logits' second and dX's.  Blocks of each, in that order.
+struct PackAll {
+  planes::PackArgs xl, xt, wl, wn;
+  unsigned nxl, nxt, nwl, nwn;
+};
+__global__ __launch_bounds__(256) void xent_pack_kernel(PackAll a) {
+  unsigned b = blockIdx.x;
+  if (b < a.nxl) return planes::pack_rows<true, kLo>(a.xl, b);
+  b -= a.nxl;
+  if (b < a.nxt) return planes::pack_cols<false, 0>(a.xt, b);
+  b -= a.nxt;
+  if (b < a.nwl) return planes::pack_cols<true, kLo>(a.wl, b);
+  planes::pack_rows<false, kLo>(a.wn, b - a.nwl);
 }
 
 struct TileArgs {
@@ -459,11 +488,13 @@ __global__ __launch_bounds__(S::NTH, 2) void xent_tile_kernel(TileArgs a) {
 }
 
 // lse and the row losses from the blocks' statistics, 64 rows to a workgroup whose
-// waves take every 16th block, and the sum of the workgroup's row losses.
+// waves take every 16th block, and the sum of the workgroup's row losses; the
+// workgroup that finishes last adds those up, in order.
 __global__ __launch_bounds__(1024) void xent_join_kernel(const float2* __restrict__ part, int blocks, int64_t padded, int nrows,
                                                          const float* __restrict__ target, const int* __restrict__ key,
                                                          float* __restrict__ lse, float* __restrict__ row_loss,
-                                                         double* __restrict__ sums) {
+                                                         double* __restrict__ sums, unsigned* __restrict__ done, float scale,
+                                                         float* __restrict__ loss, int add) {
   __shared__ float2 red[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int r = blockIdx.x * 64 + lane;  // (< padded)
@@ -498,15 +529,18 @@ __global__ __launch_bounds__(1024) void xent_join_kernel(const float2* __restric
     one = (double)v;
   }
   one = wave_sum(one);
-  if (lane == 0) sums[blockIdx.x] = one;
-}
-__global__ __launch_bounds__(NT) void xent_loss_kernel(const double* __restrict__ sums, int n, float scale,
-                                                       float* __restrict__ loss, int add) {
-  __shared__ double red[NT / 64];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += NT) s += sums[i];
-  s = block_sum<NT>(s, red);
-  if (threadIdx.x == 0) loss[0] = (float)(s * (double)scale) + (add ? loss[0] : 0.f);
+  unsigned before = 0;
+  if (lane == 0) {
+    __hip_atomic_store(&sums[blockIdx.x], one, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    before = __hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (__shfl(before, 0, 64) + 1 != gridDim.x) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  double total = 0.0;
+  for (unsigned i = lane; i < gridDim.x; i += 64)
+    total += __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  total = wave_sum(total);
+  if (lane == 0) loss[0] = (float)(total * (double)scale) + (add ? loss[0] : 0.f);
 }
 
 // What finishes a product: C (+)= 2^(exponent of its row or column) g sum.
@@ -605,40 +639,49 @@ __global__ __launch_bounds__(S::NTH, 2) void xent_products_kernel(ProductArgs w,
   else if (b >= start) xent_product<false>(x, b - start, lds);
 }
 
-// The splits' sums in order.
-__global__ __launch_bounds__(NT) void xent_reduce_kernel(ProductArgs a) {
+// The splits' sums in order: blocks [0, nw) of dW, then nx of dX.  The rest, after the
+// last piece: db (+)= g times the 64-row blocks' column sums, 64 columns to a
+// workgroup, whose waves take every fourth block; their sums in order.
+__device__ __forceinline__ void xent_reduce(const ProductArgs& a, unsigned block, unsigned blocks) {
   const int64_t ld = (int64_t)a.gx * kTile, total = (int64_t)a.out.rows * (ld / 4), step = (int64_t)a.gy * kTile * ld;
   const float g = a.out.g();
-  for (int64_t u = (int64_t)blockIdx.x * NT + threadIdx.x; u < total; u += (int64_t)gridDim.x * NT) {
+  for (int64_t u = (int64_t)block * NT + threadIdx.x; u < total; u += (int64_t)blocks * NT) {
     const int64_t row = u / (ld / 4);
     const int col = (int)(u - row * (ld / 4)) * 4;
     if (col >= a.out.cols) continue;
     const float* p = a.part + row * ld + col;
     f32x4 s = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 4
     for (int z = 1; z < a.splits; ++z) s += *reinterpret_cast<const f32x4*>(p + z * step);
     a.out.put(row, col, s, g);
   }
 }
-
-// db (+)= g times the 64-row blocks' column sums: 64 columns to a workgroup, whose
-// waves take every fourth block; their sums in order.
-__global__ __launch_bounds__(NT) void xent_db_kernel(const float* __restrict__ csum, int blocks, int64_t all, int vocab,
-                                                     float* __restrict__ db, int accumulate, float scale,
-                                                     const float* __restrict__ upstream) {
+struct BiasArgs {
+  const float* csum;
+  int blocks, vocab, accumulate;
+  int64_t all;
+  float* db;
+  float scale;
+  const float* upstream;
+};
+__global__ __launch_bounds__(NT) void xent_reduce_kernel(ProductArgs w, unsigned nw, ProductArgs x, unsigned nx, BiasArgs a) {
   __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+  const unsigned block = blockIdx.x;
+  if (block < nw) return xent_reduce(w, block, nw);
+  if (block < nw + nx) return xent_reduce(x, block - nw, nx);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (int)(block - nw - nx) * 64 + lane;
   float s = 0.f;
-  if (c < vocab) {
+  if (c < a.vocab) {
 #pragma unroll 8
-    for (int b = w; b < blocks; b += 4) s += csum[(int64_t)b * all + c];
+    for (int b = wave; b < a.blocks; b += 4) s += a.csum[(int64_t)b * a.all + c];
   }
-  red[w][lane] = s;
+  red[wave][lane] = s;
   __syncthreads();
-  if (w != 0 || c >= vocab) return;
+  if (wave != 0 || c >= a.vocab) return;
   s = ((red[0][lane] + red[1][lane]) + red[2][lane]) + red[3][lane];
-  s *= upstream ? upstream[0] * scale : scale;
-  db[c] = accumulate ? db[c] + s : s;
+  s *= a.upstream ? a.upstream[0] * a.scale : a.scale;
+  a.db[c] = a.accumulate ? a.db[c] + s : s;
 }
 
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -710,7 +753,7 @@ struct PlanePlan {
   int rows, d, vocab;
   int padded, dk, dp, piece, pieces, chunks, slabs, slab_rows;
   // offsets into the workspace
-  size_t xpart, wpart, ex, el, en, scale, key, z, target, sums, xl, wl;
+  size_t xpart, wpart, ex, el, en, scale, key, z, target, sums, done, xl, wl;
   size_t part;                                         // forward
   size_t xt, wn, prow, pcol, cfac, csum, wsplit, xsplit;  // backward, at the same place
   size_t total;
@@ -747,6 +790,7 @@ PlanePlan plane_plan(int all_rows, int d, int vocab) {
   p.z = take(padded * 4);
   p.target = take(padded * 4);
   p.sums = take(padded / 64 * 8);
+  p.done = take(4);
   p.xl = take(padded * p.dk * 32 * 4);
   p.wl = take(piece * p.dk * 32 * 4);
   const size_t both = at;
@@ -826,8 +870,8 @@ struct Chunk {
     return reinterpret_cast<T*>(ws + o);
   }
 
-  // Exponents, ids, and X packed (for dW too where `weights`).
-  void begin(const Rows& rw, const float* lse, bool weights) const {
+  // Exponents and ids.
+  void begin(const Rows& rw, const float* lse) const {
     AmaxArgs a{};
     a.X = X;
     a.ldx = ldx;
@@ -846,25 +890,32 @@ struct Chunk {
     a.padded = padded;
     a.kblocks = (padded + NT - 1) / NT;
     a.bias = bias;
+    a.xvec = aligned16(X) && ldx % 4 == 0 && p.d >= 4 && p.d % 4 == 0;
+    a.done = at<unsigned>(p.done);
     a.lse = lse;
     a.key = at<int>(p.key);
     a.z = at<float>(p.z);
     mle::launch(xent_amax_kernel, (unsigned)(a.kblocks + a.xblocks + p.pieces * p.chunks * ((p.d + kFeatures - 1) / kFeatures)), NT, 0, s, a, rw);
     mle::launch(xent_scales_kernel, (unsigned)p.pieces, 1024, 0, s, a, at<int>(p.ex), at<int>(p.el), at<int>(p.en), at<int>(p.scale));
-    const int vec = aligned16(X) && ldx % 4 == 0;
-    const planes::PackArgs l{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, nullptr, at(p.xl), vec};
-    const planes::PackArgs w{X, ldx, p.d, rows, p.dp / 16, padded / 32, at<int>(p.ex), at<int>(p.key), nullptr, at(p.xt), vec};
-    mle::launch(xent_pack_x_kernel, (unsigned)(l.rows_blocks() + (weights ? w.cols_blocks() : 0)), 256, 0, s, l, w);
   }
   int cols(int i) const { return std::min(p.piece, p.vocab - i * p.piece); }
   int pcols(int i) const { return (cols(i) + kTile - 1) / kTile * kTile; }
-  // Piece i of W for the logits, and for dX where `inputs`.
-  void pack_piece(int i, bool inputs) const {
+  // Piece i of W for the logits, and for dX where `inputs`; with the first piece, X for
+  // the logits, and for dW where `weights`.
+  void pack(int i, bool inputs, bool weights) const {
     const float* w = W + (int64_t)i * p.piece;
-    const int vec = aligned16(W) && ldw % 4 == 0;  // (pieces begin at multiples of 128)
-    const planes::PackArgs l{w, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d, nullptr, bias ? bias + (int64_t)i * p.piece : nullptr, at(p.wl), vec};
-    const planes::PackArgs x{w, ldw, p.d, cols(i), p.dp / 16, pcols(i) / 32, at<int>(p.en) + (int64_t)i * p.d, nullptr, bias ? bias + (int64_t)i * p.piece : nullptr, at(p.wn), vec};
-    mle::launch(xent_pack_w_kernel, (unsigned)(l.cols_blocks() + (inputs ? x.rows_blocks() : 0)), 256, 0, s, l, x);
+    const float* b = bias ? bias + (int64_t)i * p.piece : nullptr;
+    const int xvec = aligned16(X) && ldx % 4 == 0, wvec = aligned16(W) && ldw % 4 == 0;  // (pieces begin at multiples of 128)
+    PackAll a{{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, nullptr, at(p.xl), xvec},
+              {X, ldx, p.d, rows, p.dp / 16, padded / 32, at<int>(p.ex), at<int>(p.key), nullptr, at(p.xt), xvec},
+              {w, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d, nullptr, b, at(p.wl), wvec},
+              {w, ldw, p.d, cols(i), p.dp / 16, pcols(i) / 32, at<int>(p.en) + (int64_t)i * p.d, nullptr, b, at(p.wn), wvec},
+              0, 0, 0, 0};
+    a.nxl = i == 0 ? (unsigned)a.xl.rows_blocks() : 0u;
+    a.nxt = i == 0 && weights ? (unsigned)a.xt.cols_blocks() : 0u;
+    a.nwl = (unsigned)a.wl.cols_blocks();
+    a.nwn = inputs ? (unsigned)a.wn.rows_blocks() : 0u;
+    mle::launch(xent_pack_kernel, a.nxl + a.nxt + a.nwl + a.nwn, 256, 0, s, a);
   }
   Operand operand(size_t o, int padded_rows) const { return Operand{at(o), (int64_t)padded_rows / 16 * 2 * planes::kUnit}; }
   TileArgs tile(int i) const {
@@ -883,8 +934,9 @@ struct Chunk {
     a.pcols = pcols(i);
     return a;
   }
-  // The products of piece i; a null matrix leaves its product out.
-  void products(int i, OutArgs ow, OutArgs ox) const {
+  // The products of piece i, and what finishes them; a null matrix leaves its product
+  // out, a null db the bias gradient.
+  void products(int i, OutArgs ow, OutArgs ox, const BiasArgs& bias_grad) const {
     const PairSplit ps = pair_split(padded, p.dp, pcols(i), ow.C != nullptr, ox.C != nullptr);
     auto product = [&](Operand A, Operand B, int stages, int gx, int gy, Split sp, const OutArgs& out, size_t part) {
       ProductArgs a{};
@@ -909,9 +961,11 @@ struct Chunk {
                                   ps.x, ox, p.xsplit);
     const int start = (w.items + gemm::kXcds - 1) / gemm::kXcds * gemm::kXcds;  // (item 0 of dX on XCD 0 again)
     mle::launch(xent_products_kernel, (unsigned)(start + x.items), S::NTH, 0, s, w, x, start);
-    for (const ProductArgs& a : {w, x})
-      if (a.items && a.splits > 1)
-        mle::launch(xent_reduce_kernel, stream_grid((size_t)a.out.rows * a.gx * (kTile / 4), NT, 8192), NT, 0, s, a);
+    auto blocks = [](const ProductArgs& a) {
+      return a.items && a.splits > 1 ? stream_grid((size_t)a.out.rows * a.gx * (kTile / 4), NT, 4096) : 0u;
+    };
+    const unsigned nw = blocks(w), nx = blocks(x), nb = bias_grad.db ? (unsigned)((bias_grad.vocab + 63) / 64) : 0u;
+    if (nw + nx + nb) mle::launch(xent_reduce_kernel, nw + nx + nb, NT, 0, s, w, nw, x, nx, bias_grad);
   }
 };
 
@@ -929,10 +983,10 @@ int planes_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
   for (int r0 = 0; r0 < rows; r0 += p.rows) {
     const Chunk c = chunk_of(p, ws, s, r0, rows, X, ldx, W, ldw, bias);
     rw.r0 = r0;
-    c.begin(rw, nullptr, false);
+    c.begin(rw, nullptr);
     int blocks = 0;
     for (int i = 0; i < p.pieces; ++i) {
-      c.pack_piece(i, false);
+      c.pack(i, false, false);
       TileArgs a = c.tile(i);
       a.part = c.at<float2>(p.part) + (int64_t)blocks * c.padded;
       a.target = c.at<float>(p.target);
@@ -941,8 +995,8 @@ int planes_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
     }
     const int groups = c.padded / 64;
     mle::launch(xent_join_kernel, (unsigned)groups, 1024, 0, s, c.at<float2>(p.part), blocks, (int64_t)c.padded, c.rows,
-                c.at<float>(p.target), c.at<int>(p.key), lse + r0, row_loss ? row_loss + r0 : nullptr, c.at<double>(p.sums));
-    mle::launch(xent_loss_kernel, 1u, NT, 0, s, c.at<double>(p.sums), groups, loss_scale, loss, r0 > 0 ? 1 : 0);
+                c.at<float>(p.target), c.at<int>(p.key), lse + r0, row_loss ? row_loss + r0 : nullptr, c.at<double>(p.sums),
+                c.at<unsigned>(p.done), loss_scale, loss, r0 > 0 ? 1 : 0);
   }
   return check_launch("mle_vocab_xent_fwd");
 }
@@ -955,12 +1009,12 @@ int planes_bwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
   for (int r0 = 0; r0 < rows; r0 += p.rows) {
     const Chunk c = chunk_of(p, ws, s, r0, rows, X, ldx, W, ldw, bias);
     rw.r0 = r0;
-    c.begin(rw, lse + r0, dW != nullptr);
+    c.begin(rw, lse + r0);
     const int add = accumulate_dw || r0 > 0;
     const int64_t all = (int64_t)p.pieces * p.piece;
     for (int i = 0; i < p.pieces; ++i) {
       const int64_t v0 = (int64_t)i * p.piece;
-      c.pack_piece(i, dX != nullptr);
+      c.pack(i, dX != nullptr, dW != nullptr);
       TileArgs a = c.tile(i);
       a.lse = c.at<float>(p.z);
       a.prow = c.at(p.prow);
@@ -974,11 +1028,11 @@ int planes_bwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
       if (dX)
         ox = OutArgs{dX + (int64_t)r0 * lddx, lddx, c.rows, d, accumulate_dx || i > 0, c.at<int>(p.en) + (int64_t)i * d, 0, -kTop,
                      grad_scale, upstream, 0};
-      c.products(i, ow, ox);
+      BiasArgs bias_grad{};
+      if (db && i == p.pieces - 1)
+        bias_grad = BiasArgs{c.at<float>(p.csum), c.padded / 64, vocab, add, all, db, grad_scale, upstream};
+      c.products(i, ow, ox, bias_grad);
     }
-    if (db)
-      mle::launch(xent_db_kernel, (unsigned)((vocab + 63) / 64), NT, 0, s, c.at<float>(p.csum), c.padded / 64, all, vocab, db,
-                  add, grad_scale, upstream);
   }
   return check_launch("mle_vocab_xent_bwd");
 }
