@@ -58,31 +58,35 @@ struct RowState {
   float max, sum, target, pad;  // sum of exp(l - max)
 };
 
-// One row of a piece to a workgroup: its maximum and sum join the row's.
-__global__ __launch_bounds__(1024) void xent_stats_kernel(const float* __restrict__ l, int cols, int v0, Rows rows,
-                                                          RowState* __restrict__ state, int first) {
-  __shared__ float red[1024 / 64];
-  const int64_t r = blockIdx.x;
+// A row of a piece to L threads: its maximum and sum join the row's.  A wave to a row
+// of few columns (8192 x 300: 36 us with a workgroup to it, 5.6 so).
+template <int L>
+__global__ __launch_bounds__(L < NT ? NT : L) void xent_stats_kernel(const float* __restrict__ l, int nrows, int cols, int v0,
+                                                                     Rows rows, RowState* __restrict__ state, int first) {
+  __shared__ float red[L / 64];
+  const int64_t r = L < NT ? (int64_t)blockIdx.x * (NT / L) + threadIdx.x / L : blockIdx.x;
+  const int t = threadIdx.x % L;
+  if (r >= nrows) return;  // (a whole wave)
   const float* x = l + r * cols;
   float m = -FLT_MAX;
 #pragma unroll 4
-  for (int c = threadIdx.x; c < cols; c += 1024) m = fmaxf(m, x[c]);
-  m = block_max<1024>(m, red);
+  for (int c = t; c < cols; c += L) m = fmaxf(m, x[c]);
+  m = L == 64 ? wave_max(m) : block_max<L>(m, red);
   float s = 0.f;
 #pragma unroll 4
-  for (int c = threadIdx.x; c < cols; c += 1024) s += expf(x[c] - m);
-  s = block_sum<1024>(s, red);
-  if (threadIdx.x != 0) return;
-  RowState t{m, s, 0.f, 0.f};
+  for (int c = t; c < cols; c += L) s += expf(x[c] - m);
+  s = L == 64 ? wave_sum(s) : block_sum<L>(s, red);
+  if (t != 0) return;
+  RowState n{m, s, 0.f, 0.f};
   if (!first) {
     const RowState o = state[r];
-    t.max = fmaxf(o.max, m);
-    t.sum = o.sum * expf(o.max - t.max) + s * expf(m - t.max);
-    t.target = o.target;
+    n.max = fmaxf(o.max, m);
+    n.sum = o.sum * expf(o.max - n.max) + s * expf(m - n.max);
+    n.target = o.target;
   }
   const int k = rows.key(r);
-  if (k >= v0 && k < v0 + cols) t.target = x[k - v0];
-  state[r] = t;
+  if (k >= v0 && k < v0 + cols) n.target = x[k - v0];
+  state[r] = n;
 }
 
 // lse, the row losses and their scaled sum; one workgroup.
@@ -103,26 +107,58 @@ __global__ __launch_bounds__(1024) void xent_finish_kernel(const RowState* __res
   if (threadIdx.x == 0) loss[0] = (float)(sum * (double)scale) + (add ? loss[0] : 0.f);
 }
 
-// A piece's logits to P, in place: 1024 columns of a row to a workgroup.  Those past
-// the columns' take the rows of X that take part, the others as zeros, for dW: what
-// a row that takes no part holds, NaN included, must not reach it.
-__global__ __launch_bounds__(NT) void xent_grad_kernel(float* __restrict__ l, int cols, int v0, Rows rows,
+// A piece's logits to P, in place: 1024 of them, in the matrix's order, to a workgroup.
+// Those past the first `blocks` take the rows of X that take part, the others as zeros,
+// for dW: what a row that takes no part holds, NaN included, must not reach it.
+// db (nullable) is cleared for the product that adds to it.
+__global__ __launch_bounds__(NT) void xent_grad_kernel(float* l, int nrows, int cols, int v0, Rows rows,
                                                        const float* __restrict__ lse, const float* __restrict__ upstream,
-                                                       float scale, int blocks, const float* __restrict__ X, int64_t ldx,
-                                                       int d, float* __restrict__ out) {
-  const int64_t r = blockIdx.x;
-  const int k = rows.key(r);
-  if ((int)blockIdx.y >= blocks) {
-    for (int c = threadIdx.x; c < d; c += NT) out[r * d + c] = k >= 0 ? X[r * ldx + c] : 0.f;
-    return;
+                                                       float scale, unsigned blocks, const float* __restrict__ X, int64_t ldx,
+                                                       int d, float* __restrict__ out, float* __restrict__ db) {
+  const bool logits = blockIdx.x < blocks;
+  const unsigned n = logits ? cols : d;
+  const int64_t e0 = (int64_t)(logits ? blockIdx.x : blockIdx.x - blocks) * (4 * NT);
+  const int64_t r0 = e0 / n;
+  const unsigned c0 = (unsigned)(e0 - r0 * n);
+  const float g = upstream ? upstream[0] * scale : scale;
+  int key[4];
+  float x[4], z[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // (every load on its way before the first is used; past the end: the last row's)
+    const unsigned at = c0 + i * NT + threadIdx.x, down = at / n, c = at - down * n;
+    const int64_t r = min(r0 + down, (int64_t)nrows - 1);
+    key[i] = rows.key(r);
+    z[i] = logits ? lse[r] : 0.f;
+    x[i] = logits ? l[r * cols + c] : X[r * ldx + c];
   }
-  float* x = l + r * cols;
-  const float z = lse[r], g = upstream ? upstream[0] * scale : scale;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int c = (int)blockIdx.y * 4 * NT + i * NT + threadIdx.x;
-    if (c < cols) x[c] = k >= 0 ? g * (expf(x[c] - z) - (c + v0 == k ? 1.f : 0.f)) : 0.f;
+    const unsigned at = c0 + i * NT + threadIdx.x, down = at / n, c = at - down * n;
+    const int64_t r = r0 + down;
+    if (r >= nrows) continue;
+    if (logits) {
+      if (db && r == 0) db[v0 + c] = 0.f;
+      l[r * cols + c] = key[i] >= 0 ? g * (expf(x[i] - z[i]) - ((int)c + v0 == key[i] ? 1.f : 0.f)) : 0.f;
+    } else {
+      out[r * d + c] = key[i] >= 0 ? x[i] : 0.f;
+    }
   }
+}
+
+// dX (+)= the slices' sums in order, and the products of P's columns from `k0` on.
+__global__ __launch_bounds__(NT) void xent_slices_kernel(const float* __restrict__ part, int slices, int64_t total, int d,
+                                                         const float* __restrict__ P, int cols, int k0,
+                                                         const float* __restrict__ W, int64_t ldw, float* __restrict__ dX,
+                                                         int64_t lddx, int accumulate) {
+  const int64_t u = (int64_t)blockIdx.x * NT + threadIdx.x;
+  if (u >= total) return;
+  const int64_t r = u / d;
+  const int c = (int)(u - r * d);
+  float s = part[u];
+  for (int z = 1; z < slices; ++z) s += part[z * total + u];
+  for (int k = k0; k < cols; ++k) s = fmaf(P[r * cols + k], W[(int64_t)c * ldw + k], s);
+  float* p = dX + r * lddx + c;
+  *p = accumulate ? *p + s : s;
 }
 
 // ---------------------------------------------------------------- fp16 planes
@@ -690,10 +726,17 @@ size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 // Few rows: columns of a piece, and the workspace's parts.
 struct SmallPlan {
   int piece;
-  size_t logits, rows, state, gemm;  // bytes
-  size_t total() const { return logits + rows + state + gemm; }
+  size_t logits, rows, state, slices, gemm;  // bytes
+  size_t total() const { return logits + rows + state + slices + gemm; }
 };
 constexpr size_t kPieceBytes = (size_t)128 << 20;
+// dX of few rows and features over up to 4096 columns is a product that the library
+// leaves to one workgroup per 16 x 16 of it; it is cut into slices of about 1024
+// columns (64 x 256 over 4096: 18 -> 10.3 us with their sum).
+int dx_slices(int rows, int d, int n) {
+  const int64_t tiles = (int64_t)((rows + 15) / 16) * ((d + 15) / 16);
+  return n >= 1536 && n <= 4096 && tiles <= 128 ? (n + 1023) / 1024 : 1;
+}
 SmallPlan small_plan(int rows, int d, int vocab) {
   SmallPlan p;
   const size_t cols = kPieceBytes / sizeof(float) / (size_t)rows / 256 * 256;
@@ -702,22 +745,29 @@ SmallPlan small_plan(int rows, int d, int vocab) {
   p.rows = round256((size_t)rows * d * sizeof(float));
   p.state = round256((size_t)rows * sizeof(RowState));
   const int last = vocab % p.piece ? vocab % p.piece : p.piece;
-  p.gemm = 0;
-  for (int v : {p.piece, last})
+  p.gemm = p.slices = 0;
+  for (int v : {p.piece, last}) {
+    const int n = dx_slices(rows, d, v);
+    if (n > 1) p.slices = std::max(p.slices, round256((size_t)n * rows * d * sizeof(float)));
     p.gemm = std::max(p.gemm, std::max(mle_gemm_ws_bytes(rows, v, d, 1),
                                        std::max(mle_gemm_ws_bytes(rows, d, v, 1), mle_gemm_ws_bytes(d, v, rows, 1))));
+  }
   if (p.piece == vocab) p.gemm = std::max(p.gemm, mle_linear_bwd_ws_bytes(rows, d, vocab, 1));
   p.gemm = round256(p.gemm);
   return p;
 }
 
-// Where the products of fp16 planes run: from 128 rows (a whole tile) and 3 M logits
-// up.  Below, their eight launches more cost what the faster products save (forward
-// and backward, planes against stored pieces, us: 512 x 256 -> 4096 96 / 98, 256 x
-// 1024 -> 8000 175 / 180, 1000 x 128 -> 1000 86 / 62, 64 x 1024 -> 32000 406 / 306;
-// above: 128 x 512 -> 32000 224 / 243, 512 x 1024 -> 8000 204 / 250, 8192 x 96 ->
-// 4000 251 / 375).
-bool use_planes(int rows, int vocab) { return rows >= kTile && (double)rows * vocab >= 3e6 && vocab <= (1 << 30); }
+// Where the products of fp16 planes run: from 192 rows (a tile and a half) and a size
+// whose faster products pay for three launches more and two passes over the operands.
+// Measured at both, forward and backward, planes against stored pieces, us:
+//   small  256 x 256 -> 4096 82 / 67, 1000 x 128 -> 1000 76 / 48, 512 x 1024 -> 2000
+//          131 / 109, 512 x 256 -> 4096 89 / 86, 1000 x 64 -> 2500 79 / 71
+//   large  1000 x 512 -> 2000 106 / 124, 512 x 1024 -> 4096 147 / 161, 1000 x 64 ->
+//          4000 81 / 87, 512 x 512 -> 8000 124 / 156, 8192 x 256 -> 1000 136 / 174
+//   rows   128 x 512 -> 32000 215 / 181, 256 x 64 -> 16000 81 / 79
+bool use_planes(int rows, int d, int vocab) {
+  return rows >= 192 && (double)rows * vocab * (900.0 + d) >= 2.8e9 && vocab <= (1 << 30);
+}
 
 // The two products of a piece share a grid of two workgroups to a CU.  A product
 // whose workgroups would each take more than 5/4 of a CU slot's share of the
@@ -831,7 +881,7 @@ int check(const char* who, int rows, int d, int vocab, const float* X, int64_t l
 }
 // The planes' launches number (feature, chunk of columns) pairs in 31 bits.
 int check_planes(const char* who, int rows, int d, int vocab) {
-  if (rows <= 0 || !use_planes(rows, vocab)) return MLE_OK;
+  if (rows <= 0 || !use_planes(rows, d, vocab)) return MLE_OK;
   const PlanePlan p = plane_plan(rows, d, vocab);
   if ((double)p.pieces * p.chunks * d >= 1073741824.0 || p.dk > (1 << 26))
     return set_error(MLE_ERR_UNSUPPORTED, "%s: d %d with a vocabulary of %d is too large", who, d, vocab);
@@ -844,7 +894,7 @@ int check_ws(const char* who, size_t need, const void* ws, size_t ws_bytes) {
 }
 
 size_t ws_need(int rows, int d, int vocab) {
-  return use_planes(rows, vocab) ? plane_plan(rows, d, vocab).total : small_plan(rows, d, vocab).total();
+  return use_planes(rows, d, vocab) ? plane_plan(rows, d, vocab).total : small_plan(rows, d, vocab).total();
 }
 
 #define TRY(call)                  \
@@ -1053,7 +1103,7 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
   if (rows == 0) return mle_fill(stream, loss, 0.f, 1);
   TRY(check_planes("mle_vocab_xent_fwd", rows, d, vocab));
   TRY(check_ws("mle_vocab_xent_fwd", ws_need(rows, d, vocab), ws, ws_bytes));
-  if (use_planes(rows, vocab))
+  if (use_planes(rows, d, vocab))
     return planes_fwd(stream, rows, d, vocab, X, ldx, W, ldw, bias, Rows{keys, clen, max_clen, vocab, 0}, loss_scale, lse,
                       row_loss, loss, ws);
   const SmallPlan p = small_plan(rows, d, vocab);
@@ -1061,12 +1111,15 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
   const Rows rw{keys, clen, max_clen, vocab, 0};
   float* l = static_cast<float*>(ws);
   RowState* state = reinterpret_cast<RowState*>(static_cast<char*>(ws) + p.logits + p.rows);
-  void* gws = reinterpret_cast<char*>(state) + p.state;
+  void* gws = reinterpret_cast<char*>(state) + p.state + p.slices;
   for (int v0 = 0; v0 < vocab; v0 += p.piece) {
     const int n = std::min(p.piece, vocab - v0);
     TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr,
                     bias ? bias + v0 : nullptr, gws, p.gemm));
-    mle::launch(xent_stats_kernel, (unsigned)rows, 1024, 0, s, l, n, v0, rw, state, v0 == 0 ? 1 : 0);
+    // (with many rows a wave to each is enough to fill the chip)
+    if (n <= 1024 || rows >= 2048)
+      mle::launch(xent_stats_kernel<64>, (unsigned)(((int64_t)rows + 3) / 4), NT, 0, s, l, rows, n, v0, rw, state, v0 == 0 ? 1 : 0);
+    else mle::launch(xent_stats_kernel<1024>, (unsigned)rows, 1024, 0, s, l, rows, n, v0, rw, state, v0 == 0 ? 1 : 0);
   }
   mle::launch(xent_finish_kernel, 1u, 1024, 0, s, state, rows, rw, loss_scale, lse, row_loss, loss, 0);
   return check_launch("mle_vocab_xent_fwd");
@@ -1083,7 +1136,7 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
   MLE_CHECK_ARG(dW || !db, "mle_vocab_xent_bwd: db without dW");
   TRY(check_planes("mle_vocab_xent_bwd", rows, d, vocab));
   if (rows > 0) TRY(check_ws("mle_vocab_xent_bwd", ws_need(rows, d, vocab), ws, ws_bytes));
-  if (rows > 0 && use_planes(rows, vocab))
+  if (rows > 0 && use_planes(rows, d, vocab))
     return !dX && !dW ? MLE_OK
                       : planes_bwd(stream, rows, d, vocab, X, ldx, W, ldw, bias, Rows{keys, clen, max_clen, vocab, 0}, lse,
                                    upstream, grad_scale, dX, lddx, accumulate_dx, dW, lddw, db, accumulate_dw, ws);
@@ -1100,23 +1153,33 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
   const Rows rw{keys, clen, max_clen, vocab, 0};
   float* l = static_cast<float*>(ws);
   float* xs = reinterpret_cast<float*>(static_cast<char*>(ws) + p.logits);
-  void* gws = static_cast<char*>(ws) + p.logits + p.rows + p.state;
+  float* part = reinterpret_cast<float*>(static_cast<char*>(ws) + p.logits + p.rows + p.state);
+  void* gws = reinterpret_cast<char*>(part) + p.slices;
   // The Linear backward's own launches where its matrices are dense.
-  const bool dense = dX && dW && p.piece == vocab && ldw == vocab && lddw == vocab && lddx == d;
-  if (db && !accumulate_dw && !dense) TRY(mle_fill(stream, db, 0.f, (size_t)vocab));
+  const bool dense = dX && dW && p.piece == vocab && dx_slices(rows, d, vocab) == 1 && ldw == vocab && lddw == vocab && lddx == d;
   for (int v0 = 0; v0 < vocab; v0 += p.piece) {
-    const int n = std::min(p.piece, vocab - v0), blocks = (n + 4 * NT - 1) / (4 * NT);
+    const int n = std::min(p.piece, vocab - v0), slices = dX ? dx_slices(rows, d, n) : 1;
+    auto groups = [&](int cols) { return (unsigned)(((int64_t)rows * cols + 4 * NT - 1) / (4 * NT)); };
     TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr,
                     bias ? bias + v0 : nullptr, gws, p.gemm));
-    mle::launch(xent_grad_kernel, dim3((unsigned)rows, (unsigned)(blocks + (dW && v0 == 0 ? 1 : 0))), NT, 0, s, l, n, v0, rw, lse,
-                upstream, grad_scale, blocks, X, ldx, d, xs);
+    mle::launch(xent_grad_kernel, groups(n) + (dW && v0 == 0 ? groups(d) : 0u), NT, 0, s, l, rows, n, v0, rw, lse, upstream,
+                grad_scale, groups(n), X, ldx, d, xs, db && !accumulate_dw && !dense ? db : nullptr);
     if (dense) {
       TRY(mle_linear_bwd_ex(stream, rows, d, vocab, 1, xs, l, 0, W, 0, dX, accumulate_dx, dW, db, 0, accumulate_dw, gws, p.gemm));
       break;
     }
-    if (dX)
-      TRY(mle_gemm_ex(stream, 0, 1, rows, d, n, 1.f, l, n, 0, W + v0, ldw, 0, accumulate_dx || v0 > 0 ? 1.f : 0.f, dX,
-                      lddx, 0, 1, nullptr, nullptr, gws, p.gemm));
+    const int acc = accumulate_dx || v0 > 0;
+    if (slices > 1) {
+      const int q = n / slices / 4 * 4;
+      const int64_t total = (int64_t)rows * d;
+      TRY(mle_gemm_ex(stream, 0, 1, rows, d, q, 1.f, l, n, q, W + v0, ldw, q, 0.f, part, d, total, slices, nullptr, nullptr, gws,
+                      p.gemm));
+      mle::launch(xent_slices_kernel, (unsigned)((total + NT - 1) / NT), NT, 0, s, part, slices, total, d, l, n, slices * q,
+                  W + v0, ldw, dX, lddx, acc);
+    } else if (dX) {
+      TRY(mle_gemm_ex(stream, 0, 1, rows, d, n, 1.f, l, n, 0, W + v0, ldw, 0, acc ? 1.f : 0.f, dX, lddx, 0, 1,
+                      nullptr, nullptr, gws, p.gemm));
+    }
     if (dW)
       TRY(mle_gemm_ex(stream, 1, 0, d, n, rows, 1.f, xs, d, 0, l, n, 0, accumulate_dw ? 1.f : 0.f, dW + v0, lddw, 0, 1,
                       db ? db + v0 : nullptr, nullptr, gws, p.gemm));
