@@ -513,7 +513,8 @@ int mle_softmax_xent_keys_fwd_rowstats_read(mle_stream stream, const float* logi
  * has no finite loss.  The logits are
  * formed in pieces of the vocabulary in ws, in the forward and again in the
  * backward; ws carries nothing from one call to the next.  fp32 accuracy; sums in
- * a fixed order.  X, W, dX and dW are buffers of their own.
+ * a fixed order.  X, W, dX and dW are buffers of their own; rows, d and vocab are at
+ * most 2^30.
  * The reference forms and keeps them (SoftMaxCrossEntropy, Engine/engine.cu:2064-2124). */
 size_t mle_vocab_xent_ws_bytes(int rows, int d, int vocab);
 int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W,
@@ -547,6 +548,7 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
  *                       products exactly.  fp32 accuracy, sums in a fixed order;
  *                       an infinity or NaN in dY makes its column of dW NaN, one
  *                       among the kept values its group's rows.  rows 0 assigns zeros.
+ *                       rows, in and out are at most 2^30, lddy below 2^24.
  * Rows of 16-byte (floats) and 8-byte (codes) alignment are read and written
  * whole; any others element by element.  dx may be dy's buffer, y may be x's. */
 int mle_q8_quantize(mle_stream stream, int rows, int cols, const float* x, int64_t ldx, int8_t* q, int64_t ldq,

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int NT = 256;
 constexpr int kMaxParts = 512;  // partial weight gradients: workgroups of the backward
+constexpr int kRowsOfLaunch = 1 << 21;  // of the forward: a launch has fewer than 2^32 threads
 
 struct NormArgs {
   int rows, cols;
@@ -255,11 +256,11 @@ __global__ __launch_bounds__(1024) void rmsnorm_join_kernel(const float* __restr
 // Workgroups of the backward, each with a partial weight gradient: a function of the shape alone.
 int parts_of(int rows, int cols) {
   const int rows_of_wg = cols <= 2048 ? 4 : 1;
-  return std::max(1, std::min(kMaxParts, (rows + rows_of_wg - 1) / rows_of_wg));
+  return std::max(1, std::min(kMaxParts, (rows - 1) / rows_of_wg + 1));
 }
 
 int check(const char* who, int rows, int cols) {
-  MLE_CHECK_ARG(rows >= 0 && cols > 0, "%s: bad shape %d x %d", who, rows, cols);
+  MLE_CHECK_ARG(rows >= 0 && cols > 0 && cols <= (1 << 30), "%s: bad shape %d x %d", who, rows, cols);
   return MLE_OK;
 }
 
@@ -278,17 +279,22 @@ int mle_add_rmsnorm_q8_fwd(mle_stream stream, int rows, int cols, const float* x
                 (long long)ldq, cols, (long long)lde, q8::groups(cols));
   MLE_CHECK_ARG(eps >= 0.f, "mle_add_rmsnorm_q8_fwd: eps %g", (double)eps);
   if (rows == 0) return MLE_OK;
-  NormArgs a{rows, cols, x, r, w, h, y, rstd, q, ldq, e, lde, eps, 0, 0};
-  a.vec = cols % 4 == 0 && aligned16(x) && aligned16(r) && aligned16(w) && aligned16(h) && aligned16(y);
-  a.vq = q && q8::codes_vec(q, ldq);
+  const bool vec = cols % 4 == 0 && aligned16(x) && aligned16(r) && aligned16(w) && aligned16(h) && aligned16(y);
+  const bool vq = q && q8::codes_vec(q, ldq);
   hipStream_t s = as_stream(stream);
-  const unsigned by4 = (unsigned)((rows + 3) / 4);
-  if (cols <= 512) mle::launch(rmsnorm_q8_fwd_kernel<64, 1>, by4, NT, 0, s, a);
-  else if (cols <= 1024) mle::launch(rmsnorm_q8_fwd_kernel<64, 2>, by4, NT, 0, s, a);
-  else if (cols <= 2048) mle::launch(rmsnorm_q8_fwd_kernel<64, 4>, by4, NT, 0, s, a);
-  else if (cols <= 4096) mle::launch(rmsnorm_q8_fwd_kernel<256, 2>, (unsigned)rows, NT, 0, s, a);
-  else if (cols <= 8192) mle::launch(rmsnorm_q8_fwd_kernel<256, 4>, (unsigned)rows, NT, 0, s, a);
-  else mle::launch(rmsnorm_q8_fwd_kernel<1024, 0>, (unsigned)rows, 1024, 0, s, a);
+  for (int64_t r0 = 0; r0 < rows; r0 += kRowsOfLaunch) {
+    const int n = (int)std::min<int64_t>(rows - r0, kRowsOfLaunch);
+    const int64_t at = r0 * cols;
+    const NormArgs a{n, cols, x + at, r ? r + at : r, w, h ? h + at : h, y ? y + at : y, rstd + r0, q ? q + r0 * ldq : q, ldq,
+                     e ? e + r0 * lde : e, lde, eps, vec, vq};
+    const unsigned by4 = (unsigned)((n + 3) / 4);
+    if (cols <= 512) mle::launch(rmsnorm_q8_fwd_kernel<64, 1>, by4, NT, 0, s, a);
+    else if (cols <= 1024) mle::launch(rmsnorm_q8_fwd_kernel<64, 2>, by4, NT, 0, s, a);
+    else if (cols <= 2048) mle::launch(rmsnorm_q8_fwd_kernel<64, 4>, by4, NT, 0, s, a);
+    else if (cols <= 4096) mle::launch(rmsnorm_q8_fwd_kernel<256, 2>, (unsigned)n, NT, 0, s, a);
+    else if (cols <= 8192) mle::launch(rmsnorm_q8_fwd_kernel<256, 4>, (unsigned)n, NT, 0, s, a);
+    else mle::launch(rmsnorm_q8_fwd_kernel<1024, 0>, (unsigned)n, 1024, 0, s, a);
+  }
   return check_launch("mle_add_rmsnorm_q8_fwd");
 }
 

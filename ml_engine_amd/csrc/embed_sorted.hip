@@ -343,7 +343,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(GradArgs a, int cw) {
 }
 
 int check(const char* who, int batch, int clen, int dim, int vocab) {
-  MLE_CHECK_ARG(batch >= 0 && clen > 0 && dim > 0 && vocab > 0, "%s: bad shape (batch %d, clen %d, dim %d, vocab %d)", who,
+  MLE_CHECK_ARG(batch >= 0 && clen > 0 && dim > 0 && dim <= (1 << 30) && vocab > 0 && vocab <= (1 << 30), "%s: bad shape (batch %d, clen %d, dim %d, vocab %d)", who,
                 batch, clen, dim, vocab);
   MLE_CHECK_ARG((long long)batch * clen < 2147483647LL - IX_CHUNK, "%s: too many tokens", who);
   return MLE_OK;
@@ -427,6 +427,8 @@ int mle_embed_sorted_grad(mle_stream stream, float* dtable, const float* dy, con
   int lw = 4;  // lanes of a table row: 16, 32 or 64
   while (lw < 6 && (1 << lw) < cols) ++lw;
   const int64_t waves = a.blocks + ((int64_t)vocab + (64 >> lw) - 1) / (64 >> lw);
+  if (waves >= (1 << 26) || a.blocks >= (1 << 22))  // (a launch has fewer than 2^32 threads)
+    return set_error(MLE_ERR_UNSUPPORTED, "mle_embed_sorted_grad: %d tokens or a table of %d rows are too many", ntok, vocab);
   hipStream_t s = as_stream(stream);
   const unsigned grid = (unsigned)((waves + 3) / 4);
   if (vec) mle::launch(embed_grad_kernel<true>, grid, 256, 0, s, a, lw);

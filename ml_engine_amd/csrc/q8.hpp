@@ -20,7 +20,7 @@ namespace q8 {
 
 constexpr int kGroup = 32;
 
-inline int groups(int cols) { return (cols + kGroup - 1) / kGroup; }
+inline int groups(int cols) { return cols / kGroup + (cols % kGroup != 0); }
 
 // The value of a group's step.
 __device__ __forceinline__ float step_of(unsigned e) { return __builtin_bit_cast(float, e << 23); }
@@ -122,7 +122,7 @@ __device__ __forceinline__ void store_row8(float* __restrict__ p, const float (&
 }
 
 inline int check_shape(const char* who, int rows, int cols, const void* q, int64_t ldq, const void* e, int64_t lde) {
-  MLE_CHECK_ARG(rows >= 0 && cols > 0, "%s: bad shape %d x %d", who, rows, cols);
+  MLE_CHECK_ARG(rows >= 0 && cols > 0 && cols <= (1 << 30), "%s: bad shape %d x %d", who, rows, cols);
   MLE_CHECK_ARG(rows == 0 || (q && e), "%s: null pointer", who);
   MLE_CHECK_ARG(ldq >= cols && lde >= groups(cols), "%s: ldq %lld < %d or lde %lld < %d", who, (long long)ldq, cols,
                 (long long)lde, groups(cols));

@@ -294,6 +294,7 @@ __global__ __launch_bounds__(256) void q8_wgrad_join_kernel(WgradArgs a, unsigne
 // splits as make one workgroup to a CU of the large, two of the small, of at
 // least 8 and 4 stages, and no more than pay for their partial sums (a stage
 // takes about 1 us, a byte written and read again 0.5 ps).
+constexpr int kMost = 1 << 30;  // rows, in, out
 struct WgradPlan {
   bool large;
   int gx, gy, splits, per;
@@ -321,7 +322,7 @@ WgradPlan wgrad_plan(int rows, int in, int out) {
 extern "C" {
 
 size_t mle_q8_linear_wgrad_ws_bytes(int rows, int in, int out) {
-  return rows <= 0 || in <= 0 || out <= 0 ? 0 : std::max<size_t>(wgrad_plan(rows, in, out).bytes, 16);
+  return rows <= 0 || in <= 0 || out <= 0 || rows > kMost || in > kMost || out > kMost ? 0 : std::max<size_t>(wgrad_plan(rows, in, out).bytes, 16);
 }
 
 int mle_q8_linear_wgrad(mle_stream stream, int rows, int in, int out, const int8_t* q, int64_t ldq, const uint8_t* e,
@@ -329,8 +330,9 @@ int mle_q8_linear_wgrad(mle_stream stream, int rows, int in, int out, const int8
                         void* ws, size_t ws_bytes) {
   const int rc = q8::check_shape("mle_q8_linear_wgrad", rows, in, q, ldq, e, lde);
   if (rc) return rc;
-  MLE_CHECK_ARG(out > 0 && dW && (dY || rows == 0) && lddy >= out && lddw >= out,
-                "mle_q8_linear_wgrad: bad argument (out %d, lddy %lld, lddw %lld)", out, (long long)lddy, (long long)lddw);
+  MLE_CHECK_ARG(rows <= kMost && out > 0 && out <= kMost && dW && (dY || rows == 0) && lddy >= out && lddw >= out,
+                "mle_q8_linear_wgrad: bad argument (rows %d, out %d, lddy %lld, lddw %lld)", rows, out, (long long)lddy,
+                (long long)lddw);
   // a stage's 32 rows lie within the 31-bit offsets of buffer loads
   if (lddy > 0xffffff) return set_error(MLE_ERR_UNSUPPORTED, "mle_q8_linear_wgrad: lddy %lld above 2^24", (long long)lddy);
   if (rows == 0) {
@@ -346,7 +348,7 @@ int mle_q8_linear_wgrad(mle_stream stream, int rows, int in, int out, const int8
   if (need && (!ws || !aligned16(ws) || ws_bytes < need))
     return set_error(MLE_ERR_WORKSPACE, "mle_q8_linear_wgrad: workspace of %zu bytes, 16-byte aligned, needed", need);
   const WgradPlan p = wgrad_plan(rows, in, out);
-  MLE_CHECK_ARG((int64_t)p.gx * p.gy * p.splits < (1LL << 30), "mle_q8_linear_wgrad: grid too large");
+  MLE_CHECK_ARG((int64_t)p.gx * p.gy * p.splits * (p.large ? 512 : 256) < (1LL << 32), "mle_q8_linear_wgrad: grid too large");
   WgradArgs a{q, ldq, e, lde, dY, lddy, dW, lddw, db, rows, in, out, accumulate, p.gx, p.gy, p.splits, p.per,
               static_cast<float*>(ws), 0};
   a.vec = out % 4 == 0 && lddw % 4 == 0 && aligned16(dW);

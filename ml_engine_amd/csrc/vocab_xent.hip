@@ -720,6 +720,7 @@ __global__ __launch_bounds__(NT) void xent_reduce_kernel(ProductArgs w, unsigned
   a.db[c] = a.accumulate ? a.db[c] + s : s;
 }
 
+constexpr int kMost = 1 << 30;  // rows, d, vocab
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // ----------------------------------------------------------------------- plans
@@ -766,7 +767,7 @@ SmallPlan small_plan(int rows, int d, int vocab) {
 //          4000 81 / 87, 512 x 512 -> 8000 124 / 156, 8192 x 256 -> 1000 136 / 174
 //   rows   128 x 512 -> 32000 215 / 181, 256 x 64 -> 16000 81 / 79
 bool use_planes(int rows, int d, int vocab) {
-  return rows >= 192 && (double)rows * vocab * (900.0 + d) >= 2.8e9 && vocab <= (1 << 30);
+  return rows >= 192 && (double)rows * vocab * (900.0 + d) >= 2.8e9;
 }
 
 // The two products of a piece share a grid of two workgroups to a CU.  A product
@@ -872,7 +873,7 @@ PlanePlan plane_plan(int all_rows, int d, int vocab) {
 
 int check(const char* who, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W, int64_t ldw,
           const int32_t* keys, int clen, int max_clen) {
-  MLE_CHECK_ARG(rows >= 0 && d > 0 && vocab > 0, "%s: bad shape (rows %d, d %d, vocab %d)", who, rows, d, vocab);
+  MLE_CHECK_ARG(rows >= 0 && d > 0 && vocab > 0 && rows <= kMost && d <= kMost && vocab <= kMost, "%s: bad shape (rows %d, d %d, vocab %d)", who, rows, d, vocab);
   MLE_CHECK_ARG(W && (rows == 0 || (X && keys)), "%s: null pointer", who);
   MLE_CHECK_ARG(ldx >= d && ldw >= vocab, "%s: ldx %lld < %d or ldw %lld < %d", who, (long long)ldx, d, (long long)ldw,
                 vocab);
@@ -1092,7 +1093,7 @@ int planes_bwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
 extern "C" {
 
 size_t mle_vocab_xent_ws_bytes(int rows, int d, int vocab) {
-  return rows <= 0 || d <= 0 || vocab <= 0 ? 0 : ws_need(rows, d, vocab);
+  return rows <= 0 || d <= 0 || vocab <= 0 || rows > kMost || d > kMost || vocab > kMost ? 0 : ws_need(rows, d, vocab);
 }
 
 int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W,

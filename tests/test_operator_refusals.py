@@ -8,11 +8,12 @@ import pytest
 from ml_engine_amd import hip
 
 A = 1 << 20  # an aligned address
+BIG = (1 << 30) + 1
 
 
 def refused(match, name, *args):
     rc = getattr(hip.lib(), name)(*args)
-    assert rc in (-1, -5), (name, rc)
+    assert rc in (-1, -4, -5), (name, rc)  # argument, unsupported size, workspace
     message = hip.lib().mle_last_error().decode()
     assert re.search(match, message), message
 
@@ -40,12 +41,14 @@ EMBED_BWD = dict(stream=None, dtable=A, dy=A, index=A, index_bytes=1 << 40, batc
 CASES = [
     ("mle_vocab_xent_fwd", XENT_FWD, [dict(rows=-1), dict(d=0), dict(vocab=0), dict(X=None), dict(W=None), dict(keys=None),
                                       dict(ldx=15), dict(ldw=31), dict(clen=0), dict(max_clen=7), dict(lse=None),
-                                      dict(loss=None), dict(ws=None), dict(ws=A + 4), dict(ws_bytes=64)]),
+                                      dict(loss=None), dict(ws=None), dict(ws=A + 4), dict(ws_bytes=64),
+                                      dict(rows=BIG), dict(d=BIG, ldx=BIG), dict(vocab=BIG, ldw=BIG)]),
     ("mle_vocab_xent_bwd", XENT_BWD, [dict(rows=-1), dict(X=None), dict(W=None), dict(keys=None), dict(lse=None),
                                       dict(lddx=15), dict(lddw=31), dict(dW=None), dict(ws=None), dict(ws=A + 8),
-                                      dict(ws_bytes=64), dict(max_clen=7)]),
+                                      dict(ws_bytes=64), dict(max_clen=7), dict(rows=BIG), dict(d=BIG, ldx=BIG, lddx=BIG),
+                                      dict(vocab=BIG, ldw=BIG, lddw=BIG)]),
     ("mle_q8_quantize", QUANT, [dict(rows=-1), dict(cols=0), dict(x=None), dict(q=None), dict(e=None), dict(ldx=39),
-                                dict(ldq=39), dict(lde=1)]),
+                                dict(ldq=39), dict(lde=1), dict(cols=BIG, ldx=BIG, ldq=BIG, lde=BIG)]),
     ("mle_q8_dequantize", DEQUANT, [dict(rows=-1), dict(cols=-3), dict(y=None), dict(q=None), dict(e=None), dict(ldy=39),
                                     dict(ldq=39), dict(lde=1)]),
     ("mle_q8_act_fwd", ACT_FWD, [dict(kind=-1), dict(kind=6), dict(x=None), dict(y=None), dict(q=None), dict(ldx=39),
@@ -54,19 +57,22 @@ CASES = [
                                  dict(lddx=39), dict(ldq=39)]),
     ("mle_q8_linear_wgrad", WGRAD, [dict(rows=-1), dict(inp=0), dict(out=0), dict(q=None), dict(e=None), dict(dY=None),
                                     dict(dW=None), dict(ldq=39), dict(lde=1), dict(lddy=23), dict(lddw=23), dict(ws=None),
-                                    dict(ws=A + 4), dict(ws_bytes=64)]),
+                                    dict(ws=A + 4), dict(ws_bytes=64), dict(rows=BIG),
+                                    dict(inp=BIG, ldq=BIG, lde=BIG), dict(out=BIG, lddw=BIG), dict(lddy=1 << 24)]),
     ("mle_add_rmsnorm_q8_fwd", NORM_FWD, [dict(rows=-1), dict(cols=0), dict(x=None), dict(rstd=None), dict(q=None),
                                           dict(e=None), dict(ldq=39), dict(lde=1), dict(eps=-1.0),
-                                          dict(eps=float("nan"))]),
+                                          dict(eps=float("nan")), dict(cols=BIG, ldq=BIG, lde=BIG)]),
     ("mle_add_rmsnorm_bwd", NORM_BWD, [dict(rows=-1), dict(cols=0), dict(h=None), dict(rstd=None), dict(dy=None),
-                                       dict(dh=None), dict(ws=None), dict(ws=A + 4), dict(ws_bytes=64)]),
+                                       dict(dh=None), dict(ws=None), dict(ws=A + 4), dict(ws_bytes=64), dict(cols=BIG)]),
     ("mle_embed_scaled_fwd", EMBED_FWD, [dict(batch=-1), dict(clen=0), dict(max_clen=3), dict(dim=0), dict(vocab=0),
                                          dict(out=None), dict(table=None), dict(keys=None), dict(index=A + 4),
-                                         dict(index_bytes=64), dict(batch=1 << 20, clen=1 << 11, max_clen=1 << 11)]),
+                                         dict(index_bytes=64), dict(batch=1 << 20, clen=1 << 11, max_clen=1 << 11),
+                                         dict(dim=BIG), dict(vocab=BIG)]),
     ("mle_embed_sorted_grad", EMBED_BWD, [dict(batch=-1), dict(clen=0), dict(dim=0), dict(vocab=0), dict(dtable=None),
                                           dict(dy=None), dict(index=None), dict(index=A + 4), dict(index_bytes=64),
                                           dict(ws=None), dict(ws=A + 8), dict(ws_bytes=64),
-                                          dict(batch=1 << 20, clen=1 << 11)]),
+                                          dict(batch=1 << 20, clen=1 << 11), dict(batch=1 << 20, clen=64),
+                                          dict(vocab=1 << 30), dict(dim=BIG), dict(vocab=BIG)]),
 ]
 
 
