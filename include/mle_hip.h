@@ -549,8 +549,7 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
  *                       an infinity or NaN in dY makes its column of dW NaN, one
  *                       among the kept values its group's rows.  rows 0 assigns zeros.
  *                       rows, in and out are at most 2^30, lddy below 2^24.
- * Rows of 16-byte (floats) and 8-byte (codes) alignment are read and written
- * whole; any others element by element.  dx may be dy's buffer, y may be x's. */
+ * Rows may begin at any float and any byte.  dx may be dy's buffer, y may be x's. */
 int mle_q8_quantize(mle_stream stream, int rows, int cols, const float* x, int64_t ldx, int8_t* q, int64_t ldq,
                     uint8_t* e, int64_t lde);
 int mle_q8_dequantize(mle_stream stream, int rows, int cols, const int8_t* q, int64_t ldq, const uint8_t* e,

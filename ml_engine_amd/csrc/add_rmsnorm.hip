@@ -35,7 +35,6 @@ struct NormArgs {
   uint8_t* e;
   int64_t lde;
   float eps;
-  int vec, vq;
 };
 
 struct NormBwdArgs {
@@ -48,7 +47,6 @@ struct NormBwdArgs {
   float* dh;
   int acc_dh;
   float* part;  // [workgroups][cols]; null: no weight gradient
-  int vec;
 };
 
 // The sum of v over a row's T threads, in every one of them.
@@ -84,10 +82,10 @@ __global__ __launch_bounds__(T < NT ? NT : T) void rmsnorm_q8_fwd_kernel(NormArg
       for (int j = 0; j < 8; ++j) h[j] = 0.f;
       continue;
     }
-    q8::load_row8(a.x + base + col, n, a.vec, h);
+    q8::load_row8(a.x + base + col, n, h);
     if (a.r) {
       float r[8];
-      q8::load_row8(a.r + base + col, n, a.vec, r);
+      q8::load_row8(a.r + base + col, n, r);
 #pragma unroll
       for (int j = 0; j < 8; ++j) h[j] += r[j];
     }
@@ -103,27 +101,27 @@ __global__ __launch_bounds__(T < NT ? NT : T) void rmsnorm_q8_fwd_kernel(NormArg
     const int col = (c * T + t) * 8, n = min(max(a.cols - col, 0), 8);
     if ((c * T + (t & ~3)) * 8 >= a.cols) continue;  // no value of this quad's group
     if (C == 0) {
-      q8::load_row8(a.x + base + col, n, a.vec, h);
+      q8::load_row8(a.x + base + col, n, h);
       if (a.r) {
         float r[8];
-        q8::load_row8(a.r + base + col, n, a.vec, r);
+        q8::load_row8(a.r + base + col, n, r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[j] += r[j];
       }
     }
-    if (a.h) q8::store_row8(a.h + base + col, h, n, a.vec);
+    if (a.h) q8::store_row8(a.h + base + col, h, n);
     float y[8], w[8];
-    if (a.w) q8::load_row8(a.w + col, n, a.vec, w);
+    if (a.w) q8::load_row8(a.w + col, n, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const double u = (double)h[j] * rstd;
       y[j] = j < n ? (float)(a.w ? u * (double)w[j] : u) : 0.f;
     }
-    if (a.y) q8::store_row8(a.y + base + col, y, n, a.vec);
+    if (a.y) q8::store_row8(a.y + base + col, y, n);
     if (a.q) {
       uint2 code;
       const unsigned e = q8::quantize8(y, code);
-      q8::store_codes(a.q + row * a.ldq + col, code, n, a.vq);
+      q8::store_codes(a.q + row * a.ldq + col, code, n);
       if ((t & 3) == 0) a.e[row * a.lde + col / q8::kGroup] = (uint8_t)e;
     }
   }
@@ -144,7 +142,7 @@ __global__ __launch_bounds__(T < NT ? NT : T) void rmsnorm_bwd_kernel(NormBwdArg
     const int col = (c * T + t) * 8, n = min(max(a.cols - col, 0), 8);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[c][j] = 0.f, w[c][j] = 1.f;
-    if (a.w && n > 0) q8::load_row8(a.w + col, n, a.vec, w[c]);
+    if (a.w && n > 0) q8::load_row8(a.w + col, n, w[c]);
   }
   for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.rows; r0 += (int64_t)gridDim.x * R) {
     const int64_t row = r0 + k;
@@ -161,8 +159,8 @@ __global__ __launch_bounds__(T < NT ? NT : T) void rmsnorm_bwd_kernel(NormBwdArg
         for (int j = 0; j < 8; ++j) u[c][j] = g[c][j] = 0.f;
         continue;
       }
-      q8::load_row8(a.h + base + col, n, a.vec, u[c]);
-      q8::load_row8(a.dy + base + col, n, a.vec, g[c]);
+      q8::load_row8(a.h + base + col, n, u[c]);
+      q8::load_row8(a.dy + base + col, n, g[c]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         u[c][j] *= rstd;
@@ -177,11 +175,11 @@ __global__ __launch_bounds__(T < NT ? NT : T) void rmsnorm_bwd_kernel(NormBwdArg
       const int col = (c * T + t) * 8, n = live ? min(max(a.cols - col, 0), 8) : 0;
       if (n == 0) continue;
       float old[8] = {}, dres[8] = {}, v[8];
-      if (a.dres) q8::load_row8(a.dres + base + col, n, a.vec, dres);
-      if (a.acc_dh) q8::load_row8(a.dh + base + col, n, a.vec, old);
+      if (a.dres) q8::load_row8(a.dres + base + col, n, dres);
+      if (a.acc_dh) q8::load_row8(a.dh + base + col, n, old);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = old[j] + (dres[j] + rstd * (g[c][j] - u[c][j] * m));
-      q8::store_row8(a.dh + base + col, v, n, a.vec);
+      q8::store_row8(a.dh + base + col, v, n);
     }
   }
   if (!a.part) return;
@@ -198,7 +196,7 @@ __global__ __launch_bounds__(T < NT ? NT : T) void rmsnorm_bwd_kernel(NormBwdArg
       for (int j = 0; j < 8; ++j)
         for (int i = 1; i < R; ++i) dw[c][j] += cols_red[8 * (i * T + t) + j];
     }
-    if (n > 0) q8::store_row8(a.part + (int64_t)blockIdx.x * a.cols + col, dw[c], n, a.vec);
+    if (n > 0) q8::store_row8(a.part + (int64_t)blockIdx.x * a.cols + col, dw[c], n);
   }
 }
 
@@ -279,14 +277,12 @@ int mle_add_rmsnorm_q8_fwd(mle_stream stream, int rows, int cols, const float* x
                 (long long)ldq, cols, (long long)lde, q8::groups(cols));
   MLE_CHECK_ARG(eps >= 0.f, "mle_add_rmsnorm_q8_fwd: eps %g", (double)eps);
   if (rows == 0) return MLE_OK;
-  const bool vec = cols % 4 == 0 && aligned16(x) && aligned16(r) && aligned16(w) && aligned16(h) && aligned16(y);
-  const bool vq = q && q8::codes_vec(q, ldq);
   hipStream_t s = as_stream(stream);
   for (int64_t r0 = 0; r0 < rows; r0 += kRowsOfLaunch) {
     const int n = (int)std::min<int64_t>(rows - r0, kRowsOfLaunch);
     const int64_t at = r0 * cols;
     const NormArgs a{n, cols, x + at, r ? r + at : r, w, h ? h + at : h, y ? y + at : y, rstd + r0, q ? q + r0 * ldq : q, ldq,
-                     e ? e + r0 * lde : e, lde, eps, vec, vq};
+                     e ? e + r0 * lde : e, lde, eps};
     const unsigned by4 = (unsigned)((n + 3) / 4);
     if (cols <= 512) mle::launch(rmsnorm_q8_fwd_kernel<64, 1>, by4, NT, 0, s, a);
     else if (cols <= 1024) mle::launch(rmsnorm_q8_fwd_kernel<64, 2>, by4, NT, 0, s, a);
@@ -314,8 +310,7 @@ int mle_add_rmsnorm_bwd(mle_stream stream, int rows, int cols, const float* h, c
     return set_error(MLE_ERR_WORKSPACE, "mle_add_rmsnorm_bwd: workspace of %zu bytes, 16-byte aligned, needed",
                      mle_add_rmsnorm_ws_bytes(rows, cols));
   const int parts = parts_of(rows, cols);
-  NormBwdArgs a{rows, cols, h, w, rstd, dy, dres, dh, accumulate_dh, dw ? static_cast<float*>(ws) : nullptr, 0};
-  a.vec = cols % 4 == 0 && aligned16(h) && aligned16(w) && aligned16(dy) && aligned16(dres) && aligned16(dh);
+  const NormBwdArgs a{rows, cols, h, w, rstd, dy, dres, dh, accumulate_dh, dw ? static_cast<float*>(ws) : nullptr};
   hipStream_t s = as_stream(stream);
   if (cols <= 512) mle::launch(rmsnorm_bwd_kernel<64, 1>, (unsigned)parts, NT, 0, s, a);
   else if (cols <= 1024) mle::launch(rmsnorm_bwd_kernel<64, 2>, (unsigned)parts, NT, 0, s, a);

@@ -9,6 +9,7 @@
 #include "../../include/mle_hip.h"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // in memory, at any float's address
 
 namespace mle {
 

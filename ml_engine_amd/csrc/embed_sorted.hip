@@ -25,6 +25,20 @@ constexpr int IX_CHUNK = 8192;  // tokens that it sorts at a time
 constexpr int HEAD = 64;
 constexpr int PART = 16;        // places of the list that one partial sum covers
 
+// A row in groups of W = 4 columns (VEC: rows of 4 columns or more, at any address of a
+// float) or of one.  The last group of 4 is the row's last four columns, some of which
+// belong to the group before it.
+template <bool VEC>
+struct Cols {
+  static constexpr int W = VEC ? 4 : 1;
+  typedef float vec __attribute__((ext_vector_type(W)));
+  typedef float mem __attribute__((ext_vector_type(W), aligned(4)));  // as it lies in memory
+  static __host__ __device__ int groups(int dim) { return (dim + W - 1) / W; }
+  static __device__ __forceinline__ int at(int c, int dim) { return VEC ? min(c * 4, dim - 4) : c; }
+  static __device__ __forceinline__ vec get(const float* p) { return *reinterpret_cast<const mem*>(p); }
+  static __device__ __forceinline__ void put(float* p, vec v) { *reinterpret_cast<mem*>(p) = v; }
+};
+
 struct IndexArgs {
   const int32_t* keys;
   int clen, max_clen, ntok, vocab, rows_per_wg, nix;
@@ -189,26 +203,28 @@ __global__ __launch_bounds__(IX_NT, 8) void embed_fwd_kernel(IndexArgs a, float*
     index_rows(a, blockIdx.x, lds);
     return;
   }
-  typedef float vec __attribute__((ext_vector_type(VEC ? 4 : 1)));
-  constexpr int W = VEC ? 4 : 1, UN = 4;
-  const U stride = (U)(gridDim.x - a.nix) * IX_NT, per = (U)(dim / W);
+  typedef Cols<VEC> C;
+  typedef typename C::vec vec;
+  constexpr int UN = 4;
+  const U stride = (U)(gridDim.x - a.nix) * IX_NT, per = (U)C::groups(dim);
   for (U u0 = (U)(blockIdx.x - a.nix) * IX_NT + threadIdx.x; u0 < units; u0 += UN * stride) {
     vec v[UN];
+    int64_t to[UN];
 #pragma unroll
     for (int k = 0; k < UN; ++k) {
       const U u = u0 + k * stride;
       v[k] = vec(0.f);
       if (u < units) {
         const U t = u / per;
-        const int key = key_of(a, (int)t);
-        if (key >= 0 && key < a.vocab)
-          v[k] = scale * *reinterpret_cast<const vec*>(table + (int64_t)key * dim + (int64_t)(u - t * per) * W);
+        const int key = key_of(a, (int)t), col = C::at((int)(u - t * per), dim);
+        to[k] = (int64_t)t * dim + col;
+        if (key >= 0 && key < a.vocab) v[k] = scale * C::get(table + (int64_t)key * dim + col);
       }
     }
 #pragma unroll
     for (int k = 0; k < UN; ++k) {
       const U u = u0 + k * stride;
-      if (u < units) *reinterpret_cast<vec*>(out + (int64_t)u * W) = v[k];
+      if (u < units) C::put(out + to[k], v[k]);  // (columns of two groups: twice the same)
     }
   }
 }
@@ -220,32 +236,41 @@ struct GradArgs {
   const int2* rinfo;
   const int32_t* list;
   const int32_t* skey;
-  float* part;  // [blocks][2][dim]
+  float* part;  // [blocks][2][groups of columns]
   int dim, vocab, accumulate, blocks;
   float scale;
 };
 
 // The sum of dy's rows list[at .. at + n), column group c, in order.
-template <typename vec>
-__device__ __forceinline__ vec sum_rows(const GradArgs& a, int at, int n, int c) {
-  constexpr int W = sizeof(vec) / 4;
+template <bool VEC>
+__device__ __forceinline__ typename Cols<VEC>::vec sum_rows(const GradArgs& a, int at, int n, int c) {
+  typedef typename Cols<VEC>::vec vec;
   vec s = vec(0.f);
-  const float* dy = a.dy + (int64_t)c * W;
+  const float* dy = a.dy + Cols<VEC>::at(c, a.dim);
   int j = 0;
   for (; j + 4 <= n; j += 4) {
     vec v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const vec*>(dy + (int64_t)a.list[at + j + k] * a.dim);
+    for (int k = 0; k < 4; ++k) v[k] = Cols<VEC>::get(dy + (int64_t)a.list[at + j + k] * a.dim);
 #pragma unroll
     for (int k = 0; k < 4; ++k) s += v[k];
   }
-  for (; j < n; ++j) s += *reinterpret_cast<const vec*>(dy + (int64_t)a.list[at + j] * a.dim);
+  for (; j < n; ++j) s += Cols<VEC>::get(dy + (int64_t)a.list[at + j] * a.dim);
   return s;
 }
-template <typename vec>
-__device__ __forceinline__ void put_row(const GradArgs& a, int row, int c, vec s) {
-  vec* p = reinterpret_cast<vec*>(a.dtable + (int64_t)row * a.dim + (int64_t)c * (sizeof(vec) / 4));
-  *p = a.accumulate ? *p + a.scale * s : a.scale * s;
+template <bool VEC>
+__device__ __forceinline__ void put_row(const GradArgs& a, int row, int c, typename Cols<VEC>::vec s) {
+  typedef Cols<VEC> C;
+  const int col = C::at(c, a.dim), shared = c * C::W - col;  // columns that the group before has
+  float* p = a.dtable + (int64_t)row * a.dim + col;
+  s *= a.scale;
+  if (shared == 0) {
+    C::put(p, a.accumulate ? C::get(p) + s : s);
+  } else {
+#pragma unroll
+    for (int k = 1; k < C::W; ++k)
+      if (k >= shared) p[k] = a.accumulate ? p[k] + s[k] : s[k];
+  }
 }
 
 // A token that occurs often would keep one wave busy for long, so a row with
@@ -257,9 +282,9 @@ __device__ __forceinline__ void put_row(const GradArgs& a, int row, int c, vec s
 // by all their lanes' columns.
 template <bool VEC>
 __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, int lw) {
-  typedef float vec __attribute__((ext_vector_type(VEC ? 4 : 1)));
+  typedef Cols<VEC> C;
   const int lane = threadIdx.x & 63;
-  const int cols = a.dim / (VEC ? 4 : 1);
+  const int cols = C::groups(a.dim);
   const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   if (w < a.blocks) {
     const int total = a.head[0], p0 = (int)w * PART, n = min(PART, total - p0);
@@ -283,7 +308,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, int lw) {
       const int row = __shfl(key, b, 64);
       const int len = __popcll(__ballot(lane < n && key == row));
       for (int c = lane; c < cols; c += 64)
-        *reinterpret_cast<vec*>(a.part + (w * 2 + slot) * a.dim + (int64_t)c * (VEC ? 4 : 1)) = sum_rows<vec>(a, p0 + b, len, c);
+        C::put(a.part + ((w * 2 + slot) * cols + c) * C::W, sum_rows<VEC>(a, p0 + b, len, c));
     }
     return;
   }
@@ -291,7 +316,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, int lw) {
   if (row >= a.vocab) return;
   const int2 info = a.rinfo[row];
   if (info.y > PART || (a.accumulate && info.y == 0)) return;
-  for (int c = lane & ((1 << lw) - 1); c < cols; c += 1 << lw) put_row<vec>(a, (int)row, c, sum_rows<vec>(a, info.x, info.y, c));
+  for (int c = lane & ((1 << lw) - 1); c < cols; c += 1 << lw) put_row<VEC>(a, (int)row, c, sum_rows<VEC>(a, info.x, info.y, c));
 }
 
 // One workgroup per block of the list: joins the row that begins in it, if it
@@ -299,8 +324,8 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(GradArgs a, int lw) {
 // of them take the row's blocks in turn, and their sums are added in order.
 template <bool VEC>
 __global__ __launch_bounds__(1024) void embed_join_kernel(GradArgs a, int cw) {
-  typedef float vec __attribute__((ext_vector_type(VEC ? 4 : 1)));
-  constexpr int W = VEC ? 4 : 1;
+  typedef Cols<VEC> C;
+  typedef typename C::vec vec;
   __shared__ vec red[1024];
   const int total = a.head[0], p0 = (int)blockIdx.x * PART, n = min(PART, total - p0);
   if (n <= 0) return;
@@ -311,7 +336,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(GradArgs a, int cw) {
   const int b = __ffsll((long long)begins) - 1;
   const int row = a.skey[p0 + b], count = __shfl(info.y, b, 64);
   const int nblk = (b + count + PART - 1) / PART;
-  const int cols = a.dim / W, groups = 1024 / cw, g = threadIdx.x / cw, t = threadIdx.x % cw;
+  const int cols = C::groups(a.dim), groups = 1024 / cw, g = threadIdx.x / cw, t = threadIdx.x % cw;
   const int per = (nblk + groups - 1) / groups;  // each group a run of blocks
   for (int c0 = 0; c0 < cols; c0 += cw) {
     const int c = c0 + t;
@@ -320,24 +345,23 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(GradArgs a, int cw) {
       const int k1 = min(nblk, (g + 1) * per);
       int k = g * per;
       auto at = [&](int i) {
-        return reinterpret_cast<const vec*>(a.part + (((int64_t)blockIdx.x + i) * 2 + (i == 0 && b > 0 ? 1 : 0)) * a.dim +
-                                            (int64_t)c * W);
+        return a.part + ((((int64_t)blockIdx.x + i) * 2 + (i == 0 && b > 0 ? 1 : 0)) * cols + c) * C::W;
       };
       for (; k + 4 <= k1; k += 4) {
         vec v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = *at(k + i);
+        for (int i = 0; i < 4; ++i) v[i] = C::get(at(k + i));
 #pragma unroll
         for (int i = 0; i < 4; ++i) s += v[i];
       }
-      for (; k < k1; ++k) s += *at(k);
+      for (; k < k1; ++k) s += C::get(at(k));
     }
     __syncthreads();
     red[threadIdx.x] = s;
     __syncthreads();
     if (g == 0 && c < cols) {
       for (int i = 1; i < groups; ++i) s += red[i * cw + t];
-      put_row<vec>(a, row, c, s);
+      put_row<VEC>(a, row, c, s);
     }
   }
 }
@@ -386,8 +410,8 @@ int mle_embed_scaled_fwd(mle_stream stream, float* out, const float* table, cons
     a.list = reinterpret_cast<int32_t*>(a.rinfo + vocab);
     a.skey = a.list + ntok;
   }
-  const bool vec = dim % 4 == 0 && aligned16(out) && aligned16(table);
-  const size_t units = (size_t)ntok * (dim / (vec ? 4 : 1));
+  const bool vec = dim >= 4;
+  const size_t units = (size_t)ntok * (vec ? Cols<true>::groups(dim) : dim);
   const unsigned grid = (unsigned)a.nix + (ntok ? stream_grid((units + 3) / 4, IX_NT, 2048) : 0u);
   hipStream_t s = as_stream(stream);
   // 32-bit numbering where the unrolled walk stays below 2^32
@@ -401,7 +425,7 @@ int mle_embed_scaled_fwd(mle_stream stream, float* out, const float* table, cons
 
 size_t mle_embed_sorted_grad_ws_bytes(int batch, int clen, int dim) {
   if (batch <= 0 || clen <= 0 || dim <= 0) return 0;
-  return round256(((size_t)batch * clen + PART - 1) / PART * 2 * dim * sizeof(float));
+  return round256(((size_t)batch * clen + PART - 1) / PART * 2 * (((size_t)dim + 3) / 4 * 4) * sizeof(float));
 }
 
 int mle_embed_sorted_grad(mle_stream stream, float* dtable, const float* dy, const void* index, size_t index_bytes,
@@ -422,8 +446,8 @@ int mle_embed_sorted_grad(mle_stream stream, float* dtable, const float* dy, con
   const int32_t* list = reinterpret_cast<const int32_t*>(rinfo + vocab);
   GradArgs a{dtable, dy, head, rinfo, list, list + ntok, static_cast<float*>(ws), dim, vocab, accumulate,
              (ntok + PART - 1) / PART, scale};
-  const bool vec = dim % 4 == 0 && aligned16(dtable) && aligned16(dy);
-  const int cols = dim / (vec ? 4 : 1);
+  const bool vec = dim >= 4;
+  const int cols = vec ? Cols<true>::groups(dim) : dim;
   int lw = 4;  // lanes of a table row: 16, 32 or 64
   while (lw < 6 && (1 << lw) < cols) ++lw;
   const int64_t waves = a.blocks + ((int64_t)vocab + (64 >> lw) - 1) / (64 >> lw);

@@ -214,7 +214,6 @@ struct PackArgs {
   const int* keys;
   const float* bias;
   char* out;
-  int vec;              // 16-byte loads
   // Blocks of 256 threads that pack it.
   __host__ __device__ int64_t rows_blocks() const { return ((int64_t)blocks * kblocks + 3) / 4; }
   __host__ __device__ int64_t cols_blocks() const { return ((int64_t)(blocks / 4) * kblocks + 3) / 4; }
@@ -233,8 +232,8 @@ __device__ __forceinline__ void pack_rows(const PackArgs& a, int64_t block) {
   int e[8];
   const int n = row < a.rows ? min(max(a.k - k, 0), 8) : 0;
   const float* p = a.src + (int64_t)row * a.ld + k;
-  if (a.vec && n == 8) {
-    const f32x4 v0 = reinterpret_cast<const f32x4*>(p)[0], v1 = reinterpret_cast<const f32x4*>(p)[1];
+  if (n == 8) {
+    const f32x4 v0 = reinterpret_cast<const f32x4u*>(p)[0], v1 = reinterpret_cast<const f32x4u*>(p)[1];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       x[j] = v0[j];
@@ -271,8 +270,8 @@ __device__ __forceinline__ void pack_cols(const PackArgs& a, int64_t block) {
     const bool live = k + j < a.k && (!a.keys || a.keys[k + j] >= 0);
     const float* p = a.src + (int64_t)(k + j) * a.ld + row;
     x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (live && a.vec && row + 3 < a.rows) {
-      x[j] = *reinterpret_cast<const f32x4*>(p);
+    if (live && row + 3 < a.rows) {
+      x[j] = *reinterpret_cast<const f32x4u*>(p);
     } else if (live) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)

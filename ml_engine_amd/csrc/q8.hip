@@ -29,7 +29,6 @@ struct Q8Args {
   float* dx;
   int64_t lddx;
   int accumulate;
-  int vx, vy, vq, vdx;  // rows of x, y, q, dx eight values at a time
 };
 
 // Calls f(row, column, values left of the row (0 .. 8), lane's place in the
@@ -50,16 +49,16 @@ template <int KIND>
 __global__ __launch_bounds__(NT) void q8_quantize_kernel(Q8Args a) {
   each_unit(a, [&](int64_t row, int col, int n) {
     float x[8];
-    load_row8(a.x + row * a.ldx + col, n, a.vx, x);
+    load_row8(a.x + row * a.ldx + col, n, x);
     uint2 code;
     const unsigned e = quantize8(x, code);
-    if (n > 0) store_codes(a.q + row * a.ldq + col, code, n, a.vq);
+    if (n > 0) store_codes(a.q + row * a.ldq + col, code, n);
     if ((threadIdx.x & 3) == 0) a.e[row * a.lde + col / q8::kGroup] = (uint8_t)e;
     if (KIND >= 0) {
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = act_f<KIND < 0 ? 0 : KIND>(x[j]);
-      if (n > 0) store_row8(a.y + row * a.ldy + col, y, n, a.vy);
+      if (n > 0) store_row8(a.y + row * a.ldy + col, y, n);
     }
   });
 }
@@ -69,8 +68,8 @@ __global__ __launch_bounds__(NT) void q8_dequantize_kernel(Q8Args a) {
   each_unit(a, [&](int64_t row, int col, int n) {
     if (n == 0) return;
     float y[8];
-    values8(load_codes(a.q + row * a.ldq + col, n, a.vq), q8::step_of(a.e[row * a.lde + col / q8::kGroup]), y);
-    store_row8(a.y + row * a.ldy + col, y, n, a.vy);
+    values8(load_codes(a.q + row * a.ldq + col, n), q8::step_of(a.e[row * a.lde + col / q8::kGroup]), y);
+    store_row8(a.y + row * a.ldy + col, y, n);
   });
 }
 
@@ -80,13 +79,13 @@ __global__ __launch_bounds__(NT) void q8_act_bwd_kernel(Q8Args a) {
   each_unit(a, [&](int64_t row, int col, int n) {
     if (n == 0) return;
     float v[8], dy[8], old[8] = {};
-    values8(load_codes(a.q + row * a.ldq + col, n, a.vq), q8::step_of(a.e[row * a.lde + col / q8::kGroup]), v);
-    load_row8(a.x + row * a.ldx + col, n, a.vx, dy);
+    values8(load_codes(a.q + row * a.ldq + col, n), q8::step_of(a.e[row * a.lde + col / q8::kGroup]), v);
+    load_row8(a.x + row * a.ldx + col, n, dy);
     float* p = a.dx + row * a.lddx + col;
-    if (a.accumulate) load_row8(p, n, a.vdx, old);
+    if (a.accumulate) load_row8(p, n, old);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = act_bwd_k<KIND>(v[j], dy[j], old[j], a.accumulate != 0);
-    store_row8(p, v, n, a.vdx);
+    store_row8(p, v, n);
   });
 }
 
@@ -112,9 +111,7 @@ int mle_q8_quantize(mle_stream stream, int rows, int cols, const float* x, int64
   if (rc) return rc;
   MLE_CHECK_ARG((x || rows == 0) && ldx >= cols, "mle_q8_quantize: null pointer or ldx %lld < %d", (long long)ldx, cols);
   if (rows == 0) return MLE_OK;
-  Q8Args a{rows, cols, 4 * q8::groups(cols), x, ldx, nullptr, 0, q, ldq, e, lde, nullptr, 0, 0, 0, 0, 0, 0};
-  a.vx = q8::rows_vec(x, ldx);
-  a.vq = q8::codes_vec(q, ldq);
+  const Q8Args a{rows, cols, 4 * q8::groups(cols), x, ldx, nullptr, 0, q, ldq, e, lde, nullptr, 0, 0};
   mle::launch(q8_quantize_kernel<-1>, grid_of(a), NT, 0, as_stream(stream), a);
   return check_launch("mle_q8_quantize");
 }
@@ -125,10 +122,8 @@ int mle_q8_dequantize(mle_stream stream, int rows, int cols, const int8_t* q, in
   if (rc) return rc;
   MLE_CHECK_ARG((y || rows == 0) && ldy >= cols, "mle_q8_dequantize: null pointer or ldy %lld < %d", (long long)ldy, cols);
   if (rows == 0) return MLE_OK;
-  Q8Args a{rows, cols, 4 * q8::groups(cols), nullptr, 0, y, ldy, const_cast<int8_t*>(q), ldq, const_cast<uint8_t*>(e),
-           lde, nullptr, 0, 0, 0, 0, 0, 0};
-  a.vy = q8::rows_vec(y, ldy);
-  a.vq = q8::codes_vec(q, ldq);
+  const Q8Args a{rows, cols, 4 * q8::groups(cols), nullptr, 0, y, ldy, const_cast<int8_t*>(q), ldq, const_cast<uint8_t*>(e),
+           lde, nullptr, 0, 0};
   mle::launch(q8_dequantize_kernel, grid_of(a), NT, 0, as_stream(stream), a);
   return check_launch("mle_q8_dequantize");
 }
@@ -141,10 +136,7 @@ int mle_q8_act_fwd(mle_stream stream, int kind, int rows, int cols, const float*
   MLE_CHECK_ARG(((x && y) || rows == 0) && ldx >= cols && ldy >= cols,
                 "mle_q8_act_fwd: null pointer or a leading dimension below %d", cols);
   if (rows == 0) return MLE_OK;
-  Q8Args a{rows, cols, 4 * q8::groups(cols), x, ldx, y, ldy, q, ldq, e, lde, nullptr, 0, 0, 0, 0, 0, 0};
-  a.vx = q8::rows_vec(x, ldx);
-  a.vy = q8::rows_vec(y, ldy);
-  a.vq = q8::codes_vec(q, ldq);
+  const Q8Args a{rows, cols, 4 * q8::groups(cols), x, ldx, y, ldy, q, ldq, e, lde, nullptr, 0, 0};
   Q8_LAUNCH_ACT(q8_quantize_kernel, kind, a, as_stream(stream));
   return check_launch("mle_q8_act_fwd");
 }
@@ -157,11 +149,8 @@ int mle_q8_act_bwd(mle_stream stream, int kind, int rows, int cols, const int8_t
   MLE_CHECK_ARG(((dy && dx) || rows == 0) && lddy >= cols && lddx >= cols,
                 "mle_q8_act_bwd: null pointer or a leading dimension below %d", cols);
   if (rows == 0) return MLE_OK;
-  Q8Args a{rows, cols, 4 * q8::groups(cols), dy, lddy, nullptr, 0, const_cast<int8_t*>(q), ldq, const_cast<uint8_t*>(e),
-           lde, dx, lddx, accumulate, 0, 0, 0, 0};
-  a.vx = q8::rows_vec(dy, lddy);
-  a.vdx = q8::rows_vec(dx, lddx);
-  a.vq = q8::codes_vec(q, ldq);
+  const Q8Args a{rows, cols, 4 * q8::groups(cols), dy, lddy, nullptr, 0, const_cast<int8_t*>(q), ldq, const_cast<uint8_t*>(e),
+           lde, dx, lddx, accumulate};
   Q8_LAUNCH_ACT(q8_act_bwd_kernel, kind, a, as_stream(stream));
   return check_launch("mle_q8_act_bwd");
 }

@@ -77,48 +77,91 @@ __device__ __forceinline__ void values8(uint2 code, float step, float (&x)[8]) {
   }
 }
 
-// n <= 8 codes at p (vec: eight of them, 8-byte aligned).
-__device__ __forceinline__ uint2 load_codes(const int8_t* __restrict__ p, int n, bool vec) {
-  if (vec && n == 8) return *reinterpret_cast<const uint2*>(p);
-  unsigned w[2] = {0u, 0u};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < n) w[j >> 2] |= (unsigned)(unsigned char)p[j] << (8 * (j & 3));
-  return make_uint2(w[0], w[1]);
-}
-__device__ __forceinline__ void store_codes(int8_t* __restrict__ p, uint2 c, int n, bool vec) {
-  if (vec && n == 8) {
-    *reinterpret_cast<uint2*>(p) = c;
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < n) p[j] = (int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+// Rows start at any address of their type: loads and stores of several values at once
+// are of that alignment, which costs them little (16384 x 4093 norm, both directions and
+// the codes read back: 565 us, of 4096 columns 493; element by element 1300).  What is
+// left of a row, n < 8 values, is four at once where there are as many, and up to three
+// single ones.
+struct Left {
+  bool four;
+  int single;  // after the four
+  __device__ __forceinline__ explicit Left(int n) : four((n & 4) != 0), single(n & 3) {}
+};
+
+// a or b, by value: a plain choice between two elements of an array becomes one
+// element at an address, and the array memory.
+__device__ __forceinline__ float pick(bool first, float a, float b) {
+  const unsigned m = first ? ~0u : 0u;
+  return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, a) & m) | (__builtin_bit_cast(unsigned, b) & ~m));
 }
 
-// n <= 8 floats at p (vec: eight of them, 16-byte aligned), the rest 0.
-__device__ __forceinline__ void load_row8(const float* __restrict__ p, int n, bool vec, float (&x)[8]) {
-  if (vec && n == 8) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+// n <= 8 codes at p, the rest 0.
+__device__ __forceinline__ uint2 load_codes(const int8_t* __restrict__ p, int n) {
+  uint2 w = make_uint2(0u, 0u);
+  if (n == 8) {
+    __builtin_memcpy(&w, p, 8);
+    return w;
+  }
+  const Left l(n);
+  unsigned a = 0u, b = 0u;
+  if (l.four) __builtin_memcpy(&a, p, 4);
+  const int8_t* s = p + (n & 4);
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (j < l.single) b |= (unsigned)(unsigned char)s[j] << (8 * j);
+  return l.four ? make_uint2(a, b) : make_uint2(b, 0u);
+}
+__device__ __forceinline__ void store_codes(int8_t* __restrict__ p, uint2 c, int n) {
+  if (n == 8) {
+    __builtin_memcpy(p, &c, 8);
+    return;
+  }
+  const Left l(n);
+  if (l.four) __builtin_memcpy(p, &c.x, 4);
+  const unsigned b = l.four ? c.y : c.x;
+  int8_t* s = p + (n & 4);
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (j < l.single) s[j] = (int8_t)(b >> (8 * j));
+}
+
+// n <= 8 floats at p, the rest 0.
+__device__ __forceinline__ void load_row8(const float* __restrict__ p, int n, float (&x)[8]) {
+  if (n == 8) {
+    const f32x4u a = reinterpret_cast<const f32x4u*>(p)[0], b = reinterpret_cast<const f32x4u*>(p)[1];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       x[j] = a[j];
       x[4 + j] = b[j];
     }
-  } else {
+    return;
+  }
+  const Left l(n);
+  f32x4u a = {0.f, 0.f, 0.f, 0.f};
+  float b[4] = {};
+  if (l.four) a = *reinterpret_cast<const f32x4u*>(p);
+  const float* s = p + (n & 4);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < n ? p[j] : 0.f;
+  for (int j = 0; j < 3; ++j)
+    if (j < l.single) b[j] = s[j];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[j] = l.four ? a[j] : b[j];
+    x[4 + j] = l.four ? b[j] : 0.f;
   }
 }
-__device__ __forceinline__ void store_row8(float* __restrict__ p, const float (&x)[8], int n, bool vec) {
-  if (vec && n == 8) {
-    reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-    reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) p[j] = x[j];
+__device__ __forceinline__ void store_row8(float* __restrict__ p, const float (&x)[8], int n) {
+  if (n == 8) {
+    reinterpret_cast<f32x4u*>(p)[0] = f32x4u{x[0], x[1], x[2], x[3]};
+    reinterpret_cast<f32x4u*>(p)[1] = f32x4u{x[4], x[5], x[6], x[7]};
+    return;
   }
+  const Left l(n);
+  if (l.four) *reinterpret_cast<f32x4u*>(p) = f32x4u{x[0], x[1], x[2], x[3]};
+  float* s = p + (n & 4);
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (j < l.single) s[j] = pick(l.four, x[4 + j], x[j]);
 }
 
 inline int check_shape(const char* who, int rows, int cols, const void* q, int64_t ldq, const void* e, int64_t lde) {
@@ -128,9 +171,5 @@ inline int check_shape(const char* who, int rows, int cols, const void* q, int64
                 (long long)lde, groups(cols));
   return MLE_OK;
 }
-
-// Whether rows of a tensor can be read and written eight values at a time.
-inline bool rows_vec(const float* p, int64_t ld) { return mle::aligned16(p) && ld % 4 == 0; }
-inline bool codes_vec(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0 && ld % 8 == 0; }
 
 }  // namespace q8

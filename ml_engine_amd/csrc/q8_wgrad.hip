@@ -42,7 +42,6 @@ struct WgradArgs {
   int rows, in, out, accumulate;
   int gx, gy, splits, per;  // tiles; K splits and the stages of each
   float* part;              // [split][in][out], then [split][out] of db, where splits > 1
-  int vec;                  // rows of dW (and of the partial sums) four at a time
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, uint32_t bytes) {
@@ -242,9 +241,9 @@ __global__ __launch_bounds__(S::NTH, 2) void q8_wgrad_kernel(WgradArgs a) {
       f32x4 v;
 #pragma unroll
       for (int n = 0; n < 4; ++n) v[n] = hi[i][n][r] + lo[i][n][r];
-      if (a.vec) {
-        if (old) v += *reinterpret_cast<const f32x4*>(p);
-        *reinterpret_cast<f32x4*>(p) = v;
+      if (c0 + 3 < a.out) {
+        if (old) v += *reinterpret_cast<const f32x4u*>(p);
+        *reinterpret_cast<f32x4u*>(p) = v;
       } else {
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -273,12 +272,12 @@ __global__ __launch_bounds__(256) void q8_wgrad_join_kernel(WgradArgs a, unsigne
     const int col = (int)(u - row * groups) * 4;
     const float* p = a.part + row * a.out + col;
     float* d = a.dW + row * a.lddw + col;
-    if (a.vec) {
-      f32x4 s = *reinterpret_cast<const f32x4*>(p);
+    if (col + 3 < a.out) {
+      f32x4 s = *reinterpret_cast<const f32x4u*>(p);
 #pragma unroll 8
-      for (int z = 1; z < a.splits; ++z) s += *reinterpret_cast<const f32x4*>(p + z * mn);
-      if (a.accumulate) s += *reinterpret_cast<const f32x4*>(d);
-      *reinterpret_cast<f32x4*>(d) = s;
+      for (int z = 1; z < a.splits; ++z) s += *reinterpret_cast<const f32x4u*>(p + z * mn);
+      if (a.accumulate) s += *reinterpret_cast<const f32x4u*>(d);
+      *reinterpret_cast<f32x4u*>(d) = s;
     } else {
       for (int n = 0; n < 4 && col + n < a.out; ++n) {
         float s = p[n];
@@ -293,7 +292,9 @@ __global__ __launch_bounds__(256) void q8_wgrad_join_kernel(WgradArgs a, unsigne
 // more at a split of at least 32 stages, else small ones (128 x 128); then as many
 // splits as make one workgroup to a CU of the large, two of the small, of at
 // least 8 and 4 stages, and no more than pay for their partial sums (a stage
-// takes about 1 us, a byte written and read again 0.5 ps).
+// takes about 1 us, a byte written and read again 0.5 ps).  A large tile half of which is past
+// the matrix loses (16384 x 48 x 4096 127 us against 103), one with a third of it wins
+// (8192 x 330 x 4096 124 against 144).
 constexpr int kMost = 1 << 30;  // rows, in, out
 struct WgradPlan {
   bool large;
@@ -304,7 +305,7 @@ WgradPlan wgrad_plan(int rows, int in, int out) {
   WgradPlan p;
   const int stages = (rows + planes::kK - 1) / planes::kK;
   const int64_t big = (int64_t)((in + 255) / 256) * ((out + 127) / 128);
-  p.large = in >= 4 && big * std::max(1, stages / 32) >= gemm::kChipCus / 2;
+  p.large = in > 128 && big * std::max(1, stages / 32) >= gemm::kChipCus / 2;
   const int tm = p.large ? 256 : 128;
   p.gx = (out + 127) / 128;
   p.gy = (in + tm - 1) / tm;
@@ -349,9 +350,8 @@ int mle_q8_linear_wgrad(mle_stream stream, int rows, int in, int out, const int8
     return set_error(MLE_ERR_WORKSPACE, "mle_q8_linear_wgrad: workspace of %zu bytes, 16-byte aligned, needed", need);
   const WgradPlan p = wgrad_plan(rows, in, out);
   MLE_CHECK_ARG((int64_t)p.gx * p.gy * p.splits * (p.large ? 512 : 256) < (1LL << 32), "mle_q8_linear_wgrad: grid too large");
-  WgradArgs a{q, ldq, e, lde, dY, lddy, dW, lddw, db, rows, in, out, accumulate, p.gx, p.gy, p.splits, p.per,
-              static_cast<float*>(ws), 0};
-  a.vec = out % 4 == 0 && lddw % 4 == 0 && aligned16(dW);
+  const WgradArgs a{q, ldq, e, lde, dY, lddy, dW, lddw, db, rows, in, out, accumulate, p.gx, p.gy, p.splits, p.per,
+              static_cast<float*>(ws)};
   hipStream_t s = as_stream(stream);
   const unsigned grid = (unsigned)(p.gx * p.gy * p.splits);
   ProbeScope probe("q8_wgrad", s, 2.0 * rows * (double)in * out, rows * (double)in + 4.0 * ((double)rows * out + (double)in * out));

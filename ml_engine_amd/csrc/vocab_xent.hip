@@ -195,7 +195,6 @@ struct AmaxArgs {
   unsigned* xpart;                    // [2][slabs][d]: of rows that take part, of the others
   unsigned* wpart;                    // [pieces][chunks][d]
   int padded, kblocks;                // rows: blocks of 256
-  int xvec;                           // rows of X four at a time
   unsigned* done;                     // workgroups that have finished a later sum: 0
   const float* lse;                   // backward
   int* key;
@@ -233,7 +232,7 @@ __global__ __launch_bounds__(NT) void xent_amax_kernel(AmaxArgs a, Rows rows) {
 #pragma unroll 8
       for (int r = 0; r < nb; ++r) {
         f32x4 v;
-        if (a.xvec) v = *reinterpret_cast<const f32x4*>(x + (int64_t)r * a.ldx);
+        if (a.d >= 4) v = *reinterpret_cast<const f32x4u*>(x + (int64_t)r * a.ldx);
         else v = f32x4{x[(int64_t)r * a.ldx], x[(int64_t)r * a.ldx + min(1, a.d - 1)], x[(int64_t)r * a.ldx + min(2, a.d - 1)],
                        x[(int64_t)r * a.ldx + min(3, a.d - 1)]};
         const unsigned keep = (live >> r) & 1 ? 0xffffffffu : 0u;
@@ -588,7 +587,6 @@ struct OutArgs {
   int ex_by_row, add;  // the exponent is add - ex[row or column]
   float scale;
   const float* upstream;
-  int vec;  // four columns at a time
   __device__ __forceinline__ float g() const { return upstream ? upstream[0] * scale : scale; }
   // Columns col .. col + 3 of a row (those of the matrix).
   __device__ __forceinline__ void put(int64_t row, int col, f32x4 v, float gg) const {
@@ -596,9 +594,9 @@ struct OutArgs {
     float* p = C + row * ldc + col;
 #pragma unroll
     for (int n = 0; n < 4; ++n) v[n] = __builtin_ldexpf(v[n], add - ex[ex_by_row ? row : min(col + n, cols - 1)]) * gg;
-    if (vec) {
-      if (accumulate) v += *reinterpret_cast<const f32x4*>(p);
-      *reinterpret_cast<f32x4*>(p) = v;
+    if (col + 3 < cols) {
+      if (accumulate) v += *reinterpret_cast<const f32x4u*>(p);
+      *reinterpret_cast<f32x4u*>(p) = v;
     } else {
 #pragma unroll
       for (int n = 0; n < 4; ++n)
@@ -941,7 +939,6 @@ struct Chunk {
     a.padded = padded;
     a.kblocks = (padded + NT - 1) / NT;
     a.bias = bias;
-    a.xvec = aligned16(X) && ldx % 4 == 0 && p.d >= 4 && p.d % 4 == 0;
     a.done = at<unsigned>(p.done);
     a.lse = lse;
     a.key = at<int>(p.key);
@@ -956,11 +953,10 @@ struct Chunk {
   void pack(int i, bool inputs, bool weights) const {
     const float* w = W + (int64_t)i * p.piece;
     const float* b = bias ? bias + (int64_t)i * p.piece : nullptr;
-    const int xvec = aligned16(X) && ldx % 4 == 0, wvec = aligned16(W) && ldw % 4 == 0;  // (pieces begin at multiples of 128)
-    PackAll a{{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, nullptr, at(p.xl), xvec},
-              {X, ldx, p.d, rows, p.dp / 16, padded / 32, at<int>(p.ex), at<int>(p.key), nullptr, at(p.xt), xvec},
-              {w, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d, nullptr, b, at(p.wl), wvec},
-              {w, ldw, p.d, cols(i), p.dp / 16, pcols(i) / 32, at<int>(p.en) + (int64_t)i * p.d, nullptr, b, at(p.wn), wvec},
+    PackAll a{{X, ldx, rows, p.d, padded / 16, p.dk, at<int>(p.ex), nullptr, nullptr, at(p.xl)},
+              {X, ldx, p.d, rows, p.dp / 16, padded / 32, at<int>(p.ex), at<int>(p.key), nullptr, at(p.xt)},
+              {w, ldw, cols(i), p.d, pcols(i) / 16, p.dk, at<int>(p.el) + (int64_t)i * p.d, nullptr, b, at(p.wl)},
+              {w, ldw, p.d, cols(i), p.dp / 16, pcols(i) / 32, at<int>(p.en) + (int64_t)i * p.d, nullptr, b, at(p.wn)},
               0, 0, 0, 0};
     a.nxl = i == 0 ? (unsigned)a.xl.rows_blocks() : 0u;
     a.nxt = i == 0 && weights ? (unsigned)a.xt.cols_blocks() : 0u;
@@ -1002,7 +998,6 @@ struct Chunk {
       a.cfac = at<float>(p.cfac);
       a.pcols = pcols(i);
       a.out = out;
-      a.out.vec = aligned16(out.C) && out.ldc % 4 == 0 && out.cols % 4 == 0;
       a.part = at<float>(part);
       return a;
     };
@@ -1075,10 +1070,10 @@ int planes_bwd(mle_stream stream, int rows, int d, int vocab, const float* X, in
       a.all = all;
       mle::launch(xent_tile_kernel<true>, (unsigned)(a.gx * a.gy), S::NTH, 0, s, a);
       OutArgs ow{}, ox{};
-      if (dW) ow = OutArgs{dW + v0, lddw, d, c.cols(i), add, c.at<int>(p.ex), 1, 0, grad_scale, upstream, 0};
+      if (dW) ow = OutArgs{dW + v0, lddw, d, c.cols(i), add, c.at<int>(p.ex), 1, 0, grad_scale, upstream};
       if (dX)
         ox = OutArgs{dX + (int64_t)r0 * lddx, lddx, c.rows, d, accumulate_dx || i > 0, c.at<int>(p.en) + (int64_t)i * d, 0, -kTop,
-                     grad_scale, upstream, 0};
+                     grad_scale, upstream};
       BiasArgs bias_grad{};
       if (db && i == p.pieces - 1)
         bias_grad = BiasArgs{c.at<float>(p.csum), c.padded / 64, vocab, add, all, db, grad_scale, upstream};

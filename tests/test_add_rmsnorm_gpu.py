@@ -18,7 +18,8 @@ def at(hip, a, shift):
 
 
 SHAPES = [(1, 1), (1, 32), (3, 31), (5, 33), (64, 256), (7, 330), (130, 512), (9, 1000), (33, 1024), (6, 1500), (40, 2048),
-          (3, 2052), (5, 4096), (2, 6001), (3, 8192), (2, 8200), (3, 20001), (1500, 64)]
+          (3, 2052), (5, 4096), (2, 6001), (3, 8192), (2, 8200), (3, 20001), (1500, 64),
+          (4, 7), (6, 37), (3, 38), (5, 2049), (2, 8191)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)

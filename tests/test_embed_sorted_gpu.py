@@ -54,7 +54,10 @@ CASES = [("uniform", 1, 1, 1, 1, 1), ("uniform", 1, 1, 3, 50, 7), ("uniform", 2,
          ("one", 3, 40, 41, 9, 64), ("one", 1, 17, 17, 5, 260), ("one", 2, 5000, 5000, 40000, 16), ("outside", 5, 30, 30, 20, 32),
          ("frequent", 8, 256, 256, 8000, 512), ("frequent", 3, 3000, 3001, 33000, 100), ("uniform", 4, 4500, 4500, 300, 20),
          ("frequent", 2, 500, 512, 128000, 200), ("uniform", 1, 300, 300, 600000, 4), ("uniform", 1, 16, 16, 1, 2052),
-         ("one", 1, 16, 16, 3, 12), ("frequent", 1, 9000, 9000, 17, 1030)]
+         ("one", 1, 16, 16, 3, 12), ("frequent", 1, 9000, 9000, 17, 1030),
+         # rows whose last four columns reach into the group before
+         ("frequent", 5, 200, 200, 40, 5), ("frequent", 5, 200, 203, 300, 6), ("one", 2, 300, 300, 7, 7),
+         ("frequent", 4, 300, 301, 90, 1031), ("uniform", 2, 40, 40, 30, 3)]
 
 
 @pytest.mark.parametrize("kind,batch,clen,max_clen,vocab,dim", CASES)

@@ -39,7 +39,8 @@ def samples(r, rows, cols):
 
 
 @pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (4, 32, 0), (5, 31, 1), (7, 33, 2), (64, 96, 8), (37, 330, 3),
-                                           (3, 4096, 0), (300, 129, 0), (1, 2048, 4)])
+                                           (3, 4096, 0), (300, 129, 0), (1, 2048, 4), (5, 34, 0), (6, 35, 1), (5, 36, 0),
+                                           (7, 37, 0), (4, 38, 5), (9, 39, 0), (2, 7, 0)])
 def test_quantize_and_back(hip, rows, cols, pad):
     x = samples(rng(rows * 1000 + cols), rows, cols)
     ng = -(-cols // 32)
