@@ -21,7 +21,9 @@ namespace {
 
 constexpr int IX_NT = 1024;
 constexpr int IX_RMAX = 1024;   // table rows of an index workgroup
-constexpr int IX_CHUNK = 8192;  // tokens that it sorts at a time
+constexpr int IX_WAVES = IX_NT / 64;
+constexpr int IX_PER = 8;      // tokens of a lane, at most, in a chunk that it sorts at a time
+constexpr int IX_CHUNK = IX_PER * IX_NT;
 constexpr int HEAD = 64;
 constexpr int PART = 16;        // places of the list that one partial sum covers
 
@@ -41,7 +43,9 @@ struct Cols {
 
 struct IndexArgs {
   const int32_t* keys;
-  int clen, max_clen, ntok, vocab, rows_per_wg, nix;
+  int clen, max_clen, ntok, vocab, rows_per_wg;
+  int ranges, nix;  // of table rows; index workgroups, a multiple of ranges
+  int per;          // tokens of a lane in a chunk
   int32_t* head;
   int2* rinfo;
   int32_t* list;
@@ -51,9 +55,6 @@ struct IndexArgs {
 __device__ __forceinline__ int key_of(const IndexArgs& a, int t) {
   return a.clen == a.max_clen ? a.keys[t] : a.keys[(int64_t)(t / a.clen) * a.max_clen + t % a.clen];
 }
-
-constexpr int IX_WAVES = IX_NT / 64;
-constexpr int IX_PER = IX_CHUNK / IX_NT;  // tokens of a lane in a chunk
 
 struct IndexLds {
   int count[IX_WAVES][IX_RMAX];  // tokens of each row among a wave's, then where they go
@@ -86,32 +87,47 @@ __device__ __forceinline__ int exclusive_scan(int v, int* wave, int& sum) {
 
 // Lists the tokens of table rows [v0, v0 + nrows): every workgroup reads all
 // the keys, and counts how many lie below its rows, which is where its part of
-// the list starts.  A chunk's tokens are taken in order by the waves (512
+// the list starts.  A chunk's tokens are taken in order by the waves (64 * per
 // consecutive ones each), 64 at a time.  Lanes with equal rows find each other by a
 // ballot per bit of the row, so that a token knows its place among the wave's; the
-// waves' counts in order give the rest.
+// waves' counts in order give the rest.  Of many chunks, a range of rows has several
+// workgroups: each counts all of them and lists its own (64000 tokens, 256 rows: one
+// workgroup to a range 61 us, eight 20).
 __device__ void index_rows(const IndexArgs& a, int wg, IndexLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int v0 = wg * a.rows_per_wg, nrows = min(a.rows_per_wg, a.vocab - v0);
+  int range = wg, part = 0, parts = 1;
+  if (a.nix != a.ranges) range = wg % a.ranges, part = wg / a.ranges, parts = a.nix / a.ranges;
+  const int v0 = range * a.rows_per_wg, nrows = min(a.rows_per_wg, a.vocab - v0);
   const int rbits = 32 - __clz(max(nrows - 1, 1));
+  const int per = a.per, chunk = per * IX_NT;
   // this lane's keys of a chunk, in token order by (wave, k, lane); -1 past the end
   auto load = [&](int c0, int (&key)[IX_PER]) {
+    if (a.ntok == 0) return;
+    const int t0 = c0 + w * per * 64 + lane;
+    if (a.clen == a.max_clen) {  // (all loads on their way before the first is used)
 #pragma unroll
-    for (int k = 0; k < IX_PER; ++k) {
-      const int t = c0 + w * (IX_CHUNK / IX_WAVES) + k * 64 + lane;
-      key[k] = t < a.ntok ? key_of(a, t) : -1;
+      for (int k = 0; k < IX_PER; ++k) key[k] = a.keys[min(t0 + k * 64, a.ntok - 1)];
+    } else {
+#pragma unroll
+      for (int k = 0; k < IX_PER; ++k) key[k] = key_of(a, min(t0 + k * 64, a.ntok - 1));
     }
+#pragma unroll
+    for (int k = 0; k < IX_PER; ++k)
+      if (k >= per || t0 + k * 64 >= a.ntok) key[k] = -1;
   };
   auto clear = [&]() {
     for (int i = tid; i < IX_WAVES * nrows; i += IX_NT) s.count[i / nrows][i % nrows] = 0;
   };
-  // rank: the token's place among the wave's of its row (row: -1 for others')
-  auto rank_wave = [&](const int (&key)[IX_PER], int (&row)[IX_PER], int (&rank)[IX_PER]) {
+  auto mine_of = [&](int key, unsigned& r) {
+    r = (unsigned)key - (unsigned)v0;
+    return r < (unsigned)nrows;  // (v0 + nrows <= 2^30: a negative id is past it)
+  };
+  // rank: the token's place among the wave's of its row
+  auto rank_wave = [&](const int (&key)[IX_PER], int (&rank)[IX_PER]) {
 #pragma unroll
     for (int k = 0; k < IX_PER; ++k) {
-      const unsigned r = (unsigned)key[k] - (unsigned)v0;
-      const bool mine = key[k] >= 0 && r < (unsigned)nrows;
-      row[k] = mine ? (int)r : -1;
+      unsigned r;
+      const bool mine = mine_of(key[k], r);
       unsigned long long same = __ballot(mine);
       if (same == 0) continue;
       for (int b = 0; b < rbits; ++b) {
@@ -128,48 +144,79 @@ __device__ void index_rows(const IndexArgs& a, int wg, IndexLds& s) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's next 64 read what these wrote
     }
   };
-  const bool single = a.ntok <= IX_CHUNK;
-  int key[IX_PER], row[IX_PER], rank[IX_PER];
+  const bool single = a.ntok <= chunk;
+  int key[IX_PER] = {-1, -1, -1, -1, -1, -1, -1, -1}, rank[IX_PER];
+  static_assert(IX_PER == 8, "key");
   if (tid == 0) s.smaller = 0;
   clear();
   __syncthreads();
-  int below = 0, mine = 0;
+  // the chunks that this workgroup lists
+  int first = 0, end = a.ntok;
+  if (parts > 1) {
+    const unsigned chunks = ((unsigned)a.ntok + IX_CHUNK - 1) / IX_CHUNK;  // (whole ones: per == IX_PER)
+    first = (int)(chunks * part / parts) * IX_CHUNK;
+    end = min((int)(chunks * (part + 1) / parts) * IX_CHUNK, a.ntok);
+  }
+  int below = 0, mine = 0, before = 0;  // the row's tokens: all, and those of chunks before
+  auto add_counts = [&]() {
+    int n = 0;
+    if (tid < nrows)
+#pragma unroll
+      for (int i = 0; i < IX_WAVES; ++i) n += s.count[i][tid];
+    return n;
+  };
   if (single) {
     load(0, key);
 #pragma unroll
     for (int k = 0; k < IX_PER; ++k) below += key[k] >= 0 && key[k] < v0;
-    rank_wave(key, row, rank);
+    rank_wave(key, rank);
   } else {
-    for (int c0 = 0; c0 < a.ntok; c0 += IX_CHUNK) {
-      load(c0, key);
+    // Counted in any order: where the ids lie without gaps, four of a lane at a time.
+    const bool flat = a.clen == a.max_clen && (reinterpret_cast<uintptr_t>(a.keys) & 15) == 0;
+    auto load4 = [&](int c0, int (&key)[IX_PER]) {
+      if (!flat || c0 + chunk > a.ntok) return load(c0, key);
+#pragma unroll
+      for (int k = 0; k < IX_PER; k += 4)
+        *reinterpret_cast<int4*>(key + k) = *reinterpret_cast<const int4*>(a.keys + c0 + (w * per + k) * 64 + 4 * lane);
+    };
+    load4(0, key);
+    for (int c0 = 0; c0 < a.ntok; c0 += chunk) {
+      if (c0 == first && c0 > 0) {
+        __syncthreads();
+        before = add_counts();
+        __syncthreads();
+      }
+      int next[IX_PER];
+      load4(c0 + chunk, next);
 #pragma unroll
       for (int k = 0; k < IX_PER; ++k) {
-        below += key[k] >= 0 && key[k] < v0;
-        if (key[k] >= v0 && key[k] < v0 + nrows) atomicAdd(&s.count[w][key[k] - v0], 1);
+        below += (unsigned)key[k] < (unsigned)v0;
+        unsigned r;
+        if (mine_of(key[k], r)) atomicAdd(&s.count[w][r], 1);
       }
+#pragma unroll
+      for (int k = 0; k < IX_PER; ++k) key[k] = next[k];
     }
   }
   below = wave_sum(below);
   if (lane == 0) atomicAdd(&s.smaller, below);
   __syncthreads();
-  if (tid < nrows)
-#pragma unroll
-    for (int i = 0; i < IX_WAVES; ++i) mine += s.count[i][tid];
+  mine = add_counts();
   int kept;
   const int start = s.smaller + exclusive_scan(mine, s.wave, kept);
   if (tid < nrows) {
-    s.next[tid] = start;
-    a.rinfo[v0 + tid] = make_int2(start, mine);
+    s.next[tid] = start + before;
+    if (part == 0) a.rinfo[v0 + tid] = make_int2(start, mine);
   }
-  if (wg == a.nix - 1 && tid == 0) a.head[0] = s.smaller + kept;
+  if (wg == a.ranges - 1 && tid == 0) a.head[0] = s.smaller + kept;
   if (kept == 0) return;
-  for (int c0 = 0; c0 < a.ntok; c0 += IX_CHUNK) {
+  if (!single) load(first, key);
+  for (int c0 = first; c0 < end; c0 += chunk) {
     if (!single) {
       __syncthreads();
       clear();
       __syncthreads();
-      load(c0, key);
-      rank_wave(key, row, rank);
+      rank_wave(key, rank);
     }
     __syncthreads();
     if (tid < nrows) {
@@ -184,12 +231,14 @@ __device__ void index_rows(const IndexArgs& a, int wg, IndexLds& s) {
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < IX_PER; ++k)
-      if (row[k] >= 0) {
-        const int to = s.count[w][row[k]] + rank[k];
-        a.list[to] = c0 + w * (IX_CHUNK / IX_WAVES) + k * 64 + lane;
-        a.skey[to] = v0 + row[k];
-      }
+    for (int k = 0; k < IX_PER; ++k) {
+      unsigned r;
+      if (!mine_of(key[k], r)) continue;
+      const int to = s.count[w][r] + rank[k];
+      a.list[to] = c0 + (w * per + k) * 64 + lane;
+      a.skey[to] = key[k];
+    }
+    if (c0 + chunk < end) load(c0 + chunk, key);
   }
 }
 
@@ -369,7 +418,7 @@ __global__ __launch_bounds__(1024) void embed_join_kernel(GradArgs a, int cw) {
 int check(const char* who, int batch, int clen, int dim, int vocab) {
   MLE_CHECK_ARG(batch >= 0 && clen > 0 && dim > 0 && dim <= (1 << 30) && vocab > 0 && vocab <= (1 << 30), "%s: bad shape (batch %d, clen %d, dim %d, vocab %d)", who,
                 batch, clen, dim, vocab);
-  MLE_CHECK_ARG((long long)batch * clen < 2147483647LL - IX_CHUNK, "%s: too many tokens", who);
+  MLE_CHECK_ARG((long long)batch * clen < 2147483647LL - 2 * IX_CHUNK, "%s: too many tokens", who);
   return MLE_OK;
 }
 
@@ -401,10 +450,16 @@ int mle_embed_scaled_fwd(mle_stream stream, float* out, const float* table, cons
                      mle_embed_sorted_index_bytes(batch, clen, vocab));
   const int ntok = batch * clen;
   if (ntok == 0 && !index) return MLE_OK;
-  IndexArgs a{keys, clen, max_clen, ntok, vocab, 0, 0, nullptr, nullptr, nullptr, nullptr};
+  IndexArgs a{keys, clen, max_clen, ntok, vocab, 0, 0, 0, 1, nullptr, nullptr, nullptr, nullptr};
   if (index) {
     a.rows_per_wg = std::min(IX_RMAX, std::max(32, (vocab + 255) / 256));
-    a.nix = (vocab + a.rows_per_wg - 1) / a.rows_per_wg;
+    a.ranges = (vocab + a.rows_per_wg - 1) / a.rows_per_wg;
+    a.per = std::max(1, std::min(IX_PER, (int)(((int64_t)ntok + IX_NT - 1) / IX_NT)));
+    // workgroups to list many chunks: up to two to a CU, which delays the lookup; one where
+    // that is long (64000 tokens, 32000 rows of 512: 110 us with two, 124 with one; 32000
+    // tokens, 128000 rows of 1024: 209 / 200)
+    const int chunks = (int)(((int64_t)ntok + IX_CHUNK - 1) / IX_CHUNK);
+    a.nix = a.ranges * std::max(1, std::min(chunks, (dim <= 512 ? 512 : 256) / a.ranges));
     a.head = static_cast<int32_t*>(index);
     a.rinfo = reinterpret_cast<int2*>(a.head + HEAD);
     a.list = reinterpret_cast<int32_t*>(a.rinfo + vocab);

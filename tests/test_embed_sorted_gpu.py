@@ -12,11 +12,11 @@ F32 = 2.0 ** -24  # half a step of fp32
 def forward(hip, keys, table, clen, scale, shift=0, stream=None):
     batch, max_clen = keys.shape
     vocab, dim = table.shape
-    gk = hip.Buffer.from_array(keys)
+    gk = hip.Buffer.from_array(np.concatenate([np.zeros(shift, np.int32), keys.reshape(-1)]))
     gt = hip.Buffer.from_array(np.concatenate([np.zeros(shift, np.float32), table.reshape(-1)]))
     go = hip.Buffer.from_array(np.full(batch * clen * dim + 8, 5.0, np.float32))
     ix = hip.Buffer(hip.lib().mle_embed_sorted_index_bytes(batch, clen, vocab))
-    hip.call("mle_embed_scaled_fwd", stream, go.ptr, gt.ptr + 4 * shift, gk.ptr, batch, clen, max_clen, dim, vocab, scale,
+    hip.call("mle_embed_scaled_fwd", stream, go.ptr, gt.ptr + 4 * shift, gk.ptr + 4 * shift, batch, clen, max_clen, dim, vocab, scale,
              ix.ptr, ix.nbytes)
     out = go.numpy()
     assert (out[batch * clen * dim:] == 5.0).all()
@@ -57,7 +57,9 @@ CASES = [("uniform", 1, 1, 1, 1, 1), ("uniform", 1, 1, 3, 50, 7), ("uniform", 2,
          ("one", 1, 16, 16, 3, 12), ("frequent", 1, 9000, 9000, 17, 1030),
          # rows whose last four columns reach into the group before
          ("frequent", 5, 200, 200, 40, 5), ("frequent", 5, 200, 203, 300, 6), ("one", 2, 300, 300, 7, 7),
-         ("frequent", 4, 300, 301, 90, 1031), ("uniform", 2, 40, 40, 30, 3)]
+         ("frequent", 4, 300, 301, 90, 1031), ("uniform", 2, 40, 40, 30, 3),
+         # several index workgroups to a range of rows
+         ("frequent", 9, 4000, 4001, 300, 8), ("frequent", 4, 10000, 10000, 40000, 8), ("uniform", 2, 10001, 10001, 500, 520)]
 
 
 @pytest.mark.parametrize("kind,batch,clen,max_clen,vocab,dim", CASES)
