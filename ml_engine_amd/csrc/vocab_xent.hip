@@ -161,6 +161,117 @@ __global__ __launch_bounds__(NT) void xent_slices_kernel(const float* __restrict
   *p = accumulate ? *p + s : s;
 }
 
+// dW (+)= xs^T P and db (+)= column sums of P for few rows, where a product's tile has
+// only a stage or a few: 128 x 128 of dW to a workgroup, 64 x 64 to a wave, the
+// operands' fragments straight from memory (four neighbouring columns of eight rows to
+// a lane, transposed in its registers, as planes.hpp orders them), without LDS or
+// barriers, so that waves of different progress share a CU.  An fp32 value is the sum of
+// three bf16 planes (the first truncated: no value overflows), a product six MFMAs;
+// what is dropped is below 2^-22 of it and of either sign.  32 x 876 -> 26839 30 us, 3.2
+// TB/s written (the library's product 68); 64 x 1024 -> 32000 56 us (75).
+using planes::u32x4;
+__device__ __forceinline__ void split3(const float (&v)[8], u32x4& h, u32x4& m, u32x4& l) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned a = __builtin_bit_cast(unsigned, v[2 * j]), b = __builtin_bit_cast(unsigned, v[2 * j + 1]);
+    h[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);  // the high halves, b's above a's
+    const float ra = v[2 * j] - __builtin_bit_cast(float, a & 0xffff0000u);
+    const float rb = v[2 * j + 1] - __builtin_bit_cast(float, b & 0xffff0000u);
+    m[j] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)ra, (__bf16)rb});
+    const float sa = ra - __builtin_bit_cast(float, m[j] << 16), sb = rb - __builtin_bit_cast(float, m[j] & 0xffff0000u);
+    l[j] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)sa, (__bf16)sb});
+  }
+}
+struct DwArgs {
+  const float* X;  // [rows][d]
+  const float* P;  // [rows][cols]
+  int rows, d, cols, gx, gy, accumulate;
+  float* dW;
+  int64_t lddw;
+  float* db;
+};
+__device__ __forceinline__ f32x4 four_of(const float* p, int c, int n) {
+  if (c + 3 < n) return *reinterpret_cast<const f32x4u*>(p + c);
+  return f32x4{p[min(c, n - 1)], p[min(c + 1, n - 1)], p[min(c + 2, n - 1)], p[min(c + 3, n - 1)]};
+}
+__global__ __launch_bounds__(NT, 2) void xent_dw_kernel(DwArgs a) {
+  using T = planes::Bf16;
+  const int lane = threadIdx.x & 63, lr = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
+  int tm, tn, z;
+  gemm::item_tile(blockIdx.x, a.gx * a.gy, a.gx, a.gy, tm, tn, z);
+  const int m0 = tm * 128 + 64 * wm, c0 = tn * 128 + 64 * wn + 4 * lr;
+  if (m0 >= a.d || tn * 128 + 64 * wn >= a.cols) return;  // (a whole wave; there are no barriers)
+  f32x4 hi[4][4], lo[4][4];
+  float sum[4] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) hi[i][n] = lo[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int r0 = 0; r0 < a.rows; r0 += 32) {
+    f32x4 x[8], p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {  // (past the last row its values again, and P as zeros)
+      const int64_t r = min(r0 + 8 * q + j, a.rows - 1);
+      p[j] = four_of(a.P + r * a.cols, c0, a.cols);
+      x[j] = four_of(a.X + r * a.d, m0 + 4 * lr, a.d);
+    }
+    u32x4 b[4][3];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = r0 + 8 * q + j < a.rows ? p[j][n] : 0.f;
+        sum[n] += v[j];
+      }
+      split3(v, b[n][0], b[n][1], b[n][2]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v[8] = {x[0][i], x[1][i], x[2][i], x[3][i], x[4][i], x[5][i], x[6][i], x[7][i]};
+      u32x4 h, m, l;
+      split3(v, h, m, l);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        lo[i][n] = T::mma(l, b[n][0], lo[i][n]);
+        lo[i][n] = T::mma(h, b[n][2], lo[i][n]);
+        lo[i][n] = T::mma(m, b[n][1], lo[i][n]);
+        lo[i][n] = T::mma(m, b[n][0], lo[i][n]);
+        lo[i][n] = T::mma(h, b[n][1], lo[i][n]);
+        hi[i][n] = T::mma(h, b[n][0], hi[i][n]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = m0 + 16 * q + 4 * r + i;
+      if (row >= a.d || c0 >= a.cols) continue;
+      float* w = a.dW + (int64_t)row * a.lddw + c0;
+      f32x4 v;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[n] = hi[i][n][r] + lo[i][n][r];
+      if (c0 + 3 < a.cols) {
+        if (a.accumulate) v += *reinterpret_cast<const f32x4u*>(w);
+        *reinterpret_cast<f32x4u*>(w) = v;
+      } else {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if (c0 + n < a.cols) w[n] = a.accumulate ? w[n] + v[n] : v[n];
+      }
+    }
+  if (!a.db || m0 > 0) return;
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    sum[n] += __shfl_xor(sum[n], 16, 64);
+    sum[n] += __shfl_xor(sum[n], 32, 64);
+    if (q == 0 && c0 + n < a.cols) a.db[c0 + n] = a.accumulate ? a.db[c0 + n] + sum[n] : sum[n];
+  }
+}
+
 // ---------------------------------------------------------------- fp16 planes
 using planes::Operand;
 using S = planes::Shape<planes::Fp16, 2, 2, 2, 2>;  // 128 x 128 of C, two workgroups to a CU
@@ -772,6 +883,15 @@ bool use_planes(int rows, int d, int vocab) {
   return rows >= 192 && (double)rows * vocab * (900.0 + d) >= 2.8e9;
 }
 
+// Few logits: where dW's own kernel runs, a stage or two of rows and tiles enough to hide
+// its loads (both sides, forward and backward, own kernel / library product, us: 32 x
+// 876 -> 26839 156 / 191, 64 x 1023 -> 32001 204 / 243, 1 x 512 -> 32000 102 / 116; 95 x
+// 800 -> 7067 94 / 96, 191 x 1024 -> 16000 245 / 235, 64 x 256 -> 4096 46 / 42).
+bool short_dw(int rows, int d, int n) {
+  const int64_t tiles = ((int64_t)d + 127) / 128 * (((int64_t)n + 127) / 128);
+  return rows <= 64 && tiles >= 512 && tiles < (1 << 23);
+}
+
 // The two products of a piece share a grid of two workgroups to a CU.  A product
 // whose workgroups would each take more than 5/4 of a CU slot's share of the
 // stages has its K split, into at least 16 stages each (an even number: the column
@@ -1156,14 +1276,15 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
   float* part = reinterpret_cast<float*>(static_cast<char*>(ws) + p.logits + p.rows + p.state);
   void* gws = reinterpret_cast<char*>(part) + p.slices;
   // The Linear backward's own launches where its matrices are dense.
-  const bool dense = dX && dW && p.piece == vocab && dx_slices(rows, d, vocab) == 1 && ldw == vocab && lddw == vocab && lddx == d;
+  const bool own_dw = dW && short_dw(rows, d, p.piece);
+  const bool dense = dX && dW && !own_dw && p.piece == vocab && dx_slices(rows, d, vocab) == 1 && ldw == vocab && lddw == vocab && lddx == d;
   for (int v0 = 0; v0 < vocab; v0 += p.piece) {
     const int n = std::min(p.piece, vocab - v0), slices = dX ? dx_slices(rows, d, n) : 1;
     auto groups = [&](int cols) { return (unsigned)(((int64_t)rows * cols + 4 * NT - 1) / (4 * NT)); };
     TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr,
                     bias ? bias + v0 : nullptr, gws, p.gemm));
     mle::launch(xent_grad_kernel, groups(n) + (dW && v0 == 0 ? groups(d) : 0u), NT, 0, s, l, rows, n, v0, rw, lse, upstream,
-                grad_scale, groups(n), X, ldx, d, xs, db && !accumulate_dw && !dense ? db : nullptr);
+                grad_scale, groups(n), X, ldx, d, xs, db && !accumulate_dw && !dense && !own_dw ? db : nullptr);
     if (dense) {
       TRY(mle_linear_bwd_ex(stream, rows, d, vocab, 1, xs, l, 0, W, 0, dX, accumulate_dx, dW, db, 0, accumulate_dw, gws, p.gemm));
       break;
@@ -1180,9 +1301,13 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
       TRY(mle_gemm_ex(stream, 0, 1, rows, d, n, 1.f, l, n, 0, W + v0, ldw, 0, acc ? 1.f : 0.f, dX, lddx, 0, 1,
                       nullptr, nullptr, gws, p.gemm));
     }
-    if (dW)
+    if (own_dw) {
+      const DwArgs a{xs, l, rows, d, n, (n + 127) / 128, (d + 127) / 128, accumulate_dw, dW + v0, lddw, db ? db + v0 : nullptr};
+      mle::launch(xent_dw_kernel, (unsigned)(a.gx * a.gy), NT, 0, s, a);
+    } else if (dW) {
       TRY(mle_gemm_ex(stream, 1, 0, d, n, rows, 1.f, xs, d, 0, l, n, 0, accumulate_dw ? 1.f : 0.f, dW + v0, lddw, 0, 1,
                       db ? db + v0 : nullptr, nullptr, gws, p.gemm));
+    }
   }
   return check_launch("mle_vocab_xent_bwd");
 }

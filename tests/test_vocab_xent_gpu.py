@@ -103,7 +103,7 @@ SHAPES = [(1, 1, 1), (1, 8, 100), (3, 33, 70), (64, 64, 1000), (64, 256, 4096), 
           (2048, 64, 300), (5, 512, 20011),
           (128, 33, 24001), (300, 330, 10007), (513, 64, 6400), (1030, 65, 3001), (4001, 31, 777), (2048, 128, 1500),
           (33001, 16, 1100), (17, 40, 2051), (2100, 16, 1200), (193, 33, 24001), (200, 3, 24001),
-          (250, 1, 25000), (64, 3, 530000)]
+          (250, 1, 25000), (64, 3, 530000), (33, 300, 22001), (64, 130, 33001)]
 
 
 @pytest.mark.parametrize("rows,d,vocab", SHAPES)
