@@ -243,7 +243,7 @@ __device__ void index_rows(const IndexArgs& a, int wg, IndexLds& s) {
 }
 
 // Workgroups [0, nix) build the index, the rest look rows up.  8192 tokens x 512 with 8000
-// ids 10.4 us (the index ends last), 32000 x 1024 with 128000 66 us (4.0 TB/s).
+// ids 10.4 us (the index ends last), 32000 x 1024 with 128000 66-73 us (3.6-4.0 TB/s).
 template <bool VEC, typename U>
 __global__ __launch_bounds__(IX_NT, 8) void embed_fwd_kernel(IndexArgs a, float* __restrict__ out,
                                                           const float* __restrict__ table, int dim, float scale,
