@@ -96,9 +96,10 @@ def close(got, ref, tol, what):
     assert (err <= tol).all(), f"{what}: {np.max(err / np.maximum(tol, 1e-300)):.3g} times the bound"
 
 
-# few logits (stored in pieces), then products of fp16 planes: rows and vocabularies on
-# both sides of whole tiles, features on both sides of whole stages; the last has
-# two chunks of rows and several pieces of the vocabulary
+# few logits (stored in pieces; up to 64 rows and many columns with a kernel of their own
+# for dW), then products of fp16 planes: rows and vocabularies on both sides of whole
+# tiles, features on both sides of whole stages, several chunks of rows and pieces of
+# the vocabulary
 SHAPES = [(1, 1, 1), (1, 8, 100), (3, 33, 70), (64, 64, 1000), (64, 256, 4096), (100, 31, 257), (130, 96, 129), (300, 330, 1007),
           (2048, 64, 300), (5, 512, 20011),
           (128, 33, 24001), (300, 330, 10007), (513, 64, 6400), (1030, 65, 3001), (4001, 31, 777), (2048, 128, 1500),
@@ -134,7 +135,7 @@ def test_padded_sequences(hip, clen, max_clen):
     close(c.backward()[1], ref["dw"], tol["dw"], "dw")
 
 
-@pytest.mark.parametrize("rows,vocab", [(40, 500), (1000, 3100)])
+@pytest.mark.parametrize("rows,vocab", [(40, 500), (1000, 3100), (48, 66000)])
 def test_what_rows_outside_hold_stays_there(hip, rows, vocab):
     """NaN, infinity and huge values in rows that take no part: the loss, dW, db and the other rows' dX as without them."""
     c = Case(hip, rows, 64, vocab, ignored=0.3)
@@ -163,7 +164,7 @@ def test_no_row_takes_part(hip, rows, vocab):
     assert loss == 0 and not row_loss.any() and not dx.any() and not dw.any() and not db.any()
 
 
-@pytest.mark.parametrize("rows,vocab", [(33, 400), (1000, 4600)])
+@pytest.mark.parametrize("rows,vocab", [(33, 400), (1000, 4600), (48, 66000)])
 def test_masked_entries(hip, rows, vocab):
     """A bias of -infinity: as if the entry were not in the vocabulary."""
     c = Case(hip, rows, 64, vocab)
@@ -187,7 +188,7 @@ def test_masked_entries(hip, rows, vocab):
     assert not dw[:, out].any() and not db[out].any()
 
 
-@pytest.mark.parametrize("rows,vocab", [(40, 300), (1030, 3000)])
+@pytest.mark.parametrize("rows,vocab", [(40, 300), (1030, 3000), (48, 66000)])
 @pytest.mark.parametrize("size", [1.0, 60.0, 2.0 ** -30])
 def test_rows_outside_have_their_log_sum(hip, rows, vocab, size):
     """Ordinary values there, other than the rest's: lse is theirs.  Some features are
@@ -203,7 +204,7 @@ def test_rows_outside_have_their_log_sum(hip, rows, vocab, size):
         close(got, ref[name], tol[name], name)
 
 
-@pytest.mark.parametrize("rows,vocab", [(30, 200), (1000, 3100)])
+@pytest.mark.parametrize("rows,vocab", [(30, 200), (1000, 3100), (48, 66000)])
 def test_unaligned_buffers(hip, rows, vocab):
     """Every float buffer begins 4 bytes past an aligned address."""
     c = Case(hip, rows, 36, vocab)
@@ -223,7 +224,7 @@ def test_unaligned_buffers(hip, rows, vocab):
         close(v.numpy()[1:], np.asarray(ref[k]).reshape(-1), np.asarray(tol[k]).reshape(-1), k)
 
 
-@pytest.mark.parametrize("rows,vocab", [(20, 300), (1030, 3000)])
+@pytest.mark.parametrize("rows,vocab", [(20, 300), (1030, 3000), (48, 66000)])
 def test_not_finite_rows(hip, rows, vocab):
     """A NaN in a row that takes part: its lse and the loss are NaN, other rows' values stay."""
     c = Case(hip, rows, 64, vocab, ignored=0.0)
@@ -238,7 +239,7 @@ def test_not_finite_rows(hip, rows, vocab):
     assert np.isnan(dx[7]).all() and np.isfinite(np.delete(dx, 7, 0)).all() and np.isnan(dw).all()
 
 
-@pytest.mark.parametrize("rows,vocab", [(50, 700), (1100, 2900)])
+@pytest.mark.parametrize("rows,vocab", [(50, 700), (1100, 2900), (48, 66000)])
 def test_parts_of_the_gradient(hip, rows, vocab):
     """dX alone, dW alone, dW without db, and no row losses."""
     c = Case(hip, rows, 96, vocab)
@@ -258,7 +259,7 @@ def test_parts_of_the_gradient(hip, rows, vocab):
 
 
 @pytest.mark.parametrize("scale", [2.0 ** -40, 60.0])
-@pytest.mark.parametrize("rows,vocab", [(48, 600), (1030, 3000)])
+@pytest.mark.parametrize("rows,vocab", [(48, 600), (1030, 3000), (48, 66000)])
 def test_small_and_confident_rows(hip, rows, vocab, scale):
     """Rows of tiny values (a flat softmax), and logits up to some hundreds."""
     c = Case(hip, rows, 64, vocab, scale=scale)
@@ -273,7 +274,7 @@ def test_small_and_confident_rows(hip, rows, vocab, scale):
     close(db, ref["db"], tol["db"], "db")
 
 
-@pytest.mark.parametrize("rows,vocab", [(64, 500), (1024, 3000)])
+@pytest.mark.parametrize("rows,vocab", [(64, 500), (1024, 3000), (48, 66000)])
 def test_values_of_very_different_size(hip, rows, vocab):
     """Columns of X and rows of W from 2^-30 to 2^30 of each other."""
     c = Case(hip, rows, 64, vocab)
@@ -301,7 +302,7 @@ def test_two_norm(hip, rows, d, vocab):
         assert np.linalg.norm(got - want) <= 2e-6 * np.linalg.norm(want)
 
 
-@pytest.mark.parametrize("rows,vocab", [(60, 900), (1000, 3100)])
+@pytest.mark.parametrize("rows,vocab", [(60, 900), (1000, 3100), (48, 66000)])
 def test_repeats(hip, rows, vocab):
     c = Case(hip, rows, 80, vocab)
     c.put()
