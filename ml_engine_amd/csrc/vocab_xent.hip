@@ -764,23 +764,57 @@ __device__ __forceinline__ void xent_product(const ProductArgs& a, int item, cha
   }
   const int64_t row0 = (int64_t)tm * kTile + 64 * w.wm + (COLS ? 16 : 4) * w.q;
   const int c0 = tn * kTile + w.col();
-  const float g = a.splits > 1 ? 0.f : a.out.g();
-  const int64_t ld = (int64_t)a.gx * kTile;
-  float* p = a.part + (int64_t)z * a.gy * kTile * ld + c0;
+  auto row_of = [&](int r, int i) { return row0 + (COLS ? 4 : 16) * r + i; };
+  auto value = [&](int r, int i) { return f32x4{sum[i][0][r], sum[i][1][r], sum[i][2][r], sum[i][3][r]}; };
+  if (a.splits > 1) {
+    const int64_t ld = (int64_t)a.gx * kTile;
+    float* p = a.part + (int64_t)z * a.gy * kTile * ld + c0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<f32x4*>(p + row_of(r, i) * ld) = value(r, i);
+    return;
+  }
+  // (OutArgs::put, with every load on its way before the first store; past the last row
+  // that row again)
+  const OutArgs& o = a.out;
+  const float g = o.g();
+  const bool whole = c0 + 3 < o.cols;
+  int e[4][4];
+  f32x4 old[4][4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t row = row0 + (COLS ? 4 : 16) * r + i;
-      const f32x4 v = f32x4{sum[i][0][r], sum[i][1][r], sum[i][2][r], sum[i][3][r]};
-      if (a.splits > 1) *reinterpret_cast<f32x4*>(p + row * ld) = v;
-      else a.out.put(row, c0, v, g);
+      const int64_t row = min(row_of(r, i), (int64_t)o.rows - 1);
+      e[r][i] = COLS ? o.ex[row] : o.ex[min(c0 + i, o.cols - 1)];  // of the row, or of column c0 + i
+      old[r][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (o.accumulate && whole) old[r][i] = *reinterpret_cast<const f32x4u*>(o.C + row * o.ldc + c0);
+    }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = row_of(r, i);
+      f32x4 v = value(r, i);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[n] = __builtin_ldexpf(v[n], o.add - (COLS ? e[r][i] : e[0][n])) * g;
+      if (row >= o.rows) continue;
+      float* p = o.C + row * o.ldc + c0;
+      if (whole) {
+        *reinterpret_cast<f32x4u*>(p) = o.accumulate ? v + old[r][i] : v;
+      } else {
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if (c0 + n < o.cols) p[n] = o.accumulate ? p[n] + v[n] : v[n];
+      }
     }
 }
 
 // Both products of a piece in one launch, dW's items first (they are the longer
 // ones, or equal), so that the chip stays full to the end of the second.  Bound by the
-// matrix cores: 8192 x 1024 -> 4096 384 us, 1.07 PFLOP/s of 16 bits.
+// matrix cores: 8192 x 1024 -> 4096 384 us, 1.07 PFLOP/s of 16 bits; with the loads of dX's
+// old values and of the exponents ahead of the stores all eight pieces take 2 % less.
 __global__ __launch_bounds__(S::NTH, 2) void xent_products_kernel(ProductArgs w, ProductArgs x, int start) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
   const int b = blockIdx.x;
