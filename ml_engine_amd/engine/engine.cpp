@@ -1484,6 +1484,7 @@ graph Embedding::forward(const int32_t* keys, int batch, int clen, int max_clen)
   batch_ = batch;
   clen_ = clen;
   max_clen_ = max_clen;
+  scale_ = 1.0f;
   ws_bytes_ = mle_embed_scatter_ws_bytes(batch, clen);
   ws_ = mle::alloc_scratch(ws_bytes_);
   AdamParameter* T = &E;
@@ -1533,6 +1534,7 @@ graph Embedding::forward(const int32_t* keys, int batch, int clen, int max_clen,
   batch_ = batch;
   clen_ = clen;
   max_clen_ = max_clen;
+  scale_ = scale;
   ws_bytes_ = mle_embed_scatter_ws_bytes(batch, clen);  // UpdateSGD's
   ws_ = mle::alloc_scratch(ws_bytes_);
   AdamParameter* T = &E;
@@ -1702,7 +1704,8 @@ int Embedding::load_replace(const str& filepath, const std::unordered_map<str, i
 }
 
 void Embedding::UpdateSGD(const graph& X, float lr) {
-  check(mle_embed_scatter_add(mle::stream(), E.output, X->grad, keys_, batch_, clen_, max_clen_, dim, vocab, -lr, ws_,
-                              ws_bytes_),
+  // The lookup is scale_ times the table's rows, and so is their derivative.
+  check(mle_embed_scatter_add(mle::stream(), E.output, X->grad, keys_, batch_, clen_, max_clen_, dim, vocab, -lr * scale_,
+                              ws_, ws_bytes_),
         "Key Update in Embedding Space update");
 }

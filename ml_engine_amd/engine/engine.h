@@ -531,6 +531,8 @@ class Embedding {
   // output projection), any vocabulary; the table gradient by sorted tokens
   // (mle_embed_scaled_fwd, mle_embed_sorted_grad).
   graph forward(const int32_t* keys, int batch, int clen, int max_clen, float scale);
+  // One SGD step of the table from the gradient of X, the last forward's node (its
+  // scale included).
   void UpdateSGD(const graph& X, float lr = LEARNING_RATE);
   // AdamParameter checkpoint record of the table (with its Adam moments).
   void save(std::ofstream& f) const;
@@ -550,6 +552,7 @@ class Embedding {
  private:
   const int32_t* keys_ = nullptr;
   int batch_ = 0, clen_ = 0, max_clen_ = 0;
+  float scale_ = 1.0f;  // the last forward's
   void* ws_ = nullptr;
   size_t ws_bytes_ = 0;
 };

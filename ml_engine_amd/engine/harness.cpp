@@ -51,6 +51,7 @@ struct Model {
   bool loss_spin = false;  // the slot was cleared before the replay: spin for replay_seq
   float loss = 0.0f;
   graph target;  // C1 / C4: the one-hot target node (mle_model_target_read)
+  graph lookup;  // the embedding's node (mle_model_embed_sgd)
 };
 
 void* input_buffer(Model* m, size_t bytes) {
@@ -93,6 +94,7 @@ void build_c4(Model* m, const long long* d) {
   m->ffn2.reset(new Linear(F, D, "FFN2"));
   m->lm.reset(new Linear(D, V, "Projection"));
   auto x0 = m->emb->forward(ids, B, S, S);
+  m->lookup = x0;
   auto x = GraphOperations::MatrixPositionalEncoding(x0);
   auto h = GraphOperations::LayerNorm(x);
   auto a = m->mha->forward(h, true);
@@ -156,6 +158,7 @@ void build_c8(Model* m, const long long* d) {
   m->ffn2.reset(new Linear(F, D, "FFN2"));
   m->lm.reset(new Linear(D, V, "Projection"));
   auto x = m->emb->forward(ids, B, S, mx, sqrtf((float)D));
+  m->lookup = x;
   auto h = GraphOperations::Add(x, m->ffn2->forward(GraphOperations::GELU(m->ffn1->forward(x))));
   if (d[5]) m->root = m->lm->cross_entropy(h, tgt, S, mx);
   else m->root = GraphOperations::SoftMaxCrossEntropy(m->lm->forward(h), GraphOperations::OneHot(tgt, B, S, mx, V), true);
@@ -480,6 +483,15 @@ std::unordered_map<str, int> vocab_of(const char* const* words, int n) {
   return v;
 }
 }  // namespace
+
+// One SGD step of the embedding's table from its lookup's gradient, which the
+// last backward left there.
+int mle_model_embed_sgd(void* h, float lr) {
+  auto* m = static_cast<Model*>(h);
+  if (!m->emb || !m->lookup) return MLE_ERR_INVALID;
+  m->emb->UpdateSGD(m->lookup, lr);
+  return MLE_OK;
+}
 
 int mle_model_temb_save(void* h, const char* path, const char* const* words, int n) {
   auto* m = static_cast<Model*>(h);

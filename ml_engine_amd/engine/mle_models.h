@@ -77,6 +77,8 @@ int mle_model_node_read(void* h, int i, int which, float* host, size_t count);
 /* Checkpoint of every parameter (AdamParameter::save records, parameter order). */
 int mle_model_save(void* h, const char* path);
 int mle_model_load(void* h, const char* path);
+/* Embedding::UpdateSGD of the block and the language model's table, after a backward. */
+int mle_model_embed_sgd(void* h, float lr);
 /* TEMB file of the block model's embedding table; words[i] is the word of row
  * i (NULL skips).  load: replace = 0 full load (returns the saved vocabulary
  * size), 1 load_replace (returns the rows replaced); -1 on a bad file. */

@@ -43,6 +43,7 @@ _SIGS = {
     "mle_model_node_read": (I, [P, I, I, P, SZ]),
     "mle_model_save": (I, [P, C.c_char_p]),
     "mle_model_load": (I, [P, C.c_char_p]),
+    "mle_model_embed_sgd": (I, [P, F]),
     "mle_model_temb_save": (I, [P, C.c_char_p, C.POINTER(C.c_char_p), I]),
     "mle_model_temb_load": (I, [P, C.c_char_p, I, C.POINTER(C.c_char_p), I]),
 }
@@ -108,6 +109,10 @@ class Model:
     def step_graph(self, lr: float, mode: int = STEP_ALL) -> None:
         """The same step with zero_grad / forward / backward replayed as one recorded graph."""
         hip.check(lib().mle_model_step_graph(self.h, lr, mode))
+
+    def embed_sgd(self, lr: float) -> None:
+        """Embedding::UpdateSGD: one SGD step of the table from its lookup's gradient."""
+        hip.check(lib().mle_model_embed_sgd(self.h, lr))
 
     def grads_save(self) -> None:
         hip.check(lib().mle_model_grads_save(self.h))

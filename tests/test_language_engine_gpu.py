@@ -123,3 +123,32 @@ def test_replayed(dims):
             assert np.array_equal(a.get(i, 1), b.get(i, 1)) and np.array_equal(a.get(i), b.get(i)), (step, i)
     a.close()
     b.close()
+
+
+@pytest.mark.parametrize("kind", ["language", "block"])
+def test_sgd_step_of_the_table(kind):
+    """Embedding::UpdateSGD after a scaled lookup (and after a plain one) steps along the
+    gradient that the backward forms: the scale is part of it.  Every id occurs once,
+    so that both are one token's row, whatever the order of sums."""
+    B, S, D, V = 2, 16, 48 if kind == "language" else 64, 97
+    r = rng(5)
+    if kind == "language":
+        params, _, tgt = data(B, S, D, 32, V, S, seed=3)
+        m = Model("language", (B, S, D, 32, V, 1, S))
+    else:
+        m = Model("block", (B, S, D, 2, 32, V))
+        params, tgt = [], r.integers(0, V, (B, S)).astype(np.int32)
+    for i, p in enumerate(params):
+        m.set(i, p)
+    m.input(0, r.permutation(V)[: B * S].astype(np.int32).reshape(B, S))
+    m.input(1, tgt)
+    m.step(0.0, GRADS)
+    table, grad, lr = m.get(0).astype(np.float64), m.get(0, 1).astype(np.float64), 0.5
+    m.embed_sgd(lr)
+    m.sync()
+    assert np.count_nonzero(grad) > B * S * D // 2
+    # four roundings of the step (the gradient's, the scale's, the rate's, the product's)
+    # and one of the sum, each half a step of fp32 at most
+    tol = 2.0 ** -24 * (4 * lr * np.abs(grad) + np.abs(table) + lr * np.abs(grad))
+    assert (np.abs(m.get(0) - (table - lr * grad)) <= tol).all()
+    m.close()
