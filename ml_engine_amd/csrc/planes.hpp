@@ -44,6 +44,12 @@ struct Bf16 {
   }
 };
 
+// The high halves of two words side by side: `b` above `a`.
+__device__ __forceinline__ unsigned high_halves(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ unsigned bits(float x) { return __builtin_bit_cast(unsigned, x); }
+// x with its last 16 bits cleared: a bf16 number, exact for any x.
+__device__ __forceinline__ float top8(float x) { return __builtin_bit_cast(float, bits(x) & 0xffff0000u); }
+
 // A workgroup of CM x CN waves, each 64 x 64 of C; PA, PB planes of the operands.
 template <class T_, int CM_, int CN_, int PA_, int PB_>
 struct Shape {

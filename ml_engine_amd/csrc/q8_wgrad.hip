@@ -4,7 +4,11 @@
 // A kept value q 2^k is a bf16 number, and dY is the exact sum of three bf16 planes
 // (the top 8 bits of its magnitude, the next 8, the last 8), so three MFMAs make
 // the products exactly, where fp32 operands take six and drop terms.  The first
-// plane's products go to one accumulator, the others' to a second.
+// plane's products go to one accumulator, the others' to a second.  The later
+// planes hold 2^24 times their bits: those of values under 2^-110, which long
+// training meets, would otherwise lie below the smallest bf16 and be lost (a relative
+// 7e-5 at 2^-120, all towards zero).  Where the second accumulator overflows (sums of
+// 2^111 or more) and the first does not, fp32 products take those elements' place.
 //
 // A tile of 64 CM x 64 CN of dW, 32 rows of X and dY to a stage, double-buffered in
 // LDS in the unit layout of planes.hpp.  While a stage is multiplied, the next one's
@@ -103,10 +107,10 @@ __device__ __forceinline__ void load_stage(const WgradArgs& a, int m0, int n0, i
   }
 }
 
-// The high halves of two words side by side: `b` above `a`.
-__device__ __forceinline__ unsigned high_halves(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-__device__ __forceinline__ unsigned bits(float x) { return __builtin_bit_cast(unsigned, x); }
-__device__ __forceinline__ float top8(float x) { return __builtin_bit_cast(float, bits(x) & 0xffff0000u); }
+using planes::bits;
+using planes::high_halves;
+using planes::top8;
+constexpr float kLater = 0x1p24f;  // what the second and third plane are scaled by
 
 // Codes to bf16: exact, so the low half of the product is zero.
 template <class S>
@@ -125,7 +129,8 @@ __device__ __forceinline__ void put_codes(char* lds, const Raw<S>& x, int c) {
   }
 }
 // A column's eight floats to their three planes.  (An infinity's remainders are
-// NaN, and so are its products.)
+// NaN, and so are its products.  The remainders' scale is exact; beyond 2^111 it
+// makes infinities.)
 template <class S>
 __device__ __forceinline__ void put_floats(char* lds, const Raw<S>& x, int c) {
   const int u = threadIdx.x + c * S::NTH, lane = u & 63, g = (u >> 6) % S::CN, k8 = (u >> 6) / S::CN;
@@ -134,7 +139,7 @@ __device__ __forceinline__ void put_floats(char* lds, const Raw<S>& x, int c) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float a = x.y[c][2 * j], b = x.y[c][2 * j + 1];
-    const float ra = a - top8(a), rb = b - top8(b);
+    const float ra = (a - top8(a)) * kLater, rb = (b - top8(b)) * kLater;
     h[j] = high_halves(bits(a), bits(b));
     m[j] = high_halves(bits(ra), bits(rb));
     l[j] = high_halves(bits(ra - top8(ra)), bits(rb - top8(rb)));
@@ -142,6 +147,56 @@ __device__ __forceinline__ void put_floats(char* lds, const Raw<S>& x, int c) {
   *reinterpret_cast<u32x4*>(p) = h;
   *reinterpret_cast<u32x4*>(p + kUnit) = m;
   *reinterpret_cast<u32x4*>(p + 2 * kUnit) = l;
+}
+
+// The two sums to one, in hi.  Elements whose later planes overflowed are summed again
+// from fp32 products over rows [r0, r1), four of a lane's sixteen rows of dW at a time;
+// c0 is its first column, m0 the tile's first row.
+template <class S>
+__device__ __forceinline__ void join_planes(const WgradArgs& a, const planes::Lane<S>& w, int m0, int c0, int r0, int r1,
+                                            f32x4 (&hi)[4][4], const f32x4 (&lo)[4][4]) {
+  float finite = 0.f;  // stays zero while every sum is
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) finite = fmaf(lo[i][n][r], 0.f, finite);
+  unsigned over[4] = {};  // by r: bit 4 i + n
+  if (finite != 0.f) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if (__builtin_isfinite(hi[i][n][r]) & !__builtin_isfinite(lo[i][n][r])) over[r] |= 1u << (4 * i + n);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) hi[i][n] += lo[i][n] * (1.f / kLater);
+  if ((over[0] | over[1] | over[2] | over[3]) == 0) return;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    f32x4 sum[4] = {};
+#pragma unroll 1
+    for (int row = r0; row < r1; ++row) {
+      const float* dy = a.dY + row * a.lddy;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = min(m0 + w.row(i, r), a.in - 1);
+        const float x = (float)a.q[row * a.ldq + m] * q8::step_of(a.e[row * a.lde + m / q8::kGroup]);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) sum[i][n] = fmaf(x, dy[min(c0 + n, a.out - 1)], sum[i][n]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        if ((over[r] >> (4 * i + n)) & 1) hi[i][n][r] = sum[i][n];
+  }
 }
 
 template <class S, bool NARROW>
@@ -233,6 +288,7 @@ __global__ __launch_bounds__(S::NTH, 2) void q8_wgrad_kernel(WgradArgs a) {
   const int64_t ld = whole ? a.lddw : a.out;
   const bool old = whole && a.accumulate;
   const int c0 = n0 + w.col();
+  join_planes<S>(a, w, m0, c0, r0, r1, hi, lo);
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -242,7 +298,7 @@ __global__ __launch_bounds__(S::NTH, 2) void q8_wgrad_kernel(WgradArgs a) {
       float* p = out + row * ld + c0;
       f32x4 v;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) v[n] = hi[i][n][r] + lo[i][n][r];
+      for (int n = 0; n < 4; ++n) v[n] = hi[i][n][r];
       if (c0 + 3 < a.out) {
         if (old) v += *reinterpret_cast<const f32x4u*>(p);
         *reinterpret_cast<f32x4u*>(p) = v;

@@ -220,3 +220,38 @@ def test_linear_wgrad_repeats(hip):
     x, dy = r.standard_normal((3000, 200)).astype(np.float32), r.standard_normal((3000, 136)).astype(np.float32)
     a = [wgrad(hip, x, dy, 200, 7, 136, 136, np.zeros((200, 136), np.float32), np.zeros(136, np.float32), 0) for _ in range(2)]
     assert np.array_equal(a[0][0], a[1][0]) and np.array_equal(a[0][1], a[1][1])
+
+
+# (rows, in, out): few rows, so that the bound of their sums is tight; the narrow, the
+# small and the large tile, then row splits
+GRADIENT_SHAPES = [(8, 3, 130), (8, 64, 64), (16, 300, 40), (8, 2048, 2048), (4096, 48, 52)]
+
+
+@pytest.mark.parametrize("rows,inp,out", GRADIENT_SHAPES)
+@pytest.mark.parametrize("xs,ds", [(0, -112), (0, -117), (0, -122), (24, -130), (30, -140), (60, 55), (0, 118), (-100, 120)])
+def test_linear_wgrad_over_the_range_of_dy(hip, rows, inp, out, xs, ds):
+    """Gradients near fp32's smallest and largest keep all their bits: products are exact,
+    and a sum loses a step per term at most (and half of fp32's smallest, where it is that small)."""
+    r = rng(rows + inp)
+    x = (r.standard_normal((rows, inp)) * 2.0 ** xs).astype(np.float32)
+    dy = (np.clip(r.standard_normal((rows, out)), -4, 4) * 2.0 ** ds).astype(np.float32)
+    got, db = wgrad(hip, x, dy, inp, -(-inp // 32), out, out, np.zeros((inp, out), np.float32), np.zeros(out, np.float32), 0)
+    v, d = q8_ref.kept(x).astype(np.float64), dy.astype(np.float64)
+    tol = 2 * F32 * (rows + 4) * (np.abs(v).T @ np.abs(d)) + (rows + 4) * 2.0 ** -149
+    assert (np.abs(got - v.T @ d) <= tol).all()
+    assert (np.abs(db - d.sum(0)) <= 2 * F32 * (rows + 4) * np.abs(d).sum(0) + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("rows,inp,out,acc", [(8, 64, 64, 0), (16, 300, 40, 1), (8, 2048, 2048, 0), (4096, 48, 52, 1)])
+def test_linear_wgrad_columns_of_every_size(hip, rows, inp, out, acc):
+    """Columns of dY from 2^-122 to 2^116 beside each other in one tile."""
+    r = rng(rows + out)
+    x = r.standard_normal((rows, inp)).astype(np.float32)
+    size = r.choice(np.array([-122, -60, 0, 60, 116]), out)
+    dy = (np.clip(r.standard_normal((rows, out)), -4, 4) * np.exp2(size)).astype(np.float32)
+    old = (r.standard_normal((inp, out)) * np.exp2(size)).astype(np.float32)
+    got, _ = wgrad(hip, x, dy, inp, -(-inp // 32), out, out, old, np.zeros(out, np.float32), acc)
+    v, d = q8_ref.kept(x).astype(np.float64), dy.astype(np.float64)
+    ref = v.T @ d + (old.astype(np.float64) if acc else 0)
+    tol = 2 * F32 * ((rows + 4) * (np.abs(v).T @ np.abs(d)) + 2 * np.abs(old)) + (rows + 4) * 2.0 ** -149
+    assert (np.abs(got - ref) <= tol).all()
