@@ -31,6 +31,7 @@
 //   that read it; db's column sums are taken from the same registers.
 #include "gemm_args.hpp"
 #include "planes.hpp"
+#include "split_core.hpp"
 
 #include <float.h>
 
@@ -165,24 +166,12 @@ __global__ __launch_bounds__(NT) void xent_slices_kernel(const float* __restrict
 // only a stage or a few: 128 x 128 of dW to a workgroup, 64 x 64 to a wave, the
 // operands' fragments straight from memory (four neighbouring columns of eight rows to
 // a lane, transposed in its registers, as planes.hpp orders them), without LDS or
-// barriers, so that waves of different progress share a CU.  An fp32 value is the sum of
-// three bf16 planes (the first truncated: no value overflows), a product six MFMAs;
-// what is dropped is below 2^-22 of it and of either sign.  32 x 876 -> 26839 30 us, 3.2
-// TB/s written (the library's product 68); 64 x 1024 -> 32000 56 us (75).
+// barriers, so that waves of different progress share a CU.  The products are
+// split_core.hpp's: three bf16 planes of 2^24 times an fp32 value, six MFMAs.  Elements
+// that this scale makes infinite (values from 2^104, sums from 2^80) are summed again
+// from fp32 products.  32 x 876 -> 26839 30 us, 3.2 TB/s written (the library's product
+// 68); 64 x 1024 -> 32000 56 us (75).
 using planes::u32x4;
-__device__ __forceinline__ void split3(const float (&v)[8], u32x4& h, u32x4& m, u32x4& l) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const unsigned a = __builtin_bit_cast(unsigned, v[2 * j]), b = __builtin_bit_cast(unsigned, v[2 * j + 1]);
-    h[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);  // the high halves, b's above a's
-    const float ra = v[2 * j] - __builtin_bit_cast(float, a & 0xffff0000u);
-    const float rb = v[2 * j + 1] - __builtin_bit_cast(float, b & 0xffff0000u);
-    m[j] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)ra, (__bf16)rb});
-    const float sa = ra - __builtin_bit_cast(float, m[j] << 16), sb = rb - __builtin_bit_cast(float, m[j] & 0xffff0000u);
-    l[j] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)sa, (__bf16)sb});
-  }
-}
 struct DwArgs {
   const float* X;  // [rows][d]
   const float* P;  // [rows][cols]
@@ -223,16 +212,19 @@ __global__ __launch_bounds__(NT, 2) void xent_dw_kernel(DwArgs a) {
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = r0 + 8 * q + j < a.rows ? p[j][n] : 0.f;
-        sum[n] += v[j];
+        const float one = r0 + 8 * q + j < a.rows ? p[j][n] : 0.f;
+        sum[n] += one;
+        v[j] = one * split::kScale;
       }
-      split3(v, b[n][0], b[n][1], b[n][2]);
+      split::split8(v, b[n][0], b[n][1], b[n][2]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float v[8] = {x[0][i], x[1][i], x[2][i], x[3][i], x[4][i], x[5][i], x[6][i], x[7][i]};
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = x[j][i] * split::kScale;
       u32x4 h, m, l;
-      split3(v, h, m, l);
+      split::split8(v, h, m, l);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         lo[i][n] = T::mma(l, b[n][0], lo[i][n]);
@@ -244,6 +236,34 @@ __global__ __launch_bounds__(NT, 2) void xent_dw_kernel(DwArgs a) {
       }
     }
   }
+  float finite = 0.f;  // stays zero while every sum is
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      hi[i][n] = (hi[i][n] + lo[i][n]) * split::kUnscale;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) finite = fmaf(hi[i][n][r], 0.f, finite);
+    }
+  if (finite != 0.f) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      f32x4 again[4] = {};
+#pragma unroll 1
+      for (int k = 0; k < a.rows; ++k) {
+        const f32x4 p = four_of(a.P + (int64_t)k * a.cols, c0, a.cols), x = four_of(a.X + (int64_t)k * a.d, m0 + 16 * q + 4 * r, a.d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) again[i][n] = fmaf(x[i], p[n], again[i][n]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if (!__builtin_isfinite(hi[i][n][r])) hi[i][n][r] = again[i][n];
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -253,7 +273,7 @@ __global__ __launch_bounds__(NT, 2) void xent_dw_kernel(DwArgs a) {
       float* w = a.dW + (int64_t)row * a.lddw + c0;
       f32x4 v;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) v[n] = hi[i][n][r] + lo[i][n][r];
+      for (int n = 0; n < 4; ++n) v[n] = hi[i][n][r];
       if (c0 + 3 < a.cols) {
         if (a.accumulate) v += *reinterpret_cast<const f32x4u*>(w);
         *reinterpret_cast<f32x4u*>(w) = v;

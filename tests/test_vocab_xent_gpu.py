@@ -346,3 +346,26 @@ def test_no_rows(hip):
     assert (dw.numpy() == 1).all() and (db.numpy() == 1).all()
     hip.call("mle_vocab_xent_bwd", None, *shape, None, None, 1.0, None, 8, 0, dw.ptr, 20, db.ptr, 0, None, 0)
     assert not dw.numpy().any() and not db.numpy().any()
+
+
+@pytest.mark.parametrize("rows,d,vocab", [(8, 16, 66000), (48, 64, 66000), (8, 64, 900), (256, 16, 13000)])
+@pytest.mark.parametrize("size,upstream", [(0, -104), (-120, 40), (108, 0), (0, 90)])
+def test_gradients_near_the_smallest_and_the_largest(hip, rows, d, vocab, size, upstream):
+    """X of 2^size against W of 2^-size, and a scaled loss: P or X near fp32's smallest numbers,
+    or X near its largest, on a softmax that is the same."""
+    c = Case(hip, rows, d, vocab, ignored=0.2)
+    c.x = (c.x * 2.0 ** size).astype(np.float32)
+    c.w = (c.w * 2.0 ** min(-size, 80)).astype(np.float32)
+    if size == 108:
+        c.w = (c.w * 2.0 ** -8).astype(np.float32)
+    c.put()
+    ref, tol = c.exact(upstream=2.0 ** upstream)
+    c.forward()
+    dx, dw, db = c.backward(upstream=2.0 ** upstream)
+    # (what is below 2^-126 holds multiples of 2^-149: half a one for each P and each sum)
+    x = np.abs(np.where(c.valid()[:, None], c.x, 0).astype(np.float64))
+    w = np.abs(c.w.astype(np.float64))
+    small = 2.0 ** -149
+    close(dw, ref["dw"], tol["dw"] + small * (x.sum(0)[:, None] + rows + 4), "dw")
+    close(dx, ref["dx"], tol["dx"] + small * (w.sum(1) + vocab + 4), "dx")
+    close(db, ref["db"], tol["db"] + small * (2 * rows + 4), "db")
