@@ -512,8 +512,11 @@ int mle_softmax_xent_keys_fwd_rowstats_read(mle_stream stream, const float* logi
  * gradient 0; its weights are finite, of any size); a row with no finite logit
  * has no finite loss.  The logits are
  * formed in pieces of the vocabulary in ws, in the forward and again in the
- * backward; ws carries nothing from one call to the next.  fp32 accuracy; sums in
- * a fixed order.  X, W, dX and dW are buffers of their own; rows, d and vocab are at
+ * backward; ws carries nothing from one call to the next.  Sums are fp32's, in a
+ * fixed order.  With many logits (from 192 rows) the products' operands X, W and P
+ * are held in 22 bits under a common power of two: a feature of X or W, a row of P for
+ * dX, a column of P over 64 rows for dW; what is below 2^-28 of the largest there (of 1
+ * in a row of P) is held to 2^-50 of it.  X, W, dX and dW are buffers of their own; rows, d and vocab are at
  * most 2^30.
  * The reference forms and keeps them (SoftMaxCrossEntropy, Engine/engine.cu:2064-2124). */
 size_t mle_vocab_xent_ws_bytes(int rows, int d, int vocab);

@@ -155,27 +155,27 @@ __device__ __forceinline__ void multiply(const Operand& A, const Operand& B, int
   }
 }
 
-// The same with one accumulator, cleared every `run` stages: begin(first stage of
-// the run) is called before the run, whose loads are then there at its end, and end()
-// after it, to add the sums to what the caller keeps.  For operands whose later
-// planes are not scaled against the first, so that all products are of one scale.
+// The same with the sums cleared every `run` stages: begin(first stage of the run) is
+// called before the run, whose loads are then there at its end, and end() after it, to
+// add the sums to what the caller keeps.
 template <class S, class F, class G>
 __device__ __forceinline__ void multiply_runs(const Operand& A, const Operand& B, int tm, int tn, int k0, int k1, int run,
-                                              char* lds, const Lane<S>& w, f32x4 (&acc)[4][4], F begin, G end) {
+                                              char* lds, const Lane<S>& w, f32x4 (&hi)[4][4], f32x4 (&lo)[4][4], F begin,
+                                              G end) {
   if (k0 < k1) stage_load<S>(A, B, tm, tn, k0, lds);
   for (int kr = k0; kr < k1; kr += run) {
     begin(kr);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) acc[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < 4; ++n) hi[i][n] = lo[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int ke = min(k1, kr + run);
     for (int k = kr; k < ke; ++k) {
       char* cur = lds + ((k - k0) & 1) * S::STAGE;
       char* nxt = lds + (((k - k0) & 1) ^ 1) * S::STAGE;
       __syncthreads();
       if (k + 1 < k1) stage_load<S>(A, B, tm, tn, k + 1, nxt);
-      stage_mma<S>(cur, w, acc, acc);
+      stage_mma<S>(cur, w, hi, lo);
     }
     end();
   }

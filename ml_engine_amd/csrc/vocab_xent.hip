@@ -25,7 +25,10 @@
 //     dX      W by feature; P as it is, |P| <= 1
 //     dW      X by feature; P by column and 64 rows, whose partial sums are
 //             scaled back one by one
-//   so that a small gradient of a column or feature is as exact as a large one.
+//   so that a small gradient of a column or feature is as exact as a large one.  Within
+//   a scale, values down to 2^-28 of the largest keep their 22 bits (the second plane
+//   holds 2^11 times the remainder; without that 2^-17, and a column's small
+//   probabilities were lost beside a target's), and smaller ones are held to 2^-50 of it.
 //
 //   P leaves the tile that forms it in both orders, packed for the two products
 //   that read it; db's column sums are taken from the same registers.
@@ -296,7 +299,7 @@ __global__ __launch_bounds__(NT, 2) void xent_dw_kernel(DwArgs a) {
 using planes::Operand;
 using S = planes::Shape<planes::Fp16, 2, 2, 2, 2>;  // 128 x 128 of C, two workgroups to a CU
 constexpr int kTile = 128;
-constexpr int kLo = 11;      // the second plane's scale against the first, where it has one
+constexpr int kLo = 11;      // the second plane's scale against the first
 constexpr int kTop = 15;     // scaled magnitudes are below 2^kTop
 constexpr int kNone = -400;  // exponent of a feature that is zero everywhere
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -480,7 +483,7 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(PackAll a) {
   unsigned b = blockIdx.x;
   if (b < a.nxl) return planes::pack_rows<true, kLo>(a.xl, b);
   b -= a.nxl;
-  if (b < a.nxt) return planes::pack_cols<false, 0>(a.xt, b);
+  if (b < a.nxt) return planes::pack_cols<false, kLo>(a.xt, b);
   b -= a.nxt;
   if (b < a.nwl) return planes::pack_cols<true, kLo>(a.wl, b);
   planes::pack_rows<false, kLo>(a.wn, b - a.nwl);
@@ -632,7 +635,7 @@ __global__ __launch_bounds__(S::NTH, 2) void xent_tile_kernel(TileArgs a) {
       float x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = __builtin_ldexpf(l[j & 3][n][2 * h + (j >> 2)], ec[n]);
-      planes::put16<0>(a.pcol + planes::chunk_at<2>(a.pcols / 16, c0 + n, row0 + 8 * h), x);
+      planes::put16<kLo>(a.pcol + planes::chunk_at<2>(a.pcols / 16, c0 + n, row0 + 8 * h), x);
     }
   // by row: lanes 2 j and 2 j + 1 have 8 consecutive columns together; the even one
   // takes rows i = 0, 1, the odd one 2, 3.  Rows lie in a block by 4 r + q here (q + 4 r
@@ -750,15 +753,17 @@ struct ProductArgs {
 };
 
 // COLS false: dX = P W^T, whose rows lie in their blocks as the tile kernel left
-// them.  true: dW = X^T P, whose sums over each 64 rows (two stages) are scaled back
-// column by column.
+// them.  true: dW = X^T P, whose sums over each 64 rows (two stages) are joined and scaled
+// back column by column (192 sums to a lane, 244 registers; all three cross entropy
+// sizes of 1000 rows and more take 2 % longer than with one sum for both planes,
+// which needs them on one scale).
 template <bool COLS>
 __device__ __forceinline__ void xent_product(const ProductArgs& a, int item, char* lds) {
   const planes::Lane<S> w;
   int tm, tn, z;
   gemm::item_tile(item, a.items, a.gx, a.gy, tm, tn, z);
   const int k0 = z * a.per, k1 = min(a.nk, k0 + a.per);
-  f32x4 sum[4][4], acc[4][4];
+  f32x4 sum[4][4], hi[4][4], lo[4][4];
   if (COLS) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -767,20 +772,20 @@ __device__ __forceinline__ void xent_product(const ProductArgs& a, int item, cha
     const float* fac = a.cfac + (int64_t)tn * kTile + w.col();
     f32x4 f;
     planes::multiply_runs<S>(
-        a.A, a.B, tm, tn, k0, k1, 2, lds, w, acc,
+        a.A, a.B, tm, tn, k0, k1, 2, lds, w, hi, lo,
         [&](int k) { f = *reinterpret_cast<const f32x4*>(fac + (int64_t)(k >> 1) * a.pcols); },
         [&]() {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int n = 0; n < 4; ++n) sum[i][n] += f[n] * acc[i][n];
+            for (int n = 0; n < 4; ++n) sum[i][n] += f[n] * (hi[i][n] + lo[i][n] * (1.f / (1 << kLo)));
         });
   } else {
-    planes::multiply<S>(a.A, a.B, tm, tn, k0, k1, lds, w, sum, acc);
+    planes::multiply<S>(a.A, a.B, tm, tn, k0, k1, lds, w, sum, lo);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) sum[i][n] += acc[i][n] * (1.f / (1 << kLo));
+      for (int n = 0; n < 4; ++n) sum[i][n] += lo[i][n] * (1.f / (1 << kLo));
   }
   const int64_t row0 = (int64_t)tm * kTile + 64 * w.wm + (COLS ? 16 : 4) * w.q;
   const int c0 = tn * kTile + w.col();

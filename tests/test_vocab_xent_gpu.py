@@ -369,3 +369,59 @@ def test_gradients_near_the_smallest_and_the_largest(hip, rows, d, vocab, size, 
     close(dw, ref["dw"], tol["dw"] + small * (x.sum(0)[:, None] + rows + 4), "dw")
     close(dx, ref["dx"], tol["dx"] + small * (w.sum(1) + vocab + 4), "dx")
     close(db, ref["db"], tol["db"] + small * (2 * rows + 4), "db")
+
+
+# few logits, with the library's product and with dW's own kernel; planes of 128 and
+# of several hundred rows
+@pytest.mark.parametrize("rows,vocab", [(60, 900), (48, 66000), (256, 13000), (700, 6000)])
+@pytest.mark.parametrize("gap", [7, 12, 17])
+def test_small_probabilities_beside_targets(hip, rows, vocab, gap):
+    """Columns that are some rows' targets and hardly likely in the others, which alone have
+    certain features: those entries of dW are sums of small P and as exact as large ones,
+    down to 2^-50 of the column's largest P."""
+    r = rng(rows + gap)
+    d, hot = 8, 16
+    c = Case(hip, rows, d, vocab, bias=False, ignored=0.0)
+    target = np.arange(rows) % 64 < hot  # rows with a hot column as their id, in every 64
+    c.keys = np.where(target, np.arange(rows) % 64, r.integers(hot, vocab, rows)).astype(np.int32)
+    c.x = r.standard_normal((rows, d)).astype(np.float32)
+    c.x[target, 1:] = 0
+    c.x[:, 0] = 1
+    c.w = np.zeros((d, vocab), np.float32)  # logits: -gap in hot columns, 0 in the others
+    c.w[0, :hot] = -gap
+    c.put()
+    c.forward()
+    _, dw, _ = c.backward()
+    lse = np.log(hot * np.exp(-gap) + (vocab - hot))
+    p = np.exp(-gap - lse) * c.scale
+    x = c.x[~target, 1:].astype(np.float64)
+    # the logits are whole numbers; the sum of their exponentials, its logarithm, the
+    # difference and its exponential, the scale, then the products' sum
+    rel = STEP * (16 + np.log2(vocab) + 2 * gap + 2 * lse + rows + 4)
+    tol = np.abs(x).sum(0) * (p * rel + 2.0 ** -50 * c.scale)
+    close(dw[1:, :hot], np.repeat((x.sum(0) * p)[:, None], hot, 1), tol[:, None], "dw")
+
+
+@pytest.mark.parametrize("rows,vocab", [(60, 900), (48, 66000), (256, 13000), (700, 6000)])
+@pytest.mark.parametrize("ratio", [20, 34])
+def test_small_rows_beside_a_large_one(hip, rows, vocab, ratio):
+    """A feature that one row has 2^ratio times as large as the others: columns that this row
+    gives no probability keep the others' bits, down to 2^-50 of the feature's largest value."""
+    r = rng(rows + ratio)
+    d, cold = 8, 16
+    c = Case(hip, rows, d, vocab, bias=False, ignored=0.0)
+    c.keys = r.integers(cold, vocab, rows).astype(np.int32)
+    c.x = r.standard_normal((rows, d)).astype(np.float32)
+    c.x[:, 0] = 0
+    c.x[5, 0] = 1       # this row's logits of the cold columns are -300: their P is zero
+    c.x[5, 1:] = 2.0 ** ratio
+    c.w = np.zeros((d, vocab), np.float32)
+    c.w[0, :cold] = -300
+    c.put()
+    c.forward()
+    _, dw, _ = c.backward()
+    others = np.delete(c.x, 5, 0)[:, 1:].astype(np.float64)
+    p, lse = c.scale / vocab, np.log(vocab)
+    rel = STEP * (16 + np.log2(vocab) + 2 * lse + rows + 4)
+    tol = p * (np.abs(others).sum(0) * rel + 2.0 ** (ratio - 50) * rows)
+    close(dw[1:, :cold], np.repeat((others.sum(0) * p)[:, None], cold, 1), tol[:, None], "dw")
