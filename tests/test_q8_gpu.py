@@ -255,3 +255,42 @@ def test_linear_wgrad_columns_of_every_size(hip, rows, inp, out, acc):
     ref = v.T @ d + (old.astype(np.float64) if acc else 0)
     tol = 2 * F32 * ((rows + 4) * (np.abs(v).T @ np.abs(d)) + 2 * np.abs(old)) + (rows + 4) * 2.0 ** -149
     assert (np.abs(got - ref) <= tol).all()
+
+
+OTHERS = {  # the function and its derivative
+    "tanh": (np.tanh, lambda x: 1 - np.tanh(x) ** 2),
+    "sigmoid": (lambda x: 1 / (1 + np.exp(-x)), lambda x: 1 / (2 + np.exp(x) + np.exp(-x))),
+    "leaky_relu": (lambda x: np.where(x < 0, 0.01 * x, x), lambda x: np.where(x < 0, 0.01, 1.0)),
+}
+
+
+@pytest.mark.parametrize("kind", OTHERS)
+@pytest.mark.parametrize("rows,cols,pad,acc", [(1, 1, 0, 0), (33, 70, 2, 1), (20, 330, 0, 0)])
+def test_other_activations(hip, kind, rows, cols, pad, acc):
+    """tanh, sigmoid and leaky ReLU: each by its formula, and the elementwise calls' bits."""
+    r = rng(cols + 1)
+    f, df = OTHERS[kind]
+    x = (r.standard_normal((rows, cols)) * 3).astype(np.float32)
+    dy, old = (r.standard_normal((rows, cols)).astype(np.float32) for _ in range(2))
+    ld, ng = cols + pad, -(-cols // 32)
+    B = hip.Buffer
+    gx, gy = B.from_array(padded(x, ld, 7.0)), B.from_array(np.full((rows, ld), 5, np.float32))
+    gq, ge = B.empty((rows, ld), np.int8), B.empty((rows, ng), np.uint8)
+    hip.call("mle_q8_act_fwd", None, hip.ACT[kind], rows, cols, gx.ptr, ld, gy.ptr, ld, gq.ptr, ld, ge.ptr, ng)
+    q, e = q8_ref.quantize(x)
+    assert np.array_equal(gq.numpy()[:, :cols], q) and np.array_equal(ge.numpy(), e)
+    y = gy.numpy()
+    # an exponential or a tanh of a few steps, a division and two sums, of values up to 1 or |x|
+    assert (np.abs(y[:, :cols] - f(x.astype(np.float64))) <= 16 * F32 * (np.abs(x) + 1)).all() and (y[:, cols:] == 5).all()
+    fx, fy = B.from_array(x), B.empty((rows, cols))
+    hip.call("mle_act_fwd", None, hip.ACT[kind], fx.ptr, fy.ptr, rows * cols)
+    assert np.array_equal(fy.numpy(), y[:, :cols])
+    gdy, gdx = B.from_array(padded(dy, ld, 7.0)), B.from_array(padded(old, ld, 3.0))
+    hip.call("mle_q8_act_bwd", None, hip.ACT[kind], rows, cols, gq.ptr, ld, ge.ptr, ng, gdy.ptr, ld, gdx.ptr, ld, acc)
+    dx, v = gdx.numpy(), q8_ref.values(q, e).astype(np.float64)
+    ref = df(v) * dy + (old if acc else 0)
+    # the same operations again, of a derivative of at most 1
+    assert (np.abs(dx[:, :cols] - ref) <= F32 * (16 * np.abs(dy) + 2 * np.abs(old))).all() and (dx[:, cols:] == 3).all()
+    fv, fdy, fdx = B.from_array(v.astype(np.float32)), B.from_array(dy), B.from_array(old)
+    hip.call("mle_act_bwd", None, hip.ACT[kind], fv.ptr, fdy.ptr, fdx.ptr, rows * cols, acc)
+    assert np.array_equal(fdx.numpy(), dx[:, :cols])
