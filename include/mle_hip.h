@@ -518,6 +518,14 @@ int mle_softmax_xent_keys_fwd_rowstats_read(mle_stream stream, const float* logi
  * dX, a column of P over 64 rows for dW; what is below 2^-28 of the largest there (of 1
  * in a row of P) is held to 2^-50 of it.  X, W, dX and dW are buffers of their own; rows, d and vocab are at
  * most 2^30.
+ * The workspace is no fraction of the logits but about a constant: with many logits
+ * 8 bytes for each of a piece (256 MiB of them at most, what the logits and their gradient
+ * take), each element of X (32768 rows at most) and of the piece's columns of W, and
+ * the products' partial sums.  It is below the logits with their gradient where these
+ * are well above 256 MiB (8192 x 512 -> 8000 393 MB against 524, 8192 x 1024 ->
+ * 32000 422 against 2097), and above them for smaller problems (1000 x 330 -> 10007 176
+ * against 80, 2048 x 1024 -> 16000 448 against 262, 300 x 4096 -> 128000 2345 against
+ * 307, where W is 2097): a program short of memory there keeps its logits.
  * The reference forms and keeps them (SoftMaxCrossEntropy, Engine/engine.cu:2064-2124). */
 size_t mle_vocab_xent_ws_bytes(int rows, int d, int vocab);
 int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const float* X, int64_t ldx, const float* W,

@@ -104,3 +104,18 @@ def test_vocab_xent_workspace_stays_below_the_logits(rows, d, vocab):
     gradient, which it replaces, beside what the weights and inputs take anyway."""
     need = hip.lib().mle_vocab_xent_ws_bytes(rows, d, vocab)
     assert need <= 0.6 * 8 * rows * vocab + 3 * 4 * (rows * d + d * vocab), need
+
+
+@pytest.mark.parametrize("rows,d,vocab", [(1000, 330, 10007), (2048, 1024, 16000), (200, 1024, 32000), (300, 4096, 128000),
+                                          (512, 1024, 4096), (192, 64, 16000), (4096, 512, 8000), (8192, 256, 1000),
+                                          (200000, 16, 1100), (1000, 5000, 1000)])
+def test_vocab_xent_workspace_of_middle_sizes(rows, d, vocab):
+    """Where the logits themselves are no more than the workspace: 8 bytes for each logit of a
+    piece (256 MiB at most), each element of X and of the piece's columns of W, in whole
+    tiles of 128, and as much again for partial sums and statistics at most."""
+    up = lambda n: -(-n // 128) * 128  # noqa: E731
+    r, f = up(min(rows, 32768)), up(d)
+    pieces = -(-vocab // max(128, (1 << 25) // r // 128 * 128))
+    piece = up(-(-vocab // pieces))
+    need = hip.lib().mle_vocab_xent_ws_bytes(rows, d, vocab)
+    assert 0 < need <= 2 * 8 * (r * piece + f * (r + piece)), need
