@@ -254,7 +254,8 @@ __global__ __launch_bounds__(NT, 2) void xent_dw_kernel(DwArgs a) {
       f32x4 again[4] = {};
 #pragma unroll 1
       for (int k = 0; k < a.rows; ++k) {
-        const f32x4 p = four_of(a.P + (int64_t)k * a.cols, c0, a.cols), x = four_of(a.X + (int64_t)k * a.d, m0 + 16 * q + 4 * r, a.d);
+        const f32x4 p = four_of(a.P + (int64_t)k * a.cols, c0, a.cols);
+        const f32x4 x = four_of(a.X + (int64_t)k * a.d, m0 + 16 * q + 4 * r, a.d);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -526,10 +527,12 @@ __device__ __forceinline__ float row_add(float x) {
   return x + rotated<0x121>(x);
 }
 
-// A tile of logits, and from them the rows' statistics or P.  Bound by the matrix cores
-// (128 x 128 tiles keep two workgroups of 64 KB to a CU, so that one's epilogue runs beside
-// the other's products): 8192 x 1024 -> 4096 190 us with the statistics, 1.08 PFLOP/s
-// of 16 bits; 217 us with P, whose two packed copies are 268 MB written.
+// A tile of logits, and from them the rows' statistics or P.  Bound by the products' loop,
+// matrix cores 54 and 46 % busy at 2.03-2.1 GHz (128 x 128 tiles keep two workgroups of
+// 64 KB to a CU, so that one's epilogue runs beside the other's products): 8192 x 1024 -> 4096 182 us with the statistics, 1.13 PFLOP/s
+// of 16 bits; 208 us with P, whose two packed copies are 268 MB written.
+// Exponentials are the hardware's, exp2 of the logit less its maximum or log-sum, times
+// log2 e: that product's rounding is no larger than the difference's own.
 template <bool GRAD>
 __global__ __launch_bounds__(S::NTH, 2) void xent_tile_kernel(TileArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
@@ -838,7 +841,8 @@ __device__ __forceinline__ void xent_product(const ProductArgs& a, int item, cha
 
 // Both products of a piece in one launch, dW's items first (they are the longer
 // ones, or equal), so that the chip stays full to the end of the second.  Bound by the
-// matrix cores: 8192 x 1024 -> 4096 384 us, 1.07 PFLOP/s of 16 bits; with the loads of dX's
+// products' loop (matrix cores 53 % busy at 2.05 GHz): 8192 x 1024 -> 4096 375 us, 1.10
+// PFLOP/s of 16 bits; with the loads of dX's
 // old values and of the exponents ahead of the stores all eight pieces take 2 % less.
 __global__ __launch_bounds__(S::NTH, 2) void xent_products_kernel(ProductArgs w, ProductArgs x, int start) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];

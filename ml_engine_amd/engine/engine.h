@@ -440,7 +440,8 @@ class Linear {
   // SoftMaxCrossEntropy(forward(X), OneHot(keys, batch, clen, max_clen, out_features()), last)
   // in one node that keeps no logits and no gradient of them (mle_vocab_xent_*):
   // the same loss, and the same gradients of X, W1 and B1, for ids in the
-  // vocabulary.  A position whose id is outside it (INT_MIN past a sequence's
+  // vocabulary, to the rounding of fp32 sums (from 192 rows the products'
+  // operands are held in 22 bits).  A position whose id is outside it (INT_MIN past a sequence's
   // end) has no loss and no gradient.  X is [batch, 1, clen, in_features()];
   // keys are device ids [batch][max_clen].
   graph cross_entropy(const graph& X, const int32_t* keys, int clen, int max_clen, const bool last = true);
