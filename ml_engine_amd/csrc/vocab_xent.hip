@@ -62,11 +62,18 @@ struct RowState {
   float max, sum, target, pad;  // sum of exp(l - max)
 };
 
+// A stored logit x of a piece's column c: -infinity where the bias (the piece's, or
+// null) takes the entry out, also if its weights' product is infinite or a NaN.
+__device__ __forceinline__ float logit(float x, const float* bias, int c) {
+  return x != x && bias && bias[c] == -INFINITY ? -INFINITY : x;
+}
+
 // A row of a piece to L threads: its maximum and sum join the row's.  A wave to a row
 // of few columns (8192 x 300: 36 us with a workgroup to it, 5.6 so).
 template <int L>
 __global__ __launch_bounds__(L < NT ? NT : L) void xent_stats_kernel(const float* __restrict__ l, int nrows, int cols, int v0,
-                                                                     Rows rows, RowState* __restrict__ state, int first) {
+                                                                     const float* __restrict__ bias, Rows rows,
+                                                                     RowState* __restrict__ state, int first) {
   __shared__ float red[L / 64];
   const int64_t r = L < NT ? (int64_t)blockIdx.x * (NT / L) + threadIdx.x / L : blockIdx.x;
   const int t = threadIdx.x % L;
@@ -74,12 +81,17 @@ __global__ __launch_bounds__(L < NT ? NT : L) void xent_stats_kernel(const float
   const float* x = l + r * cols;
   float m = -FLT_MAX;
 #pragma unroll 4
-  for (int c = t; c < cols; c += L) m = fmaxf(m, x[c]);
+  for (int c = t; c < cols; c += L) m = fmaxf(m, x[c]);  // (not of a NaN)
   m = L == 64 ? wave_max(m) : block_max<L>(m, red);
   float s = 0.f;
 #pragma unroll 4
   for (int c = t; c < cols; c += L) s += expf(x[c] - m);
   s = L == 64 ? wave_sum(s) : block_sum<L>(s, red);
+  if (s != s && bias) {  // a NaN: those of entries that the bias takes out do not count
+    s = 0.f;
+    for (int c = t; c < cols; c += L) s += expf(logit(x[c], bias, c) - m);
+    s = L == 64 ? wave_sum(s) : block_sum<L>(s, red);
+  }
   if (t != 0) return;
   RowState n{m, s, 0.f, 0.f};
   if (!first) {
@@ -89,7 +101,7 @@ __global__ __launch_bounds__(L < NT ? NT : L) void xent_stats_kernel(const float
     n.target = o.target;
   }
   const int k = rows.key(r);
-  if (k >= v0 && k < v0 + cols) n.target = x[k - v0];
+  if (k >= v0 && k < v0 + cols) n.target = logit(x[k - v0], bias, k - v0);
   state[r] = n;
 }
 
@@ -118,7 +130,8 @@ __global__ __launch_bounds__(1024) void xent_finish_kernel(const RowState* __res
 __global__ __launch_bounds__(NT) void xent_grad_kernel(float* l, int nrows, int cols, int v0, Rows rows,
                                                        const float* __restrict__ lse, const float* __restrict__ upstream,
                                                        float scale, unsigned blocks, const float* __restrict__ X, int64_t ldx,
-                                                       int d, float* __restrict__ out, float* __restrict__ db) {
+                                                       int d, float* __restrict__ out, float* __restrict__ db,
+                                                       const float* __restrict__ bias) {
   const bool logits = blockIdx.x < blocks;
   const unsigned n = logits ? cols : d;
   const int64_t e0 = (int64_t)(logits ? blockIdx.x : blockIdx.x - blocks) * (4 * NT);
@@ -142,7 +155,7 @@ __global__ __launch_bounds__(NT) void xent_grad_kernel(float* l, int nrows, int 
     if (r >= nrows) continue;
     if (logits) {
       if (db && r == 0) db[v0 + c] = 0.f;
-      l[r * cols + c] = key[i] >= 0 ? g * (expf(x[i] - z[i]) - ((int)c + v0 == key[i] ? 1.f : 0.f)) : 0.f;
+      l[r * cols + c] = key[i] >= 0 ? g * (expf(logit(x[i], bias, (int)c) - z[i]) - ((int)c + v0 == key[i] ? 1.f : 0.f)) : 0.f;
     } else {
       out[r * d + c] = key[i] >= 0 ? x[i] : 0.f;
     }
@@ -1301,8 +1314,8 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
                     bias ? bias + v0 : nullptr, gws, p.gemm));
     // (with many rows a wave to each is enough to fill the chip)
     if (n <= 1024 || rows >= 2048)
-      mle::launch(xent_stats_kernel<64>, (unsigned)(((int64_t)rows + 3) / 4), NT, 0, s, l, rows, n, v0, rw, state, v0 == 0 ? 1 : 0);
-    else mle::launch(xent_stats_kernel<1024>, (unsigned)rows, 1024, 0, s, l, rows, n, v0, rw, state, v0 == 0 ? 1 : 0);
+      mle::launch(xent_stats_kernel<64>, (unsigned)(((int64_t)rows + 3) / 4), NT, 0, s, l, rows, n, v0, bias ? bias + v0 : nullptr, rw, state, v0 == 0 ? 1 : 0);
+    else mle::launch(xent_stats_kernel<1024>, (unsigned)rows, 1024, 0, s, l, rows, n, v0, bias ? bias + v0 : nullptr, rw, state, v0 == 0 ? 1 : 0);
   }
   mle::launch(xent_finish_kernel, 1u, 1024, 0, s, state, rows, rw, loss_scale, lse, row_loss, loss, 0);
   return check_launch("mle_vocab_xent_fwd");
@@ -1347,7 +1360,7 @@ int mle_vocab_xent_bwd(mle_stream stream, int rows, int d, int vocab, const floa
     TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr,
                     bias ? bias + v0 : nullptr, gws, p.gemm));
     mle::launch(xent_grad_kernel, groups(n) + (dW && v0 == 0 ? groups(d) : 0u), NT, 0, s, l, rows, n, v0, rw, lse, upstream,
-                grad_scale, groups(n), X, ldx, d, xs, db && !accumulate_dw && !dense && !own_dw ? db : nullptr);
+                grad_scale, groups(n), X, ldx, d, xs, db && !accumulate_dw && !dense && !own_dw ? db : nullptr, bias ? bias + v0 : nullptr);
     if (dense) {
       TRY(mle_linear_bwd_ex(stream, rows, d, vocab, 1, xs, l, 0, W, 0, dX, accumulate_dx, dW, db, 0, accumulate_dw, gws, p.gemm));
       break;

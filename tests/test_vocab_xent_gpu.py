@@ -425,3 +425,30 @@ def test_small_rows_beside_a_large_one(hip, rows, vocab, ratio):
     rel = STEP * (16 + np.log2(vocab) + 2 * lse + rows + 4)
     tol = p * (np.abs(others).sum(0) * rel + 2.0 ** (ratio - 50) * rows)
     close(dw[1:, :cold], np.repeat((others.sum(0) * p)[:, None], cold, 1), tol[:, None], "dw")
+
+
+@pytest.mark.parametrize("rows,vocab", [(33, 400), (5, 20011), (48, 66000), (1000, 4600)])
+@pytest.mark.parametrize("big", [3e38, 1e20])
+def test_masked_entries_of_any_weights(hip, rows, vocab, big):
+    """Entries that the bias takes out, with weights whose products overflow (both signs in a
+    sum): as if their weights were zero."""
+    c = Case(hip, rows, 64, vocab)
+    out = np.arange(0, vocab, 3)
+    c.keys[np.isin(c.keys, out) & c.valid()] += 1
+    c.b[out] = 0
+    c.w[:, out] = 0
+    ref_b = c.b.copy()
+    c.b[out] = -1e9  # no probability left in 64 bits either
+    ref, tol = c.exact()
+    c.b = ref_b
+    c.b[out] = -np.inf
+    c.w[:, out] = (big * rng(vocab).choice(np.array([-1, 1]), (64, out.size))).astype(np.float32)
+    c.put()
+    lse, row_loss, loss = c.forward()
+    dx, dw, db = c.backward()
+    keep = np.setdiff1d(np.arange(vocab), out)
+    close(lse, ref["lse"], tol["lse"] + STEP * np.abs(ref["lse"]), "lse")
+    close(row_loss, ref["row_loss"], tol["row_loss"] + STEP * np.abs(ref["row_loss"]), "row_loss")
+    close(dx, ref["dx"], tol["dx"], "dx")
+    close(dw[:, keep], ref["dw"][:, keep], tol["dw"][:, keep], "dw")
+    assert not dw[:, out].any() and not db[out].any()
