@@ -516,8 +516,9 @@ int mle_softmax_xent_keys_fwd_rowstats_read(mle_stream stream, const float* logi
  * fixed order.  With many logits (from 192 rows) the products' operands X, W and P
  * are held in 22 bits under a common power of two: a feature of X or W, a row of P for
  * dX, a column of P over 64 rows for dW; what is below 2^-28 of the largest there (of 1
- * in a row of P) is held to 2^-50 of it.  X, W, dX and dW are buffers of their own; rows, d and vocab are at
- * most 2^30.
+ * in a row of P) is held to 2^-50 of it, and each product in a logit to 2^-50 of the
+ * largest of 32768 rows and a piece.  X, W, dX and dW are buffers of their own; rows,
+ * d and vocab are at most 2^30.
  * The workspace is no fraction of the logits but about a constant: with many logits
  * 8 bytes for each of a piece (256 MiB of them at most, what the logits and their gradient
  * take), each element of X (32768 rows at most) and of the piece's columns of W, and
