@@ -163,14 +163,14 @@ __device__ __forceinline__ void join_planes(const WgradArgs& a, const planes::La
 #pragma unroll
       for (int r = 0; r < 4; ++r) finite = fmaf(lo[i][n][r], 0.f, finite);
   unsigned over[4] = {};  // by r: bit 4 i + n
-  if (finite != 0.f) {
+  if (finite != 0.f) {  // (what lies past dY's columns may be anything: those are not stored)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int n = 0; n < 4; ++n)
-          if (__builtin_isfinite(hi[i][n][r]) & !__builtin_isfinite(lo[i][n][r])) over[r] |= 1u << (4 * i + n);
+          if ((c0 + n < a.out) & __builtin_isfinite(hi[i][n][r]) & !__builtin_isfinite(lo[i][n][r])) over[r] |= 1u << (4 * i + n);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)

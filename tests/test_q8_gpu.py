@@ -294,3 +294,18 @@ def test_other_activations(hip, kind, rows, cols, pad, acc):
     fv, fdy, fdx = B.from_array(v.astype(np.float32)), B.from_array(dy), B.from_array(old)
     hip.call("mle_act_bwd", None, hip.ACT[kind], fv.ptr, fdy.ptr, fdx.ptr, rows * cols, acc)
     assert np.array_equal(fdx.numpy(), dx[:, :cols])
+
+
+@pytest.mark.parametrize("rows,inp,out", [(100, 96, 40), (8, 2048, 2048), (3000, 48, 52), (20, 3, 70)])
+@pytest.mark.parametrize("bad", [0x7F800000, 0xFF800000, 0x7FC00000, 0x7F800001])
+def test_linear_wgrad_not_finite_gradients_stay_in_their_column(hip, rows, inp, out, bad):
+    """An infinity or a NaN (also one whose payload is in the last bits only) in dY: its
+    column of dW is NaN, the others are as they were."""
+    r = rng(rows)
+    x, dy = r.standard_normal((rows, inp)).astype(np.float32), r.standard_normal((rows, out)).astype(np.float32)
+    args = (inp, -(-inp // 32), out, out, np.zeros((inp, out), np.float32), np.zeros(out, np.float32), 0)
+    want, want_db = wgrad(hip, x, dy, *args)
+    dy.view(np.uint32)[rows // 2, 17] = bad
+    got, db = wgrad(hip, x, dy, *args)
+    assert np.isnan(got[:, 17]).all() and not np.isfinite(db[17])
+    assert np.array_equal(np.delete(got, 17, 1), np.delete(want, 17, 1)) and np.array_equal(np.delete(db, 17), np.delete(want_db, 17))
