@@ -542,8 +542,9 @@ __device__ __forceinline__ float row_add(float x) {
 
 // A tile of logits, and from them the rows' statistics or P.  Bound by the products' loop,
 // matrix cores 54 and 46 % busy at 2.03-2.1 GHz (128 x 128 tiles keep two workgroups of
-// 64 KB to a CU, so that one's epilogue runs beside the other's products): 8192 x 1024 -> 4096 182 us with the statistics, 1.13 PFLOP/s
-// of 16 bits; 208 us with P, whose two packed copies are 268 MB written.
+// 64 KB to a CU, so that one's epilogue runs beside the other's products): 8192 x 1024 ->
+// 4096 182 us with the statistics, 1.13 PFLOP/s of 16 bits; 208 us with P, whose two
+// packed copies are 268 MB written.
 // Exponentials are the hardware's, exp2 of the logit less its maximum or log-sum, times
 // log2 e: that product's rounding is no larger than the difference's own.
 template <bool GRAD>
@@ -855,8 +856,8 @@ __device__ __forceinline__ void xent_product(const ProductArgs& a, int item, cha
 // Both products of a piece in one launch, dW's items first (they are the longer
 // ones, or equal), so that the chip stays full to the end of the second.  Bound by the
 // products' loop (matrix cores 53 % busy at 2.05 GHz): 8192 x 1024 -> 4096 375 us, 1.10
-// PFLOP/s of 16 bits; with the loads of dX's
-// old values and of the exponents ahead of the stores all eight pieces take 2 % less.
+// PFLOP/s of 16 bits; with the loads of dX's old values and of the exponents ahead of
+// the stores all eight pieces take 2 % less.
 __global__ __launch_bounds__(S::NTH, 2) void xent_products_kernel(ProductArgs w, ProductArgs x, int start) {
   __shared__ __attribute__((aligned(16))) char lds[S::LDS];
   const int b = blockIdx.x;
@@ -1309,13 +1310,13 @@ int mle_vocab_xent_fwd(mle_stream stream, int rows, int d, int vocab, const floa
   RowState* state = reinterpret_cast<RowState*>(static_cast<char*>(ws) + p.logits + p.rows);
   void* gws = reinterpret_cast<char*>(state) + p.state + p.slices;
   for (int v0 = 0; v0 < vocab; v0 += p.piece) {
-    const int n = std::min(p.piece, vocab - v0);
-    TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr,
-                    bias ? bias + v0 : nullptr, gws, p.gemm));
+    const int n = std::min(p.piece, vocab - v0), first = v0 == 0 ? 1 : 0;
+    const float* b = bias ? bias + v0 : nullptr;
+    TRY(mle_gemm_ex(stream, 0, 0, rows, n, d, 1.f, X, ldx, 0, W + v0, ldw, 0, 0.f, l, n, 0, 1, nullptr, b, gws, p.gemm));
     // (with many rows a wave to each is enough to fill the chip)
     if (n <= 1024 || rows >= 2048)
-      mle::launch(xent_stats_kernel<64>, (unsigned)(((int64_t)rows + 3) / 4), NT, 0, s, l, rows, n, v0, bias ? bias + v0 : nullptr, rw, state, v0 == 0 ? 1 : 0);
-    else mle::launch(xent_stats_kernel<1024>, (unsigned)rows, 1024, 0, s, l, rows, n, v0, bias ? bias + v0 : nullptr, rw, state, v0 == 0 ? 1 : 0);
+      mle::launch(xent_stats_kernel<64>, (unsigned)(((int64_t)rows + 3) / 4), NT, 0, s, l, rows, n, v0, b, rw, state, first);
+    else mle::launch(xent_stats_kernel<1024>, (unsigned)rows, 1024, 0, s, l, rows, n, v0, b, rw, state, first);
   }
   mle::launch(xent_finish_kernel, 1u, 1024, 0, s, state, rows, rw, loss_scale, lse, row_loss, loss, 0);
   return check_launch("mle_vocab_xent_fwd");
