@@ -182,6 +182,25 @@ int mle_add_broadcast(mle_stream stream, const float* x, const float* t, float* 
 /* Timestep embedding: cos half then sin half.  PEncoding (Engine/kernels.cu:147-164). */
 int mle_timestep_pe(mle_stream stream, float* y, int t, int dim);
 
+/* Rotary positions: pair p of every head of q [rows, ldq] and k [rows, ldk] is turned by the
+ * angle positions[axis][row] * frequency,
+ *   (a, b) -> (a cos - b sin, a sin + b cos),
+ * the first sections[0] pairs by axis 0, the next sections[1] by axis 1, and so on (1 to 8 axes;
+ * sections is a host array, n = their sum, at most head_dim / 2 and 128; values 2n .. of a head
+ * stay).  positions is device int32 [axes][rows], any value.  By default pair p is values p and
+ * n + p and its frequency base^(-p / n).  Flags:
+ *   MLE_ROTARY_NEIGHBOURS  pair p is values 2p and 2p + 1
+ *   MLE_ROTARY_BY_AXIS     the frequencies start anew in every axis: base^(-i / sections[axis]) for
+ *                          the axis's pair i (rows and columns of an image)
+ * inverse 1 turns back: the gradient of the forward.  accumulate 1 adds to the outputs.  An output
+ * may be its input.  k with kv_heads 0 is left out.  Angles are formed and reduced in 64 bits.
+ * No counterpart in the reference, whose transformer adds MatPEncoding (mle_matpe). */
+enum mle_rotary_flags { MLE_ROTARY_NEIGHBOURS = 1, MLE_ROTARY_BY_AXIS = 2 };
+int mle_rotary(mle_stream stream, int rows, int head_dim, const float* q, int64_t ldq, float* q_out, int64_t ldqo,
+               int heads, const float* k, int64_t ldk, float* k_out, int64_t ldko, int kv_heads,
+               const int32_t* positions, int axes, const int* sections, double base, int flags, int inverse,
+               int accumulate);
+
 /* ------------------------------------------------------------------------- */
 /* Activations                                                               */
 /* ------------------------------------------------------------------------- */
@@ -391,6 +410,52 @@ int mle_attention_fwd(mle_stream stream, const float* q, const float* k, const f
 int mle_attention_bwd(mle_stream stream, const float* q, const float* k, const float* v, const float* dout, float* dq,
                       float* dk, float* dv, int batch, int heads, int seq, int head_dim, int ld, float scale,
                       int causal, int acc_q, int acc_k, int acc_v, int k_reference_grad, void* ws, size_t ws_bytes);
+
+/* Attention along rows over the keys that a causal sliding window and a few first
+ * positions leave visible.  Tensors are [batch, seq, ld], head h in columns
+ * h*head_dim ..; heads come in heads / kv_heads groups of consecutive heads, each with one
+ * head of k and v (kv_heads divides heads; head_dim 1 to 128; any alignment of a float).
+ * The query at position p sees key j when
+ *   j <= p  and  (p - j < window  or  j < sinks)  and  j < length,
+ * window >= 1, sinks >= 0; window >= seq is plain causal attention.  lengths (device
+ * int32 [batch], nullable: seq) are taken as at most seq and at least 0.
+ *   S = scale q k^T,  P = exp(S - lse),  lse = log sum exp S,  out = P v
+ * over the visible keys, whatever the others hold.  Rows at or past a length have out 0 and
+ * lse -infinity, and their gradients take no part; their k and v rows get gradients of 0.
+ * lse [batch, heads, seq] is nullable where no backward follows.
+ * The products' operands are held in 22 bits (two fp16 parts and a power of two per tile,
+ * row or column); sums, statistics and exponentials are fp32.  A tile that holds an infinity or
+ * a NaN is computed with fp32 products, key by key.  Results do not depend on timing.
+ * MultiHeadAttention's softmax (mle_attention_fwd) is over columns; this is SOFTMAX type 0
+ * (Engine/engine.cu:2430-2505) with a mask, without storing scores. */
+int mle_window_attention_fwd(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
+                             const float* v, int64_t ldv, float* out, int64_t ldo, float* lse, const int32_t* lengths,
+                             int batch, int seq, int heads, int kv_heads, int head_dim, float scale, int window,
+                             int sinks);
+/* Its backward, given dout and the forward's out and lse:
+ *   D = <dout, out>,  dS = P (dout v^T - D),
+ *   dq (+)= scale dS k,  dk (+)= scale dS^T q,  dv (+)= P^T dout
+ * with dk and dv summed over the heads of a group.  acc_*: 1 adds, 0 assigns.  The gradients
+ * are distinct buffers and none of the inputs.  ws: 16-byte aligned. */
+size_t mle_window_attention_ws_bytes(int batch, int seq, int heads, int kv_heads, int head_dim, int window, int sinks);
+int mle_window_attention_bwd(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
+                             const float* v, int64_t ldv, const float* out, int64_t ldo, const float* lse,
+                             const float* dout, int64_t lddo, float* dq, int64_t lddq, int acc_q, float* dk,
+                             int64_t lddk, int acc_k, float* dv, int64_t lddv, int acc_v, const int32_t* lengths,
+                             int batch, int seq, int heads, int kv_heads, int head_dim, float scale, int window,
+                             int sinks, void* ws, size_t ws_bytes);
+/* The forward for the newest `tokens` positions of each sequence over a cache of keys and values
+ * [batch, capacity, ld], the newest positions' own among them: row i of sequence b's queries
+ * [batch, tokens, ldq] is at position lengths[b] - tokens + i (lengths taken as at most capacity
+ * and at least 0; rows at a position below 0 get zeros).  Cache rows at or past a length are not
+ * read.  The keys are shared out over the chip and the parts joined in order; ws: 16-byte aligned,
+ * two calls that run at once need one each. */
+size_t mle_window_attention_step_ws_bytes(int batch, int tokens, int capacity, int heads, int kv_heads, int head_dim,
+                                          int window, int sinks);
+int mle_window_attention_step(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
+                              const float* v, int64_t ldv, float* out, int64_t ldo, const int32_t* lengths, int batch,
+                              int tokens, int capacity, int heads, int kv_heads, int head_dim, float scale, int window,
+                              int sinks, void* ws, size_t ws_bytes);
 
 size_t mle_loss_ws_bytes(size_t n);
 /* loss[0] = sum((t - x)^2) / n.  scalar_mse_kernel (Engine/kernels.cu:1808-1816). */
@@ -704,6 +769,23 @@ size_t mle_add_rmsnorm_ws_bytes(int rows, int cols);
 int mle_add_rmsnorm_bwd(mle_stream stream, int rows, int cols, const float* h, const float* w, const float* rstd,
                         const float* dy, const float* dres, float* dh, int accumulate_dh, float* dw, int accumulate_dw,
                         void* ws, size_t ws_bytes);
+
+/* The residual Add and the layer norm that reads it, with a learned weight and bias:
+ *   h = x + r,  u = (h - mean) rstd,  rstd = 1 / sqrt(var + eps),  y = u w + b
+ * along each row, var the mean of (h - mean)^2.  r, w (1), b (0), h and y are nullable; h may be x or
+ * r.  mean and rstd [rows] are the backward's.  Backward, given y's gradient and, nullable, that of
+ * h by other ways (dres): with g = dy w
+ *   dh (+)= dres + rstd (g - mean(g) - u mean(g u)),  dw (+)= sum over rows of dy u,  db (+)= sum of dy
+ * h is the forward's (x without r).  dw and db are nullable, the workspace (16-byte aligned) is
+ * needed with either of them; dh may be dy, dres or h.  accumulate_*: 1 adds, 0 assigns.  LayerNorm
+ * (Engine/engine.cu:3080-3146, mle_norm_fwd) has neither weight nor bias, and one mean to a whole
+ * sample. */
+int mle_add_layernorm_fwd(mle_stream stream, int rows, int cols, const float* x, const float* r, const float* w,
+                          const float* b, float eps, float* h, float* y, float* mean, float* rstd);
+size_t mle_add_layernorm_ws_bytes(int rows, int cols);
+int mle_add_layernorm_bwd(mle_stream stream, int rows, int cols, const float* h, const float* w, const float* mean,
+                          const float* rstd, const float* dy, const float* dres, float* dh, int accumulate_dh,
+                          float* dw, float* db, int accumulate_dw, void* ws, size_t ws_bytes);
 
 /* ------------------------------------------------------------------------- */
 /* Layout (U-Net skip concatenation, transposed-convolution weights)         */

@@ -1,0 +1,375 @@
+// The residual Add and the layer norm that reads it, with a learned weight and
+// bias, and the backward of both.
+//
+//   h = x + r,  u = (h - mean) rstd,  rstd = 1 / sqrt(mean of (h - mean)^2 + eps),  y = u w + b
+//   g = dy w:  dh = dres + rstd (g - mean(g) - u mean(g u)),  dw = sum over rows of dy u,  db = sum of dy
+//
+// One pass over a row: T lanes of a wave, or a workgroup of T threads, hold it
+// in registers, eight consecutive values to a thread and chunk.  The variance is
+// that of the centred values, so a mean far above the spread costs no bits; the
+// row's sums are in 64 bits.  The weight's and the bias's gradients are summed per
+// workgroup in registers and joined in order.
+#include "q8.hpp"
+
+#include <algorithm>
+
+using namespace mle;
+
+namespace {
+
+constexpr int NT = 256;
+constexpr int kMaxParts = 512;          // partial weight gradients: workgroups of the backward
+constexpr int kRowsOfLaunch = 1 << 21;  // of a launch of one workgroup to a row: fewer than 2^32 threads
+
+struct LnArgs {
+  int rows, cols;
+  const float* x;
+  const float* r;
+  const float* w;
+  const float* b;
+  float* h;
+  float* y;
+  float* mean;
+  float* rstd;
+  float eps;
+};
+
+struct LnBwdArgs {
+  int rows, cols;
+  const float* h;
+  const float* w;
+  const float* mean;
+  const float* rstd;
+  const float* dy;
+  const float* dres;
+  float* dh;
+  int acc_dh;
+  float* part;  // [workgroups][2][cols], dw's and db's; null: neither
+};
+
+// The sums of a and b over a row's T threads, in every one of them.
+template <int T>
+__device__ __forceinline__ double2 row_sums(double a, double b, double (*red)[2]) {
+#pragma unroll
+  for (int o = (T < 64 ? T : 64) / 2; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o, 64);
+    b += __shfl_xor(b, o, 64);
+  }
+  if (T <= 64) return make_double2(a, b);
+  __syncthreads();  // the last sums have been read
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6][0] = a;
+    red[threadIdx.x >> 6][1] = b;
+  }
+  __syncthreads();
+  a = b = 0.0;
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i) {
+    a += red[i][0];
+    b += red[i][1];
+  }
+  return make_double2(a, b);
+}
+
+__device__ __forceinline__ void load_sum8(const LnArgs& a, int64_t at, int n, float (&h)[8]) {
+  q8::load_row8(a.x + at, n, h);
+  if (a.r) {
+    float r[8];
+    q8::load_row8(a.r + at, n, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] += r[j];
+  }
+}
+
+// T threads to a row, C chunks of 8 values each (T * 8 * C >= cols); C == 0: any
+// width, the row read three times.
+template <int T, int C>
+__global__ __launch_bounds__(T < NT ? NT : T) void layernorm_fwd_kernel(LnArgs a) {
+  constexpr int B = T < NT ? NT : T, R = B / T;  // rows of a workgroup
+  __shared__ double red[B / 64][2];
+  const int t = threadIdx.x % T;
+  const int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / T;
+  if (row >= a.rows) return;  // (T < B: whole waves; T == B: the workgroup)
+  const int64_t base = row * a.cols;
+  const int chunks = C > 0 ? C : (a.cols + 8 * T - 1) / (8 * T);
+  float keep[C > 0 ? C : 1][8];
+  double s = 0.0;
+#pragma unroll C > 0 ? C : 1
+  for (int c = 0; c < chunks; ++c) {
+    float(&h)[8] = keep[C > 0 ? c : 0];
+    const int col = (c * T + t) * 8, n = min(max(a.cols - col, 0), 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = 0.f;
+    if (n == 0) continue;
+    load_sum8(a, base + col, n, h);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += (double)h[j];
+  }
+  const double mean = row_sums<T>(s, 0.0, red).x / a.cols;
+  s = 0.0;
+#pragma unroll C > 0 ? C : 1
+  for (int c = 0; c < chunks; ++c) {
+    float(&h)[8] = keep[C > 0 ? c : 0];
+    const int col = (c * T + t) * 8, n = min(max(a.cols - col, 0), 8);
+    if (n == 0) continue;
+    if (C == 0) load_sum8(a, base + col, n, h);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = (float)((double)h[j] - mean);
+      s += j < n ? (double)d * (double)d : 0.0;
+    }
+  }
+  const double rstd = 1.0 / sqrt(row_sums<T>(s, 0.0, red).x / a.cols + (double)a.eps);
+  if (t == 0) {
+    a.mean[row] = (float)mean;
+    a.rstd[row] = (float)rstd;
+  }
+#pragma unroll C > 0 ? C : 1
+  for (int c = 0; c < chunks; ++c) {
+    float(&h)[8] = keep[C > 0 ? c : 0];
+    const int col = (c * T + t) * 8, n = min(max(a.cols - col, 0), 8);
+    if (n == 0) continue;
+    if (C == 0) load_sum8(a, base + col, n, h);
+    if (a.h) q8::store_row8(a.h + base + col, h, n);
+    if (!a.y) continue;
+    float w[8], b[8], y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = 1.f, b[j] = 0.f;
+    if (a.w) q8::load_row8(a.w + col, n, w);
+    if (a.b) q8::load_row8(a.b + col, n, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = fmaf((float)(((double)h[j] - mean) * rstd), w[j], b[j]);
+    q8::store_row8(a.y + base + col, y, n);
+  }
+}
+
+// A workgroup takes rows blockIdx.x * R + i * gridDim.x * R and keeps its
+// threads' columns of dw and db in registers; the R rows that it walks at a time
+// add theirs through LDS at the end.
+template <int T, int C>
+__global__ __launch_bounds__(T < NT ? NT : T) void layernorm_bwd_kernel(LnBwdArgs a) {
+  constexpr int B = T < NT ? NT : T, R = B / T;
+  __shared__ double red[B / 64][2];
+  __shared__ float cols_red[R > 1 ? 8 * B : 1];
+  const int t = threadIdx.x % T, k = threadIdx.x / T;
+  float dw[C][8], db[C][8], w[C][8];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int col = (c * T + t) * 8, n = min(max(a.cols - col, 0), 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[c][j] = db[c][j] = 0.f, w[c][j] = 1.f;
+    if (a.w && n > 0) q8::load_row8(a.w + col, n, w[c]);
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.rows; r0 += (int64_t)gridDim.x * R) {
+    const int64_t row = r0 + k;
+    const bool live = row < a.rows;
+    const int64_t base = (live ? row : a.rows - 1) * a.cols;
+    const float rstd = live ? a.rstd[row] : 0.f, mean = live ? a.mean[row] : 0.f;
+    float u[C][8], g[C][8];
+    double s1 = 0.0, s2 = 0.0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * T + t) * 8, n = live ? min(max(a.cols - col, 0), 8) : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[c][j] = g[c][j] = 0.f;
+      if (n == 0) continue;
+      q8::load_row8(a.h + base + col, n, u[c]);
+      q8::load_row8(a.dy + base + col, n, g[c]);  // (0 past the row's end, whatever u is there)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        u[c][j] = (u[c][j] - mean) * rstd;
+        dw[c][j] += g[c][j] * u[c][j];
+        db[c][j] += g[c][j];
+        g[c][j] *= w[c][j];
+        s1 += (double)g[c][j];
+        s2 += (double)(g[c][j] * u[c][j]);
+      }
+    }
+    const double2 m = row_sums<T>(s1, s2, red);
+    const float m1 = (float)(m.x / a.cols), m2 = (float)(m.y / a.cols);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * T + t) * 8, n = live ? min(max(a.cols - col, 0), 8) : 0;
+      if (n == 0) continue;
+      float old[8] = {}, dres[8] = {}, v[8];
+      if (a.dres) q8::load_row8(a.dres + base + col, n, dres);
+      if (a.acc_dh) q8::load_row8(a.dh + base + col, n, old);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = old[j] + (dres[j] + rstd * ((g[c][j] - m1) - u[c][j] * m2));
+      q8::store_row8(a.dh + base + col, v, n);
+    }
+  }
+  if (!a.part) return;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    float(&sum)[C][8] = p ? db : dw;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * T + t) * 8, n = min(max(a.cols - col, 0), 8);
+      if (R > 1) {  // the rows' sums in order
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cols_red[8 * threadIdx.x + j] = sum[c][j];
+        __syncthreads();
+        if (k > 0) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          for (int i = 1; i < R; ++i) sum[c][j] += cols_red[8 * (i * T + t) + j];
+      }
+      if (n > 0) q8::store_row8(part + (int64_t)p * a.cols + col, sum[c], n);
+    }
+  }
+}
+
+// Rows wider than the register kernels take: h and dy read twice; the weight's and the
+// bias's gradients in a pass of their own (layernorm_dw_kernel).
+__global__ __launch_bounds__(1024) void layernorm_bwd_wide_kernel(LnBwdArgs a) {
+  __shared__ double red[16][2];
+  const int64_t base = (int64_t)blockIdx.x * a.cols;
+  const float rstd = a.rstd[blockIdx.x], mean = a.mean[blockIdx.x];
+  double s1 = 0.0, s2 = 0.0;
+  for (int i = threadIdx.x; i < a.cols; i += 1024) {
+    const float g = a.dy[base + i] * (a.w ? a.w[i] : 1.f), u = (a.h[base + i] - mean) * rstd;
+    s1 += (double)g;
+    s2 += (double)(g * u);
+  }
+  const double2 m = row_sums<1024>(s1, s2, red);
+  const float m1 = (float)(m.x / a.cols), m2 = (float)(m.y / a.cols);
+  for (int i = threadIdx.x; i < a.cols; i += 1024) {
+    const float g = a.dy[base + i] * (a.w ? a.w[i] : 1.f), u = (a.h[base + i] - mean) * rstd;
+    const float v = (a.dres ? a.dres[base + i] : 0.f) + rstd * ((g - m1) - u * m2);
+    a.dh[base + i] = (a.acc_dh ? a.dh[base + i] : 0.f) + v;
+  }
+}
+// part[block y][.][col] = sums over rows y, y + gridDim.y, ...
+__global__ __launch_bounds__(NT) void layernorm_dw_kernel(LnBwdArgs a) {
+  const int col = blockIdx.x * NT + threadIdx.x;
+  if (col >= a.cols) return;
+  float s = 0.f, b = 0.f;
+  for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+    const float dy = a.dy[r * a.cols + col];
+    s += dy * ((a.h[r * a.cols + col] - a.mean[r]) * a.rstd[r]);
+    b += dy;
+  }
+  float* part = a.part + (int64_t)blockIdx.y * 2 * a.cols;
+  part[col] = s;
+  part[a.cols + col] = b;
+}
+
+// dw (+)= and db (+)= the partial sums: 16 columns of one of them to a workgroup, 64
+// threads to a column, each adding every 64th part, and the threads' sums in order.
+__global__ __launch_bounds__(1024) void layernorm_join_kernel(const float* __restrict__ part, int parts, int cols,
+                                                              float* __restrict__ dw, float* __restrict__ db,
+                                                              int accumulate) {
+  __shared__ float red[64][17];
+  float* out = blockIdx.y ? db : dw;
+  if (!out) return;
+  const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
+  float s = 0.f;
+  if (col < cols) {
+#pragma unroll 8
+    for (int p = g; p < parts; p += 64) s += part[((int64_t)p * 2 + blockIdx.y) * cols + col];
+  }
+  red[g][c] = s;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  // a quarter of the threads' sums to each of four lanes, then the quarters
+  s = 0.f;
+  const int q = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += red[16 * q + i][c];
+  const float x0 = __shfl(s, c, 64), x1 = __shfl(s, 16 + c, 64), x2 = __shfl(s, 32 + c, 64), x3 = __shfl(s, 48 + c, 64);
+  if (q != 0 || col >= cols) return;
+  const float v = ((x0 + x1) + x2) + x3;
+  out[col] = accumulate ? out[col] + v : v;
+}
+
+// Workgroups of the backward, each with partial gradients: a function of the shape alone.
+int parts_of(int rows, int cols) {
+  const int rows_of_wg = cols <= 2048 ? 4 : 1;
+  return std::max(1, std::min(kMaxParts, (rows - 1) / rows_of_wg + 1));
+}
+
+int check(const char* who, int rows, int cols) {
+  MLE_CHECK_ARG(rows >= 0 && cols > 0 && cols <= (1 << 30), "%s: bad shape %d x %d", who, rows, cols);
+  return MLE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mle_add_layernorm_fwd(mle_stream stream, int rows, int cols, const float* x, const float* r, const float* w,
+                          const float* b, float eps, float* h, float* y, float* mean, float* rstd) {
+  const int rc = check("mle_add_layernorm_fwd", rows, cols);
+  if (rc) return rc;
+  MLE_CHECK_ARG(rows == 0 || (x && mean && rstd), "mle_add_layernorm_fwd: null pointer");
+  MLE_CHECK_ARG(eps >= 0.f, "mle_add_layernorm_fwd: eps %g", (double)eps);
+  if (rows == 0) return MLE_OK;
+  hipStream_t s = as_stream(stream);
+  for (int64_t r0 = 0; r0 < rows; r0 += kRowsOfLaunch) {
+    const int n = (int)std::min<int64_t>(rows - r0, kRowsOfLaunch);
+    const int64_t at = r0 * cols;
+    const LnArgs a{n, cols, x + at, r ? r + at : r, w, b, h ? h + at : h, y ? y + at : y, mean + r0, rstd + r0, eps};
+    const unsigned by4 = (unsigned)((n + 3) / 4);
+    if (cols <= 512) mle::launch(layernorm_fwd_kernel<64, 1>, by4, NT, 0, s, a);
+    else if (cols <= 1024) mle::launch(layernorm_fwd_kernel<64, 2>, by4, NT, 0, s, a);
+    else if (cols <= 2048) mle::launch(layernorm_fwd_kernel<64, 4>, by4, NT, 0, s, a);
+    else if (cols <= 4096) mle::launch(layernorm_fwd_kernel<256, 2>, (unsigned)n, NT, 0, s, a);
+    else if (cols <= 8192) mle::launch(layernorm_fwd_kernel<256, 4>, (unsigned)n, NT, 0, s, a);
+    else mle::launch(layernorm_fwd_kernel<1024, 0>, (unsigned)n, 1024, 0, s, a);
+  }
+  return check_launch("mle_add_layernorm_fwd");
+}
+
+size_t mle_add_layernorm_ws_bytes(int rows, int cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return (size_t)parts_of(rows, cols) * 2 * cols * sizeof(float);
+}
+
+int mle_add_layernorm_bwd(mle_stream stream, int rows, int cols, const float* h, const float* w, const float* mean,
+                          const float* rstd, const float* dy, const float* dres, float* dh, int accumulate_dh,
+                          float* dw, float* db, int accumulate_dw, void* ws, size_t ws_bytes) {
+  const int rc = check("mle_add_layernorm_bwd", rows, cols);
+  if (rc) return rc;
+  MLE_CHECK_ARG(rows == 0 || (h && mean && rstd && dy && dh), "mle_add_layernorm_bwd: null pointer");
+  if (rows == 0) {
+    if (accumulate_dw) return MLE_OK;
+    if (dw) {
+      const int e = mle_fill(stream, dw, 0.f, (size_t)cols);
+      if (e) return e;
+    }
+    return db ? mle_fill(stream, db, 0.f, (size_t)cols) : MLE_OK;
+  }
+  const bool sums = dw || db;
+  if (sums && (!ws || !aligned16(ws) || ws_bytes < mle_add_layernorm_ws_bytes(rows, cols)))
+    return set_error(MLE_ERR_WORKSPACE, "mle_add_layernorm_bwd: workspace of %zu bytes, 16-byte aligned, needed",
+                     mle_add_layernorm_ws_bytes(rows, cols));
+  const int parts = parts_of(rows, cols);
+  LnBwdArgs a{rows, cols, h, w, mean, rstd, dy, dres, dh, accumulate_dh, sums ? static_cast<float*>(ws) : nullptr};
+  hipStream_t s = as_stream(stream);
+  if (cols <= 512) mle::launch(layernorm_bwd_kernel<64, 1>, (unsigned)parts, NT, 0, s, a);
+  else if (cols <= 1024) mle::launch(layernorm_bwd_kernel<64, 2>, (unsigned)parts, NT, 0, s, a);
+  else if (cols <= 2048) mle::launch(layernorm_bwd_kernel<64, 4>, (unsigned)parts, NT, 0, s, a);
+  else if (cols <= 4096) mle::launch(layernorm_bwd_kernel<256, 2>, (unsigned)parts, NT, 0, s, a);
+  else if (cols <= 8192) mle::launch(layernorm_bwd_kernel<256, 4>, (unsigned)parts, NT, 0, s, a);
+  else {
+    // the weight's sums first: dh may be dy's or h's buffer
+    if (sums) mle::launch(layernorm_dw_kernel, dim3((unsigned)((cols + NT - 1) / NT), (unsigned)parts), NT, 0, s, a);
+    for (int64_t r0 = 0; r0 < rows; r0 += kRowsOfLaunch) {
+      const int n = (int)std::min<int64_t>(rows - r0, kRowsOfLaunch);
+      const int64_t at = r0 * cols;
+      const LnBwdArgs b{n, cols, h + at, w, mean + r0, rstd + r0, dy + at, dres ? dres + at : dres, dh + at, accumulate_dh,
+                        nullptr};
+      mle::launch(layernorm_bwd_wide_kernel, (unsigned)n, 1024, 0, s, b);
+    }
+  }
+  if (sums)
+    mle::launch(layernorm_join_kernel, dim3((unsigned)((cols + 15) / 16), 2), 1024, 0, s, static_cast<const float*>(ws), parts,
+                cols, dw, db, accumulate_dw);
+  return check_launch("mle_add_layernorm_bwd");
+}
+
+}  // extern "C"

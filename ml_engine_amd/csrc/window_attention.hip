@@ -1,0 +1,194 @@
+// Attention with a causal sliding window and sinks (window_attention.hpp): a wave
+// to a row or a key.
+#include "window_attention.hpp"
+
+#include <math.h>
+#include <algorithm>
+
+using namespace mle;
+using namespace wattn;
+
+namespace {
+
+// A wave to a row: row index over [batch][head][row].
+__global__ __launch_bounds__(256) void rows_fwd_kernel(Args a, int64_t first) {
+  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (int64_t)a.batch * a.heads * a.rows) return;
+  const int64_t bh = w / a.rows;
+  plain_row(a, (int)(bh / a.heads), (int)(bh % a.heads), (int)(w - bh * a.rows));
+}
+
+__global__ __launch_bounds__(256) void delta_kernel(Args a, int64_t first) {
+  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (int64_t)a.batch * a.heads * a.rows) return;
+  const int64_t bh = w / a.rows;
+  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads), i = (int)(w - bh * a.rows), lane = threadIdx.x & 63;
+  const int64_t at = (int64_t)b * a.rows + i;
+  float s = 0.f;
+  for (int d = lane; d < a.dim; d += 64)
+    s = fmaf(a.dout[at * a.lddo + (int64_t)h * a.dim + d], a.out_in[at * a.ldo + (int64_t)h * a.dim + d], s);
+  s = wave_sum(s);
+  if (lane == 0) a.delta[w] = s;
+}
+
+__global__ __launch_bounds__(256) void rows_dq_kernel(Args a, int64_t first) {
+  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (int64_t)a.batch * a.heads * a.rows) return;
+  const int64_t bh = w / a.rows;
+  plain_dq(a, (int)(bh / a.heads), (int)(bh % a.heads), (int)(w - bh * a.rows));
+}
+
+__global__ __launch_bounds__(256) void keys_dkv_kernel(Args a, int64_t first) {
+  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (w >= (int64_t)a.batch * a.kv_heads * a.keys) return;
+  const int64_t be = w / a.keys;
+  const int b = (int)(be / a.kv_heads), e = (int)(be % a.kv_heads), j = (int)(w - be * a.keys), lane = threadIdx.x & 63;
+  const Seq s(a, b);
+  float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
+  const int end = j < a.sinks ? s.len : (int)min((int64_t)s.len, (int64_t)j + a.window);
+  for (int g = 0; g < a.group; ++g) plain_kv_sums(a, b, e * a.group + g, j, j, end, sk, sv);
+  float* dk = a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim;
+  float* dv = a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int d = lane + 64 * r;
+    if (d < a.dim) {
+      dk[d] = (a.acc_k ? dk[d] : 0.f) + sk[r];
+      dv[d] = (a.acc_v ? dv[d] : 0.f) + sv[r];
+    }
+  }
+}
+
+constexpr int64_t kWavesOfLaunch = 1 << 25;  // fewer than 2^32 threads
+
+// Waves [0, n) of `kernel` in launches of bounded size.
+template <class K>
+void launch_waves(K kernel, int64_t n, hipStream_t s, const Args& a) {
+  for (int64_t w = 0; w < n; w += kWavesOfLaunch)
+    mle::launch(kernel, (unsigned)((std::min(n - w, kWavesOfLaunch) + 3) / 4), 256, 0, s, a, w);
+}
+
+int check(const char* who, int batch, int rows, int keys, int heads, int kv_heads, int dim, float scale, int window,
+          int sinks) {
+  MLE_CHECK_ARG(batch >= 0 && batch <= (1 << 24) && rows >= 0 && keys >= 0 && rows <= (1 << 30) && keys <= (1 << 30),
+                "%s: bad shape, %d sequences of %d rows and %d keys", who, batch, rows, keys);
+  MLE_CHECK_ARG(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= (1 << 16), "%s: %d heads on %d of keys", who,
+                heads, kv_heads);
+  MLE_CHECK_ARG(dim > 0, "%s: head_dim %d", who, dim);
+  MLE_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %d (at least 1), sinks %d (at least 0)", who, window, sinks);
+  MLE_CHECK_ARG(isfinite(scale), "%s: scale %g", who, (double)scale);
+  if (dim > kMaxDim) return set_error(MLE_ERR_UNSUPPORTED, "%s: head_dim %d, at most %d", who, dim, kMaxDim);
+  return MLE_OK;
+}
+
+int check_ld(const char* who, const char* name, int64_t ld, int heads, int dim) {
+  MLE_CHECK_ARG(ld >= (int64_t)heads * dim && ld <= ((int64_t)1 << 32), "%s: %s %lld for %d heads of %d", who, name,
+                (long long)ld, heads, dim);
+  return MLE_OK;
+}
+
+Args make_args(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t ldo,
+               const int32_t* lengths, int batch, int rows, int keys, int heads, int kv_heads, int dim, float scale,
+               int window, int sinks) {
+  Args a{};
+  a.q = q, a.k = k, a.v = v;
+  a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo;
+  a.lengths = lengths;
+  a.batch = batch, a.rows = rows, a.keys = keys;
+  a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim;
+  a.window = std::min(window, std::max(keys, 1)), a.sinks = std::min(sinks, keys);
+  a.scale = scale;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mle_window_attention_fwd(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
+                             const float* v, int64_t ldv, float* out, int64_t ldo, float* lse, const int32_t* lengths,
+                             int batch, int seq, int heads, int kv_heads, int head_dim, float scale, int window,
+                             int sinks) {
+  const char* who = "mle_window_attention_fwd";
+  int rc = check(who, batch, seq, seq, heads, kv_heads, head_dim, scale, window, sinks);
+  if (!rc) rc = check_ld(who, "ldq", ldq, heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldk", ldk, kv_heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldv", ldv, kv_heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldo", ldo, heads, head_dim);
+  if (rc) return rc;
+  if (batch == 0 || seq == 0) return MLE_OK;
+  MLE_CHECK_ARG(q && k && v && out, "%s: null pointer", who);
+  Args a = make_args(q, ldq, k, ldk, v, ldv, ldo, lengths, batch, seq, seq, heads, kv_heads, head_dim, scale, window, sinks);
+  a.out = out;
+  a.lse = lse;
+  launch_waves(rows_fwd_kernel, (int64_t)batch * heads * seq, as_stream(stream), a);
+  return check_launch(who);
+}
+
+size_t mle_window_attention_ws_bytes(int batch, int seq, int heads, int kv_heads, int head_dim, int window, int sinks) {
+  if (batch <= 0 || seq <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  return ((size_t)batch * heads * seq * sizeof(float) + 15) & ~(size_t)15;
+}
+
+int mle_window_attention_bwd(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
+                             const float* v, int64_t ldv, const float* out, int64_t ldo, const float* lse,
+                             const float* dout, int64_t lddo, float* dq, int64_t lddq, int acc_q, float* dk,
+                             int64_t lddk, int acc_k, float* dv, int64_t lddv, int acc_v, const int32_t* lengths,
+                             int batch, int seq, int heads, int kv_heads, int head_dim, float scale, int window,
+                             int sinks, void* ws, size_t ws_bytes) {
+  const char* who = "mle_window_attention_bwd";
+  int rc = check(who, batch, seq, seq, heads, kv_heads, head_dim, scale, window, sinks);
+  if (!rc) rc = check_ld(who, "ldq", ldq, heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldk", ldk, kv_heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldv", ldv, kv_heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldo", ldo, heads, head_dim);
+  if (!rc) rc = check_ld(who, "lddo", lddo, heads, head_dim);
+  if (!rc) rc = check_ld(who, "lddq", lddq, heads, head_dim);
+  if (!rc) rc = check_ld(who, "lddk", lddk, kv_heads, head_dim);
+  if (!rc) rc = check_ld(who, "lddv", lddv, kv_heads, head_dim);
+  if (rc) return rc;
+  if (batch == 0 || seq == 0) return MLE_OK;
+  MLE_CHECK_ARG(q && k && v && out && lse && dout && dq && dk && dv, "%s: null pointer", who);
+  const size_t need = mle_window_attention_ws_bytes(batch, seq, heads, kv_heads, head_dim, window, sinks);
+  if (!ws || !aligned16(ws) || ws_bytes < need)
+    return set_error(MLE_ERR_WORKSPACE, "%s: workspace of %zu bytes, 16-byte aligned, needed", who, need);
+  Args a = make_args(q, ldq, k, ldk, v, ldv, ldo, lengths, batch, seq, seq, heads, kv_heads, head_dim, scale, window, sinks);
+  a.out_in = out, a.lse_in = lse, a.dout = dout, a.lddo = lddo;
+  a.dq = dq, a.dk = dk, a.dv = dv;
+  a.lddq = lddq, a.lddk = lddk, a.lddv = lddv;
+  a.acc_q = acc_q != 0, a.acc_k = acc_k != 0, a.acc_v = acc_v != 0;
+  a.delta = static_cast<float*>(ws);
+  hipStream_t s = as_stream(stream);
+  launch_waves(delta_kernel, (int64_t)batch * heads * seq, s, a);
+  launch_waves(rows_dq_kernel, (int64_t)batch * heads * seq, s, a);
+  launch_waves(keys_dkv_kernel, (int64_t)batch * kv_heads * seq, s, a);
+  return check_launch(who);
+}
+
+size_t mle_window_attention_step_ws_bytes(int batch, int tokens, int capacity, int heads, int kv_heads, int head_dim,
+                                          int window, int sinks) {
+  return 0;
+}
+
+int mle_window_attention_step(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
+                              const float* v, int64_t ldv, float* out, int64_t ldo, const int32_t* lengths, int batch,
+                              int tokens, int capacity, int heads, int kv_heads, int head_dim, float scale, int window,
+                              int sinks, void* ws, size_t ws_bytes) {
+  const char* who = "mle_window_attention_step";
+  int rc = check(who, batch, tokens, capacity, heads, kv_heads, head_dim, scale, window, sinks);
+  if (!rc) rc = check_ld(who, "ldq", ldq, heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldk", ldk, kv_heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldv", ldv, kv_heads, head_dim);
+  if (!rc) rc = check_ld(who, "ldo", ldo, heads, head_dim);
+  if (rc) return rc;
+  if (batch == 0 || tokens == 0) return MLE_OK;
+  MLE_CHECK_ARG(q && out && lengths && (capacity == 0 || (k && v)), "%s: null pointer", who);
+  Args a = make_args(q, ldq, k, ldk, v, ldv, ldo, lengths, batch, tokens, capacity, heads, kv_heads, head_dim, scale, window,
+                     sinks);
+  a.out = out;
+  a.at_end = 1;
+  launch_waves(rows_fwd_kernel, (int64_t)batch * heads * tokens, as_stream(stream), a);
+  return check_launch(who);
+}
+
+}  // extern "C"

@@ -65,6 +65,7 @@ SIGNATURES: dict[str, tuple] = {
     "mle_timestep_pe": (I, [P, P, I, I]),
     "mle_matpe_table": (I, [P, P, I, I, I]),
     "mle_add_broadcast": (I, [P, P, P, P, I, SZ]),
+    "mle_rotary": (I, [P, I, I, P, I64, P, I64, I, P, I64, P, I64, I, P, I, P, D, I, I, I]),
     "mle_act_fwd": (I, [P, I, P, P, SZ]),
     "mle_act_bwd": (I, [P, I, P, P, P, SZ, I]),
     "mle_gemm": (I, [P, I, I, I, I, I, F, P, I64, I64, P, I64, I64, F, P, I64, I64, I, P]),
@@ -91,6 +92,12 @@ SIGNATURES: dict[str, tuple] = {
     "mle_attention_ws_bytes": (SZ, [I, I, I]),
     "mle_attention_fwd": (I, [P, P, P, P, P, I, I, I, I, I, F, I, P, SZ]),
     "mle_attention_bwd": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I, F, I, I, I, I, I, P, SZ]),
+    "mle_window_attention_fwd": (I, [P, P, I64, P, I64, P, I64, P, I64, P, P, I, I, I, I, I, F, I, I]),
+    "mle_window_attention_ws_bytes": (SZ, [I, I, I, I, I, I, I]),
+    "mle_window_attention_bwd": (I, [P, P, I64, P, I64, P, I64, P, I64, P, P, I64, P, I64, I, P, I64, I, P, I64, I, P,
+                                     I, I, I, I, I, F, I, I, P, SZ]),
+    "mle_window_attention_step_ws_bytes": (SZ, [I, I, I, I, I, I, I, I]),
+    "mle_window_attention_step": (I, [P, P, I64, P, I64, P, I64, P, I64, P, I, I, I, I, I, I, F, I, I, P, SZ]),
     "mle_loss_ws_bytes": (SZ, [SZ]),
     "mle_mse_fwd": (I, [P, P, P, SZ, P, P, SZ]),
     "mle_mse_fwd_read": (I, [P, P, P, SZ, P, P, SZ, P]),
@@ -131,6 +138,9 @@ SIGNATURES: dict[str, tuple] = {
     "mle_add_rmsnorm_q8_fwd": (I, [P, I, I, P, P, P, F, P, P, P, P, I64, P, I64]),
     "mle_add_rmsnorm_ws_bytes": (SZ, [I, I]),
     "mle_add_rmsnorm_bwd": (I, [P, I, I, P, P, P, P, P, P, I, P, I, P, SZ]),
+    "mle_add_layernorm_fwd": (I, [P, I, I, P, P, P, P, F, P, P, P, P]),
+    "mle_add_layernorm_ws_bytes": (SZ, [I, I]),
+    "mle_add_layernorm_bwd": (I, [P, I, I, P, P, P, P, P, P, P, I, P, P, I, P, SZ]),
     "mle_copy_crop_fwd": (I, [P, P, P, P, I, I, I, I, I, I, I]),
     "mle_copy_crop_bwd": (I, [P, P, P, P, I, I, I, I, I, I, I, I, I]),
     "mle_weight_swap": (I, [P, P, P, I, I, I, I]),
