@@ -1,6 +1,7 @@
 // Attention with a causal sliding window and sinks (window_attention.hpp): a wave
 // to a row or a key.
 #include "window_attention.hpp"
+#include "window_kernels.hpp"
 
 #include <math.h>
 #include <algorithm>
@@ -16,47 +17,6 @@ __global__ __launch_bounds__(256) void rows_fwd_kernel(Args a, int64_t first) {
   if (w >= (int64_t)a.batch * a.heads * a.rows) return;
   const int64_t bh = w / a.rows;
   plain_row(a, (int)(bh / a.heads), (int)(bh % a.heads), (int)(w - bh * a.rows));
-}
-
-__global__ __launch_bounds__(256) void delta_kernel(Args a, int64_t first) {
-  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.batch * a.heads * a.rows) return;
-  const int64_t bh = w / a.rows;
-  const int b = (int)(bh / a.heads), h = (int)(bh % a.heads), i = (int)(w - bh * a.rows), lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)b * a.rows + i;
-  float s = 0.f;
-  for (int d = lane; d < a.dim; d += 64)
-    s = fmaf(a.dout[at * a.lddo + (int64_t)h * a.dim + d], a.out_in[at * a.ldo + (int64_t)h * a.dim + d], s);
-  s = wave_sum(s);
-  if (lane == 0) a.delta[w] = s;
-}
-
-__global__ __launch_bounds__(256) void rows_dq_kernel(Args a, int64_t first) {
-  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.batch * a.heads * a.rows) return;
-  const int64_t bh = w / a.rows;
-  plain_dq(a, (int)(bh / a.heads), (int)(bh % a.heads), (int)(w - bh * a.rows));
-}
-
-__global__ __launch_bounds__(256) void keys_dkv_kernel(Args a, int64_t first) {
-  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.batch * a.kv_heads * a.keys) return;
-  const int64_t be = w / a.keys;
-  const int b = (int)(be / a.kv_heads), e = (int)(be % a.kv_heads), j = (int)(w - be * a.keys), lane = threadIdx.x & 63;
-  const Seq s(a, b);
-  float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
-  const int end = j < a.sinks ? s.len : (int)min((int64_t)s.len, (int64_t)j + a.window);
-  for (int g = 0; g < a.group; ++g) plain_kv_sums(a, b, e * a.group + g, j, j, end, sk, sv);
-  float* dk = a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim;
-  float* dv = a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int d = lane + 64 * r;
-    if (d < a.dim) {
-      dk[d] = (a.acc_k ? dk[d] : 0.f) + sk[r];
-      dv[d] = (a.acc_v ? dv[d] : 0.f) + sv[r];
-    }
-  }
 }
 
 constexpr int64_t kWavesOfLaunch = 1 << 25;  // fewer than 2^32 threads
@@ -76,6 +36,8 @@ int check(const char* who, int batch, int rows, int keys, int heads, int kv_head
                 heads, kv_heads);
   MLE_CHECK_ARG(dim > 0, "%s: head_dim %d", who, dim);
   MLE_CHECK_ARG(window >= 1 && sinks >= 0, "%s: window %d (at least 1), sinks %d (at least 0)", who, window, sinks);
+  MLE_CHECK_ARG((double)batch * heads * std::max(rows, keys) <= 1e12, "%s: %d sequences of %d rows, %d heads", who, batch, rows,
+                heads);
   MLE_CHECK_ARG(isfinite(scale), "%s: scale %g", who, (double)scale);
   if (dim > kMaxDim) return set_error(MLE_ERR_UNSUPPORTED, "%s: head_dim %d, at most %d", who, dim, kMaxDim);
   return MLE_OK;
@@ -121,13 +83,15 @@ int mle_window_attention_fwd(mle_stream stream, const float* q, int64_t ldq, con
   Args a = make_args(q, ldq, k, ldk, v, ldv, ldo, lengths, batch, seq, seq, heads, kv_heads, head_dim, scale, window, sinks);
   a.out = out;
   a.lse = lse;
-  launch_waves(rows_fwd_kernel, (int64_t)batch * heads * seq, as_stream(stream), a);
+  tile_forward(a, as_stream(stream));
   return check_launch(who);
 }
 
 size_t mle_window_attention_ws_bytes(int batch, int seq, int heads, int kv_heads, int head_dim, int window, int sinks) {
   if (batch <= 0 || seq <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
-  return ((size_t)batch * heads * seq * sizeof(float) + 15) & ~(size_t)15;
+  Args a = make_args(nullptr, 0, nullptr, 0, nullptr, 0, 0, nullptr, batch, seq, seq, heads, kv_heads, head_dim, 1.f,
+                     std::max(window, 1), std::max(sinks, 0));
+  return BwdWork(a).place(a, nullptr);
 }
 
 int mle_window_attention_bwd(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
@@ -157,11 +121,9 @@ int mle_window_attention_bwd(mle_stream stream, const float* q, int64_t ldq, con
   a.dq = dq, a.dk = dk, a.dv = dv;
   a.lddq = lddq, a.lddk = lddk, a.lddv = lddv;
   a.acc_q = acc_q != 0, a.acc_k = acc_k != 0, a.acc_v = acc_v != 0;
-  a.delta = static_cast<float*>(ws);
-  hipStream_t s = as_stream(stream);
-  launch_waves(delta_kernel, (int64_t)batch * heads * seq, s, a);
-  launch_waves(rows_dq_kernel, (int64_t)batch * heads * seq, s, a);
-  launch_waves(keys_dkv_kernel, (int64_t)batch * kv_heads * seq, s, a);
+  BwdWork w(a);
+  w.place(a, ws);
+  tile_backward(a, w, as_stream(stream));
   return check_launch(who);
 }
 

@@ -1,0 +1,110 @@
+// The launches of the windowed attention's tiled kernels, and how their workgroups
+// are numbered.
+#pragma once
+#include "window_attention.hpp"
+
+#include <algorithm>
+
+namespace wattn {
+
+constexpr int kKeyBlock = 128;  // keys of a workgroup of the backward
+
+// The backward's workspace, and what follows from the sizes.
+struct BwdWork {
+  int* ex;        // exponent of each row of dout, [batch, heads, rows]
+  int* tile_ex;   // the largest of 64 rows, [batch, heads, tiles]
+  float* part;    // far sums of the sinks, [batch, kv_heads, sink_blocks, fars, dk and dv, kKeyBlock, dim]
+  int tiles, key_blocks, sink_blocks;
+  int fars, far_rows;  // chunks of rows past a block's window, and their rows
+  // Rows from here on see a block's sinks alone.
+  __host__ __device__ int near_end(const Args& a, int k0, int kb) const {
+    const int64_t n = ((int64_t)k0 + kb + a.window + 62) / 64 * 64;
+    return (int)(n < tiles * 64ll ? n : tiles * 64ll);
+  }
+  explicit BwdWork(const Args& a) : ex(nullptr), tile_ex(nullptr), part(nullptr) {
+    tiles = (a.rows + 63) / 64;
+    key_blocks = (a.keys + kKeyBlock - 1) / kKeyBlock;
+    sink_blocks = (a.sinks + kKeyBlock - 1) / kKeyBlock;
+    // short, so that they fill in behind the blocks of keys
+    far_rows = std::max(256, (a.window / 4 + 63) / 64 * 64);
+    const int after = a.rows - near_end(a, 0, kKeyBlock);
+    fars = sink_blocks > 0 && after > 0 ? (after + far_rows - 1) / far_rows : 0;
+  }
+  // Lays it out from `ws` (which may be null) after D; the bytes of all of it.
+  size_t place(Args& a, void* ws) {
+    char* p = static_cast<char*>(ws);
+    size_t n = 0;
+    auto take = [&](size_t bytes) {
+      char* at = p ? p + n : nullptr;
+      n += (bytes + 15) & ~(size_t)15;
+      return at;
+    };
+    const size_t rows = (size_t)a.batch * a.heads * a.rows;
+    a.delta = reinterpret_cast<float*>(take(rows * sizeof(float)));
+    ex = reinterpret_cast<int*>(take(rows * sizeof(int)));
+    tile_ex = reinterpret_cast<int*>(take((size_t)a.batch * a.heads * tiles * sizeof(int)));
+    part = reinterpret_cast<float*>(
+        take((size_t)a.batch * a.kv_heads * sink_blocks * fars * 2 * kKeyBlock * a.dim * sizeof(float)));
+    return n;
+  }
+};
+
+void tile_forward(const Args& a, hipStream_t s);
+void tile_backward(const Args& a, const BwdWork& w, hipStream_t s);
+
+struct Block {
+  int b, h, row;
+};
+struct Place {
+  int64_t group;
+  int item;
+};
+
+// Workgroups: sequence, head, block of rows.  The blocks of one sequence and group of heads
+// read the same keys and values: where the groups fill the 8 XCDs evenly, each XCD (a
+// workgroup's number modulo 8) takes whole groups, so that its L2 holds them.  The last rows,
+// which see the most, come first.  (A kernel may number a group's items by itself: Place.)
+struct Grid {
+  int64_t first, total;
+  int groups, per_group, per_head, blocks;  // per_head: heads of a group; blocks: of rows
+  int xcd;
+  Grid(const Args& a, int heads, int blocks_) : first(0) {
+    groups = a.batch * a.kv_heads;
+    per_head = heads / a.kv_heads;
+    blocks = blocks_;
+    per_group = per_head * blocks;
+    total = (int64_t)groups * per_group;
+    xcd = groups % 8 == 0;
+  }
+  __device__ __forceinline__ Place place() const {
+    const int64_t id = first + blockIdx.x;
+    Place p;
+    if (xcd) {
+      const int64_t k = id >> 3;
+      p.group = (k / per_group) * 8 + (id & 7);
+      p.item = (int)(k % per_group);
+    } else {
+      p.group = id / per_group;
+      p.item = (int)(id - p.group * per_group);
+    }
+    return p;
+  }
+  __device__ __forceinline__ Block block(const Args& a, int rows) const {
+    const Place p = place();
+    Block r;
+    r.b = (int)(p.group / a.kv_heads);
+    r.h = (int)(p.group % a.kv_heads) * per_head + p.item % per_head;
+    r.row = (blocks - 1 - p.item / per_head) * rows;
+    return r;
+  }
+};
+
+// All of the grid in launches of fewer than 2^32 threads.
+template <class K, class... More>
+void launch_blocks(K kernel, Grid g, int threads, hipStream_t s, const Args& a, const More&... more) {
+  constexpr int64_t kBlocks = 1 << 22;
+  for (; g.first < g.total; g.first += kBlocks)
+    mle::launch(kernel, (unsigned)std::min<int64_t>(g.total - g.first, kBlocks), threads, 0, s, a, more..., g);
+}
+
+}  // namespace wattn
