@@ -1,5 +1,4 @@
-// Attention with a causal sliding window and sinks (window_attention.hpp): a wave
-// to a row or a key.
+// The entry points of the windowed attention: checks, workspaces, and which kernels run.
 #include "window_attention.hpp"
 #include "window_kernels.hpp"
 
@@ -10,23 +9,6 @@ using namespace mle;
 using namespace wattn;
 
 namespace {
-
-// A wave to a row: row index over [batch][head][row].
-__global__ __launch_bounds__(256) void rows_fwd_kernel(Args a, int64_t first) {
-  const int64_t w = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (int64_t)a.batch * a.heads * a.rows) return;
-  const int64_t bh = w / a.rows;
-  plain_row(a, (int)(bh / a.heads), (int)(bh % a.heads), (int)(w - bh * a.rows));
-}
-
-constexpr int64_t kWavesOfLaunch = 1 << 25;  // fewer than 2^32 threads
-
-// Waves [0, n) of `kernel` in launches of bounded size.
-template <class K>
-void launch_waves(K kernel, int64_t n, hipStream_t s, const Args& a) {
-  for (int64_t w = 0; w < n; w += kWavesOfLaunch)
-    mle::launch(kernel, (unsigned)((std::min(n - w, kWavesOfLaunch) + 3) / 4), 256, 0, s, a, w);
-}
 
 int check(const char* who, int batch, int rows, int keys, int heads, int kv_heads, int dim, float scale, int window,
           int sinks) {
@@ -129,7 +111,10 @@ int mle_window_attention_bwd(mle_stream stream, const float* q, int64_t ldq, con
 
 size_t mle_window_attention_step_ws_bytes(int batch, int tokens, int capacity, int heads, int kv_heads, int head_dim,
                                           int window, int sinks) {
-  return 0;
+  if (batch <= 0 || tokens <= 0 || capacity <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  const Args a = make_args(nullptr, 0, nullptr, 0, nullptr, 0, 0, nullptr, batch, tokens, capacity, heads, kv_heads, head_dim,
+                           1.f, std::max(window, 1), std::max(sinks, 0));
+  return StepWork::few(tokens) ? StepWork(a).bytes(a) : 0;
 }
 
 int mle_window_attention_step(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
@@ -149,7 +134,16 @@ int mle_window_attention_step(mle_stream stream, const float* q, int64_t ldq, co
                      sinks);
   a.out = out;
   a.at_end = 1;
-  launch_waves(rows_fwd_kernel, (int64_t)batch * heads * tokens, as_stream(stream), a);
+  if (!StepWork::few(tokens)) {
+    tile_forward(a, as_stream(stream));
+    return check_launch(who);
+  }
+  StepWork w(a);
+  const size_t need = w.bytes(a);
+  if (need > 0 && (!ws || !aligned16(ws) || ws_bytes < need))
+    return set_error(MLE_ERR_WORKSPACE, "%s: workspace of %zu bytes, 16-byte aligned, needed", who, need);
+  w.part = static_cast<float*>(ws);
+  step_forward(a, w, as_stream(stream));
   return check_launch(who);
 }
 

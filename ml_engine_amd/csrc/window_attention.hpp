@@ -48,8 +48,10 @@ struct Seen {
   __device__ __forceinline__ int key(int t) const { return t < before ? t : low + t - before; }
 };
 
+// (Without branches, and its users choose values by it: a vector's element set to minus
+// infinity under a condition has been compiled into a copy that some lanes skip.)
 __device__ __forceinline__ bool sees(const Args& a, int p, int j) {
-  return j <= p && (p - j < a.window || j < a.sinks);
+  return (j <= p) & ((p - j < a.window) | (j < a.sinks));
 }
 
 // ---------------------------------------------------------------- plain forms

@@ -315,7 +315,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
         s[r] = fmaf(s[r], ct, -lse[r >> 2][r & 3]);
         if (!all) {
           const int i = i0 + 8 * (r >> 2) + 4 * half + (r & 3);
-          if (!live || !sees(a, i, j)) s[r] = -INFINITY;
+          s[r] = live & sees(a, i, j) ? s[r] : -INFINITY;
         }
         mx = fmaxf(mx, s[r]);
       }
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
         float p = fmaf(s[r], ct, -lse);
         if (!all) {
           const int j = jb + 8 * (r >> 2) + 4 * half + (r & 3);
-          if (!live || !sees(a, i, j)) p = -INFINITY;
+          p = live & sees(a, i, j) ? p : -INFINITY;
         }
         x[r] = __builtin_amdgcn_exp2f(p) * fmaf(x[r], cd, -dd);
         mx = fmaxf(mx, fabsf(x[r]));

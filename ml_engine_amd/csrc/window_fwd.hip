@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int j = j0 + 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
-            if (!live || !sees(a, p, j)) s[n][r] = -INFINITY;
+            s[n][r] = live & sees(a, p, j) ? s[n][r] : -INFINITY;
           }
       }
       // (never 0, so that what is hidden stays at minus infinity)

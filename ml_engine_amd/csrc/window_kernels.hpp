@@ -49,7 +49,30 @@ struct BwdWork {
   }
 };
 
+// A step's: few rows (heads of a group times tokens) over many keys.
+struct StepWork {
+  float* part;     // [batch, kv_heads, row_blocks, splits, 16 rows, dim and (maximum, sum)]
+  int row_blocks;  // of 16 rows of a group
+  int splits;      // of the keys
+  // From 32 tokens on their rows fill a wave's 32 in the tiled forward.
+  static bool few(int tokens) { return tokens < 32; }
+  explicit StepWork(const Args& a) : part(nullptr) {
+    row_blocks = (a.group * a.rows + 15) / 16;
+    const int64_t groups = (int64_t)a.batch * a.kv_heads * row_blocks;
+    const int64_t keys = std::min<int64_t>(a.keys, (int64_t)a.sinks + a.window + a.rows - 1);
+    // enough workgroups for the chip's 256 CUs twice, 128 keys (a block to a wave) or more
+    // to each; one launch where a second would cost what it saves
+    splits = 1;
+    if (groups < 200 && keys > 256)
+      splits = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + groups - 1) / groups, (keys + 127) / 128, 64}));
+  }
+  size_t bytes(const Args& a) const {
+    return splits == 1 ? 0 : (size_t)a.batch * a.kv_heads * row_blocks * splits * 16 * (a.dim + 2) * sizeof(float);
+  }
+};
+
 void tile_forward(const Args& a, hipStream_t s);
+void step_forward(const Args& a, const StepWork& w, hipStream_t s);
 void tile_backward(const Args& a, const BwdWork& w, hipStream_t s);
 
 struct Block {
