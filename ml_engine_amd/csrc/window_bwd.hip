@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kOdd = 1 << 20;   // in place of a row's exponent: something in it is not finite
 constexpr int kNone = -(1 << 20);
+constexpr int kTileRows = 64;   // of wk.tile_ex
 constexpr int kUnit = -10;  // dP and D of a row are taken times 2^(kUnit - exponents of its dout and of V): below 1
 
 // D, and the exponents, of 64 rows of a head; four lanes to a row.
@@ -34,7 +35,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(Args a, BwdWork wk, int64_
   const int tile = (int)(id % wk.tiles);
   const int64_t bh = id / wk.tiles;
   const int b = (int)(bh / a.heads), h = (int)(bh % a.heads);
-  const int sub = threadIdx.x & 3, i = tile * TR + (threadIdx.x >> 2);
+  const int sub = threadIdx.x & 3, i = tile * kTileRows + (threadIdx.x >> 2);
   const Seq seq(a, b);
   float s = 0.f, m = 0.f;
   if (i < seq.len) {
@@ -125,20 +126,22 @@ __device__ __forceinline__ void store_plain(const Args& a, float* part, int kb, 
 }
 
 // A row's part in the kv pass, by row of a tile.
+template <int R>
 struct Rows {
-  float lse[TR];    // its log-sum less its exponent (log2 units); infinity: not there
-  float delta[TR];  // D in the units of dP
-  int ex[TR];
+  float lse[R];    // its log-sum less its exponent (log2 units); infinity: not there
+  float delta[R];  // D in the units of dP
+  int ex[R];
+  unsigned odd;    // set where one is not finite
 };
 
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, BwdWork wk, Grid g) {
   using T = Tile<DP>;
-  constexpr int NT = 64 * NW, KB = 32 * NW;
+  constexpr int NT = 64 * NW, KB = 32 * NW, R = T::R, AHEAD = 1;
   __shared__ __attribute__((aligned(16))) char lds[2][2][T::BYTES];  // [buffer][Q, dout]
-  __shared__ __attribute__((aligned(16))) Rows rows[4];
-  __shared__ Tops tops;
-  __shared__ int shared_ex, shared_ev;
+  __shared__ __attribute__((aligned(16))) Rows<R> rows[4];
+  __shared__ __attribute__((aligned(16))) Tops<NW> tops;
+  __shared__ int shared_ex[NW], shared_ev[NW];
   const Place pl = g.place();
   const int b = (int)(pl.group / a.kv_heads), e = (int)(pl.group % a.kv_heads);
   const Seq seq(a, b);
@@ -152,20 +155,38 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, half = lane >> 5;
   const int kw = k0 + 32 * w, j = kw + c;  // of this wave, of this lane
   const bool live = j < seq.len;
-  const int per_head = i_begin < i_end ? (i_end - i_begin + TR - 1) / TR : 0;
+  const int per_head = i_begin < i_end ? (i_end - i_begin + R - 1) / R : 0;
   const int count = per_head * a.group;
+  float* part = far ? wk.part + ((pl.group * wk.sink_blocks + kb) * wk.fars + chunk) * 2 * KB * a.dim : nullptr;
+  // This wave's keys with fp32 products.
+  const auto plain = [&]() {
+    for (int r = 0; r < 32; ++r) {
+      const int key = kw + r;
+      if (key >= a.keys) break;
+      float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
+      const int end = key < a.sinks ? i_end : (int)min((int64_t)i_end, (int64_t)key + a.window);
+      if (key < seq.len)
+        for (int q = 0; q < a.group; ++q) plain_kv_sums(a, b, e * a.group + q, key, max(key, i_begin), end, sk, sv);
+      store_plain(a, part, KB, b, e, key, key - k0, sk, sv);
+    }
+  };
+  if (count == 0 || a.dim < 4) {  // (the workgroup) nobody sees them, or rows too short to load
+    plain();
+    return;
+  }
   const Places<DP> at(lane);
 
-  if (threadIdx.x < 8) tops.v[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
-  if (threadIdx.x == 0) {
-    shared_ex = kNone;
-    shared_ev = kNone;
-  }
-  __syncthreads();
-  // the largest exponent of the rows of dout to come
-  for (int t = threadIdx.x; t < count; t += NT) {
-    const int64_t bh = (int64_t)b * a.heads + e * a.group + t / per_head;
-    atomicMax(&shared_ex, wk.tile_ex[bh * wk.tiles + i_begin / TR + t % per_head]);
+  // The largest exponent of the rows of dout to come.
+  int ex0 = kNone;
+  {
+    const int n = (i_end - i_begin + kTileRows - 1) / kTileRows;
+    for (int t = threadIdx.x; t < n * a.group; t += NT) {
+      const int64_t bh = (int64_t)b * a.heads + e * a.group + t / n;
+      ex0 = max(ex0, wk.tile_ex[bh * wk.tiles + i_begin / kTileRows + t % n]);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) ex0 = max(ex0, __shfl_xor(ex0, x, 64));
+    if (lane == 0) shared_ex[w] = ex0;
   }
   // this lane's rows of K, at a power of two of its own, and of V, at the workgroup's
   Frag kf[T::KS], vf[T::KS];
@@ -183,11 +204,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
     odd |= !(m < INFINITY);
     const int ex = exponent(m);
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) x[s][n] = __builtin_amdgcn_ldexpf(x[s][n], kTop - ex);
-      kf[s] = split8(x[s]);
-    }
+    for (int s = 0; s < T::KS; ++s) kf[s] = split8(x[s], scale(ex));
     ek = ex;
   }
   int ev;
@@ -200,58 +217,59 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
       m = fmaxf(m, top8(x[s]));
     }
     odd |= !(m < INFINITY);
-    m = fmaxf(row16_max(m), __shfl_xor(row16_max(m), 16, 64));
-    m = fmaxf(m, other_half(m));
-    if (lane == 0) atomicMax(&shared_ev, exponent(m));
+    m = wave_top(m);
+    if (lane == 63) shared_ev[w] = exponent(m);
     __syncthreads();
-    ev = shared_ev;
+    ev = shared_ev[0], ex0 = shared_ex[0];
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
+    for (int i = 1; i < NW; ++i) ev = max(ev, shared_ev[i]), ex0 = max(ex0, shared_ex[i]);
 #pragma unroll
-      for (int n = 0; n < 8; ++n) x[s][n] = __builtin_amdgcn_ldexpf(x[s][n], kTop - ev);
-      vf[s] = split8(x[s]);
-    }
+    for (int s = 0; s < T::KS; ++s) vf[s] = split8(x[s], scale(ev));
   }
-  const int ex0 = shared_ex;
-
   Share<DP, NT> rq, rg;
   float r_lse = 0.f, r_delta = 0.f;  // of row threadIdx.x of the tile to come
   int r_ex = 0;
-  const auto head_of = [&](int t) { return e * a.group + t / per_head; };
-  const auto row_of = [&](int t) { return i_begin + TR * (t % per_head); };
+  // Tiles past the last are the last once more, which nobody reads: no branches around loads.
+  struct At {
+    int h, r0;
+  };
+  const auto at_tile = [&](int t) {
+    t = min(t, count - 1);
+    return At{e * a.group + t / per_head, i_begin + R * (t % per_head)};
+  };
   auto fetch = [&](int t) {
-    const int h = head_of(t), r0 = row_of(t);
-    rq.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)h * a.dim, a.ldq, r0, i_end, a.dim);
-    rg.load(a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)h * a.dim, a.lddo, r0, i_end, a.dim);
-    if (threadIdx.x < TR) {
-      const int i = r0 + (int)threadIdx.x;
-      r_lse = INFINITY, r_delta = 0.f, r_ex = 0;
-      if (i < i_end) {
-        const int64_t st = ((int64_t)b * a.heads + h) * a.rows + i;
-        r_lse = a.lse_in[st];
-        r_delta = a.delta[st];
-        r_ex = wk.ex[st];
-      }
-    }
+    const At x = at_tile(t);
+    rq.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)x.h * a.dim, a.ldq, x.r0, i_end, a.dim);
+    rg.load(a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)x.h * a.dim, a.lddo, x.r0, i_end, a.dim);
+    const int64_t st = ((int64_t)b * a.heads + x.h) * a.rows + min(x.r0 + (int)threadIdx.x % R, i_end - 1);
+    r_lse = a.lse_in[st];
+    r_delta = a.delta[st];
+    r_ex = wk.ex[st];
   };
   // The tile's largest of Q, and what its rows are scaled by: one step ahead of put().
   auto tell = [&](int t) {
-    add_top(&tops.v[t & 3][0], rq.top());
-    if (threadIdx.x < TR) {
-      Rows& r = rows[t & 3];
-      if (r_ex == kOdd) atomicMax(&tops.v[t & 3][1], 1u);
-      const int ex = r_ex == kOdd ? 0 : r_ex;
-      r.ex[threadIdx.x] = ex;
-      r.lse[threadIdx.x] = r_lse * kLog2e - (float)(ex - ex0);
-      r.delta[threadIdx.x] = __builtin_amdgcn_ldexpf(r_delta, kUnit - ex - ev);
+    const At x = at_tile(t);
+    rq.clear(x.r0, i_end, a.dim);
+    rg.clear(x.r0, i_end, a.dim);
+    tops.add(0, t, rq.top());
+    if (threadIdx.x < 64) {
+      Rows<R>& r = rows[t & 3];
+      const int n = threadIdx.x % R;
+      const bool there = x.r0 + n < i_end, bad = there && r_ex == kOdd;
+      const int ex = there && !bad ? r_ex : 0;
+      r.ex[n] = ex;
+      r.lse[n] = there ? r_lse * kLog2e - (float)(ex - ex0) : INFINITY;
+      r.delta[n] = there ? __builtin_amdgcn_ldexpf(r_delta, kUnit - ex - ev) : 0.f;
+      const unsigned any = __any(bad) ? 1u : 0u;
+      if (threadIdx.x == 0) r.odd = any;
     }
   };
   int eq = kNone, eq_next = kNone;
   auto put = [&](int t) {
-    const float mq = __builtin_bit_cast(float, tops.v[t & 3][0]);
-    odd |= !(mq < INFINITY) || tops.v[t & 3][1] != 0u;
+    const float mq = tops.get(0, t);
+    odd |= !(mq < INFINITY) || rows[t & 3].odd != 0u;
     eq_next = max(eq_next, exponent(mq));
-    rq.put(lds[t & 1][0], kTop - eq_next);
+    rq.put(lds[t & 1][0], eq_next);
     rg.put_rows(lds[t & 1][1], rows[t & 3].ex);
   };
   f32x16 dk[T::DB], dv[T::DB];
@@ -262,24 +280,20 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
   // this key's P is held at 2^sj (times its row's power of two), its dS at 2^(sj + tj)
   float sj = 100.f;
   int tj = 100;
-  if (count > 0) {
-    fetch(0);
-    tell(0);
-  }
+  fetch(0);
+  tell(0);
   __syncthreads();
-  if (count > 0) put(0);
-  if (count > 1) {
-    fetch(1);
-    tell(1);
-  }
+  put(0);
+  fetch(1);
+  tell(1);
   for (int t = 0; t < count; ++t) {
     __syncthreads();  // tile t lies in its buffer, nobody reads the other, tile t + 1 is announced
     const int eqt = eq_next;
-    if (t + 1 < count) put(t + 1);
-    if (threadIdx.x < 2) tops.v[(t + 3) & 3][threadIdx.x] = 0u;
+    put(t + 1);
+    fetch(t + 2);
     const char *tq = lds[t & 1][0], *tg = lds[t & 1][1];
-    const Rows& rw = rows[t & 3];
-    const int r0 = row_of(t);
+    const Rows<R>& rw = rows[t & 3];
+    const int r0 = at_tile(t).r0;
     if (eqt != eq) {  // Q's operand has a larger power of two from here on
 #pragma unroll
       for (int d = 0; d < T::DB; ++d)
@@ -287,21 +301,20 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
         for (int r = 0; r < 16; ++r) dk[d][r] = __builtin_amdgcn_ldexpf(dk[d][r], eq - eqt);
       eq = eqt;
     }
-    if (t + 2 < count) fetch(t + 2);
     const float ct = __builtin_amdgcn_ldexpf(a.scale * kLog2e, ek + eqt - 2 * kTop);
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < T::NB; ++n) {
       const int i0 = r0 + 32 * n;  // rows of this block
       // some pair of it visible?
       if (i0 >= i_end || kw >= seq.len || i0 + 31 < kw || (i0 - (kw + 31) >= a.window && kw >= a.sinks)) continue;
       f32x16 s, x;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = x[r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < T::KS; ++k) {
-        mma3(frag_row<DP>(tq, at, n, k), kf[k], s);
-        mma3(frag_row<DP>(tg, at, n, k), vf[k], x);
-      }
+      steps<2 * T::KS, AHEAD>([&](int i) { return frag_row<DP>(i & 1 ? tg : tq, at, n, i >> 1); },
+                              [&](int i, const Frag& f) {
+                                if (i & 1) mma3(f, vf[i >> 1], x);
+                                else mma3(f, kf[i >> 1], s);
+                              });
       const bool all = kw + 31 <= i0 && (i0 + 31 - kw < a.window || kw + 31 < a.sinks) && kw + 32 <= seq.len;
       f32x4 lse[4], delta[4];
 #pragma unroll
@@ -315,7 +328,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
         s[r] = fmaf(s[r], ct, -lse[r >> 2][r & 3]);
         if (!all) {
           const int i = i0 + 8 * (r >> 2) + 4 * half + (r & 3);
-          s[r] = live & sees(a, i, j) ? s[r] : -INFINITY;
+          s[r] = (live & sees(a, i, j)) ? s[r] : -INFINITY;
         }
         mx = fmaxf(mx, s[r]);
       }
@@ -339,36 +352,23 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
       }
       rescale(mx, tj, dk);
       const float ft = __builtin_amdgcn_ldexpf(1.f, tj);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] *= ft;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const Frag pf = split_rows(s, k), df = split_rows(x, k);
-#pragma unroll
-        for (int d = 0; d < T::DB; ++d) {
-          mma3(frag_col<DP>(tg, at, 2 * n + k, d), pf, dv[d]);
-          mma3(frag_col<DP>(tq, at, 2 * n + k, d), df, dk[d]);
-        }
-      }
+      const Frag pf[2] = {split_rows(s, 0), split_rows(s, 1)}, df[2] = {split_rows(x, 0, ft), split_rows(x, 1, ft)};
+      steps<4 * T::DB, AHEAD>([&](int i) { return frag_col<DP>(i & 1 ? tq : tg, at, 2 * n + i / (2 * T::DB), (i >> 1) % T::DB); },
+                              [&](int i, const Frag& f) {
+                                const int k = i / (2 * T::DB), d = (i >> 1) % T::DB;
+                                if (i & 1) mma3(f, df[k], dk[d]);
+                                else mma3(f, pf[k], dv[d]);
+                              });
     }
-    if (t + 2 < count) tell(t + 2);
+    tell(t + 2);
   }
   float mark = 0.f;
 #pragma unroll
   for (int d = 0; d < T::DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) mark = fmaf(0.f, dk[d][r], fmaf(0.f, dv[d][r], mark));
-  float* part = far ? wk.part + ((pl.group * wk.sink_blocks + kb) * wk.fars + chunk) * 2 * KB * a.dim : nullptr;
   if (__any(odd || mark != 0.f)) {  // (mark is 0 or NaN)
-    for (int r = 0; r < 32; ++r) {
-      const int key = kw + r;
-      if (key >= a.keys) break;
-      float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
-      const int end = key < a.sinks ? i_end : (int)min((int64_t)i_end, (int64_t)key + a.window);
-      if (key < seq.len)
-        for (int q = 0; q < a.group; ++q) plain_kv_sums(a, b, e * a.group + q, key, max(key, i_begin), end, sk, sv);
-      store_plain(a, part, KB, b, e, key, key - k0, sk, sv);
-    }
+    plain();
     return;
   }
   if (j >= a.keys) return;
@@ -376,8 +376,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
   const float* old_v = a.acc_v && !far ? a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim : nullptr;
   float* out_k = far ? part + (j - k0) * a.dim : a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim;
   float* out_v = far ? part + (KB + j - k0) * a.dim : a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim;
-  const int sh_v = live && count > 0 ? -(int)sj + ex0 - kTop : 0;
-  const int sh_k = live && count > 0 ? -(int)sj - tj + ex0 + ev - kUnit + eq - kTop : 0;
+  const int sh_v = live ? -(int)sj + ex0 - kTop : 0;
+  const int sh_k = live ? -(int)sj - tj + ex0 + ev - kUnit + eq - kTop : 0;
 #pragma unroll
   for (int d = 0; d < T::DB; ++d)
 #pragma unroll
@@ -398,9 +398,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, BwdWork wk, Grid g) {
   using T = Tile<DP>;
-  constexpr int NT = 64 * NW;
+  constexpr int NT = 64 * NW, R = T::R, AHEAD = 1;
   __shared__ __attribute__((aligned(16))) char lds[2][2][T::BYTES];  // [buffer][K, V]
-  __shared__ Tops tops;
+  __shared__ __attribute__((aligned(16))) Tops<NW> tops;
   const Block blk = g.block(a, 32 * NW);
   const int b = blk.b, h = blk.h, e = h / a.group;
   const Seq seq(a, b);
@@ -410,18 +410,34 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
   const int first = blk.row, last = min(blk.row + 32 * NW, seq.len) - 1;
   const int wlast = min(row0 + 32, seq.len) - 1;
   const bool any = first <= last;
-  const Tiles tiles(a, first, last);
+  const Tiles<R> tiles(a, first, last);
   const int count = any ? tiles.count : 0;
+  const auto plain = [&]() {  // this wave's rows with fp32 products
+    for (int r = 0; r < 32; ++r)
+      if (row0 + r < a.rows) plain_dq(a, b, h, row0 + r);
+  };
+  if (count == 0 || a.dim < 4) {  // (the workgroup) nothing to see, or rows too short to load
+    plain();
+    return;
+  }
   const float* K = a.k + (int64_t)b * a.keys * a.ldk + (int64_t)e * a.dim;
   const float* V = a.v + (int64_t)b * a.keys * a.ldv + (int64_t)e * a.dim;
   const Places<DP> at(lane);
 
   Share<DP, NT> rk, rv;
-  if (threadIdx.x < 8) tops.v[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
-  if (count > 0) {
-    rk.load(K, a.ldk, tiles.row(0), seq.len, a.dim);
-    rv.load(V, a.ldv, tiles.row(0), seq.len, a.dim);
-  }
+  // Tiles past the last are the last once more, which nobody reads: no branches around loads.
+  auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
+  auto fetch = [&](int t) {
+    rk.load(K, a.ldk, row_of(t), seq.len, a.dim);
+    rv.load(V, a.ldv, row_of(t), seq.len, a.dim);
+  };
+  auto tell = [&](int t) {
+    rk.clear(row_of(t), seq.len, a.dim);
+    rv.clear(row_of(t), seq.len, a.dim);
+    tops.add(0, t, rk.top());
+    tops.add(1, t, rv.top());
+  };
+  fetch(0);
   Frag q[T::KS], go[T::KS];
   int eq, eg;
   bool odd = false;
@@ -437,11 +453,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
     odd |= !(m < INFINITY);
     const int ex = exponent(m);
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) x[s][n] = __builtin_amdgcn_ldexpf(x[s][n], kTop - ex);
-      q[s] = split8(x[s]);
-    }
+    for (int s = 0; s < T::KS; ++s) q[s] = split8(x[s], scale(ex));
     eq = ex;
   }
   {
@@ -456,34 +468,21 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
     odd |= !(m < INFINITY);
     eg = exponent(m);
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) x[s][n] = __builtin_amdgcn_ldexpf(x[s][n], kTop - eg);
-      go[s] = split8(x[s]);
-    }
+    for (int s = 0; s < T::KS; ++s) go[s] = split8(x[s], scale(eg));
   }
   const int64_t st = ((int64_t)b * a.heads + h) * a.rows + (live ? i : 0);
   const float delta = live ? a.delta[st] : 0.f, lse = live ? a.lse_in[st] * kLog2e : 0.f;
   odd |= !(fabsf(delta) < INFINITY) || !(fabsf(lse) < INFINITY);
-  __syncthreads();  // tops are clear
   int ek = kNone, ek_next = kNone, ev = 0;
   auto put = [&](int t) {
-    const float mk = __builtin_bit_cast(float, tops.v[t & 3][0]), mv = __builtin_bit_cast(float, tops.v[t & 3][1]);
+    const float mk = tops.get(0, t), mv = tops.get(1, t);
     odd |= !(fmaxf(mk, mv) < INFINITY);
     ek_next = max(ek_next, exponent(mk));
     ev = exponent(mv);
-    rk.put(lds[t & 1][0], kTop - ek_next);
-    rv.put(lds[t & 1][1], kTop - ev);
+    rk.put(lds[t & 1][0], ek_next);
+    rv.put(lds[t & 1][1], ev);
   };
-  auto fetch = [&](int t) {
-    rk.load(K, a.ldk, tiles.row(t), seq.len, a.dim);
-    rv.load(V, a.ldv, tiles.row(t), seq.len, a.dim);
-  };
-  auto tell = [&](int t) {
-    add_top(&tops.v[t & 3][0], rk.top());
-    add_top(&tops.v[t & 3][1], rv.top());
-  };
-  if (count > 0) tell(0);
+  tell(0);
   __syncthreads();
   f32x16 dq[T::DB];
 #pragma unroll
@@ -492,17 +491,14 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
   int ti = 100;  // this row's dS is held at 2^ti (and below)
   const float dd = __builtin_amdgcn_ldexpf(delta, -eg);
-  if (count > 0) put(0);
-  if (count > 1) {
-    fetch(1);
-    tell(1);
-  }
+  put(0);
+  fetch(1);
+  tell(1);
   for (int t = 0; t < count; ++t) {
     __syncthreads();
     const int ekt = ek_next, evt = ev;
-    if (t + 1 < count) put(t + 1);
-    if (threadIdx.x < 2) tops.v[(t + 3) & 3][threadIdx.x] = 0u;
-    if (t + 2 < count) fetch(t + 2);
+    put(t + 1);
+    fetch(t + 2);
     const char *tk = lds[t & 1][0], *tv = lds[t & 1][1];
     const int j0 = tiles.row(t);
     if (ekt != ek) {  // K's operand has a larger power of two from here on
@@ -515,17 +511,17 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
     const float ct = __builtin_amdgcn_ldexpf(a.scale * kLog2e, eq + ekt - 2 * kTop);
     const float cd = __builtin_amdgcn_ldexpf(1.f, evt - 2 * kTop);  // dP - D at 2^-eg
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < T::NB; ++n) {
       const int jb = j0 + 32 * n;
       if (row0 > wlast || jb > wlast || (row0 - (jb + 31) >= a.window && jb >= a.sinks)) continue;
       f32x16 s, x;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = x[r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < T::KS; ++k) {
-        mma3(frag_row<DP>(tk, at, n, k), q[k], s);
-        mma3(frag_row<DP>(tv, at, n, k), go[k], x);
-      }
+      steps<2 * T::KS, AHEAD>([&](int i) { return frag_row<DP>(i & 1 ? tv : tk, at, n, i >> 1); },
+                              [&](int i, const Frag& f) {
+                                if (i & 1) mma3(f, go[i >> 1], x);
+                                else mma3(f, q[i >> 1], s);
+                              });
       const bool all = jb + 31 <= row0 && (wlast - jb < a.window || jb + 31 < a.sinks) && row0 + 32 <= seq.len;
       float mx = 0.f;
 #pragma unroll
@@ -533,23 +529,18 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
         float p = fmaf(s[r], ct, -lse);
         if (!all) {
           const int j = jb + 8 * (r >> 2) + 4 * half + (r & 3);
-          p = live & sees(a, i, j) ? p : -INFINITY;
+          p = (live & sees(a, i, j)) ? p : -INFINITY;
         }
         x[r] = __builtin_amdgcn_exp2f(p) * fmaf(x[r], cd, -dd);
         mx = fmaxf(mx, fabsf(x[r]));
       }
       rescale(mx, ti, dq);
       const float ft = __builtin_amdgcn_ldexpf(1.f, ti);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] *= ft;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const Frag df = split_rows(x, k);
-#pragma unroll
-        for (int d = 0; d < T::DB; ++d) mma3(frag_col<DP>(tk, at, 2 * n + k, d), df, dq[d]);
-      }
+      const Frag df[2] = {split_rows(x, 0, ft), split_rows(x, 1, ft)};
+      steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<DP>(tk, at, 2 * n + i / T::DB, i % T::DB); },
+                              [&](int i, const Frag& f) { mma3(f, df[i / T::DB], dq[i % T::DB]); });
     }
-    if (t + 2 < count) tell(t + 2);
+    tell(t + 2);
   }
   float mark = 0.f;
 #pragma unroll
@@ -557,8 +548,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
 #pragma unroll
     for (int r = 0; r < 16; ++r) mark = fmaf(0.f, dq[d][r], mark);
   if (__any(odd || mark != 0.f)) {
-    for (int r = 0; r < 32; ++r)
-      if (row0 + r < a.rows) plain_dq(a, b, h, row0 + r);
+    plain();
     return;
   }
   if (i >= a.rows) return;

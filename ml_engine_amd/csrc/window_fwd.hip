@@ -3,24 +3,25 @@
 // softmax.
 //
 // Scores come out as S^T = K Q^T, rows to lanes, so a row's statistics are a lane's
-// (two lanes hold 16 keys of a row each), and P^T is the operand of O^T += V^T P^T as
-// it lies in the accumulators.  P is held as 2^15 P.
+// (two lanes hold 16 of every 32 keys of a row each), and P^T is the operand of
+// O^T += V^T P^T as it lies in the accumulators.  P is held at 2^8 for a row's maximum so
+// far; the sums are rescaled only when a score passes that by 2^7.
 #include "window_tile.hpp"
 #include "window_kernels.hpp"
-
-#include <type_traits>
 
 using namespace mle;
 
 namespace wattn {
 namespace {
 
+constexpr float kHead = 8.f;
+
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
   using T = Tile<DP>;
-  constexpr int NT = 64 * NW;
+  constexpr int NT = 64 * NW, R = T::R, AHEAD = 2;
   __shared__ __attribute__((aligned(16))) char lds[2][2][T::BYTES];  // [buffer][K, V]
-  __shared__ Tops tops;
+  __shared__ __attribute__((aligned(16))) Tops<NW> tops;
   const Block blk = g.block(a, 32 * NW);
   const int b = blk.b, h = blk.h, e = h / a.group;
   const Seq seq(a, b);
@@ -32,18 +33,31 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
   const int first = max(seq.first + blk.row, 0), last = min(seq.first + min(blk.row + 32 * NW, a.rows), seq.len) - 1;
   const int wfirst = max(seq.first + row0, 0), wlast = min(seq.first + min(row0 + 32, a.rows), seq.len) - 1;
   const bool any = first <= last;
-  const Tiles tiles(a, first, last);
+  const Tiles<R> tiles(a, first, last);
   const int count = any ? tiles.count : 0;
+  if (count == 0 || a.dim < 4) {  // (the workgroup) nothing to see, or rows too short to load
+    for (int r = 0; r < 32; ++r)
+      if (row0 + r < a.rows) plain_row(a, b, h, row0 + r);
+    return;
+  }
   const float* K = a.k + (int64_t)b * a.keys * a.ldk + (int64_t)e * a.dim;
   const float* V = a.v + (int64_t)b * a.keys * a.ldv + (int64_t)e * a.dim;
   const Places<DP> at(lane);
 
   Share<DP, NT> rk, rv;
-  if (threadIdx.x < 8) tops.v[threadIdx.x >> 1][threadIdx.x & 1] = 0u;
-  if (count > 0) {
-    rk.load(K, a.ldk, tiles.row(0), seq.len, a.dim);
-    rv.load(V, a.ldv, tiles.row(0), seq.len, a.dim);
-  }
+  // Tiles past the last are the last once more, which nobody reads: no branches around loads.
+  auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
+  auto fetch = [&](int t) {
+    rk.load(K, a.ldk, row_of(t), seq.len, a.dim);
+    rv.load(V, a.ldv, row_of(t), seq.len, a.dim);
+  };
+  auto tell = [&](int t) {
+    rk.clear(row_of(t), seq.len, a.dim);
+    rv.clear(row_of(t), seq.len, a.dim);
+    tops.add(0, t, rk.top());
+    tops.add(1, t, rv.top());
+  };
+  fetch(0);
   // this lane's row of Q, at a power of two of its own
   Frag q[T::KS];
   int eq;
@@ -59,117 +73,108 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
     m = fmaxf(m, other_half(m));
     odd = !(m < INFINITY);
     const int ex = exponent(m);
+    const float sc = a.scale < 0.f ? -scale(ex) : scale(ex);
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[s][j] = __builtin_amdgcn_ldexpf(a.scale < 0.f ? -x[s][j] : x[s][j], kTop - ex);
-      q[s] = split8(x[s]);
-    }
+    for (int s = 0; s < T::KS; ++s) q[s] = split8(x[s], sc);
     eq = ex;
   }
-  __syncthreads();  // tops are clear
   int ek = 0, ev = -1000, ev_next = -1000;  // exponents: of the tile of K at hand, of V's operand so far
   auto put = [&](int t) {  // tile t from the registers to its buffer
-    const float mk = __builtin_bit_cast(float, tops.v[t & 3][0]), mv = __builtin_bit_cast(float, tops.v[t & 3][1]);
+    const float mk = tops.get(0, t), mv = tops.get(1, t);
     odd |= !(fmaxf(mk, mv) < INFINITY);
     ek = exponent(mk);
     ev_next = max(ev_next, exponent(mv));
-    rk.put(lds[t & 1][0], kTop - ek);
-    rv.put(lds[t & 1][1], kTop - ev_next);
+    rk.put(lds[t & 1][0], ek);
+    rv.put(lds[t & 1][1], ev_next);
   };
-  auto fetch = [&](int t) {
-    rk.load(K, a.ldk, tiles.row(t), seq.len, a.dim);
-    rv.load(V, a.ldv, tiles.row(t), seq.len, a.dim);
-  };
-  auto tell = [&](int t) {
-    add_top(&tops.v[t & 3][0], rk.top());
-    add_top(&tops.v[t & 3][1], rv.top());
-  };
-  if (count > 0) tell(0);
+  tell(0);
   __syncthreads();
   f32x16 o[T::DB];
 #pragma unroll
   for (int d = 0; d < T::DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-  float m = -3e38f, l = 0.f;  // log2 units; m is 15 below the maximum
-  if (count > 0) {
-    put(0);
-    if (count > 1) {
-      fetch(1);
-      tell(1);
-    }
-  }
-  for (int t = 0; t < count; ++t) {
-    __syncthreads();  // tile t lies in its buffer, nobody reads the other, tile t + 1's tops are known
-    const int ekt = ek, evt = ev_next;
-    if (t + 1 < count) put(t + 1);
-    if (threadIdx.x < 2) tops.v[(t + 3) & 3][threadIdx.x] = 0u;
-    if (t + 2 < count) fetch(t + 2);
-    const char *tk = lds[t & 1][0], *tv = lds[t & 1][1];
+  float m = -3e38f, l = 0.f;  // log2 units; m is kHead below the maximum
+  const auto some = [&](int t) {  // does the wave see any of tile t?
     const int j0 = tiles.row(t);
-    const bool some = wfirst <= wlast && j0 <= wlast && (wfirst - (j0 + TR - 1) < a.window || j0 < a.sinks);
-    if (evt != ev) {  // V's operand has a larger power of two from here on
+    return wfirst <= wlast && j0 <= wlast && (wfirst - (j0 + R - 1) < a.window || j0 < a.sinks);
+  };
+  Frag pf[2 * T::NB];  // P of a tile
+  // P of tile t, whose K has exponent e.
+  const auto weights = [&](int t, int e) {
+    const char* tk = lds[t & 1][0];
+    const int j0 = tiles.row(t);
+    f32x16 s[T::NB];
+#pragma unroll
+    for (int n = 0; n < T::NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
+    steps<T::KS * T::NB, AHEAD>([&](int i) { return frag_row<DP>(tk, at, i % T::NB, i / T::NB); },
+                                [&](int i, const Frag& f) { mma3(f, q[i / T::NB], s[i % T::NB]); });
+    const bool all = j0 + R - 1 <= wfirst && (wlast - j0 < a.window || j0 + R - 1 < a.sinks) && row0 + 32 <= a.rows &&
+                     seq.first + row0 >= 0 && seq.first + row0 + 32 <= seq.len;
+    if (!all) {
+#pragma unroll
+      for (int n = 0; n < T::NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int j = j0 + 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
+          s[n][r] = (live & sees(a, p, j)) ? s[n][r] : -INFINITY;
+        }
+    }
+    // (never 0, so that what is hidden stays at minus infinity)
+    const float ct = fmaxf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, eq + e - 2 * kTop), 0x1p-126f);
+    float mx = s[0][0];
+#pragma unroll
+    for (int n = 0; n < T::NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx *= ct;
+    if (__any(mx > m + 15.f)) {
+      const float mn = fmaxf(m, fmaxf(mx, other_half(mx)) - kHead), f = __builtin_amdgcn_exp2f(m - mn);
+      l *= f;
 #pragma unroll
       for (int d = 0; d < T::DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] = __builtin_amdgcn_ldexpf(o[d][r], ev - evt);
-      ev = evt;
+        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+      m = mn;
     }
-    if (some) {
-      f32x16 s[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < T::NB; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < T::KS; ++k)
-#pragma unroll
-        for (int n = 0; n < 2; ++n) mma3(frag_row<DP>(tk, at, n, k), q[k], s[n]);
-      const bool all = j0 + TR - 1 <= wfirst && (wlast - j0 < a.window || j0 + TR - 1 < a.sinks) && row0 + 32 <= a.rows &&
-                       seq.first + row0 >= 0 && seq.first + row0 + 32 <= seq.len;
-      if (!all) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = j0 + 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
-            s[n][r] = live & sees(a, p, j) ? s[n][r] : -INFINITY;
-          }
-      }
-      // (never 0, so that what is hidden stays at minus infinity)
-      const float ct = fmaxf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, eq + ekt - 2 * kTop), 0x1p-126f);
-      float mx = s[0][0];
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-      mx = fmaxf(mx, other_half(mx));
-      const float mn = fmaxf(m, mx * ct - 15.f);
-      if (__any(mn > m)) {
-        const float f = __builtin_amdgcn_exp2f(m - mn);
-        l *= f;
-#pragma unroll
-        for (int d = 0; d < T::DB; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[d][r] *= f;
-        m = mn;
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], ct, -m));
+        l += s[n][r];
       }
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int k = 0; k < 2 * T::NB; ++k) pf[k] = split_rows(s[k >> 1], k & 1);
+  };
+  // O += P V of tile t, whose operand of V has exponent e.
+  const auto values = [&](int t, int e) {
+    if (e != ev) {  // V's operand has a larger power of two from here on
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], ct, -m));
-          l += s[n][r];
-        }
+      for (int d = 0; d < T::DB; ++d)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const Frag pf = split_rows(s[k >> 1], k & 1);
-#pragma unroll
-        for (int d = 0; d < T::DB; ++d) mma3(frag_col<DP>(tv, at, k, d), pf, o[d]);
-      }
+        for (int r = 0; r < 16; ++r) o[d][r] = __builtin_amdgcn_ldexpf(o[d][r], ev - e);
+      ev = e;
     }
-    if (t + 2 < count) tell(t + 2);
+    const char* tv = lds[t & 1][1];
+    steps<2 * T::NB * T::DB, AHEAD>([&](int i) { return frag_col<DP>(tv, at, i / T::DB, i % T::DB); },
+                                    [&](int i, const Frag& f) { mma3(f, pf[i / T::DB], o[i % T::DB]); });
+  };
+  put(0);
+  fetch(1);
+  tell(1);
+  for (int t = 0; t < count; ++t) {
+    __syncthreads();  // tile t lies in its buffer, nobody reads the other, tile t + 1's tops are known
+    const int ekt = ek, evt = ev_next;
+    put(t + 1);
+    fetch(t + 2);
+    if (some(t)) {
+      weights(t, ekt);
+      values(t, evt);
+    }
+    tell(t + 2);
   }
   l += other_half(l);
   float mark = l;  // not finite where a score or a sum is not
@@ -205,8 +210,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
 
 template <int DP>
 void launch_dim(const Args& a, hipStream_t s) {
-  // 8 waves share a tile of 64 keys, 4 a smaller window: a workgroup walks over window +
-  // rows keys, of which a wave computes window + 32
+  // 8 waves share a tile, 4 where the window is small: a workgroup walks over window + rows
+  // keys, of which a wave computes window + 32.
   const bool wide = a.window >= 512 && (int64_t)a.batch * a.heads * ((a.rows + 255) / 256) >= 256;
   const int nw = wide ? 8 : 4;
   const Grid g(a, a.heads, (a.rows + 32 * nw - 1) / (32 * nw));

@@ -1,4 +1,4 @@
-// Tiles of 64 rows for the attention kernels, and products of them on the matrix
+// Tiles of 64 or 32 rows for the attention kernels, and products of them on the matrix
 // cores with fp32 accuracy.
 //
 // Products.  An fp32 value x, scaled by a power of two so that its tile's largest is in
@@ -24,6 +24,8 @@
 #pragma once
 #include "window_attention.hpp"
 
+#include <type_traits>
+
 namespace wattn {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -32,14 +34,15 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int TR = 64;      // rows of a tile
 constexpr int kTop = 14;    // exponent of a tile's largest value
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// DP: columns, the head's dimension rounded up to 64, 96 or 128.
+// DP: columns, the head's dimension rounded up to 64, 96 or 128.  Fewer rows of wide heads:
+// as many products to a tile, half the registers on the way to LDS.
 template <int DP>
 struct Tile {
-  static constexpr int UNITS = DP / 8, PITCH = DP <= 64 ? 128 : 256, PLANE = TR * PITCH, BYTES = 2 * PLANE;
+  static constexpr int R = DP <= 64 ? 64 : 32, NB = R / 32;  // rows, blocks of 32
+  static constexpr int UNITS = DP / 8, PITCH = DP <= 64 ? 128 : 256, PLANE = R * PITCH, BYTES = 2 * PLANE;
   static constexpr int KS = DP / 16, DB = DP / 32;  // steps over the columns; blocks of 32 columns
 };
 
@@ -62,14 +65,31 @@ __device__ __forceinline__ void mma3(const Frag& a, const Frag& b, f32x16& c) {
   c = mma(a.hi, b.hi, c);
 }
 
+// x in two parts: hi its first 11 bits, lo the next 11.  (Masked and subtracted: 5.1 ns a wave
+// and value; two v_fma_mix_f16 take 7.2.)
 __device__ __forceinline__ Frag split8(const float (&x)[8]) {
-  Frag f;
+  f16x2 h[4], l[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    f.hi[j] = (_Float16)x[j];
-    f.lo[j] = (_Float16)(x[j] - (float)f.hi[j]);
+  for (int j = 0; j < 4; ++j) {
+    float a[2], b[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      a[n] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x[2 * j + n]) & 0xffffe000u);
+      b[n] = x[2 * j + n] - a[n];
+    }
+    h[j] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a[0], a[1]));
+    l[j] = f16x2{(_Float16)b[0], (_Float16)b[1]};
   }
-  return f;
+  return Frag{__builtin_shufflevector(__builtin_shufflevector(h[0], h[1], 0, 1, 2, 3),
+                                      __builtin_shufflevector(h[2], h[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7),
+              __builtin_shufflevector(__builtin_shufflevector(l[0], l[1], 0, 1, 2, 3),
+                                      __builtin_shufflevector(l[2], l[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7)};
+}
+__device__ __forceinline__ Frag split8(const float (&x)[8], float s) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = x[j] * s;
+  return split8(v);
 }
 
 // Eight of a block's 16 rows as an operand.
@@ -79,27 +99,29 @@ __device__ __forceinline__ Frag split_rows(const f32x16& x, int s) {
   for (int j = 0; j < 8; ++j) v[j] = x[8 * s + j];
   return split8(v);
 }
+__device__ __forceinline__ Frag split_rows(const f32x16& x, int s, float scale) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = x[8 * s + j];
+  return split8(v, scale);
+}
 
-// A lane's places in a tile.
+// A lane's places in a tile: of frag_row's first step and of frag_col's first columns.  Later
+// ones differ in bits that the swizzle only flips.
 template <int DP>
 struct Places {
-  int row[Tile<DP>::KS];  // of frag_row: row lane % 32, columns 16 s + 8 (lane / 32) ..
-  int col[Tile<DP>::DB];  // of frag_col
+  int row, col;
   __device__ __forceinline__ Places(int lane) {
-    const int c = lane & 31, h = lane >> 5, i = lane & 15, g = (lane >> 4) & 1;
-#pragma unroll
-    for (int s = 0; s < Tile<DP>::KS; ++s) row[s] = c * Tile<DP>::PITCH + (((2 * s + h) ^ swizzle<DP>(c)) << 4);
-    const int r = 4 * h + (i >> 2);
-#pragma unroll
-    for (int d = 0; d < Tile<DP>::DB; ++d)
-      col[d] = r * Tile<DP>::PITCH + (((4 * d + 2 * g + ((i & 3) >> 1)) ^ swizzle<DP>(r)) << 4) + 8 * (i & 1);
+    const int c = lane & 31, h = lane >> 5, i = lane & 15, g = (lane >> 4) & 1, r = 4 * h + (i >> 2);
+    row = c * Tile<DP>::PITCH + ((h ^ swizzle<DP>(c)) << 4);  // row c, columns 16 s + 8 h ..
+    col = r * Tile<DP>::PITCH + (((2 * g + ((i & 3) >> 1)) ^ swizzle<DP>(r)) << 4) + 8 * (i & 1);
   }
 };
 
-// Rows 32 b + lane % 32, columns of step s.
+// Row 32 b + lane % 32, columns of step s.
 template <int DP>
 __device__ __forceinline__ Frag frag_row(const char* t, const Places<DP>& p, int b, int s) {
-  const char* at = t + p.row[s] + 32 * b * Tile<DP>::PITCH;
+  const char* at = t + (p.row ^ (s << 5)) + 32 * b * Tile<DP>::PITCH;
   Frag f;
   f.hi = *reinterpret_cast<const f16x8*>(at);
   f.lo = *reinterpret_cast<const f16x8*>(at + Tile<DP>::PLANE);
@@ -113,8 +135,9 @@ __device__ __forceinline__ s16x4 read_tr(const char* p) {
 // Columns 32 d + lane % 32, the 16 rows of step s in the accumulators' order.
 template <int DP>
 __device__ __forceinline__ Frag frag_col(const char* t, const Places<DP>& p, int s, int d) {
-  const char* a = t + p.col[d] + 16 * s * Tile<DP>::PITCH;
-  const char* b = t + (p.col[d] ^ 16) + (16 * s + 8) * Tile<DP>::PITCH;  // 8 rows on: the swizzle's last bit
+  const int c = p.col ^ (d << 6);
+  const char* a = t + c + 16 * s * Tile<DP>::PITCH;
+  const char* b = t + (c ^ 16) + (16 * s + 8) * Tile<DP>::PITCH;  // 8 rows on: the swizzle's last bit
   Frag f;
   const f16x4 h0 = __builtin_bit_cast(f16x4, read_tr(a)), h1 = __builtin_bit_cast(f16x4, read_tr(b));
   const f16x4 l0 = __builtin_bit_cast(f16x4, read_tr(a + Tile<DP>::PLANE)),
@@ -153,39 +176,80 @@ __device__ __forceinline__ float top8(const float (&x)[8]) {
   return m;
 }
 
-// The largest over 16 lanes, in each of them.
-__device__ __forceinline__ float row16_max(float v) {
-  auto dpp = [](float x, auto ctrl) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+// The largest of a wave's values, all at least 0, in lane 63.
+__device__ __forceinline__ float wave_top(float v) {
+  auto step = [](float x, auto ctrl, auto rows) {
+    return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                                          decltype(rows)::value, 0xF, false)));
   };
-  v = fmaxf(v, dpp(v, std::integral_constant<int, 0xB1>{}));   // lanes 1 0 3 2
-  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x4E>{}));   // lanes 2 3 0 1
-  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x124>{}));  // four lanes round
-  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x128>{}));  // eight
-  return v;
+  typedef std::integral_constant<int, 0xF> All;
+  v = step(v, std::integral_constant<int, 0xB1>{}, All{});   // lanes 1 0 3 2
+  v = step(v, std::integral_constant<int, 0x4E>{}, All{});   // lanes 2 3 0 1
+  v = step(v, std::integral_constant<int, 0x124>{}, All{});  // four lanes round
+  v = step(v, std::integral_constant<int, 0x128>{}, All{});  // eight: a row of 16
+  v = step(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // rows 0, 2 to 1, 3
+  return step(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // half to half
 }
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
-// floor(log2) of a magnitude (0 and subnormals as 2^-127, infinity as the largest number).
+// floor(log2) of a magnitude, within what scale() can raise (smaller ones, 0 among them, as
+// 2^-112; infinity as the largest number).
 __device__ __forceinline__ int exponent(float m) {
   const int e = (int)(__builtin_bit_cast(unsigned, m) >> 23);
-  return min(e, 254) - 127;
+  return min(max(e, 15), 254) - 127;
 }
+// The power of two that brings values of this exponent to [2^kTop, 2^(kTop + 1)).
+__device__ __forceinline__ float scale(int e) { return __builtin_bit_cast(float, (unsigned)(kTop - e + 127) << 23); }
 
 // A thread's share of a tile of NT threads: N chunks of eight columns.
 template <int DP, int NT>
 struct Share {
-  static constexpr int ALL = TR * Tile<DP>::UNITS, N = (ALL + NT - 1) / NT;
+  static constexpr int ALL = Tile<DP>::R * Tile<DP>::UNITS, N = (ALL + NT - 1) / NT;
   float x[N][8];
-  static __device__ __forceinline__ int unit(int c) { return c * NT + (int)threadIdx.x; }
   static constexpr bool whole = ALL % NT == 0;
-  // Rows r0 .. r0 + 63 of a tensor from `base`, those in [r0, end).
+  // (a chunk past the last is the last, read again and not put)
+  static __device__ __forceinline__ int unit(int c) {
+    const int id = c * NT + (int)threadIdx.x;
+    return whole ? id : min(id, ALL - 1);
+  }
+  static __device__ __forceinline__ bool has(int c) {
+    return whole || c * NT + (int)threadIdx.x < ALL;
+  }
+  // Rows r0 .. r0 + R - 1 (r0 < end) of a tensor from `base`, dim >= 4.  What is not there is read
+  // at a place that is, and put right by clear() once it has come: two ways of loading would
+  // meet in a copy of the registers, which waits for the loads.
   __device__ __forceinline__ void load(const float* __restrict__ base, int64_t ld, int r0, int end, int dim) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       const int id = unit(c), row = id / Tile<DP>::UNITS, u = id % Tile<DP>::UNITS;
-      const bool there = (whole || id < ALL) && r0 + row < end;
-      load8(base + (int64_t)(there ? r0 + row : 0) * ld, u, dim, there, x[c]);
+      const float* p = base + (int64_t)min(r0 + row, end - 1) * ld;
+      const f32x4u v0 = *reinterpret_cast<const f32x4u*>(p + min(8 * u, dim - 4)),
+                   v1 = *reinterpret_cast<const f32x4u*>(p + min(8 * u + 4, dim - 4));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[c][j] = v0[j];
+        x[c][4 + j] = v1[j];
+      }
+    }
+  }
+  // Zeros from row `end` and column `dim` on; four values that reach past dim have been read as the
+  // last four.
+  __device__ __forceinline__ void clear(int r0, int end, int dim) {
+    if (r0 + Tile<DP>::R <= end && dim == DP) return;
+    const int cut = dim & 3;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int id = unit(c), row = id / Tile<DP>::UNITS, u = id % Tile<DP>::UNITS;
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
+        const int n = r0 + row < end ? dim - 8 * u - k : 0;
+        const float v[4] = {x[c][k], x[c][k + 1], x[c][k + 2], x[c][k + 3]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float late = cut == 3 ? v[min(j + 1, 3)] : cut == 2 ? v[min(j + 2, 3)] : v[3];
+          x[c][k + j] = n >= 4 ? v[j] : j < n ? late : 0.f;
+        }
+      }
     }
   }
   __device__ __forceinline__ float top() const {
@@ -194,24 +258,21 @@ struct Share {
     for (int c = 0; c < N; ++c) m = fmaxf(m, top8(x[c]));
     return m;
   }
-  // Split at 2^shift into a tile; put_rows: at 2^(kTop - ex) of each row.
-  __device__ __forceinline__ void put(char* t, int shift) const {
-    put_with(t, [=](int) { return shift; });
+  // Split at the scale of exponent e into a tile; put_rows: of each row's.
+  __device__ __forceinline__ void put(char* t, int e) const {
+    const float s = scale(e);
+    put_with(t, [=](int) { return s; });
   }
   __device__ __forceinline__ void put_rows(char* t, const int* ex) const {
-    put_with(t, [=](int row) { return kTop - ex[row]; });
+    put_with(t, [=](int row) { return scale(ex[row]); });
   }
   template <class F>
-  __device__ __forceinline__ void put_with(char* t, F shift_of) const {
+  __device__ __forceinline__ void put_with(char* t, F scale_of) const {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       const int id = unit(c), row = id / Tile<DP>::UNITS, u = id % Tile<DP>::UNITS;
-      if (!whole && id >= ALL) break;
-      const int shift = shift_of(row);
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = __builtin_amdgcn_ldexpf(x[c][j], shift);
-      const Frag f = split8(v);
+      if (!has(c)) break;
+      const Frag f = split8(x[c], scale_of(row));
       char* at = t + row * Tile<DP>::PITCH + ((u ^ swizzle<DP>(row)) << 4);
       *reinterpret_cast<f16x8*>(at) = f.hi;
       *reinterpret_cast<f16x8*>(at + Tile<DP>::PLANE) = f.lo;
@@ -219,24 +280,55 @@ struct Share {
   }
 };
 
-// The largest magnitudes of coming tiles: slot t of four takes tile t's, a wave at a time.
+// The largest magnitudes of coming tiles of two tensors: slot t of four takes tile t's, a value
+// from each wave.  (Not an atomic maximum: the compiler makes a loop over lanes of it, some 700
+// cycles a tile.)
+template <int NW>
 struct Tops {
-  unsigned v[4][2];
+  float v[2][4][NW];
+  __device__ __forceinline__ void add(int tensor, int t, float m) {
+    m = wave_top(m);
+    if ((threadIdx.x & 63) == 63) v[tensor][t & 3][threadIdx.x >> 6] = m;
+  }
+  __device__ __forceinline__ float get(int tensor, int t) const {
+    float m = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; w += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&v[tensor][t & 3][w]);
+      m = fmaxf(fmaxf(fmaxf(m, x[0]), fmaxf(x[1], x[2])), x[3]);
+    }
+    return m;
+  }
 };
-__device__ __forceinline__ void add_top(unsigned* slot, float m) {
-  m = row16_max(m);
-  if ((threadIdx.x & 15) == 0) atomicMax(slot, __builtin_bit_cast(unsigned, m));
+
+// N steps, each using a fragment that has been read from LDS AHEAD steps before.  The barriers hold
+// the scheduler to it: left to itself it waits for every read where it is used, which
+// costs a step more than its three products.
+template <int N, int AHEAD, class Load, class Use>
+__device__ __forceinline__ void steps(Load load, Use use) {
+  Frag f[AHEAD + 1];
+#pragma unroll
+  for (int i = 0; i < AHEAD && i < N; ++i) f[i] = load(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i + AHEAD < N) f[(i + AHEAD) % (AHEAD + 1)] = load(i + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+    use(i, f[i % (AHEAD + 1)]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
-// The tiles that rows at positions first .. last (0 <= first <= last) see: sinks before the window, then the window.
+// The tiles of R keys that rows at positions first .. last (0 <= first <= last) see: sinks before
+// the window, then the window.
+template <int R>
 struct Tiles {
   int before, low, count;
   __device__ __forceinline__ Tiles(const Args& a, int first, int last) {
-    low = max(first - a.window + 1, 0) / TR;
-    before = min((a.sinks + TR - 1) / TR, low);
-    count = before + last / TR + 1 - low;
+    low = max(first - a.window + 1, 0) / R;
+    before = min((a.sinks + R - 1) / R, low);
+    count = before + last / R + 1 - low;
   }
-  __device__ __forceinline__ int row(int t) const { return TR * (t < before ? t : low + t - before); }
+  __device__ __forceinline__ int row(int t) const { return R * (t < before ? t : low + t - before); }
 };
 
 }  // namespace wattn
