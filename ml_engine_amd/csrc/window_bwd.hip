@@ -15,18 +15,12 @@
 // own column, a lane's: a key's P and dS (kv), a row's dS (q) have the largest seen so far
 // between 2^8 and 2^15, and a larger one rescales the lane's sums.  Rows of dout are at powers
 // of two of their own too; P takes those up in its exponent.
-#include "window_tile.hpp"
-#include "window_kernels.hpp"
+#include "window_bwd.hpp"
 
 using namespace mle;
 
 namespace wattn {
 namespace {
-
-constexpr int kOdd = 1 << 20;   // in place of a row's exponent: something in it is not finite
-constexpr int kNone = -(1 << 20);
-constexpr int kTileRows = 64;   // of wk.tile_ex
-constexpr int kUnit = -10;  // dP and D of a row are taken times 2^(kUnit - exponents of its dout and of V): below 1
 
 // D, and the exponents, of 64 rows of a head; four lanes to a row.
 __global__ __launch_bounds__(256) void prepare_kernel(Args a, BwdWork wk, int64_t first) {
@@ -80,197 +74,86 @@ __global__ __launch_bounds__(256) void prepare_kernel(Args a, BwdWork wk, int64_
   if (threadIdx.x == 0) wk.tile_ex[id] = max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
-// A column's operand held at 2^t: where its largest, mx of a lane and of the lane's other
-// half, would reach 2^15, t is lowered to bring it to 2^8 .. 2^9, and the sums follow.
-template <int N>
-__device__ __forceinline__ void rescale(float mx, int& t, f32x16 (&sums)[N]) {
-  mx = fmaxf(mx, other_half(mx));
-  const int e = exponent(mx);
-  const bool over = e + t > 14 || t > 120;
-  if (!__any(over)) return;
-  const int to = over ? min(8 - e, 120) : t;
-#pragma unroll
-  for (int d = 0; d < N; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sums[d][r] = __builtin_amdgcn_ldexpf(sums[d][r], to - t);
-  t = to;
-}
-
-// Four of a row's values from column `col`, added to `old` where that is not null.
-__device__ __forceinline__ void store4(float* out, const float* old, int col, int dim, float (&x)[4]) {
-  if (col + 4 <= dim) {
-    f32x4u v = {x[0], x[1], x[2], x[3]};
-    if (old) v += *reinterpret_cast<const f32x4u*>(old + col);
-    *reinterpret_cast<f32x4u*>(out + col) = v;
-  } else {
-#pragma unroll
-    for (int n = 0; n < 4; ++n)
-      if (col + n < dim) out[col + n] = old ? old[col + n] + x[n] : x[n];
-  }
-}
-
-// A key's sums as plain_kv_sums leaves them in a wave, to its gradients or (part) to the
-// workgroup's share of far sums.
-__device__ __forceinline__ void store_plain(const Args& a, float* part, int kb, int b, int e, int key, int local,
-                                            const float (&sk)[2], const float (&sv)[2]) {
-  const int lane = threadIdx.x & 63;
-  float* ok = part ? part + local * a.dim : a.dk + ((int64_t)b * a.keys + key) * a.lddk + (int64_t)e * a.dim;
-  float* ov = part ? part + (kb + local) * a.dim : a.dv + ((int64_t)b * a.keys + key) * a.lddv + (int64_t)e * a.dim;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int d = lane + 64 * r;
-    if (d >= a.dim) continue;
-    ok[d] = (a.acc_k && !part ? ok[d] : 0.f) + sk[r];
-    ov[d] = (a.acc_v && !part ? ov[d] : 0.f) + sv[r];
-  }
-}
-
-// A row's part in the kv pass, by row of a tile.
-template <int R>
-struct Rows {
-  float lse[R];    // its log-sum less its exponent (log2 units); infinity: not there
-  float delta[R];  // D in the units of dP
-  int ex[R];
-  unsigned odd;    // set where one is not finite
+template <int DP, int NW>
+struct Shared {
+  alignas(16) char lds[2][2][Tile<DP, 64>::BYTES];  // [buffer][Q, dout or K, V]
+  alignas(16) Rows<64> rows[4];
+  alignas(16) Tops<NW> tops;
+  int ex[NW];
 };
 
+// dk and dv of 32 keys to a wave.
 template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, BwdWork wk, Grid g) {
-  using T = Tile<DP>;
+__device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const Place& place, Shared<DP, NW>& m) {
+  using T = Tile<DP, 64>;
   constexpr int NT = 64 * NW, KB = 32 * NW, R = T::R, AHEAD = 1;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][T::BYTES];  // [buffer][Q, dout]
-  __shared__ __attribute__((aligned(16))) Rows<R> rows[4];
-  __shared__ __attribute__((aligned(16))) Tops<NW> tops;
-  __shared__ int shared_ex[NW], shared_ev[NW];
-  const Place pl = g.place();
-  const int b = (int)(pl.group / a.kv_heads), e = (int)(pl.group % a.kv_heads);
+  static_assert(KB == kKeyBlock, "keys of a workgroup");
+  const KvJob job(a, wk, place);
+  const int b = job.b, e = job.e, k0 = job.k0, i_end = job.i_end;
   const Seq seq(a, b);
-  const int fi = pl.item - wk.key_blocks;  // (the far blocks last: they are short)
-  const bool far = fi >= 0;
-  const int kb = far ? fi / wk.fars : pl.item, chunk = far ? fi % wk.fars : 0;
-  const int k0 = kb * KB;
-  const int near_end = wk.near_end(a, k0, KB);
-  const int i_begin = far ? near_end + chunk * wk.far_rows : k0;
-  const int i_end = min(far ? i_begin + wk.far_rows : near_end, seq.len);
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, half = lane >> 5;
   const int kw = k0 + 32 * w, j = kw + c;  // of this wave, of this lane
   const bool live = j < seq.len;
-  const int per_head = i_begin < i_end ? (i_end - i_begin + R - 1) / R : 0;
+  const int per_head = job.i_begin < i_end ? (i_end - job.i_begin + R - 1) / R : 0;
   const int count = per_head * a.group;
-  float* part = far ? wk.part + ((pl.group * wk.sink_blocks + kb) * wk.fars + chunk) * 2 * KB * a.dim : nullptr;
-  // This wave's keys with fp32 products.
-  const auto plain = [&]() {
-    for (int r = 0; r < 32; ++r) {
-      const int key = kw + r;
-      if (key >= a.keys) break;
-      float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
-      const int end = key < a.sinks ? i_end : (int)min((int64_t)i_end, (int64_t)key + a.window);
-      if (key < seq.len)
-        for (int q = 0; q < a.group; ++q) plain_kv_sums(a, b, e * a.group + q, key, max(key, i_begin), end, sk, sv);
-      store_plain(a, part, KB, b, e, key, key - k0, sk, sv);
-    }
-  };
   if (count == 0 || a.dim < 4) {  // (the workgroup) nobody sees them, or rows too short to load
-    plain();
+    job.plain(a, kw, true, true);
     return;
   }
-  const Places<DP> at(lane);
-
-  // The largest exponent of the rows of dout to come.
-  int ex0 = kNone;
-  {
-    const int n = (i_end - i_begin + kTileRows - 1) / kTileRows;
-    for (int t = threadIdx.x; t < n * a.group; t += NT) {
-      const int64_t bh = (int64_t)b * a.heads + e * a.group + t / n;
-      ex0 = max(ex0, wk.tile_ex[bh * wk.tiles + i_begin / kTileRows + t % n]);
-    }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) ex0 = max(ex0, __shfl_xor(ex0, x, 64));
-    if (lane == 0) shared_ex[w] = ex0;
-  }
-  // this lane's rows of K, at a power of two of its own, and of V, at the workgroup's
+  const Places<T> at(lane);
+  job.largest(a, wk, m.ex);
+  // this lane's rows of K, at a power of two of its own, and of V, at the wave's
   Frag kf[T::KS], vf[T::KS];
-  int ek;
+  int ek, ev;
   bool odd = false;
   {
-    float x[T::KS][8], m = 0.f;
-    const float* K = a.k + ((int64_t)b * a.keys + (live ? j : 0)) * a.ldk + (int64_t)e * a.dim;
+    float x[T::KS][8];
+    const float top = load_row<T::KS>(a.k + ((int64_t)b * a.keys + (live ? j : 0)) * a.ldk + (int64_t)e * a.dim, half, a.dim, live, x);
+    odd |= !(top < INFINITY);
+    ek = exponent(fmaxf(top, other_half(top)));
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-      load8(K, 2 * s + half, a.dim, live, x[s]);
-      m = fmaxf(m, top8(x[s]));
-    }
-    m = fmaxf(m, other_half(m));
-    odd |= !(m < INFINITY);
-    const int ex = exponent(m);
-#pragma unroll
-    for (int s = 0; s < T::KS; ++s) kf[s] = split8(x[s], scale(ex));
-    ek = ex;
+    for (int s = 0; s < T::KS; ++s) kf[s] = split8(x[s], scale(ek));
   }
-  int ev;
   {
-    float x[T::KS][8], m = 0.f;
-    const float* V = a.v + ((int64_t)b * a.keys + (live ? j : 0)) * a.ldv + (int64_t)e * a.dim;
-#pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-      load8(V, 2 * s + half, a.dim, live, x[s]);
-      m = fmaxf(m, top8(x[s]));
-    }
-    odd |= !(m < INFINITY);
-    m = wave_top(m);
-    if (lane == 63) shared_ev[w] = exponent(m);
-    __syncthreads();
-    ev = shared_ev[0], ex0 = shared_ex[0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) ev = max(ev, shared_ev[i]), ex0 = max(ex0, shared_ex[i]);
+    float x[T::KS][8];
+    const float top = load_row<T::KS>(a.v + ((int64_t)b * a.keys + (live ? j : 0)) * a.ldv + (int64_t)e * a.dim, half, a.dim, live, x);
+    odd |= !(top < INFINITY);
+    ev = __builtin_amdgcn_readlane(exponent(wave_top(top)), 63);
 #pragma unroll
     for (int s = 0; s < T::KS; ++s) vf[s] = split8(x[s], scale(ev));
   }
-  Share<DP, NT> rq, rg;
-  float r_lse = 0.f, r_delta = 0.f;  // of row threadIdx.x of the tile to come
-  int r_ex = 0;
-  // Tiles past the last are the last once more, which nobody reads: no branches around loads.
-  struct At {
-    int h, r0;
-  };
-  const auto at_tile = [&](int t) {
-    t = min(t, count - 1);
-    return At{e * a.group + t / per_head, i_begin + R * (t % per_head)};
-  };
-  auto fetch = [&](int t) {
-    const At x = at_tile(t);
-    rq.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)x.h * a.dim, a.ldq, x.r0, i_end, a.dim);
-    rg.load(a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)x.h * a.dim, a.lddo, x.r0, i_end, a.dim);
-    const int64_t st = ((int64_t)b * a.heads + x.h) * a.rows + min(x.r0 + (int)threadIdx.x % R, i_end - 1);
+  const float cd = __builtin_amdgcn_ldexpf(1.f, ev + kUnit - 2 * kTop);
+  __syncthreads();
+  int ex0 = m.ex[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) ex0 = max(ex0, m.ex[i]);
+  Share<T, NT> in;  // of Q and dout
+  float r_lse, r_delta;  // of row threadIdx.x % 64 of the tile to come
+  int r_ex;
+  Walk<R> ahead(a, job), here(a, job);
+  auto fetch = [&]() {
+    in.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)ahead.h * a.dim, a.ldq,
+            a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)ahead.h * a.dim, a.lddo, ahead.r0, i_end, a.dim);
+    const int64_t st = ((int64_t)b * a.heads + ahead.h) * a.rows + min(ahead.r0 + (int)threadIdx.x % R, i_end - 1);
     r_lse = a.lse_in[st];
     r_delta = a.delta[st];
     r_ex = wk.ex[st];
   };
   // The tile's largest of Q, and what its rows are scaled by: one step ahead of put().
   auto tell = [&](int t) {
-    const At x = at_tile(t);
-    rq.clear(x.r0, i_end, a.dim);
-    rg.clear(x.r0, i_end, a.dim);
-    tops.add(0, t, rq.top());
-    if (threadIdx.x < 64) {
-      Rows<R>& r = rows[t & 3];
-      const int n = threadIdx.x % R;
-      const bool there = x.r0 + n < i_end, bad = there && r_ex == kOdd;
-      const int ex = there && !bad ? r_ex : 0;
-      r.ex[n] = ex;
-      r.lse[n] = there ? r_lse * kLog2e - (float)(ex - ex0) : INFINITY;
-      r.delta[n] = there ? __builtin_amdgcn_ldexpf(r_delta, kUnit - ex - ev) : 0.f;
-      const unsigned any = __any(bad) ? 1u : 0u;
-      if (threadIdx.x == 0) r.odd = any;
-    }
+    in.clear(ahead.r0, i_end, a.dim);
+    m.tops.add(0, t, in.top(false));
+    m.rows[t & 3].put(ahead.r0, i_end, ex0, r_lse, r_delta, r_ex);
+    ahead.next();
   };
-  int eq = kNone, eq_next = kNone;
+  int eq = kNone, eq_next = kNone;  // the exponent of Q's operand, that dk is at and of the tile to come
   auto put = [&](int t) {
-    const float mq = tops.get(0, t);
-    odd |= !(mq < INFINITY) || rows[t & 3].odd != 0u;
+    const float mq = m.tops.get(0, t);
+    const Rows<R>& r = m.rows[t & 3];
+    odd |= !(mq < INFINITY) || r.odd != 0u;
     eq_next = max(eq_next, exponent(mq));
-    rq.put(lds[t & 1][0], eq_next);
-    rg.put_rows(lds[t & 1][1], rows[t & 3].ex);
+    const float sq = scale(eq_next);
+    in.put(m.lds[t & 1][0], m.lds[t & 1][1], [&](bool g, int row) { return g ? scale(r.ex[row]) : sq; });
   };
   f32x16 dk[T::DB], dv[T::DB];
 #pragma unroll
@@ -280,20 +163,21 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
   // this key's P is held at 2^sj (times its row's power of two), its dS at 2^(sj + tj)
   float sj = 100.f;
   int tj = 100;
-  fetch(0);
+  fetch();
   tell(0);
   __syncthreads();
   put(0);
-  fetch(1);
+  fetch();
   tell(1);
   for (int t = 0; t < count; ++t) {
     __syncthreads();  // tile t lies in its buffer, nobody reads the other, tile t + 1 is announced
     const int eqt = eq_next;
     put(t + 1);
-    fetch(t + 2);
-    const char *tq = lds[t & 1][0], *tg = lds[t & 1][1];
-    const Rows<R>& rw = rows[t & 3];
-    const int r0 = at_tile(t).r0;
+    fetch();
+    const char *tq = m.lds[t & 1][0], *tg = m.lds[t & 1][1];
+    const Rows<R>& rw = m.rows[t & 3];
+    const int r0 = here.r0;
+    here.next();
     if (eqt != eq) {  // Q's operand has a larger power of two from here on
 #pragma unroll
       for (int d = 0; d < T::DB; ++d)
@@ -310,7 +194,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
       f32x16 s, x;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = x[r] = 0.f;
-      steps<2 * T::KS, AHEAD>([&](int i) { return frag_row<DP>(i & 1 ? tg : tq, at, n, i >> 1); },
+      steps<2 * T::KS, AHEAD>([&](int i) { return frag_row<T>(i & 1 ? tg : tq, at, n, i >> 1); },
                               [&](int i, const Frag& f) {
                                 if (i & 1) mma3(f, vf[i >> 1], x);
                                 else mma3(f, kf[i >> 1], s);
@@ -347,13 +231,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[r] = __builtin_amdgcn_exp2f(s[r] + sj);
-        x[r] = s[r] * fmaf(x[r], 0x1p-38f, -delta[r >> 2][r & 3]);
+        x[r] = s[r] * fmaf(x[r], cd, -delta[r >> 2][r & 3]);
         mx = fmaxf(mx, fabsf(x[r]));
       }
       rescale(mx, tj, dk);
       const float ft = __builtin_amdgcn_ldexpf(1.f, tj);
       const Frag pf[2] = {split_rows(s, 0), split_rows(s, 1)}, df[2] = {split_rows(x, 0, ft), split_rows(x, 1, ft)};
-      steps<4 * T::DB, AHEAD>([&](int i) { return frag_col<DP>(i & 1 ? tq : tg, at, 2 * n + i / (2 * T::DB), (i >> 1) % T::DB); },
+      steps<4 * T::DB, AHEAD>([&](int i) { return frag_col<T>(i & 1 ? tq : tg, at, 2 * n + i / (2 * T::DB), (i >> 1) % T::DB); },
                               [&](int i, const Frag& f) {
                                 const int k = i / (2 * T::DB), d = (i >> 1) % T::DB;
                                 if (i & 1) mma3(f, df[k], dk[d]);
@@ -368,16 +252,16 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
 #pragma unroll
     for (int r = 0; r < 16; ++r) mark = fmaf(0.f, dk[d][r], fmaf(0.f, dv[d][r], mark));
   if (__any(odd || mark != 0.f)) {  // (mark is 0 or NaN)
-    plain();
+    job.plain(a, kw, true, true);
     return;
   }
   if (j >= a.keys) return;
-  const float* old_k = a.acc_k && !far ? a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim : nullptr;
-  const float* old_v = a.acc_v && !far ? a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim : nullptr;
-  float* out_k = far ? part + (j - k0) * a.dim : a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim;
-  float* out_v = far ? part + (KB + j - k0) * a.dim : a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim;
+  const float* old_k = a.acc_k && !job.part ? a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim : nullptr;
+  const float* old_v = a.acc_v && !job.part ? a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim : nullptr;
+  float* out_k = job.part ? job.part + (j - k0) * a.dim : a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim;
+  float* out_v = job.part ? job.part + (KB + j - k0) * a.dim : a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim;
   const int sh_v = live ? -(int)sj + ex0 - kTop : 0;
-  const int sh_k = live ? -(int)sj - tj + ex0 + ev - kUnit + eq - kTop : 0;
+  const int sh_k = live ? -(int)sj - tj + ex0 - kUnit + eq - kTop : 0;
 #pragma unroll
   for (int d = 0; d < T::DB; ++d)
 #pragma unroll
@@ -396,12 +280,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void kv_kernel(Args a, B
 
 // dq of 32 rows to a wave; rows to lanes, as in the forward.
 template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, BwdWork wk, Grid g) {
-  using T = Tile<DP>;
+__device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<DP, NW>& m) {
+  using T = Tile<DP, 64>;
   constexpr int NT = 64 * NW, R = T::R, AHEAD = 1;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][T::BYTES];  // [buffer][K, V]
-  __shared__ __attribute__((aligned(16))) Tops<NW> tops;
-  const Block blk = g.block(a, 32 * NW);
   const int b = blk.b, h = blk.h, e = h / a.group;
   const Seq seq(a, b);
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, half = lane >> 5;
@@ -422,65 +303,42 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
   }
   const float* K = a.k + (int64_t)b * a.keys * a.ldk + (int64_t)e * a.dim;
   const float* V = a.v + (int64_t)b * a.keys * a.ldv + (int64_t)e * a.dim;
-  const Places<DP> at(lane);
+  const Places<T> at(lane);
 
-  Share<DP, NT> rk, rv;
+  Share<T, NT> in;
   // Tiles past the last are the last once more, which nobody reads: no branches around loads.
   auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
-  auto fetch = [&](int t) {
-    rk.load(K, a.ldk, row_of(t), seq.len, a.dim);
-    rv.load(V, a.ldv, row_of(t), seq.len, a.dim);
-  };
+  auto fetch = [&](int t) { in.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim); };
   auto tell = [&](int t) {
-    rk.clear(row_of(t), seq.len, a.dim);
-    rv.clear(row_of(t), seq.len, a.dim);
-    tops.add(0, t, rk.top());
-    tops.add(1, t, rv.top());
+    in.clear(row_of(t), seq.len, a.dim);
+    m.tops.add(0, t, in.top(false));
+    m.tops.add(1, t, in.top(true));
   };
   fetch(0);
   Frag q[T::KS], go[T::KS];
-  int eq, eg;
   bool odd = false;
-  {
-    const float* Q = a.q + ((int64_t)b * a.rows + (live ? i : 0)) * a.ldq + (int64_t)h * a.dim;
-    float x[T::KS][8], m = 0.f;
+  auto own = [&](const float* p, Frag (&f)[T::KS]) {  // a row at a power of two of its own
+    float x[T::KS][8];
+    float top = load_row<T::KS>(p, half, a.dim, live, x);
+    top = fmaxf(top, other_half(top));
+    odd |= !(top < INFINITY);
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-      load8(Q, 2 * s + half, a.dim, live, x[s]);
-      m = fmaxf(m, top8(x[s]));
-    }
-    m = fmaxf(m, other_half(m));
-    odd |= !(m < INFINITY);
-    const int ex = exponent(m);
-#pragma unroll
-    for (int s = 0; s < T::KS; ++s) q[s] = split8(x[s], scale(ex));
-    eq = ex;
-  }
-  {
-    const float* G = a.dout + ((int64_t)b * a.rows + (live ? i : 0)) * a.lddo + (int64_t)h * a.dim;
-    float x[T::KS][8], m = 0.f;
-#pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-      load8(G, 2 * s + half, a.dim, live, x[s]);
-      m = fmaxf(m, top8(x[s]));
-    }
-    m = fmaxf(m, other_half(m));
-    odd |= !(m < INFINITY);
-    eg = exponent(m);
-#pragma unroll
-    for (int s = 0; s < T::KS; ++s) go[s] = split8(x[s], scale(eg));
-  }
+    for (int s = 0; s < T::KS; ++s) f[s] = split8(x[s], scale(exponent(top)));
+    return exponent(top);
+  };
+  const int64_t row = (int64_t)b * a.rows + (live ? i : 0);
+  const int eq = own(a.q + row * a.ldq + (int64_t)h * a.dim, q), eg = own(a.dout + row * a.lddo + (int64_t)h * a.dim, go);
   const int64_t st = ((int64_t)b * a.heads + h) * a.rows + (live ? i : 0);
   const float delta = live ? a.delta[st] : 0.f, lse = live ? a.lse_in[st] * kLog2e : 0.f;
   odd |= !(fabsf(delta) < INFINITY) || !(fabsf(lse) < INFINITY);
   int ek = kNone, ek_next = kNone, ev = 0;
   auto put = [&](int t) {
-    const float mk = tops.get(0, t), mv = tops.get(1, t);
+    const float mk = m.tops.get(0, t), mv = m.tops.get(1, t);
     odd |= !(fmaxf(mk, mv) < INFINITY);
     ek_next = max(ek_next, exponent(mk));
     ev = exponent(mv);
-    rk.put(lds[t & 1][0], ek_next);
-    rv.put(lds[t & 1][1], ev);
+    const float sk = scale(ek_next), sv = scale(ev);
+    in.put(m.lds[t & 1][0], m.lds[t & 1][1], [=](bool v, int) { return v ? sv : sk; });
   };
   tell(0);
   __syncthreads();
@@ -499,7 +357,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
     const int ekt = ek_next, evt = ev;
     put(t + 1);
     fetch(t + 2);
-    const char *tk = lds[t & 1][0], *tv = lds[t & 1][1];
+    const char *tk = m.lds[t & 1][0], *tv = m.lds[t & 1][1];
     const int j0 = tiles.row(t);
     if (ekt != ek) {  // K's operand has a larger power of two from here on
 #pragma unroll
@@ -517,7 +375,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
       f32x16 s, x;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = x[r] = 0.f;
-      steps<2 * T::KS, AHEAD>([&](int i) { return frag_row<DP>(i & 1 ? tv : tk, at, n, i >> 1); },
+      steps<2 * T::KS, AHEAD>([&](int i) { return frag_row<T>(i & 1 ? tv : tk, at, n, i >> 1); },
                               [&](int i, const Frag& f) {
                                 if (i & 1) mma3(f, go[i >> 1], x);
                                 else mma3(f, q[i >> 1], s);
@@ -537,7 +395,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
       rescale(mx, ti, dq);
       const float ft = __builtin_amdgcn_ldexpf(1.f, ti);
       const Frag df[2] = {split_rows(x, 0, ft), split_rows(x, 1, ft)};
-      steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<DP>(tk, at, 2 * n + i / T::DB, i % T::DB); },
+      steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<T>(tk, at, 2 * n + i / T::DB, i % T::DB); },
                               [&](int i, const Frag& f) { mma3(f, df[i / T::DB], dq[i % T::DB]); });
     }
     tell(t + 2);
@@ -566,32 +424,45 @@ __global__ __launch_bounds__(64 * NW, DP <= 64 ? 2 : 1) void q_kernel(Args a, Bw
     }
 }
 
-// Adds the far sums of the sinks, chunk by chunk: a thread to a value.
-__global__ __launch_bounds__(256) void join_kernel(Args a, BwdWork wk, int64_t first) {
-  const int64_t id = (first + blockIdx.x) * 256 + threadIdx.x;
-  const int64_t n = (int64_t)a.sinks * a.dim, group = id / n;  // of a head
-  if (group >= (int64_t)a.batch * a.kv_heads) return;
-  const int at = (int)(id - group * n), j = at / a.dim, d = at - j * a.dim, blk = j / kKeyBlock;
-  const int b = (int)(group / a.kv_heads), e = (int)(group % a.kv_heads);
-  const Seq seq(a, b);
-  const int begin = wk.near_end(a, blk * kKeyBlock, kKeyBlock);
-  if (j >= seq.len || begin >= seq.len) return;
-  float sk = 0.f, sv = 0.f;
-  const float* p = wk.part + ((group * wk.sink_blocks + blk) * wk.fars) * 2 * kKeyBlock * a.dim + (j - blk * kKeyBlock) * a.dim + d;
-  for (int i = begin; i < seq.len; i += wk.far_rows, p += 2 * kKeyBlock * a.dim) {
-    sk += p[0];
-    sv += p[kKeyBlock * a.dim];
-  }
-  a.dk[((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim + d] += sk;
-  a.dv[((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim + d] += sv;
+// Both passes in one launch, the longer kv pass first: the one fills in behind the other.
+template <int DP, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void narrow_kernel(Args a, BwdWork wk, Grid kv, Grid q, int64_t first) {
+  __shared__ Shared<DP, NW> m;
+  const int64_t id = first + blockIdx.x;
+  if (id < kv.total)
+    kv_rows<DP, NW>(a, wk, kv.place(id), m);
+  else
+    q_rows<DP, NW>(a, q.block(a, 32 * NW, id - kv.total), m);
 }
 
-constexpr int kWaves = kKeyBlock / 32;  // of a workgroup
-
-template <int DP>
-void launch_dim(const Args& a, const BwdWork& wk, hipStream_t s) {
-  launch_blocks(kv_kernel<DP, kWaves>, Grid(a, a.kv_heads, wk.key_blocks + wk.sink_blocks * wk.fars), 64 * kWaves, s, a, wk);
-  launch_blocks(q_kernel<DP, kWaves>, Grid(a, a.heads, (a.rows + 32 * kWaves - 1) / (32 * kWaves)), 64 * kWaves, s, a, wk);
+// Adds the parts of a key's sums, in order, and to its gradients: a thread to a value.
+__global__ __launch_bounds__(256) void join_kernel(Args a, BwdWork wk, int keys, int64_t first) {
+  const int64_t id = (first + blockIdx.x) * 256 + threadIdx.x;
+  const int64_t n = (int64_t)keys * a.dim, group = id / n;  // of a head
+  if (group >= (int64_t)a.batch * a.kv_heads) return;
+  const int at = (int)(id - group * n), j = at / a.dim, d = at - j * a.dim, blk = j / kKeyBlock, k0 = blk * kKeyBlock;
+  const int b = (int)(group / a.kv_heads), e = (int)(group % a.kv_heads);
+  const int len = Seq(a, b).len, size = 2 * kKeyBlock * a.dim, place = (j - k0) * a.dim + d, begin = wk.near_end(a, k0);
+  float sk = 0.f, sv = 0.f;
+  if (wk.nears > 1 && j < len) {
+    const float* p = wk.near + (group * wk.key_blocks + blk) * wk.nears * size + place;
+    for (int i = k0; i < min(begin, len); i += wk.near_rows, p += size) {
+      sk += p[0];
+      sv += p[kKeyBlock * a.dim];
+    }
+  }
+  if (j < a.sinks && j < len) {
+    const float* p = wk.far + (group * wk.sink_blocks + blk) * wk.fars * size + place;
+    for (int i = begin; i < len; i += wk.far_rows, p += size) {
+      sk += p[0];
+      sv += p[kKeyBlock * a.dim];
+    }
+  }
+  // (with one near part a sink's gradients hold that part already)
+  float* dk = a.dk + ((int64_t)b * a.keys + j) * a.lddk + (int64_t)e * a.dim + d;
+  float* dv = a.dv + ((int64_t)b * a.keys + j) * a.lddv + (int64_t)e * a.dim + d;
+  *dk = (wk.nears == 1 || a.acc_k ? *dk : 0.f) + sk;
+  *dv = (wk.nears == 1 || a.acc_v ? *dv : 0.f) + sv;
 }
 
 }  // namespace
@@ -601,13 +472,17 @@ void tile_backward(const Args& a, const BwdWork& wk, hipStream_t s) {
   constexpr int64_t kBlocks = 1 << 23;
   for (int64_t f = 0; f < tiles; f += kBlocks)
     mle::launch(prepare_kernel, (unsigned)std::min(tiles - f, kBlocks), 256, 0, s, a, wk, f);
-  if (a.dim <= 64) launch_dim<64>(a, wk, s);
-  else if (a.dim <= 96) launch_dim<96>(a, wk, s);
-  else launch_dim<128>(a, wk, s);
-  if (wk.fars == 0) return;
-  const int64_t joins = ((int64_t)a.batch * a.kv_heads * a.sinks * a.dim + 255) / 256;
+  if (a.dim <= 64) {
+    constexpr int NW = kKeyBlock / 32;
+    launch_both(narrow_kernel<64, NW>, Grid(a, a.kv_heads, wk.kv_items()), Grid(a, a.heads, (a.rows + 32 * NW - 1) / (32 * NW)),
+                64 * NW, s, a, wk);
+  } else {
+    launch_wide(a, wk, s);
+  }
+  const int keys = wk.nears > 1 ? a.keys : wk.fars > 0 ? std::min(a.sinks, a.keys) : 0;
+  const int64_t joins = ((int64_t)a.batch * a.kv_heads * keys * a.dim + 255) / 256;
   for (int64_t f = 0; f < joins; f += kBlocks)
-    mle::launch(join_kernel, (unsigned)std::min(joins - f, kBlocks), 256, 0, s, a, wk, f);
+    mle::launch(join_kernel, (unsigned)std::min(joins - f, kBlocks), 256, 0, s, a, wk, keys, f);
 }
 
 }  // namespace wattn

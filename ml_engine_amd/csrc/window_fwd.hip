@@ -18,7 +18,7 @@ constexpr float kHead = 8.f;
 
 template <int DP, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
-  using T = Tile<DP>;
+  using T = Tile<DP, DP <= 64 ? 64 : 32>;  // as many products to a tile of wide heads, half the registers to LDS
   constexpr int NT = 64 * NW, R = T::R, AHEAD = 2;
   __shared__ __attribute__((aligned(16))) char lds[2][2][T::BYTES];  // [buffer][K, V]
   __shared__ __attribute__((aligned(16))) Tops<NW> tops;
@@ -42,20 +42,18 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
   }
   const float* K = a.k + (int64_t)b * a.keys * a.ldk + (int64_t)e * a.dim;
   const float* V = a.v + (int64_t)b * a.keys * a.ldv + (int64_t)e * a.dim;
-  const Places<DP> at(lane);
+  const Places<T> at(lane);
 
-  Share<DP, NT> rk, rv;
+  Share<T, NT> kv;
   // Tiles past the last are the last once more, which nobody reads: no branches around loads.
   auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
   auto fetch = [&](int t) {
-    rk.load(K, a.ldk, row_of(t), seq.len, a.dim);
-    rv.load(V, a.ldv, row_of(t), seq.len, a.dim);
+    kv.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim);
   };
   auto tell = [&](int t) {
-    rk.clear(row_of(t), seq.len, a.dim);
-    rv.clear(row_of(t), seq.len, a.dim);
-    tops.add(0, t, rk.top());
-    tops.add(1, t, rv.top());
+    kv.clear(row_of(t), seq.len, a.dim);
+    tops.add(0, t, kv.top(false));
+    tops.add(1, t, kv.top(true));
   };
   fetch(0);
   // this lane's row of Q, at a power of two of its own
@@ -84,8 +82,8 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
     odd |= !(fmaxf(mk, mv) < INFINITY);
     ek = exponent(mk);
     ev_next = max(ev_next, exponent(mv));
-    rk.put(lds[t & 1][0], ek);
-    rv.put(lds[t & 1][1], ev_next);
+    const float sk = scale(ek), sv = scale(ev_next);
+    kv.put(lds[t & 1][0], lds[t & 1][1], [=](bool v, int) { return v ? sv : sk; });
   };
   tell(0);
   __syncthreads();
@@ -109,7 +107,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
     for (int n = 0; n < T::NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-    steps<T::KS * T::NB, AHEAD>([&](int i) { return frag_row<DP>(tk, at, i % T::NB, i / T::NB); },
+    steps<T::KS * T::NB, AHEAD>([&](int i) { return frag_row<T>(tk, at, i % T::NB, i / T::NB); },
                                 [&](int i, const Frag& f) { mma3(f, q[i / T::NB], s[i % T::NB]); });
     const bool all = j0 + R - 1 <= wfirst && (wlast - j0 < a.window || j0 + R - 1 < a.sinks) && row0 + 32 <= a.rows &&
                      seq.first + row0 >= 0 && seq.first + row0 + 32 <= seq.len;
@@ -159,7 +157,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
       ev = e;
     }
     const char* tv = lds[t & 1][1];
-    steps<2 * T::NB * T::DB, AHEAD>([&](int i) { return frag_col<DP>(tv, at, i / T::DB, i % T::DB); },
+    steps<2 * T::NB * T::DB, AHEAD>([&](int i) { return frag_col<T>(tv, at, i / T::DB, i % T::DB); },
                                     [&](int i, const Frag& f) { mma3(f, pf[i / T::DB], o[i % T::DB]); });
   };
   put(0);

@@ -13,23 +13,32 @@ constexpr int kKeyBlock = 128;  // keys of a workgroup of the backward
 struct BwdWork {
   int* ex;        // exponent of each row of dout, [batch, heads, rows]
   int* tile_ex;   // the largest of 64 rows, [batch, heads, tiles]
-  float* part;    // far sums of the sinks, [batch, kv_heads, sink_blocks, fars, dk and dv, kKeyBlock, dim]
+  float* near;    // parts of the keys' sums, [batch, kv_heads, key_blocks, nears, dk and dv, kKeyBlock, dim]
+  float* far;     // far sums of the sinks, [batch, kv_heads, sink_blocks, fars, dk and dv, kKeyBlock, dim]
   int tiles, key_blocks, sink_blocks;
-  int fars, far_rows;  // chunks of rows past a block's window, and their rows
+  int nears, near_rows;  // chunks of rows of a block's own and window, and their rows
+  int fars, far_rows;    // chunks of rows past that
   // Rows from here on see a block's sinks alone.
-  __host__ __device__ int near_end(const Args& a, int k0, int kb) const {
-    const int64_t n = ((int64_t)k0 + kb + a.window + 62) / 64 * 64;
+  __host__ __device__ int near_end(const Args& a, int k0) const {
+    const int64_t n = ((int64_t)k0 + kKeyBlock + a.window + 62) / 64 * 64;
     return (int)(n < tiles * 64ll ? n : tiles * 64ll);
   }
-  explicit BwdWork(const Args& a) : ex(nullptr), tile_ex(nullptr), part(nullptr) {
+  explicit BwdWork(const Args& a) : ex(nullptr), tile_ex(nullptr), near(nullptr), far(nullptr) {
     tiles = (a.rows + 63) / 64;
     key_blocks = (a.keys + kKeyBlock - 1) / kKeyBlock;
-    sink_blocks = (a.sinks + kKeyBlock - 1) / kKeyBlock;
+    sink_blocks = (std::min(a.sinks, a.keys) + kKeyBlock - 1) / kKeyBlock;
+    // Too few blocks of keys for the chip's 256 CUs: their rows in parts.
+    const int64_t blocks = (int64_t)a.batch * a.kv_heads * key_blocks;
+    const int rows = near_end(a, 0);
+    near_rows = rows;
+    if (blocks > 0 && blocks < 256) near_rows = (int)std::max<int64_t>(64, (rows * blocks / 256 + 63) / 64 * 64);
+    nears = rows > 0 ? (rows + near_rows - 1) / near_rows : 1;
     // short, so that they fill in behind the blocks of keys
     far_rows = std::max(256, (a.window / 4 + 63) / 64 * 64);
-    const int after = a.rows - near_end(a, 0, kKeyBlock);
+    const int after = a.rows - rows;
     fars = sink_blocks > 0 && after > 0 ? (after + far_rows - 1) / far_rows : 0;
   }
+  int kv_items() const { return key_blocks * nears + sink_blocks * fars; }  // workgroups of the kv pass to a head
   // Lays it out from `ws` (which may be null) after D; the bytes of all of it.
   size_t place(Args& a, void* ws) {
     char* p = static_cast<char*>(ws);
@@ -43,8 +52,9 @@ struct BwdWork {
     a.delta = reinterpret_cast<float*>(take(rows * sizeof(float)));
     ex = reinterpret_cast<int*>(take(rows * sizeof(int)));
     tile_ex = reinterpret_cast<int*>(take((size_t)a.batch * a.heads * tiles * sizeof(int)));
-    part = reinterpret_cast<float*>(
-        take((size_t)a.batch * a.kv_heads * sink_blocks * fars * 2 * kKeyBlock * a.dim * sizeof(float)));
+    const size_t part = (size_t)a.batch * a.kv_heads * 2 * kKeyBlock * a.dim * sizeof(float);
+    if (nears > 1) near = reinterpret_cast<float*>(take(part * key_blocks * nears));
+    far = reinterpret_cast<float*>(take(part * sink_blocks * fars));
     return n;
   }
 };
@@ -99,8 +109,7 @@ struct Grid {
     total = (int64_t)groups * per_group;
     xcd = groups % 8 == 0;
   }
-  __device__ __forceinline__ Place place() const {
-    const int64_t id = first + blockIdx.x;
+  __device__ __forceinline__ Place place(int64_t id) const {
     Place p;
     if (xcd) {
       const int64_t k = id >> 3;
@@ -112,8 +121,9 @@ struct Grid {
     }
     return p;
   }
-  __device__ __forceinline__ Block block(const Args& a, int rows) const {
-    const Place p = place();
+  __device__ __forceinline__ Block block(const Args& a, int rows) const { return block(a, rows, first + blockIdx.x); }
+  __device__ __forceinline__ Block block(const Args& a, int rows, int64_t id) const {
+    const Place p = place(id);
     Block r;
     r.b = (int)(p.group / a.kv_heads);
     r.h = (int)(p.group % a.kv_heads) * per_head + p.item % per_head;
@@ -128,6 +138,15 @@ void launch_blocks(K kernel, Grid g, int threads, hipStream_t s, const Args& a, 
   constexpr int64_t kBlocks = 1 << 22;
   for (; g.first < g.total; g.first += kBlocks)
     mle::launch(kernel, (unsigned)std::min<int64_t>(g.total - g.first, kBlocks), threads, 0, s, a, more..., g);
+}
+
+// The same for two grids one after the other.
+template <class K>
+void launch_both(K kernel, const Grid& g0, const Grid& g1, int threads, hipStream_t s, const Args& a, const BwdWork& wk) {
+  constexpr int64_t kBlocks = 1 << 22;
+  const int64_t total = g0.total + g1.total;
+  for (int64_t f = 0; f < total; f += kBlocks)
+    mle::launch(kernel, (unsigned)std::min(total - f, kBlocks), threads, 0, s, a, wk, g0, g1, f);
 }
 
 }  // namespace wattn

@@ -37,11 +37,10 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kTop = 14;    // exponent of a tile's largest value
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// DP: columns, the head's dimension rounded up to 64, 96 or 128.  Fewer rows of wide heads:
-// as many products to a tile, half the registers on the way to LDS.
-template <int DP>
+// DP: columns, the head's dimension rounded up to 64, 96 or 128; R rows.
+template <int DP_, int R_>
 struct Tile {
-  static constexpr int R = DP <= 64 ? 64 : 32, NB = R / 32;  // rows, blocks of 32
+  static constexpr int DP = DP_, R = R_, NB = R / 32;  // blocks of 32 rows
   static constexpr int UNITS = DP / 8, PITCH = DP <= 64 ? 128 : 256, PLANE = R * PITCH, BYTES = 2 * PLANE;
   static constexpr int KS = DP / 16, DB = DP / 32;  // steps over the columns; blocks of 32 columns
 };
@@ -108,23 +107,23 @@ __device__ __forceinline__ Frag split_rows(const f32x16& x, int s, float scale) 
 
 // A lane's places in a tile: of frag_row's first step and of frag_col's first columns.  Later
 // ones differ in bits that the swizzle only flips.
-template <int DP>
+template <class T>
 struct Places {
   int row, col;
   __device__ __forceinline__ Places(int lane) {
     const int c = lane & 31, h = lane >> 5, i = lane & 15, g = (lane >> 4) & 1, r = 4 * h + (i >> 2);
-    row = c * Tile<DP>::PITCH + ((h ^ swizzle<DP>(c)) << 4);  // row c, columns 16 s + 8 h ..
-    col = r * Tile<DP>::PITCH + (((2 * g + ((i & 3) >> 1)) ^ swizzle<DP>(r)) << 4) + 8 * (i & 1);
+    row = c * T::PITCH + ((h ^ swizzle<T::DP>(c)) << 4);  // row c, columns 16 s + 8 h ..
+    col = r * T::PITCH + (((2 * g + ((i & 3) >> 1)) ^ swizzle<T::DP>(r)) << 4) + 8 * (i & 1);
   }
 };
 
 // Row 32 b + lane % 32, columns of step s.
-template <int DP>
-__device__ __forceinline__ Frag frag_row(const char* t, const Places<DP>& p, int b, int s) {
-  const char* at = t + (p.row ^ (s << 5)) + 32 * b * Tile<DP>::PITCH;
+template <class T>
+__device__ __forceinline__ Frag frag_row(const char* t, const Places<T>& p, int b, int s) {
+  const char* at = t + (p.row ^ (s << 5)) + 32 * b * T::PITCH;
   Frag f;
   f.hi = *reinterpret_cast<const f16x8*>(at);
-  f.lo = *reinterpret_cast<const f16x8*>(at + Tile<DP>::PLANE);
+  f.lo = *reinterpret_cast<const f16x8*>(at + T::PLANE);
   return f;
 }
 
@@ -133,15 +132,15 @@ __device__ __forceinline__ s16x4 read_tr(const char* p) {
 }
 
 // Columns 32 d + lane % 32, the 16 rows of step s in the accumulators' order.
-template <int DP>
-__device__ __forceinline__ Frag frag_col(const char* t, const Places<DP>& p, int s, int d) {
+template <class T>
+__device__ __forceinline__ Frag frag_col(const char* t, const Places<T>& p, int s, int d) {
   const int c = p.col ^ (d << 6);
-  const char* a = t + c + 16 * s * Tile<DP>::PITCH;
-  const char* b = t + (c ^ 16) + (16 * s + 8) * Tile<DP>::PITCH;  // 8 rows on: the swizzle's last bit
+  const char* a = t + c + 16 * s * T::PITCH;
+  const char* b = t + (c ^ 16) + (16 * s + 8) * T::PITCH;  // 8 rows on: the swizzle's last bit
   Frag f;
   const f16x4 h0 = __builtin_bit_cast(f16x4, read_tr(a)), h1 = __builtin_bit_cast(f16x4, read_tr(b));
-  const f16x4 l0 = __builtin_bit_cast(f16x4, read_tr(a + Tile<DP>::PLANE)),
-              l1 = __builtin_bit_cast(f16x4, read_tr(b + Tile<DP>::PLANE));
+  const f16x4 l0 = __builtin_bit_cast(f16x4, read_tr(a + T::PLANE)),
+              l1 = __builtin_bit_cast(f16x4, read_tr(b + T::PLANE));
   f.hi = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
   f.lo = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
   return f;
@@ -201,30 +200,38 @@ __device__ __forceinline__ int exponent(float m) {
 // The power of two that brings values of this exponent to [2^kTop, 2^(kTop + 1)).
 __device__ __forceinline__ float scale(int e) { return __builtin_bit_cast(float, (unsigned)(kTop - e + 127) << 23); }
 
-// A thread's share of a tile of NT threads: N chunks of eight columns.
-template <int DP, int NT>
+// A thread's share of two tensors' tiles among NT threads: N chunks of eight columns, the
+// first tensor's tile and then the second's.  A wave's chunk is of one tensor.
+template <class T, int NT>
 struct Share {
-  static constexpr int ALL = Tile<DP>::R * Tile<DP>::UNITS, N = (ALL + NT - 1) / NT;
+  static constexpr int ALL = T::R * T::UNITS, N = (2 * ALL + NT - 1) / NT;
+  static_assert(ALL % 64 == 0 && NT % 64 == 0, "whole waves");
   float x[N][8];
-  static constexpr bool whole = ALL % NT == 0;
   // (a chunk past the last is the last, read again and not put)
   static __device__ __forceinline__ int unit(int c) {
     const int id = c * NT + (int)threadIdx.x;
-    return whole ? id : min(id, ALL - 1);
+    return (2 * ALL) % NT == 0 ? id : min(id, 2 * ALL - 1);
   }
-  static __device__ __forceinline__ bool has(int c) {
-    return whole || c * NT + (int)threadIdx.x < ALL;
+  static __device__ __forceinline__ bool has(int c) { return (2 * ALL) % NT == 0 || c * NT + (int)threadIdx.x < 2 * ALL; }
+  // Of the second tensor?  (the same for all of a wave)
+  static __device__ __forceinline__ bool second(int c) {
+    if ((c + 1) * NT <= ALL) return false;
+    if (c * NT >= ALL) return true;
+    return c * NT + __builtin_amdgcn_readfirstlane((int)threadIdx.x) >= ALL;
   }
-  // Rows r0 .. r0 + R - 1 (r0 < end) of a tensor from `base`, dim >= 4.  What is not there is read
-  // at a place that is, and put right by clear() once it has come: two ways of loading would
-  // meet in a copy of the registers, which waits for the loads.
-  __device__ __forceinline__ void load(const float* __restrict__ base, int64_t ld, int r0, int end, int dim) {
+  static __device__ __forceinline__ int row(int c) { return (unit(c) - (second(c) ? ALL : 0)) / T::UNITS; }
+  static __device__ __forceinline__ int col(int c) { return 8 * ((unit(c) - (second(c) ? ALL : 0)) % T::UNITS); }
+  // Rows r0 .. r0 + R - 1 (r0 < end) of both, dim >= 4.  What is not there is read at a place that
+  // is, and put right by clear() once it has come: two ways of loading would meet in a copy of
+  // the registers, which waits for the loads.
+  __device__ __forceinline__ void load(const float* __restrict__ base0, int64_t ld0, const float* __restrict__ base1,
+                                       int64_t ld1, int r0, int end, int dim) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int id = unit(c), row = id / Tile<DP>::UNITS, u = id % Tile<DP>::UNITS;
-      const float* p = base + (int64_t)min(r0 + row, end - 1) * ld;
-      const f32x4u v0 = *reinterpret_cast<const f32x4u*>(p + min(8 * u, dim - 4)),
-                   v1 = *reinterpret_cast<const f32x4u*>(p + min(8 * u + 4, dim - 4));
+      const bool s = second(c);
+      const float* p = (s ? base1 : base0) + (int64_t)min(r0 + row(c), end - 1) * (s ? ld1 : ld0);
+      const f32x4u v0 = *reinterpret_cast<const f32x4u*>(p + min(col(c), dim - 4)),
+                   v1 = *reinterpret_cast<const f32x4u*>(p + min(col(c) + 4, dim - 4));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[c][j] = v0[j];
@@ -235,14 +242,13 @@ struct Share {
   // Zeros from row `end` and column `dim` on; four values that reach past dim have been read as the
   // last four.
   __device__ __forceinline__ void clear(int r0, int end, int dim) {
-    if (r0 + Tile<DP>::R <= end && dim == DP) return;
+    if (r0 + T::R <= end && dim == T::DP) return;
     const int cut = dim & 3;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int id = unit(c), row = id / Tile<DP>::UNITS, u = id % Tile<DP>::UNITS;
 #pragma unroll
       for (int k = 0; k < 8; k += 4) {
-        const int n = r0 + row < end ? dim - 8 * u - k : 0;
+        const int n = r0 + row(c) < end ? dim - col(c) - k : 0;
         const float v[4] = {x[c][k], x[c][k + 1], x[c][k + 2], x[c][k + 3]};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -252,30 +258,25 @@ struct Share {
       }
     }
   }
-  __device__ __forceinline__ float top() const {
+  // The largest magnitude of the first (second) tensor's chunks.
+  __device__ __forceinline__ float top(bool of_second) const {
     float m = 0.f;
 #pragma unroll
-    for (int c = 0; c < N; ++c) m = fmaxf(m, top8(x[c]));
+    for (int c = 0; c < N; ++c) m = fmaxf(m, second(c) == of_second ? top8(x[c]) : 0.f);
     return m;
   }
-  // Split at the scale of exponent e into a tile; put_rows: of each row's.
-  __device__ __forceinline__ void put(char* t, int e) const {
-    const float s = scale(e);
-    put_with(t, [=](int) { return s; });
-  }
-  __device__ __forceinline__ void put_rows(char* t, const int* ex) const {
-    put_with(t, [=](int row) { return scale(ex[row]); });
-  }
+  // Split into the two tiles, at the scales that scale_of(second tensor?, row) gives.
   template <class F>
-  __device__ __forceinline__ void put_with(char* t, F scale_of) const {
+  __device__ __forceinline__ void put(char* t0, char* t1, F scale_of) const {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int id = unit(c), row = id / Tile<DP>::UNITS, u = id % Tile<DP>::UNITS;
       if (!has(c)) break;
-      const Frag f = split8(x[c], scale_of(row));
-      char* at = t + row * Tile<DP>::PITCH + ((u ^ swizzle<DP>(row)) << 4);
+      const bool s = second(c);
+      const int r = row(c), u = col(c) / 8;
+      const Frag f = split8(x[c], scale_of(s, r));
+      char* at = (s ? t1 : t0) + r * T::PITCH + ((u ^ swizzle<T::DP>(r)) << 4);
       *reinterpret_cast<f16x8*>(at) = f.hi;
-      *reinterpret_cast<f16x8*>(at + Tile<DP>::PLANE) = f.lo;
+      *reinterpret_cast<f16x8*>(at + T::PLANE) = f.lo;
     }
   }
 };
