@@ -27,11 +27,13 @@ struct BwdWork {
     tiles = (a.rows + 63) / 64;
     key_blocks = (a.keys + kKeyBlock - 1) / kKeyBlock;
     sink_blocks = (std::min(a.sinks, a.keys) + kKeyBlock - 1) / kKeyBlock;
-    // Too few blocks of keys for the chip's 256 CUs: their rows in parts.
+    // Too few blocks of keys for half of the chip's 256 CUs: their rows in parts, the dq pass
+    // taking the other half (4 heads of 2048 x 64, window 512, us: whole 82, in parts for 128
+    // CUs 61, for 256 68; 6 heads of 777 x 80: 128, 97, 101).
     const int64_t blocks = (int64_t)a.batch * a.kv_heads * key_blocks;
     const int rows = near_end(a, 0);
     near_rows = rows;
-    if (blocks > 0 && blocks < 256) near_rows = (int)std::max<int64_t>(64, (rows * blocks / 256 + 63) / 64 * 64);
+    if (blocks > 0 && blocks < 128) near_rows = (int)std::max<int64_t>(64, (rows * blocks / 128 + 63) / 64 * 64);
     nears = rows > 0 ? (rows + near_rows - 1) / near_rows : 1;
     // short, so that they fill in behind the blocks of keys
     far_rows = std::max(256, (a.window / 4 + 63) / 64 * 64);
