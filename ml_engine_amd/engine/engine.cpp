@@ -1125,6 +1125,117 @@ graph Linear::cross_entropy(const graph& X, const int32_t* keys, int clen, int m
 }
 
 // ---------------------------------------------------------------------------
+// AffineLayerNorm (see engine.h).
+AffineLayerNorm::AffineLayerNorm(const int features_, const str name, const float eps_)
+    : features(features_), eps(eps_), W1(name + " W1", 1, 1, 1, features_), B1(name + " B1", 1, 1, 1, features_) {
+  if (name != "") op_name = name;
+  check(mle_fill(mle::stream(), W1.output, 1.0f, W1.total), op_name + " weight");
+  check(mle_fill(mle::stream(), B1.output, 0.0f, B1.total), op_name + " bias");
+}
+void AffineLayerNorm::save(std::ofstream& f) const {
+  W1.save(f);
+  B1.save(f);
+}
+void AffineLayerNorm::load(std::ifstream& f) {
+  W1.load(f);
+  B1.load(f);
+}
+void AffineLayerNorm::operator=(const AffineLayerNorm& other) {
+  W1 = other.W1;
+  B1 = other.B1;
+}
+
+graph AffineLayerNorm::forward(const graph& X) {
+  const long long lines = (long long)X->dim[0] * X->dim[1] * X->dim[2];
+  if (X->dim[3] != features || lines > (1ll << 30)) {
+    std::cout << "Shape Mismatch in " << op_name << ": \n";
+    Dimension(X);
+    std::cout << "Expected rows of " << features << " \n";
+    std::exit(1);
+  }
+  auto node = std::make_shared<NodeBackProp>(op_name, X->dim[0], X->dim[1], X->dim[2], X->dim[3], 1);
+  node->lazy_grad_writer = true;
+  node->reads_grad_alias = true;
+  node->inputs = {X};
+  const int rows = (int)lines, cols = features;
+  const float e = eps;
+  AdamParameter *W = &W1, *Bb = &B1;
+  NodeBackProp *nd = node.get(), *x = X.get();
+  const str name = op_name;
+  node->params = {W, Bb};
+  float* mean = mle::alloc_output(rows);
+  float* rstd = mle::alloc_output(rows);
+  GraphOperations::GB += (double)(node->total + 2 * lines) * sizeof(float) / (1ULL << 30);
+  const size_t ws_bytes = mle_add_layernorm_ws_bytes(rows, cols);
+  void* ws = mle::gemm_workspace(ws_bytes);
+  node->forward = [=]() {
+    check(mle_add_layernorm_fwd(mle::stream(), rows, cols, x->output, nullptr, W->output, Bb->output, e, nullptr,
+                                nd->output, mean, rstd),
+          name + " forward");
+  };
+  if (mle::fusion_enabled() && X->forward_layernorm) {
+    auto sum = X->forward_layernorm;
+    auto alone = X->forward;
+    auto written = std::make_shared<bool>(false);  // y is of the sum's last forward
+    std::weak_ptr<NodeBackProp> here = node;
+    X->forward = [=]() {
+      auto n = here.lock();
+      if (!n || !n->output) return alone();  // this node is gone
+      sum(rows, cols, W->output, Bb->output, e, n->output, mean, rstd);
+      *written = true;
+    };
+    X->forward_layernorm = nullptr;  // one takeover per producer
+    X->forward_normstats = nullptr;
+    X->forward_act = nullptr;
+    X->forward_act_mse = nullptr;
+    auto by_itself = node->forward;
+    node->forward = [=]() {
+      if (!*written) by_itself();
+      *written = false;
+    };
+  }
+  node->backward = [=]() {
+    // The gradient that reaches x past this node, read where it lies (see can_alias_grad).
+    const float* past = x->grad_src;
+    int acc = 0;
+    if (past) {
+      x->grad_src = nullptr;
+      x->grad_pending_zero = false;
+    } else {
+      acc = mle::accumulate_flag(x);
+    }
+    check(mle_add_layernorm_bwd(mle::stream(), rows, cols, x->output, W->output, mean, rstd, mle::grad_of(nd), past,
+                                x->grad, acc, W->grad, Bb->grad, mle::params_write_flag({W, Bb}), ws, ws_bytes),
+          name + " backward");
+  };
+  node->free = [=]() {
+    nd->clear();
+    mle::release(mean, rows, false);
+    mle::release(rstd, rows, false);
+  };
+  node->serious_free = [=]() {};
+  node->zero_grad = [=]() {
+    mle::defer_zero(nd);
+    mle::defer_zero(W);
+    mle::defer_zero(Bb);
+  };
+  node->accumulate = [=](double* s) {
+    W->accumulate_grad(s);
+    Bb->accumulate_grad(s);
+  };
+  node->clipnorm = [=](const double* s) {
+    W->gradnorm(s);
+    Bb->gradnorm(s);
+  };
+  node->updateParams = [=](const float lr, const bool adamw) {
+    W->update(lr, adamw);
+    Bb->update(lr, adamw);
+  };
+  node->printparams = [=](const bool) {};
+  return node;
+}
+
+// ---------------------------------------------------------------------------
 // Sibling Linear fusion (see engine.h).
 namespace mle {
 

@@ -227,6 +227,10 @@ struct NodeBackProp {
   // activation: out = act(y) + cbias[channel], the activation's own output
   // not written (mle_norm_fwd_act_bias).
   std::function<void(int kind, float* out, const float* cbias)> forward_act_bias;
+  // Set by Add (additive): its forward with the layer norm of its rows after
+  // it (AffineLayerNorm), one pass.
+  std::function<void(int rows, int cols, const float* w, const float* b, float eps, float* y, float* mean, float* rstd)>
+      forward_layernorm;
   // Set by Add (additive): its forward with the activation after it and the
   // last MSE node on that activation's output, one pass
   // (mle_add_mse_act_fwd_bwd_read): the loss and its read-back and the early
@@ -406,6 +410,20 @@ class GraphOperations {
   // seq a multiple of 64.  Returns nullptr (building nothing) for other shapes.
   static graph HeadAttention(const graph& Q, const graph& K, const graph& V, const int heads, const float scale,
                              const bool causal);
+  // Attention along rows (SOFTMAX type 0 of the scaled scores, masked) over the keys that a
+  // causal sliding window and the first `sinks` positions leave visible, no scores stored
+  // (mle_window_attention_*; no counterpart in the reference): Q [batch, 1, seq, heads * dim],
+  // K and V [batch, 1, seq, kv_heads * dim], kv_heads dividing heads; nodes of their own each.
+  // window >= seq is plain causal attention.  lengths: device ids [batch] of the padded
+  // sequences' lengths, or nullptr.
+  static graph WindowAttention(const graph& Q, const graph& K, const graph& V, const int heads, const int kv_heads,
+                               const float scale, const int window, const int sinks = 0,
+                               const int32_t* lengths = nullptr);
+  // Rotary positions (mle_rotary; no counterpart in the reference) of X [batch, 1, seq, heads * dim]: the first
+  // sections[0] pairs of each head turn by axis 0's positions, the next by axis 1's, ..
+  // positions: device ids [sections.size()][batch * seq].  flags: mle_rotary_flags.
+  static graph Rotary(const graph& X, const int heads, const int32_t* positions, const std::vector<int>& sections,
+                      const double base = 10000.0, const int flags = 0);
   static graph SOFTMAX(const graph& X, const int type = 0);
   static graph SOFTMASK(const graph& X, const int type = 0);
   static graph RELU(const graph& input);
@@ -451,6 +469,28 @@ class Linear {
   void save(std::ofstream& f) const;
   void load(std::ifstream& f);
   void operator=(const Linear& other);
+};
+
+// Layer norm of each row (the last dimension) with a learned weight and bias
+// (mle_add_layernorm_*): y = (x - mean) / sqrt(var + eps) * W1 + B1.
+// GraphOperations::LayerNorm has neither, and one mean to a whole sample.
+// W1 [1, 1, 1, features] starts at 1, B1 at 0.  When X is an Add's output (and
+// the fusions are on) the sum and its norm are one pass, and the norm's
+// backward adds to the gradient that reaches the sum past it.
+class AffineLayerNorm {
+ private:
+  int features;
+  float eps;
+
+ public:
+  AdamParameter W1;
+  AdamParameter B1;
+  str op_name = "Affine Layer Norm";
+  AffineLayerNorm(const int features, const str name = "", const float eps = 1e-5f);
+  graph forward(const graph& X);
+  void save(std::ofstream& f) const;
+  void load(std::ifstream& f);
+  void operator=(const AffineLayerNorm& other);
 };
 
 // Horizontal fusion of Linear layers that read the same input (e.g. the Q, K

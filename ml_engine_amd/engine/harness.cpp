@@ -31,6 +31,8 @@ struct Model {
   // owned modules
   std::unique_ptr<Linear> l1, l2, ffn1, ffn2, lm;
   std::unique_ptr<MultiHeadAttention> mha;
+  std::unique_ptr<WindowSelfAttention> wattn;
+  std::unique_ptr<AffineLayerNorm> n1, n2, n3;
   std::unique_ptr<Embedding> emb;
   std::unique_ptr<ResidualBlock> rb;
   std::unique_ptr<Convolute2DT> up;
@@ -165,6 +167,38 @@ void build_c8(Model* m, const long long* d) {
   m->params = {&m->emb->E, &m->ffn1->W1, &m->ffn1->B1, &m->ffn2->W1, &m->ffn2->B1, &m->lm->W1, &m->lm->B1};
 }
 
+// A transformer block of a language model over padded sequences: scaled embedding, layer norms
+// with weights, windowed attention with rotary positions of `axes` axes, a feed-forward, the
+// vocabulary's cross entropy.
+// dims {B, S, D, heads, kv_heads, head_dim, F, V, window, sinks, axes}
+void build_c9(Model* m, const long long* d) {
+  const int B = (int)d[0], S = (int)d[1], D = (int)d[2], H = (int)d[3], G = (int)d[4], hd = (int)d[5], F = (int)d[6],
+            V = (int)d[7], axes = (int)d[10];
+  auto* ids = static_cast<int32_t*>(input_buffer(m, sizeof(int32_t) * B * S));
+  auto* tgt = static_cast<int32_t*>(input_buffer(m, sizeof(int32_t) * B * S));
+  auto* positions = static_cast<int32_t*>(input_buffer(m, sizeof(int32_t) * axes * B * S));
+  auto* lengths = static_cast<int32_t*>(input_buffer(m, sizeof(int32_t) * B));
+  std::vector<int> sections(axes);
+  for (int i = 0; i < axes; ++i) sections[i] = hd / 2 * (i + 1) / axes - hd / 2 * i / axes;
+  m->emb.reset(new Embedding(V, D, "Token Embedding"));
+  m->n1.reset(new AffineLayerNorm(D, "Norm 1"));
+  m->wattn.reset(new WindowSelfAttention(D, H, G, hd, (int)d[8], (int)d[9], "Block"));
+  m->n2.reset(new AffineLayerNorm(D, "Norm 2"));
+  m->ffn1.reset(new Linear(D, F, "FFN1"));
+  m->ffn2.reset(new Linear(F, D, "FFN2"));
+  m->n3.reset(new AffineLayerNorm(D, "Norm 3"));
+  m->lm.reset(new Linear(D, V, "Projection"));
+  auto x = m->emb->forward(ids, B, S, S, sqrtf((float)D));
+  m->lookup = x;
+  auto h = GraphOperations::Add(x, m->wattn->forward(m->n1->forward(x), positions, sections, lengths));
+  auto f = m->ffn2->forward(GraphOperations::GELU(m->ffn1->forward(m->n2->forward(h))));
+  m->root = m->lm->cross_entropy(m->n3->forward(GraphOperations::Add(h, f)), tgt, S, S);
+  auto& a = *m->wattn;
+  m->params = {&m->emb->E, &m->n1->W1, &m->n1->B1, &a.q.W1, &a.q.B1, &a.k.W1, &a.k.B1, &a.v.W1, &a.v.B1,
+               &a.o.W1, &a.o.B1, &m->n2->W1, &m->n2->B1, &m->ffn1->W1, &m->ffn1->B1, &m->ffn2->W1, &m->ffn2->B1,
+               &m->n3->W1, &m->n3->B1, &m->lm->W1, &m->lm->B1};
+}
+
 // C2: a flat set of parameters; each parameter is carried by a hook node (as
 // Linear's output node carries W1/B1) under one track() root.
 void build_c2(Model* m, const long long* d, int nd) {
@@ -230,6 +264,7 @@ void* mle_model_create(int kind, const long long* dims, int ndims) {
     case 6: build_c6(m, dims); break;
     case 7: build_c7(m, dims); break;
     case 8: build_c8(m, dims); break;
+    case 9: build_c9(m, dims); break;
     default:
       delete m;
       return nullptr;

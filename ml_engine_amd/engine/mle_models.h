@@ -24,7 +24,12 @@ enum { MLE_STEP_CLOBBER_SCALE = 16 };
  *                                                             inputs: x, target f32
  * kind 8: scaled embedding -> x + FFN(x) -> vocabulary cross entropy, in one node
  *         without logits (whole 1) or through them  dims {B, S, D, F, V, whole, max_clen}
- *                                                             inputs: ids i32, targets i32 [B][max_clen] */
+ *                                                             inputs: ids i32, targets i32 [B][max_clen]
+ * kind 9: scaled embedding -> transformer block (AffineLayerNorm, WindowSelfAttention, FFN) ->
+ *         AffineLayerNorm -> vocabulary cross entropy
+ *         dims {B, S, D, heads, kv_heads, head_dim, F, V, window, sinks, axes}
+ *                                                             inputs: ids, targets i32 [B][S],
+ *                                                             positions i32 [axes][B][S], lengths i32 [B] */
 void* mle_model_create(int kind, const long long* dims, int ndims);
 void mle_model_destroy(void* h);
 /* Reference bugs reproduced (1, default) or fixed (0); see mle::Quirks. */

@@ -56,6 +56,48 @@ graph MultiHeadAttention::forward(const graph& X, const bool mask) {
   return output;
 }
 
+WindowSelfAttention::WindowSelfAttention(const int embed_dim_, const int num_heads_, const int kv_heads_,
+                                         const int head_dim_, const int window_, const int sinks_, const str& name_)
+    : embed_dim(embed_dim_),
+      num_heads(num_heads_),
+      kv_heads(kv_heads_),
+      head_dim(head_dim_),
+      window(window_),
+      sinks(sinks_),
+      name(name_),
+      q(embed_dim_, num_heads_ * head_dim_, name_ + " Query"),
+      k(embed_dim_, kv_heads_ * head_dim_, name_ + " Key"),
+      v(embed_dim_, kv_heads_ * head_dim_, name_ + " Value"),
+      o(num_heads_ * head_dim_, embed_dim_, name_ + " Output") {}
+
+void WindowSelfAttention::save(std::ofstream& f) const {
+  q.save(f);
+  k.save(f);
+  v.save(f);
+  o.save(f);
+}
+void WindowSelfAttention::load(std::ifstream& f) {
+  q.load(f);
+  k.load(f);
+  v.load(f);
+  o.load(f);
+}
+
+graph WindowSelfAttention::forward(const graph& X, const int32_t* positions, const std::vector<int>& sections,
+                                   const int32_t* lengths, const double base, const int rotary_flags) {
+  auto Q = q.forward(X);
+  auto K = k.forward(X);
+  auto V = v.forward(X);
+  if (kv_heads == num_heads) mle::fuse_sibling_linears({Q, K, V}, {&q, &k, &v});
+  else mle::fuse_sibling_linears({K, V}, {&k, &v});
+  auto mixed = GraphOperations::WindowAttention(GraphOperations::Rotary(Q, num_heads, positions, sections, base, rotary_flags),
+                                                GraphOperations::Rotary(K, kv_heads, positions, sections, base, rotary_flags),
+                                                V, num_heads, kv_heads, 1.0f / sqrtf((float)head_dim), window, sinks, lengths);
+  auto output = o.forward(mixed);
+  output->op_name = name + " Output";
+  return output;
+}
+
 // ResidualBlock (Engine/diffusion.cu:109-137).
 ResidualBlock::ResidualBlock(const int in_channels, const int out_channels, const int t_hidden, const int stride_,
                              const int groups_)

@@ -1,9 +1,10 @@
 // Layer compositions used by the benchmark configurations, built only from
 // GraphOperations ops: MultiHeadAttention (Includes/transformer.h,
-// Engine/transformer.cu:635-661) and the diffusion ResidualBlock
-// (Includes/diffusion.h:35-46, Engine/diffusion.cu:109-137).
+// Engine/transformer.cu:635-661), WindowSelfAttention and the diffusion
+// ResidualBlock (Includes/diffusion.h:35-46, Engine/diffusion.cu:109-137).
 #pragma once
 #include <memory>
+#include <vector>
 
 #include "engine.h"
 
@@ -15,6 +16,24 @@ class MultiHeadAttention {
   bool qkv_fused = false;  // set by forward: dX of the Q, K, V projections is one grouped GEMM
   MultiHeadAttention(const int embed_dim, const int hidden, const int num_heads, const str& name = "MHA");
   graph forward(const graph& X, const bool mask = true);
+  void save(std::ofstream& f) const;
+  void load(std::ifstream& f);
+};
+
+// Self-attention with rotary positions over a causal window and sinks, the heads of Q in
+// groups that share a head of K and V (no counterpart in the reference, whose
+// MultiHeadAttention adds positions to its input and softmaxes whole columns).
+class WindowSelfAttention {
+ public:
+  int embed_dim, num_heads, kv_heads, head_dim, window, sinks;
+  str name;
+  Linear q, k, v, o;
+  WindowSelfAttention(const int embed_dim, const int num_heads, const int kv_heads, const int head_dim,
+                      const int window, const int sinks = 0, const str& name = "Window Attention");
+  // positions: device ids [sections.size()][batch * seq], sections the pairs of a head that turn
+  // by each axis; lengths: device ids [batch] or nullptr.
+  graph forward(const graph& X, const int32_t* positions, const std::vector<int>& sections,
+                const int32_t* lengths = nullptr, const double base = 10000.0, const int rotary_flags = 0);
   void save(std::ofstream& f) const;
   void load(std::ifstream& f);
 };

@@ -132,6 +132,7 @@ graph act_node(const graph& input, int kind, const str& name) {
     input->forward = [fa, kind, nd]() { fa(kind, nd->output); };
     input->forward_act = nullptr;  // one takeover per producer
     input->forward_normstats = nullptr;
+    input->forward_layernorm = nullptr;
     input->forward_rowstats = nullptr;
     input->forward_xent_small = nullptr;
     node->forward = []() {};
@@ -195,6 +196,7 @@ graph norm_node(const graph& X, int groups, const str& name) {
     auto fs = X->forward_normstats;
     X->forward = [fs, groups, ws, ws_bytes]() { fs(groups, ws, ws_bytes); };
     X->forward_normstats = nullptr;  // one takeover per producer
+    X->forward_layernorm = nullptr;
     X->forward_act = nullptr;
     X->forward_act_mse = nullptr;
     ready = 1;
@@ -504,6 +506,11 @@ graph GraphOperations::Add(const graph& A, const graph& B, const bool last) {
       check(mle_add_norm_partials(S(), pa->output, pb->output, (size_t)nd->total, nd->output, d0, d1, d23, groups, ws,
                                   ws_bytes),
             "Add forward (with the normalisation statistics)");
+    };
+    node->forward_layernorm = [=](int rows, int cols, const float* w, const float* b, float eps, float* y, float* mean,
+                                  float* rstd) {
+      check(mle_add_layernorm_fwd(S(), rows, cols, pa->output, pb->output, w, b, eps, nd->output, y, mean, rstd),
+            "Add forward (with the layer norm after it)");
     };
     node->forward_act = [=](int kind, float* act_out) {
       check(mle_add_act_fwd(S(), pa->output, pb->output, nd->output, act_out, kind, nd->total),
@@ -1022,6 +1029,76 @@ graph GraphOperations::HeadAttention(const graph& Q, const graph& K, const graph
                             seq, hd, E, scale, causal ? 1 : 0, aq, ak, av, kref ? 1 : 0, ws, wsb),
           "Attention backward");
   };
+  std_hooks(node);
+  return node;
+}
+
+// Windowed attention (see engine.h).
+graph GraphOperations::WindowAttention(const graph& Q, const graph& K, const graph& V, const int heads,
+                                       const int kv_heads, const float scale, const int window, const int sinks,
+                                       const int32_t* lengths) {
+  const int b = Q->dim[0], seq = Q->dim[2], E = Q->dim[3], G = K->dim[3], hd = heads > 0 ? E / heads : 0;
+  bool fits = heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && E == heads * hd && G == kv_heads * hd && window >= 1 &&
+              sinks >= 0 && Q != K && Q != V && K != V && Q->dim[1] == 1;
+  for (int i = 0; i < 4; ++i) fits = fits && K->dim[i] == V->dim[i] && (i == 3 || Q->dim[i] == K->dim[i]);
+  if (!fits) {
+    std::cout << "Shape Mismatch in WindowAttention: " << heads << " heads, " << kv_heads << " of keys, window " << window
+              << ", " << sinks << " sinks \n";
+    Dimension(Q);
+    Dimension(K);
+    Dimension(V);
+    std::exit(1);
+  }
+  auto node = make_node("Window Attention", b, 1, seq, E);
+  node->inputs = {Q, K, V};
+  node->reads_grad_alias = true;
+  NodeBackProp *nd = node.get(), *pq = Q.get(), *pk = K.get(), *pv = V.get();
+  const size_t stats = (size_t)b * heads * seq;
+  float* lse = mle::alloc_output(stats);
+  GraphOperations::GB += (double)stats * sizeof(float) / (1ULL << 30);
+  const size_t ws_bytes = mle_window_attention_ws_bytes(b, seq, heads, kv_heads, hd, window, sinks);
+  void* ws = mle::gemm_workspace(ws_bytes);  // carries nothing from one call to the next
+  node->forward = [=]() {
+    check(mle_window_attention_fwd(S(), pq->output, E, pk->output, G, pv->output, G, nd->output, E, lse, lengths, b, seq,
+                                   heads, kv_heads, hd, scale, window, sinks),
+          "Window Attention forward");
+  };
+  node->backward = [=]() {
+    const int aq = mle::accumulate_flag(pq), ak = mle::accumulate_flag(pk), av = mle::accumulate_flag(pv);
+    check(mle_window_attention_bwd(S(), pq->output, E, pk->output, G, pv->output, G, nd->output, E, lse,
+                                   mle::grad_of(nd), E, pq->grad, E, aq, pk->grad, G, ak, pv->grad, G, av, lengths, b,
+                                   seq, heads, kv_heads, hd, scale, window, sinks, ws, ws_bytes),
+          "Window Attention backward");
+  };
+  std_hooks(node);
+  node->free = [=]() {
+    nd->clear();
+    mle::release(lse, stats, false);
+  };
+  return node;
+}
+
+// Rotary positions (see engine.h); the gradient turns back.
+graph GraphOperations::Rotary(const graph& X, const int heads, const int32_t* positions,
+                              const std::vector<int>& sections, const double base, const int flags) {
+  const int E = X->dim[3];
+  const long long rows = (long long)X->dim[0] * X->dim[2];
+  if (X->dim[1] != 1 || heads <= 0 || E % heads != 0 || rows > (1ll << 30)) {
+    std::cout << "Shape Mismatch in Rotary: " << heads << " heads \n";
+    Dimension(X);
+    std::exit(1);
+  }
+  auto node = make_node("Rotary", X->dim[0], 1, X->dim[2], E);
+  node->inputs = {X};
+  node->reads_grad_alias = true;
+  NodeBackProp *nd = node.get(), *x = X.get();
+  auto turn = [=](const float* in, float* out, int inverse, int accumulate, const char* what) {
+    check(mle_rotary(S(), (int)rows, E / heads, in, E, out, E, heads, nullptr, 0, nullptr, 0, 0, positions,
+                     (int)sections.size(), sections.data(), base, flags, inverse, accumulate),
+          what);
+  };
+  node->forward = [=]() { turn(x->output, nd->output, 0, 0, "Rotary forward"); };
+  node->backward = [=]() { turn(mle::grad_of(nd), x->grad, 1, mle::accumulate_flag(x), "Rotary backward"); };
   std_hooks(node);
   return node;
 }
