@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(Args a, BwdWork wk, int64_
 template <int DP, int NW>
 struct Shared {
   alignas(16) char lds[2][2][Tile<DP, 64>::BYTES];  // [buffer][Q, dout or K, V]
-  alignas(16) Rows<64> rows[4];
+  alignas(16) Rows<32> rows[4];
   alignas(16) Tops<NW> tops;
   int ex[NW];
 };
@@ -85,7 +85,7 @@ struct Shared {
 // dk and dv of 32 keys to a wave.
 template <int DP, int NW>
 __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const Place& place, Shared<DP, NW>& m) {
-  using T = Tile<DP, 64>;
+  using T = Tile<DP, 32>;
   constexpr int NT = 64 * NW, KB = 32 * NW, R = T::R, AHEAD = 1;
   static_assert(KB == kKeyBlock, "keys of a workgroup");
   const KvJob job(a, wk, place);
@@ -128,7 +128,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
 #pragma unroll
   for (int i = 1; i < NW; ++i) ex0 = max(ex0, m.ex[i]);
   Share<T, NT> in;  // of Q and dout
-  float r_lse, r_delta;  // of row threadIdx.x % 64 of the tile to come
+  float r_lse, r_delta;  // of row threadIdx.x % 32 of the tile to come
   int r_ex;
   Walk<R> ahead(a, job), here(a, job);
   auto fetch = [&]() {
