@@ -1,6 +1,6 @@
-// Forward of the windowed attention: 32 rows to a wave, 32 NW to a workgroup, one
-// pass over the tiles of keys that they see with the running maximum and sum of a
-// softmax.
+// Forward of the windowed attention: 32 rows to a wave, or (KW 2) to two waves that take half
+// of each tile's keys and join at the end, one pass over the tiles of keys that the rows of a
+// workgroup see with the running maximum and sum of a softmax.
 //
 // Scores come out as S^T = K Q^T, rows to lanes, so a row's statistics are a lane's
 // (two lanes hold 16 of every 32 keys of a row each), and P^T is the operand of
@@ -16,27 +16,30 @@ namespace {
 
 constexpr float kHead = 8.f;
 
-template <int DP, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
-  using T = Tile<DP, DP <= 64 ? 64 : 32>;  // as many products to a tile of wide heads, half the registers to LDS
+template <int DP, int NW, int KW>
+__global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile_fwd_kernel(Args a, Grid g) {
+  // as many products to a wave and tile of wide heads, half the registers to LDS
+  using T = Tile<DP, DP <= 64 || KW == 2 ? 64 : 32>;
   constexpr int NT = 64 * NW, R = T::R, AHEAD = 2;
+  constexpr int NB = T::NB / KW;  // a wave's blocks of a tile
   __shared__ __attribute__((aligned(16))) char lds[2][2][T::BYTES];  // [buffer][K, V]
   __shared__ __attribute__((aligned(16))) Tops<NW> tops;
-  const Block blk = g.block(a, 32 * NW);
+  const Block blk = g.block(a, 32 * NW / KW);
   const int b = blk.b, h = blk.h, e = h / a.group;
   const Seq seq(a, b);
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, half = lane >> 5;
-  const int row0 = blk.row + 32 * w;          // of this wave
+  const int kw = w % KW, n0 = kw * NB;        // which of the rows' waves, its first block of a tile
+  const int row0 = blk.row + 32 * (w / KW);   // of this wave
   const int i = row0 + c, p = seq.first + i;  // of this lane
   const bool live = i < a.rows && p >= 0 && p < seq.len;
   // positions of the workgroup's and the wave's rows that are there
-  const int first = max(seq.first + blk.row, 0), last = min(seq.first + min(blk.row + 32 * NW, a.rows), seq.len) - 1;
+  const int first = max(seq.first + blk.row, 0), last = min(seq.first + min(blk.row + 32 * NW / KW, a.rows), seq.len) - 1;
   const int wfirst = max(seq.first + row0, 0), wlast = min(seq.first + min(row0 + 32, a.rows), seq.len) - 1;
   const bool any = first <= last;
   const Tiles<R> tiles(a, first, last);
   const int count = any ? tiles.count : 0;
   if (count == 0 || a.dim < 4) {  // (the workgroup) nothing to see, or rows too short to load
-    for (int r = 0; r < 32; ++r)
+    for (int r = kw; r < 32; r += KW)
       if (row0 + r < a.rows) plain_row(a, b, h, row0 + r);
     return;
   }
@@ -94,26 +97,26 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m = -3e38f, l = 0.f;  // log2 units; m is kHead below the maximum
   const auto some = [&](int t) {  // does the wave see any of tile t?
-    const int j0 = tiles.row(t);
-    return wfirst <= wlast && j0 <= wlast && (wfirst - (j0 + R - 1) < a.window || j0 < a.sinks);
+    const int j0 = tiles.row(t) + 32 * n0;
+    return wfirst <= wlast && j0 <= wlast && (wfirst - (j0 + 32 * NB - 1) < a.window || j0 < a.sinks);
   };
-  Frag pf[2 * T::NB];  // P of a tile
+  Frag pf[2 * NB];  // P of a tile
   // P of tile t, whose K has exponent e.
   const auto weights = [&](int t, int e) {
     const char* tk = lds[t & 1][0];
-    const int j0 = tiles.row(t);
-    f32x16 s[T::NB];
+    const int j0 = tiles.row(t) + 32 * n0;
+    f32x16 s[NB];
 #pragma unroll
-    for (int n = 0; n < T::NB; ++n)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[n][r] = 0.f;
-    steps<T::KS * T::NB, AHEAD>([&](int i) { return frag_row<T>(tk, at, i % T::NB, i / T::NB); },
-                                [&](int i, const Frag& f) { mma3(f, q[i / T::NB], s[i % T::NB]); });
-    const bool all = j0 + R - 1 <= wfirst && (wlast - j0 < a.window || j0 + R - 1 < a.sinks) && row0 + 32 <= a.rows &&
+    steps<T::KS * NB, AHEAD>([&](int i) { return frag_row<T>(tk, at, n0 + i % NB, i / NB); },
+                                [&](int i, const Frag& f) { mma3(f, q[i / NB], s[i % NB]); });
+    const bool all = j0 + 32 * NB - 1 <= wfirst && (wlast - j0 < a.window || j0 + 32 * NB - 1 < a.sinks) && row0 + 32 <= a.rows &&
                      seq.first + row0 >= 0 && seq.first + row0 + 32 <= seq.len;
     if (!all) {
 #pragma unroll
-      for (int n = 0; n < T::NB; ++n)
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int j = j0 + 32 * n + 8 * (r >> 2) + 4 * half + (r & 3);
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
     const float ct = fmaxf(__builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, eq + e - 2 * kTop), 0x1p-126f);
     float mx = s[0][0];
 #pragma unroll
-    for (int n = 0; n < T::NB; ++n)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx *= ct;
@@ -138,14 +141,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
       m = mn;
     }
 #pragma unroll
-    for (int n = 0; n < T::NB; ++n)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], ct, -m));
         l += s[n][r];
       }
 #pragma unroll
-    for (int k = 0; k < 2 * T::NB; ++k) pf[k] = split_rows(s[k >> 1], k & 1);
+    for (int k = 0; k < 2 * NB; ++k) pf[k] = split_rows(s[k >> 1], k & 1);
   };
   // O += P V of tile t, whose operand of V has exponent e.
   const auto values = [&](int t, int e) {
@@ -157,7 +160,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
       ev = e;
     }
     const char* tv = lds[t & 1][1];
-    steps<2 * T::NB * T::DB, AHEAD>([&](int i) { return frag_col<T>(tv, at, i / T::DB, i % T::DB); },
+    steps<2 * NB * T::DB, AHEAD>([&](int i) { return frag_col<T>(tv, at, 2 * n0 + i / T::DB, i % T::DB); },
                                     [&](int i, const Frag& f) { mma3(f, pf[i / T::DB], o[i % T::DB]); });
   };
   put(0);
@@ -175,6 +178,34 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
     tell(t + 2);
   }
   l += other_half(l);
+  if constexpr (KW == 2) {
+    // the second wave's sums to the first, both at the larger maximum and power of two
+    static_assert(NW / 2 * 64 * (16 * T::DB + 3) * sizeof(float) <= sizeof(lds), "room for a wave's sums");
+    float* at_lane = reinterpret_cast<float*>(lds) + (w / 2) * 64 * (16 * T::DB + 3) + lane;
+    __syncthreads();  // the tiles have been read
+    if (kw == 1) {
+#pragma unroll
+      for (int d = 0; d < T::DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) at_lane[64 * (16 * d + r)] = o[d][r];
+      at_lane[64 * 16 * T::DB] = m;
+      at_lane[64 * (16 * T::DB + 1)] = l;
+      at_lane[64 * (16 * T::DB + 2)] = (float)ev;
+    }
+    __syncthreads();
+    if (kw == 1) return;
+    const float m1 = at_lane[64 * 16 * T::DB], l1 = at_lane[64 * (16 * T::DB + 1)], mj = fmaxf(m, m1);
+    const int ev1 = (int)at_lane[64 * (16 * T::DB + 2)], evj = max(ev, ev1);
+    const float f0 = __builtin_amdgcn_exp2f(m - mj), f1 = __builtin_amdgcn_exp2f(m1 - mj);
+    l = fmaf(l, f0, l1 * f1);
+#pragma unroll
+    for (int d = 0; d < T::DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        o[d][r] = fmaf(__builtin_amdgcn_ldexpf(o[d][r], ev - evj), f0,
+                       __builtin_amdgcn_ldexpf(at_lane[64 * (16 * d + r)], ev1 - evj) * f1);
+    m = mj, ev = evj;
+  }
   float mark = l;  // not finite where a score or a sum is not
 #pragma unroll
   for (int d = 0; d < T::DB; ++d)
@@ -209,12 +240,19 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(Args a, Grid g) {
 template <int DP>
 void launch_dim(const Args& a, hipStream_t s) {
   // 8 waves share a tile, 4 where the window is small: a workgroup walks over window + rows
-  // keys, of which a wave computes window + 32.
-  const bool wide = a.window >= 512 && (int64_t)a.batch * a.heads * ((a.rows + 255) / 256) >= 256;
-  const int nw = wide ? 8 : 4;
-  const Grid g(a, a.heads, (a.rows + 32 * nw - 1) / (32 * nw));
-  if (wide) launch_blocks(tile_fwd_kernel<DP, 8>, g, 512, s, a);
-  else launch_blocks(tile_fwd_kernel<DP, 4>, g, 256, s, a);
+  // keys, of which a wave computes window + 32.  Where that leaves CUs idle two waves share 32 rows'
+  // keys: 64 rows to a workgroup (6 heads of 777 x 80, window 200: 33 us against 40, 4 of 2048 x 64:
+  // 26 against 34), or 128 where 64 would be no more workgroups or too many (32 heads of
+  // 1024 x 64, all keys: 40 against 46).
+  const auto blocks = [&](int rows) { return (int64_t)a.batch * a.heads * ((a.rows + rows - 1) / rows); };
+  if (a.window >= 512 && blocks(256) >= 256)
+    launch_blocks(tile_fwd_kernel<DP, 8, 1>, Grid(a, a.heads, (a.rows + 255) / 256), 512, s, a);
+  else if (blocks(64) <= 256 && blocks(64) > blocks(128))
+    launch_blocks(tile_fwd_kernel<DP, 4, 2>, Grid(a, a.heads, (a.rows + 63) / 64), 256, s, a);
+  else if (blocks(128) <= 256)
+    launch_blocks(tile_fwd_kernel<DP, 8, 2>, Grid(a, a.heads, (a.rows + 127) / 128), 512, s, a);
+  else
+    launch_blocks(tile_fwd_kernel<DP, 4, 1>, Grid(a, a.heads, (a.rows + 127) / 128), 256, s, a);
 }
 
 }  // namespace
