@@ -106,6 +106,21 @@ CASES = [
 ]
 
 
+# many heads: every number of waves and of key blocks that the launches choose from, at each width
+CASES += [
+    (40, 140, 8, 4, 64, 60, 2, None, 0, 0, 0),
+    (24, 150, 6, 6, 90, 70, 3, [150, 0, 1, 149, 128, 33] * 4, 0, 0, 0),
+    (20, 131, 8, 2, 128, 40, 0, None, 0, 0, 7),
+    (32, 40, 8, 8, 64, 600, 1, [40, 3] * 16, 0, 0, 2),
+    (16, 300, 8, 4, 128, 512, 0, None, 0, 0, 0),
+    (32, 33, 8, 1, 72, 512, 2, None, 1, 2, 0),
+    (16, 200, 5, 5, 64, 50, 1, None, 0, 0, 0),
+    (16, 129, 6, 3, 96, 300, 0, [129, 128, 65, 64] * 4, 0, 0, 0),
+    (12, 256, 8, 8, 128, 90, 2, None, 0, 0, 0),
+    (1, 3, 300, 100, 5, 2, 1, None, 0, 0, 0),
+]
+
+
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x).replace(" ", "") for x in c))
 def test_forward_and_backward(hip, case):
     b, n, h, kv, d, w, s, lengths, pad, shift, acc = case
