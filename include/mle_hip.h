@@ -422,10 +422,12 @@ int mle_attention_bwd(mle_stream stream, const float* q, const float* k, const f
  *   S = scale q k^T,  P = exp(S - lse),  lse = log sum exp S,  out = P v
  * over the visible keys, whatever the others hold.  Rows at or past a length have out 0 and
  * lse -infinity, and their gradients take no part; their k and v rows get gradients of 0.
- * lse [batch, heads, seq] is nullable where no backward follows.
- * The products' operands are held in 22 bits (two fp16 parts and a power of two per tile,
- * row or column); sums, statistics and exponentials are fp32.  A tile that holds an infinity or
- * a NaN is computed with fp32 products, key by key.  Results do not depend on timing.
+ * lse [batch, heads, seq] is nullable where no backward follows; out is none of the inputs.
+ * The products' operands are held in 22 bits (two fp16 parts and a power of two per tile of 32
+ * or 64 positions, row or column): what is below 2^-18 of a tile's largest, hidden entries
+ * among them, is held to 2^-40 of it.  Sums, statistics and exponentials are fp32.  Where a tile
+ * holds an infinity or a NaN, or lies far below an earlier one, rows are computed with fp32
+ * products, key by key.  Results do not depend on timing.
  * MultiHeadAttention's softmax (mle_attention_fwd) is over columns; this is SOFTMAX type 0
  * (Engine/engine.cu:2430-2505) with a mask, without storing scores. */
 int mle_window_attention_fwd(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,
@@ -448,8 +450,8 @@ int mle_window_attention_bwd(mle_stream stream, const float* q, int64_t ldq, con
  * [batch, capacity, ld], the newest positions' own among them: row i of sequence b's queries
  * [batch, tokens, ldq] is at position lengths[b] - tokens + i (lengths taken as at most capacity
  * and at least 0; rows at a position below 0 get zeros).  Cache rows at or past a length are not
- * read.  The keys are shared out over the chip and the parts joined in order; ws: 16-byte aligned,
- * two calls that run at once need one each. */
+ * read.  The keys are shared out over the chip and the parts joined in order; ws: 16-byte aligned
+ * (NULL where 0 bytes are needed), two calls that run at once need one each. */
 size_t mle_window_attention_step_ws_bytes(int batch, int tokens, int capacity, int heads, int kv_heads, int head_dim,
                                           int window, int sinks);
 int mle_window_attention_step(mle_stream stream, const float* q, int64_t ldq, const float* k, int64_t ldk,

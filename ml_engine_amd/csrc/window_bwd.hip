@@ -102,7 +102,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
   }
   const Places<T> at(lane);
   job.largest(a, wk, m.ex);
-  // this lane's rows of K, at a power of two of its own, and of V, at the wave's
+  // this lane's rows of K and V, each at a power of two of its own
   Frag kf[T::KS], vf[T::KS];
   int ek, ev;
   bool odd = false;
@@ -118,7 +118,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
     float x[T::KS][8];
     const float top = load_row<T::KS>(a.v + ((int64_t)b * a.keys + (live ? j : 0)) * a.ldv + (int64_t)e * a.dim, half, a.dim, live, x);
     odd |= !(top < INFINITY);
-    ev = __builtin_amdgcn_readlane(exponent(wave_top(top)), 63);
+    ev = exponent(fmaxf(top, other_half(top)));
 #pragma unroll
     for (int s = 0; s < T::KS; ++s) vf[s] = split8(x[s], scale(ev));
   }
@@ -151,7 +151,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
     const float mq = m.tops.get(0, t);
     const Rows<R>& r = m.rows[t & 3];
     odd |= !(mq < INFINITY) || r.odd != 0u;
-    eq_next = max(eq_next, exponent(mq));
+    eq_next = raised(eq_next, mq, odd);
     const float sq = scale(eq_next);
     in.put(m.lds[t & 1][0], m.lds[t & 1][1], [&](bool g, int row) { return g ? scale(r.ex[row]) : sq; });
   };
@@ -335,7 +335,7 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
   auto put = [&](int t) {
     const float mk = m.tops.get(0, t), mv = m.tops.get(1, t);
     odd |= !(fmaxf(mk, mv) < INFINITY);
-    ek_next = max(ek_next, exponent(mk));
+    ek_next = raised(ek_next, mk, odd);
     ev = exponent(mv);
     const float sk = scale(ek_next), sv = scale(ev);
     in.put(m.lds[t & 1][0], m.lds[t & 1][1], [=](bool v, int) { return v ? sv : sk; });

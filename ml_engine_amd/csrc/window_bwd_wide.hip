@@ -66,7 +66,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
   // Which of the pair this is tells its code: each has the registers to itself.
   const auto pass = [&](auto which) {
     constexpr bool second = decltype(which)::value;
-    // This lane's row of K, at a power of two of its own, or of V, at the wave's.
+    // This lane's row of K or V, at a power of two of its own.
     Frag own[T::KS];
     bool odd = false;
     int eo;
@@ -75,7 +75,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
       const float* p = (second ? a.v : a.k) + ((int64_t)b * a.keys + (live ? j : 0)) * (second ? a.ldv : a.ldk) + (int64_t)e * a.dim;
       const float top = load_row<T::KS>(p, half, a.dim, live, x);
       odd |= !(top < INFINITY);
-      eo = second ? __builtin_amdgcn_readlane(exponent(wave_top(top)), 63) : exponent(fmaxf(top, other_half(top)));
+      eo = exponent(fmaxf(top, other_half(top)));
 #pragma unroll
       for (int s = 0; s < T::KS; ++s) own[s] = split8(x[s], scale(eo));
     }
@@ -108,7 +108,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
       const float mq = m.tops.get(0, t);
       const Rows<R>& r = m.rows[t & 3];
       odd |= !(mq < INFINITY) || r.odd != 0u;
-      eq_next = max(eq_next, exponent(mq));
+      eq_next = raised(eq_next, mq, odd);
       const float sq = scale(eq_next);
       in.put(buf[0], buf[1], [&](bool g, int row) { return g ? scale(r.ex[row]) : sq; });
     };
@@ -306,7 +306,7 @@ __device__ __forceinline__ void q_pairs(const Args& a, const Block& blk, Shared<
     auto put = [&](int t, char (*buf)[T::BYTES]) {
       const float mk = m.tops.get(0, t), mv = m.tops.get(1, t);
       odd |= !(fmaxf(mk, mv) < INFINITY);
-      ek_next = max(ek_next, exponent(mk));
+      ek_next = raised(ek_next, mk, odd);
       ev = exponent(mv);
       const float sk = scale(ek_next), sv = scale(ev);
       in.put(buf[0], buf[1], [=](bool v, int) { return v ? sv : sk; });

@@ -84,7 +84,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile
     const float mk = tops.get(0, t), mv = tops.get(1, t);
     odd |= !(fmaxf(mk, mv) < INFINITY);
     ek = exponent(mk);
-    ev_next = max(ev_next, exponent(mv));
+    ev_next = raised(ev_next, mv, odd);
     const float sk = scale(ek), sv = scale(ev_next);
     kv.put(lds[t & 1][0], lds[t & 1][1], [=](bool v, int) { return v ? sv : sk; });
   };

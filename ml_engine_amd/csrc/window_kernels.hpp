@@ -35,9 +35,12 @@ struct BwdWork {
     near_rows = rows;
     if (blocks > 0 && blocks < 128) near_rows = (int)std::max<int64_t>(64, (rows * blocks / 128 + 63) / 64 * 64);
     nears = rows > 0 ? (rows + near_rows - 1) / near_rows : 1;
-    // short, so that they fill in behind the blocks of keys
-    far_rows = std::max(256, (a.window / 4 + 63) / 64 * 64);
-    const int after = a.rows - rows;
+    // short, so that they fill in behind the blocks of keys; longer where sinks are so many
+    // that their blocks alone fill the chip, and their parts the memory
+    const int after = std::max(a.rows - rows, 0);
+    const int64_t sets = (int64_t)a.batch * a.kv_heads * sink_blocks, most = std::max<int64_t>(1, 2048 / std::max<int64_t>(sets, 1));
+    far_rows = (int)std::max<int64_t>({256, a.window / 4, (after + most - 1) / most});
+    far_rows = (far_rows + 63) / 64 * 64;
     fars = sink_blocks > 0 && after > 0 ? (after + far_rows - 1) / far_rows : 0;
   }
   int kv_items() const { return key_blocks * nears + sink_blocks * fars; }  // workgroups of the kv pass to a head

@@ -200,6 +200,15 @@ __device__ __forceinline__ int exponent(float m) {
 // The power of two that brings values of this exponent to [2^kTop, 2^(kTop + 1)).
 __device__ __forceinline__ float scale(int e) { return __builtin_bit_cast(float, (unsigned)(kTop - e + 127) << 23); }
 
+// An operand's exponent from a tile on whose largest magnitude is `top`, the sums being at the
+// largest exponent so far.  A tile far below that would lose bits that rows need which no
+// longer see the large one: `odd`, then (fp32 products).
+__device__ __forceinline__ int raised(int so_far, float top, bool& odd) {
+  const int e = exponent(top);
+  odd |= top > 0.f && so_far - e > 16;
+  return max(so_far, e);
+}
+
 // A thread's share of two tensors' tiles among NT threads: N chunks of eight columns, the
 // first tensor's tile and then the second's.  A wave's chunk is of one tensor.
 template <class T, int NT>

@@ -70,6 +70,15 @@ def test_queries_take_zeros():
     assert L.mle_add_layernorm_ws_bytes(0, 40) == 0 == L.mle_add_layernorm_ws_bytes(40, 0)
 
 
+def test_workspace_of_many_sinks():
+    """The far parts of sinks take no more than some tensors of the keys' size."""
+    lib = hip.lib()
+    for batch, seq, kv, dim in ((1, 8192, 8, 128), (8, 8192, 8, 128), (1, 100000, 1, 64), (64, 4096, 4, 64)):
+        for sinks in (1, 1000, seq // 2, seq):
+            tensor = 4 * batch * seq * kv * dim
+            assert lib.mle_window_attention_ws_bytes(batch, seq, kv, kv, dim, 1, sinks) <= (1 << 29) + 4 * tensor
+
+
 def test_workspaces_stay_small():
     """The backward's is a number per row and head and a share of the sinks' gradients; a step's, partial rows."""
     L = hip.lib()

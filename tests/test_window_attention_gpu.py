@@ -118,6 +118,8 @@ CASES += [
     (16, 129, 6, 3, 96, 300, 0, [129, 128, 65, 64] * 4, 0, 0, 0),
     (12, 256, 8, 8, 128, 90, 2, None, 0, 0, 0),
     (1, 3, 300, 100, 5, 2, 1, None, 0, 0, 0),
+    (1, 1500, 2, 2, 32, 3, 1400, [1499], 0, 0, 2),
+    (2, 900, 4, 2, 100, 1, 900, [900, 40], 0, 0, 0),
 ]
 
 
@@ -147,6 +149,32 @@ def test_rows_of_unlike_size(hip):
         for a in (c.v, c.dout):
             a *= (10.0 ** r.uniform(-4, 0, a.shape[:2] + (1, 1))).astype(np.float32)
     c = Case(hip, 2, 400, 4, 2, 64, 150, 4, spoil=spoil)
+    c.forward()
+    c.backward()
+    c.check()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+def test_what_the_window_has_left_may_be_large(hip, which, dim):
+    """Entries 2^30 times the others' that a row no longer sees cost it no bits."""
+    small, large = Case(hip, 1, 400, 4, 2, dim, 40, 0), Case(
+        hip, 1, 400, 4, 2, dim, 40, 0, spoil=lambda c: getattr(c, which).__setitem__((0, slice(0, 60)), getattr(c, which)[0, :60] * np.float32(2 ** 30)))
+    for c in (small, large):
+        c.forward()
+        c.backward()
+    r, got = small.expected(), large.results()
+    at = slice(192, None)  # tiles after the large ones' and the window's
+    for name in ("out", "dq", "dk", "dv"):
+        ref.check(got[name][:, at], {name: r[name][:, at], "e_" + name: r["e_" + name][:, at]}, name)
+    ref.check(got["lse"][:, :, at], {"lse": r["lse"][:, :, at], "e_lse": r["e_lse"][:, :, at]}, "lse")
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-6])
+@pytest.mark.parametrize("dim", [48, 120])
+def test_scales(hip, scale, dim):
+    c = Case(hip, 2, 150, 4, 2, dim, 60, 2, lengths=[150, 90])
+    c.scale = float(np.float32(scale))
     c.forward()
     c.backward()
     c.check()
