@@ -101,6 +101,25 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
     return;
   }
   const Places<T> at(lane);
+  typedef Share<T, NT> Part;
+  struct In {  // of Q and dout, and of row threadIdx.x % 32 of them
+    Part x;
+    float lse, delta;
+    int ex;
+  } in0, in;  // tile 0's, and the others'
+  Walk<R> ahead(a, job), here(a, job);
+  auto fetch = [&](In& in) {
+    in.x.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)ahead.h * a.dim, a.ldq,
+              a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)ahead.h * a.dim, a.lddo, ahead.r0, i_end, a.dim);
+    const int64_t st = ((int64_t)b * a.heads + ahead.h) * a.rows + min(ahead.r0 + (int)threadIdx.x % R, i_end - 1);
+    in.lse = a.lse_in[st];
+    in.delta = a.delta[st];
+    in.ex = wk.ex[st];
+  };
+  fetch(in0);
+  const int first_row = ahead.r0;
+  ahead.next();
+  fetch(in);
   job.largest(a, wk, m.ex);
   // this lane's rows of K and V, each at a power of two of its own
   Frag kf[T::KS], vf[T::KS];
@@ -127,33 +146,20 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
   int ex0 = m.ex[0];
 #pragma unroll
   for (int i = 1; i < NW; ++i) ex0 = max(ex0, m.ex[i]);
-  Share<T, NT> in;  // of Q and dout
-  float r_lse, r_delta;  // of row threadIdx.x % 32 of the tile to come
-  int r_ex;
-  Walk<R> ahead(a, job), here(a, job);
-  auto fetch = [&]() {
-    in.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)ahead.h * a.dim, a.ldq,
-            a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)ahead.h * a.dim, a.lddo, ahead.r0, i_end, a.dim);
-    const int64_t st = ((int64_t)b * a.heads + ahead.h) * a.rows + min(ahead.r0 + (int)threadIdx.x % R, i_end - 1);
-    r_lse = a.lse_in[st];
-    r_delta = a.delta[st];
-    r_ex = wk.ex[st];
-  };
-  // The tile's largest of Q, and what its rows are scaled by: one step ahead of put().
-  auto tell = [&](int t) {
-    in.clear(ahead.r0, i_end, a.dim);
-    m.tops.add(0, t, in.top(false));
-    m.rows[t & 3].put(ahead.r0, i_end, ex0, r_lse, r_delta, r_ex);
-    ahead.next();
+  // The largest of Q in tile t from row r0, and what its rows are scaled by: one step ahead of put().
+  auto tell = [&](In& in, int t, int r0) {
+    in.x.clear(r0, i_end, a.dim);
+    m.tops.add(0, t, in.x.top(false));
+    m.rows[t & 3].put(r0, i_end, ex0, in.lse, in.delta, in.ex);
   };
   int eq = kNone, eq_next = kNone;  // the exponent of Q's operand, that dk is at and of the tile to come
-  auto put = [&](int t) {
+  auto put = [&](const Part& x, int t) {
     const float mq = m.tops.get(0, t);
     const Rows<R>& r = m.rows[t & 3];
     odd |= !(mq < INFINITY) || r.odd != 0u;
     eq_next = raised(eq_next, mq, odd);
     const float sq = scale(eq_next);
-    in.put(m.lds[t & 1][0], m.lds[t & 1][1], [&](bool g, int row) { return g ? scale(r.ex[row]) : sq; });
+    x.put(m.lds[t & 1][0], m.lds[t & 1][1], [&](bool g, int row) { return g ? scale(r.ex[row]) : sq; });
   };
   f32x16 dk[T::DB], dv[T::DB];
 #pragma unroll
@@ -163,17 +169,16 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
   // this key's P is held at 2^sj (times its row's power of two), its dS at 2^(sj + tj)
   float sj = 100.f;
   int tj = 100;
-  fetch();
-  tell(0);
+  tell(in0, 0, first_row);
+  tell(in, 1, ahead.r0);
+  ahead.next();
   __syncthreads();
-  put(0);
-  fetch();
-  tell(1);
+  put(in0.x, 0);
   for (int t = 0; t < count; ++t) {
     __syncthreads();  // tile t lies in its buffer, nobody reads the other, tile t + 1 is announced
     const int eqt = eq_next;
-    put(t + 1);
-    fetch();
+    if (t + 1 < count) put(in.x, t + 1);
+    fetch(in);
     const char *tq = m.lds[t & 1][0], *tg = m.lds[t & 1][1];
     const Rows<R>& rw = m.rows[t & 3];
     const int r0 = here.r0;
@@ -244,7 +249,10 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
                                 else mma3(f, pf[k], dv[d]);
                               });
     }
-    tell(t + 2);
+    if (t + 2 < count) {
+      tell(in, t + 2, ahead.r0);
+      ahead.next();
+    }
   }
   float mark = 0.f;
 #pragma unroll
@@ -305,16 +313,18 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
   const float* V = a.v + (int64_t)b * a.keys * a.ldv + (int64_t)e * a.dim;
   const Places<T> at(lane);
 
-  Share<T, NT> in;
-  // Tiles past the last are the last once more, which nobody reads: no branches around loads.
+  typedef Share<T, NT> Part;
+  Part kv0, kv;  // tile 0's registers, and the others'
+  // Loads past the last tile are of the last once more and go unused: no branches around loads.
   auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
-  auto fetch = [&](int t) { in.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim); };
-  auto tell = [&](int t) {
-    in.clear(row_of(t), seq.len, a.dim);
-    m.tops.add(0, t, in.top(false));
-    m.tops.add(1, t, in.top(true));
+  auto fetch = [&](Part& x, int t) { x.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim); };
+  auto tell = [&](Part& x, int t) {
+    x.clear(row_of(t), seq.len, a.dim);
+    m.tops.add(0, t, x.top(false));
+    m.tops.add(1, t, x.top(true));
   };
-  fetch(0);
+  fetch(kv0, 0);
+  fetch(kv, 1);
   Frag q[T::KS], go[T::KS];
   bool odd = false;
   auto own = [&](const float* p, Frag (&f)[T::KS]) {  // a row at a power of two of its own
@@ -332,15 +342,16 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
   const float delta = live ? a.delta[st] : 0.f, lse = live ? a.lse_in[st] * kLog2e : 0.f;
   odd |= !(fabsf(delta) < INFINITY) || !(fabsf(lse) < INFINITY);
   int ek = kNone, ek_next = kNone, ev = 0;
-  auto put = [&](int t) {
+  auto put = [&](const Part& x, int t) {
     const float mk = m.tops.get(0, t), mv = m.tops.get(1, t);
     odd |= !(fmaxf(mk, mv) < INFINITY);
     ek_next = raised(ek_next, mk, odd);
     ev = exponent(mv);
     const float sk = scale(ek_next), sv = scale(ev);
-    in.put(m.lds[t & 1][0], m.lds[t & 1][1], [=](bool v, int) { return v ? sv : sk; });
+    x.put(m.lds[t & 1][0], m.lds[t & 1][1], [=](bool v, int) { return v ? sv : sk; });
   };
-  tell(0);
+  tell(kv0, 0);
+  tell(kv, 1);
   __syncthreads();
   f32x16 dq[T::DB];
 #pragma unroll
@@ -349,14 +360,12 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
   int ti = 100;  // this row's dS is held at 2^ti (and below)
   const float dd = __builtin_amdgcn_ldexpf(delta, -eg);
-  put(0);
-  fetch(1);
-  tell(1);
+  put(kv0, 0);
   for (int t = 0; t < count; ++t) {
     __syncthreads();
     const int ekt = ek_next, evt = ev;
-    put(t + 1);
-    fetch(t + 2);
+    if (t + 1 < count) put(kv, t + 1);
+    fetch(kv, t + 2);
     const char *tk = m.lds[t & 1][0], *tv = m.lds[t & 1][1];
     const int j0 = tiles.row(t);
     if (ekt != ek) {  // K's operand has a larger power of two from here on
@@ -398,7 +407,7 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
       steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<T>(tk, at, 2 * n + i / T::DB, i % T::DB); },
                               [&](int i, const Frag& f) { mma3(f, df[i / T::DB], dq[i % T::DB]); });
     }
-    tell(t + 2);
+    if (t + 2 < count) tell(kv, t + 2);
   }
   float mark = 0.f;
 #pragma unroll

@@ -77,18 +77,6 @@ struct Rows {
   }
 };
 
-// A row of a wave's own operand, columns 16 s + 8 half .. of step s; the largest magnitude.
-template <int KS>
-__device__ __forceinline__ float load_row(const float* __restrict__ p, int half, int dim, bool there, float (&x)[KS][8]) {
-  float m = 0.f;
-#pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    load8(p, 2 * s + half, dim, there, x[s]);
-    m = fmaxf(m, top8(x[s]));
-  }
-  return m;
-}
-
 // A workgroup's part of the kv pass: kKeyBlock keys, and rows of every head of the group.
 struct KvJob {
   int b, e, k0, i_begin, i_end;
@@ -137,8 +125,8 @@ struct KvJob {
   }
 };
 
-// The tiles of R rows of each head in turn; those past the last are the last once more, which
-// nobody reads: no branches around loads.
+// The tiles of R rows of each head in turn; past the last comes the last once more (loads of it go
+// unused: no branches around loads).
 template <int R>
 struct Walk {
   int h, r0, h_end, begin, end;

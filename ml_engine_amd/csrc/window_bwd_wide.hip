@@ -62,10 +62,29 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
     return;
   }
   const Places<T> at(lane);
-  job.largest(a, wk, m.ex);
+  typedef Share<T, NT> Part;
   // Which of the pair this is tells its code: each has the registers to itself.
   const auto pass = [&](auto which) {
     constexpr bool second = decltype(which)::value;
+    struct In {  // of Q and dout, and of row threadIdx.x % 32 of them
+      Part x;
+      float lse, delta;
+      int ex;
+    } in0, in;  // tile 0's, and the others'
+    Walk<R> ahead(a, job), here(a, job);
+    auto fetch = [&](In& in) {
+      in.x.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)ahead.h * a.dim, a.ldq,
+                a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)ahead.h * a.dim, a.lddo, ahead.r0, i_end, a.dim);
+      const int64_t st = ((int64_t)b * a.heads + ahead.h) * a.rows + min(ahead.r0 + (int)threadIdx.x % R, i_end - 1);
+      in.lse = a.lse_in[st];
+      in.delta = a.delta[st];
+      in.ex = wk.ex[st];
+    };
+    fetch(in0);
+    const int first_row = ahead.r0;
+    ahead.next();
+    fetch(in);
+    job.largest(a, wk, m.ex);
     // This lane's row of K or V, at a power of two of its own.
     Frag own[T::KS];
     bool odd = false;
@@ -84,33 +103,20 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
 #pragma unroll
     for (int i = 1; i < NW; ++i) ex0 = max(ex0, m.ex[i]);
 
-    Share<T, NT> in;       // of Q and dout
-    float r_lse, r_delta;  // of row threadIdx.x % 32 of the tile to come
-    int r_ex;
-    Walk<R> ahead(a, job), here(a, job);
-    auto fetch = [&]() {
-      in.load(a.q + (int64_t)b * a.rows * a.ldq + (int64_t)ahead.h * a.dim, a.ldq,
-              a.dout + (int64_t)b * a.rows * a.lddo + (int64_t)ahead.h * a.dim, a.lddo, ahead.r0, i_end, a.dim);
-      const int64_t st = ((int64_t)b * a.heads + ahead.h) * a.rows + min(ahead.r0 + (int)threadIdx.x % R, i_end - 1);
-      r_lse = a.lse_in[st];
-      r_delta = a.delta[st];
-      r_ex = wk.ex[st];
-    };
-    // The tile's largest of Q, and what its rows are scaled by: one step ahead of put().
-    auto tell = [&](int t) {
-      in.clear(ahead.r0, i_end, a.dim);
-      m.tops.add(0, t, in.top(false));
-      m.rows[t & 3].put(ahead.r0, i_end, ex0, r_lse, r_delta, r_ex);
-      ahead.next();
+    // The largest of Q in tile t from row r0, and what its rows are scaled by: one step ahead of put().
+    auto tell = [&](In& in, int t, int r0) {
+      in.x.clear(r0, i_end, a.dim);
+      m.tops.add(0, t, in.x.top(false));
+      m.rows[t & 3].put(r0, i_end, ex0, in.lse, in.delta, in.ex);
     };
     int eq_next = kNone;  // the exponent of Q's operand so far
-    auto put = [&](int t, char (*buf)[T::BYTES]) {
+    auto put = [&](const Part& x, int t, char (*buf)[T::BYTES]) {
       const float mq = m.tops.get(0, t);
       const Rows<R>& r = m.rows[t & 3];
       odd |= !(mq < INFINITY) || r.odd != 0u;
       eq_next = raised(eq_next, mq, odd);
       const float sq = scale(eq_next);
-      in.put(buf[0], buf[1], [&](bool g, int row) { return g ? scale(r.ex[row]) : sq; });
+      x.put(buf[0], buf[1], [&](bool g, int row) { return g ? scale(r.ex[row]) : sq; });
     };
     f32x16 sum[T::DB];  // dv^T or dk^T
 #pragma unroll
@@ -192,24 +198,26 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
       steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<T>(buf[!second], at, i / T::DB, i % T::DB); },
                               [&](int i, const Frag& f) { mma3(f, op[i / T::DB], sum[i % T::DB]); });
     };
-    fetch();
-    tell(0);
+    tell(in0, 0, first_row);
+    tell(in, 1, ahead.r0);
+    ahead.next();
     __syncthreads();
-    put(0, m.lds[0]);
-    fetch();
-    tell(1);
+    put(in0.x, 0, m.lds[0]);
     int e_last = 0, now = 0, old = 2;  // the buffers of tiles t and t - 1
     for (int t = 0; t <= count; ++t) {
       __syncthreads();  // tile t lies in its buffer, nobody reads that of t + 1, which is announced; P of t - 1 is there
       const int et = eq_next, coming = now == 2 ? 0 : now + 1;
-      put(t + 1, m.lds[coming]);
-      fetch();
+      if (t + 1 < count) put(in.x, t + 1, m.lds[coming]);
+      fetch(in);
       if (second ? t > 0 : t < count) {
         block(second ? t - 1 : t, m.lds[second ? old : now], second ? e_last : et);
         here.next();
       }
       e_last = et, old = now, now = coming;
-      tell(t + 2);
+      if (t + 2 < count) {
+        tell(in, t + 2, ahead.r0);
+        ahead.next();
+      }
     }
     float mark = 0.f;
 #pragma unroll
@@ -275,16 +283,18 @@ __device__ __forceinline__ void q_pairs(const Args& a, const Block& blk, Shared<
   // Which of the pair this is tells its code: each has the registers to itself.
   const auto pass = [&](auto which) {
     constexpr bool second = decltype(which)::value;
-    Share<T, NT> in;
-    // Tiles past the last are the last once more, which nobody reads: no branches around loads.
+    typedef Share<T, NT> Part;
+    Part kv0, kv;  // tile 0's registers, and the others'
+    // Loads past the last tile are of the last once more and go unused: no branches around loads.
     auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
-    auto fetch = [&](int t) { in.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim); };
-    auto tell = [&](int t) {
-      in.clear(row_of(t), seq.len, a.dim);
-      m.tops.add(0, t, in.top(false));
-      m.tops.add(1, t, in.top(true));
+    auto fetch = [&](Part& x, int t) { x.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim); };
+    auto tell = [&](Part& x, int t) {
+      x.clear(row_of(t), seq.len, a.dim);
+      m.tops.add(0, t, x.top(false));
+      m.tops.add(1, t, x.top(true));
     };
-    fetch(0);
+    fetch(kv0, 0);
+    fetch(kv, 1);
     // this lane's row of Q or of dout, at a power of two of its own
     Frag own[T::KS];
     int eo;
@@ -303,13 +313,13 @@ __device__ __forceinline__ void q_pairs(const Args& a, const Block& blk, Shared<
     const float delta = live ? a.delta[st] : 0.f, lse = live ? a.lse_in[st] * kLog2e : 0.f;
     odd |= !(fabsf(delta) < INFINITY) || !(fabsf(lse) < INFINITY);
     int ek_next = kNone, ev = 0;
-    auto put = [&](int t, char (*buf)[T::BYTES]) {
+    auto put = [&](const Part& x, int t, char (*buf)[T::BYTES]) {
       const float mk = m.tops.get(0, t), mv = m.tops.get(1, t);
       odd |= !(fmaxf(mk, mv) < INFINITY);
       ek_next = raised(ek_next, mk, odd);
       ev = exponent(mv);
       const float sk = scale(ek_next), sv = scale(ev);
-      in.put(buf[0], buf[1], [=](bool v, int) { return v ? sv : sk; });
+      x.put(buf[0], buf[1], [=](bool v, int) { return v ? sv : sk; });
     };
     f32x16 dq[T::DB];
 #pragma unroll
@@ -363,20 +373,19 @@ __device__ __forceinline__ void q_pairs(const Args& a, const Block& blk, Shared<
                                 [&](int i, const Frag& f) { mma3(f, op[i / T::DB], dq[i % T::DB]); });
       }
     };
-    tell(0);
+    tell(kv0, 0);
+    tell(kv, 1);
     __syncthreads();
-    put(0, m.lds[0]);
-    fetch(1);
-    tell(1);
+    put(kv0, 0, m.lds[0]);
     int ek_last = 0, ev_last = 0, now = 0, old = 2;  // the buffers of tiles t and t - 1
     for (int t = 0; t <= count; ++t) {
       __syncthreads();  // tile t lies in its buffer, nobody reads that of t + 1, which is announced; P of t - 1 is there
       const int ekt = ek_next, evt = ev, coming = now == 2 ? 0 : now + 1;
-      put(t + 1, m.lds[coming]);
-      fetch(t + 2);
+      if (t + 1 < count) put(kv, t + 1, m.lds[coming]);
+      fetch(kv, t + 2);
       if (second ? t > 0 : t < count) block(second ? t - 1 : t, m.lds[second ? old : now], second ? ek_last : ekt, ev_last);
       ek_last = ekt, ev_last = evt, old = now, now = coming;
-      tell(t + 2);
+      if (t + 2 < count) tell(kv, t + 2);
     }
     if constexpr (second) {
       float mark = 0.f;

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile
   const Places<T> at(lane);
 
   Share<T, NT> kv;
-  // Tiles past the last are the last once more, which nobody reads: no branches around loads.
+  // Loads past the last tile are of the last once more and go unused: no branches around loads.
   auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
   auto fetch = [&](int t) {
     kv.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim);
@@ -65,12 +65,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile
   bool odd = false;  // an infinity among the rows or the tiles, whose powers of two then say nothing
   {
     const float* Q = a.q + ((int64_t)b * a.rows + (live ? i : 0)) * a.ldq + (int64_t)h * a.dim;
-    float x[T::KS][8], m = 0.f;
-#pragma unroll
-    for (int s = 0; s < T::KS; ++s) {
-      load8(Q, 2 * s + half, a.dim, live, x[s]);
-      m = fmaxf(m, top8(x[s]));
-    }
+    float x[T::KS][8], m = load_row<T::KS>(Q, half, a.dim, live, x);
     m = fmaxf(m, other_half(m));
     odd = !(m < INFINITY);
     const int ex = exponent(m);
@@ -169,13 +164,13 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile
   for (int t = 0; t < count; ++t) {
     __syncthreads();  // tile t lies in its buffer, nobody reads the other, tile t + 1's tops are known
     const int ekt = ek, evt = ev_next;
-    put(t + 1);
+    if (t + 1 < count) put(t + 1);
     fetch(t + 2);
     if (some(t)) {
       weights(t, ekt);
       values(t, evt);
     }
-    tell(t + 2);
+    if (t + 2 < count) tell(t + 2);
   }
   l += other_half(l);
   if constexpr (KW == 2) {

@@ -146,28 +146,6 @@ __device__ __forceinline__ Frag frag_col(const char* t, const Places<T>& p, int 
   return f;
 }
 
-// Eight columns from 8 u of a row, zeros past `dim` and of a row that is not there.
-__device__ __forceinline__ void load8(const float* __restrict__ row, int u, int dim, bool there, float (&x)[8]) {
-  const int n = there ? dim - 8 * u : 0;
-  const float* p = row + 8 * u;
-  if (n >= 8) {
-    const f32x4u a = reinterpret_cast<const f32x4u*>(p)[0], b = reinterpret_cast<const f32x4u*>(p)[1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[j] = a[j];
-      x[4 + j] = b[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (n > 0) {
-#pragma unroll
-      for (int j = 0; j < 7; ++j)
-        if (j < n) x[j] = p[j];
-    }
-  }
-}
-
 __device__ __forceinline__ float top8(const float (&x)[8]) {
   float m = 0.f;
 #pragma unroll
@@ -199,6 +177,45 @@ __device__ __forceinline__ int exponent(float m) {
 }
 // The power of two that brings values of this exponent to [2^kTop, 2^(kTop + 1)).
 __device__ __forceinline__ float scale(int e) { return __builtin_bit_cast(float, (unsigned)(kTop - e + 127) << 23); }
+
+// Eight values read as four from column col and four from col + 4 of n that are there (by now
+// or never), where four that reach past the end were read as the last four.
+__device__ __forceinline__ void cut8(float (&x)[8], int n, int cut) {
+#pragma unroll
+  for (int k = 0; k < 8; k += 4) {
+    const float v[4] = {x[k], x[k + 1], x[k + 2], x[k + 3]};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float late = cut == 3 ? v[min(j + 1, 3)] : cut == 2 ? v[min(j + 2, 3)] : v[3];
+      x[k + j] = n - k >= 4 ? v[j] : j < n - k ? late : 0.f;
+    }
+  }
+}
+
+// A row of a wave's own operand (dim >= 4; zeros of one that is not there, p being one that
+// is), columns 16 s + 8 half .. of step s; the largest magnitude.  All loads before any use.
+template <int KS>
+__device__ __forceinline__ float load_row(const float* __restrict__ p, int half, int dim, bool there, float (&x)[KS][8]) {
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int c = 16 * s + 8 * half;
+    const f32x4u v0 = *reinterpret_cast<const f32x4u*>(p + min(c, dim - 4)),
+                 v1 = *reinterpret_cast<const f32x4u*>(p + min(c + 4, dim - 4));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[s][j] = v0[j];
+      x[s][4 + j] = v1[j];
+    }
+  }
+  if (dim < 16 * KS || !__all(there)) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) cut8(x[s], there ? dim - 16 * s - 8 * half : 0, dim & 3);
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) m = fmaxf(m, top8(x[s]));
+  return m;
+}
 
 // An operand's exponent from a tile on whose largest magnitude is `top`, the sums being at the
 // largest exponent so far.  A tile far below that would lose bits that rows need which no
@@ -252,20 +269,8 @@ struct Share {
   // last four.
   __device__ __forceinline__ void clear(int r0, int end, int dim) {
     if (r0 + T::R <= end && dim == T::DP) return;
-    const int cut = dim & 3;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-#pragma unroll
-      for (int k = 0; k < 8; k += 4) {
-        const int n = r0 + row(c) < end ? dim - col(c) - k : 0;
-        const float v[4] = {x[c][k], x[c][k + 1], x[c][k + 2], x[c][k + 3]};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float late = cut == 3 ? v[min(j + 1, 3)] : cut == 2 ? v[min(j + 2, 3)] : v[3];
-          x[c][k + j] = n >= 4 ? v[j] : j < n ? late : 0.f;
-        }
-      }
-    }
+    for (int c = 0; c < N; ++c) cut8(x[c], r0 + row(c) < end ? dim - col(c) : 0, dim & 3);
   }
   // The largest magnitude of the first (second) tensor's chunks.
   __device__ __forceinline__ float top(bool of_second) const {
