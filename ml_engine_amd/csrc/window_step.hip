@@ -204,13 +204,14 @@ __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(Args a, StepWo
   }
 }
 
-// Joins the splits of a row, in order: a wave to a row.
+// Joins the splits of a row: a quarter of them to each of four waves, eight at a time (one after
+// the other, 64 splits were 36 us of 88 at 32 heads over 32768 keys), then the quarters in order.
 __global__ __launch_bounds__(256) void step_join_kernel(Args a, StepWork wk, int64_t first) {
-  const int64_t id = first + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, all_rows = a.group * a.rows;
+  __shared__ float quarter[4][kMaxDim];
+  const int64_t id = first + blockIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, all_rows = a.group * a.rows;
   const int64_t group = id / all_rows;
   const int g = (int)(id - group * all_rows);
-  if (group >= (int64_t)a.batch * a.kv_heads) return;
   const int b = (int)(group / a.kv_heads), h = (int)(group % a.kv_heads) * a.group + g / a.rows, tok = g % a.rows;
   const Seq seq(a, b);
   const int pos = seq.first + tok, n = part_size(a);
@@ -223,24 +224,43 @@ __global__ __launch_bounds__(256) void step_join_kernel(Args a, StepWork wk, int
     m = p[lane * stride + a.dim];
     l = p[lane * stride + a.dim + 1];
   }
+  const int per = (wk.splits + 3) / 4, s0 = w * per, s1 = min(s0 + per, wk.splits);
+  const int d0 = min(lane, a.dim - 1), d1 = min(lane + 64, a.dim - 1);
   const float f = __builtin_amdgcn_exp2f(m - wave_max(m));
   l = wave_sum(l * f);
-  float* out = a.out + ((int64_t)b * a.rows + tok) * a.ldo + (int64_t)h * a.dim;
   float x[2] = {0.f, 0.f};
-  for (int s = 0; s < wk.splits; ++s) {
-    const float fs = __shfl(f, s, 64);
+  for (int s = s0; s < s1; s += 8) {
+    float v[8][2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (lane + 64 * k < a.dim) x[k] = fmaf(fs, p[s * stride + lane + 64 * k], x[k]);
+    for (int k = 0; k < 8; ++k) {
+      const float* r = p + min(s + k, s1 - 1) * stride;
+      v[k][0] = r[d0];
+      v[k][1] = r[d1];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool is = s + k < s1;
+      const float fs = __shfl(f, is ? s + k : 0, 64);
+      x[0] = is ? fmaf(fs, v[k][0], x[0]) : x[0];
+      x[1] = is ? fmaf(fs, v[k][1], x[1]) : x[1];
+    }
   }
-  bool bad = false;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (lane + 64 * k < a.dim) {
-      x[k] = there ? x[k] / l : 0.f;
-      bad |= !(fabsf(x[k]) < INFINITY);
-      out[lane + 64 * k] = x[k];
+    if (lane + 64 * k < a.dim) quarter[w][lane + 64 * k] = x[k];
+  __syncthreads();
+  if (w != 0) return;
+  float* out = a.out + ((int64_t)b * a.rows + tok) * a.ldo + (int64_t)h * a.dim;
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int d = lane + 64 * k;
+    if (d < a.dim) {
+      const float y = there ? (quarter[0][d] + quarter[1][d] + quarter[2][d] + quarter[3][d]) / l : 0.f;
+      bad |= !(fabsf(y) < INFINITY);
+      out[d] = y;
     }
+  }
   if (a.rows > 1 && __any(bad)) plain_row(a, b, h, tok);
 }
 
@@ -258,8 +278,8 @@ void step_forward(const Args& a, const StepWork& wk, hipStream_t s) {
   }
   if (wk.splits == 1) return;
   const int64_t rows = (int64_t)a.batch * a.heads * a.rows;
-  for (int64_t f = 0; f < rows; f += 4 * kBlocks)
-    mle::launch(step_join_kernel, (unsigned)((std::min(rows - f, 4 * kBlocks) + 3) / 4), 256, 0, s, a, wk, f);
+  for (int64_t f = 0; f < rows; f += kBlocks)
+    mle::launch(step_join_kernel, (unsigned)std::min(rows - f, kBlocks), 256, 0, s, a, wk, f);
 }
 
 }  // namespace wattn
