@@ -169,6 +169,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
   // this key's P is held at 2^sj (times its row's power of two), its dS at 2^(sj + tj)
   float sj = 100.f;
   int tj = 100;
+  const unsigned most = !live ? 0u : j < a.sinks ? 0x7fffffffu : (unsigned)a.window;  // how far its rows go
   tell(in0, 0, first_row);
   tell(in, 1, ahead.r0);
   ahead.next();
@@ -215,12 +216,10 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[r] = fmaf(s[r], ct, -lse[r >> 2][r & 3]);
-        if (!all) {
-          const int i = i0 + 8 * (r >> 2) + 4 * half + (r & 3);
-          s[r] = (live & sees(a, i, j)) ? s[r] : -INFINITY;
-        }
-        mx = fmaxf(mx, s[r]);
       }
+      if (!all) hide_rows(s, i0 + 4 * half - j, most);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
       mx = fmaxf(mx, other_half(mx));
       if (__any(mx + sj > 15.f)) {
         const float to = mx + sj > 15.f ? floorf(8.f - mx) : sj;
@@ -392,13 +391,11 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
       const bool all = jb + 31 <= row0 && (wlast - jb < a.window || jb + 31 < a.sinks) && row0 + 32 <= seq.len;
       float mx = 0.f;
 #pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], ct, -lse);
+      if (!all) hide_keys(s, live ? i - jb - 4 * half : -1, a.window, a.sinks - jb - 4 * half, jb < a.sinks);
+#pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float p = fmaf(s[r], ct, -lse);
-        if (!all) {
-          const int j = jb + 8 * (r >> 2) + 4 * half + (r & 3);
-          p = (live & sees(a, i, j)) ? p : -INFINITY;
-        }
-        x[r] = __builtin_amdgcn_exp2f(p) * fmaf(x[r], cd, -dd);
+        x[r] = __builtin_amdgcn_exp2f(s[r]) * fmaf(x[r], cd, -dd);
         mx = fmaxf(mx, fabsf(x[r]));
       }
       rescale(mx, ti, dq);

@@ -126,6 +126,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
     // this key's P is held at 2^sj (times its row's power of two), its dS at 2^(sj + tj)
     float sj = 100.f;
     int tj = 100, eq = kNone;
+    const unsigned most = !live ? 0u : j < a.sinks ? 0x7fffffffu : (unsigned)a.window;  // how far its rows go
     // Tile t in buf, Q's exponent there being e.
     const auto block = [&](int t, const char (*buf)[T::BYTES], int e) {
       const Rows<R>& rw = m.rows[t & 3];
@@ -155,10 +156,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[4 * q + r] = fmaf(x[4 * q + r], ct, -lse[r]);
         }
-        if (!all) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = (live & sees(a, i0 + 8 * (r >> 2) + 4 * half + (r & 3), j)) ? x[r] : -INFINITY;
-        }
+        if (!all) hide_rows(x, i0 + 4 * half - j, most);
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[r]);
         if (__any(mx + sj > 15.f)) {
@@ -349,10 +347,7 @@ __device__ __forceinline__ void q_pairs(const Args& a, const Block& blk, Shared<
         const bool all = j0 + 31 <= row0 && (wlast - j0 < a.window || j0 + 31 < a.sinks) && row0 + 32 <= seq.len;
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], ct, -lse);
-        if (!all) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = (live & sees(a, i, j0 + 8 * (r >> 2) + 4 * half + (r & 3))) ? x[r] : -INFINITY;
-        }
+        if (!all) hide_keys(x, live ? i - j0 - 4 * half : -1, a.window, a.sinks - j0 - 4 * half, j0 < a.sinks);
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r]);
         h.put(lane, x, 0.f);

@@ -333,6 +333,24 @@ __device__ __forceinline__ void steps(Load load, Use use) {
   }
 }
 
+// A block's scores set to minus infinity where a row does not see a key, one unsigned comparison
+// for both ends of the window.  Rows in lanes: `base` is the row's position less the block's first
+// key and 4 (lane / 32) (negative: not there); `sinks` those from that key on, of use if `some`.
+__device__ __forceinline__ void hide_keys(f32x16& x, int base, int window, int sinks, bool some) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int c = 8 * (r >> 2) + (r & 3);
+    const unsigned most = some && c < sinks ? 0x7fffffffu : (unsigned)window;
+    x[r] = (unsigned)(base - c) < most ? x[r] : -INFINITY;
+  }
+}
+// Keys in lanes: `base` is the block's first row and 4 (lane / 32) less the key's position, `most`
+// how far from a row on it is seen (0: not there).
+__device__ __forceinline__ void hide_rows(f32x16& x, int base, unsigned most) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = (unsigned)(base + 8 * (r >> 2) + (r & 3)) < most ? x[r] : -INFINITY;
+}
+
 // The tiles of R keys that rows at positions first .. last (0 <= first <= last) see: sinks before
 // the window, then the window.
 template <int R>
