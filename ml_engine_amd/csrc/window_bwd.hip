@@ -220,8 +220,8 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
       if (!all) hide_rows(s, i0 + 4 * half - j, most);
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
-      mx = fmaxf(mx, other_half(mx));
       if (__any(mx + sj > 15.f)) {
+        mx = fmaxf(mx, other_half(mx));
         const float to = mx + sj > 15.f ? floorf(8.f - mx) : sj;
         const int by = (int)(to - sj);
 #pragma unroll

@@ -14,10 +14,9 @@ constexpr int kUnit = -10;  // dP and D of a row are taken times 2^(kUnit - expo
 // half, would reach 2^15, t is lowered to bring it to 2^8 .. 2^9, and the sums follow.
 template <int N>
 __device__ __forceinline__ void rescale(float mx, int& t, f32x16 (&sums)[N]) {
-  mx = fmaxf(mx, other_half(mx));
-  const int e = exponent(mx);
+  if (!__any(exponent(mx) + t > 14 || t > 120)) return;
+  const int e = exponent(fmaxf(mx, other_half(mx)));
   const bool over = e + t > 14 || t > 120;
-  if (!__any(over)) return;
   const int to = over ? min(8 - e, 120) : t;
 #pragma unroll
   for (int d = 0; d < N; ++d)
