@@ -3,8 +3,8 @@
 //   prepare   D and the exponent of each row of dout
 //   kv        dk and dv of 32 keys to a wave, over the tiles of rows that see them
 //   q         dq of 32 rows to a wave, over the tiles of keys that they see
-//   join      sinks: the sums over rows past their own window, added in order
-// S and dP = dout v^T are computed again in both.
+//   join      the parts of sums over rows, added in order
+// S and dP = dout v^T are computed again in both; kv and q are one launch.
 //
 // Sinks are seen by every later row.  Blocks of keys with sinks take the rows up to their
 // window like all others ("near"); the rows after it ("far") are shared out over workgroups
@@ -15,6 +15,12 @@
 // own column, a lane's: a key's P and dS (kv), a row's dS (q) have the largest seen so far
 // between 2^8 and 2^15, and a larger one rescales the lane's sums.  Rows of dout are at powers
 // of two of their own too; P takes those up in its exponent.
+//
+// Here for heads of up to 64, a wave with 32 keys (rows) to itself: two workgroups of four waves
+// to a CU, out of step.  Tiles of 32 rows in the kv pass, whose staging then fits beside the
+// sums (64-row tiles spilled, and every reload waited for the loads under way: 555 us against
+// 523 at 4 x 8 heads of 4096, window 1024); 64 keys in the q pass (528 with 32).  That
+// case takes 495 us (fp32 products at 152 TFLOP/s), 32 x 8 heads of 256 under a window of 128 81 us.
 #include "window_bwd.hpp"
 
 using namespace mle;

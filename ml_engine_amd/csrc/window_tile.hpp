@@ -2,7 +2,7 @@
 // cores with fp32 accuracy.
 //
 // Products.  An fp32 value x, scaled by a power of two so that its tile's largest is in
-// [2^14, 2^15), is held as two fp16 parts, hi = fp16(x) and lo = fp16(x - hi): 22 bits of
+// [2^14, 2^15), is held as two fp16 parts, hi its first 11 bits and lo the next 11: 22 bits of
 // every value down to 2^-18 of the largest, and 2^-40 of the largest below (the matrix
 // cores keep fp16's subnormals).  A product is hi hi + hi lo + lo hi, three
 // v_mfma_f32_32x32x16_f16, where three bf16 parts (split_core.hpp) take six.
