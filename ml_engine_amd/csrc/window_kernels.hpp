@@ -35,11 +35,13 @@ struct BwdWork {
     near_rows = rows;
     if (blocks > 0 && blocks < 128) near_rows = (int)std::max<int64_t>(64, (rows * blocks / 128 + 63) / 64 * 64);
     nears = rows > 0 ? (rows + near_rows - 1) / near_rows : 1;
-    // short, so that they fill in behind the blocks of keys; longer where sinks are so many
-    // that their blocks alone fill the chip, and their parts the memory
+    // short, so that they fill in behind the blocks of keys, no longer than those' parts (18 heads
+    // of 777 x 80, us: 92 with twice as long ones, 86 so); longer where sinks are so many that
+    // their blocks alone fill the chip, and their parts the memory
     const int after = std::max(a.rows - rows, 0);
     const int64_t sets = (int64_t)a.batch * a.kv_heads * sink_blocks, most = std::max<int64_t>(1, 2048 / std::max<int64_t>(sets, 1));
-    far_rows = (int)std::max<int64_t>({256, a.window / 4, (after + most - 1) / most});
+    far_rows = nears > 1 ? near_rows : std::max(256, a.window / 4);
+    far_rows = (int)std::max<int64_t>(far_rows, (after + most - 1) / most);
     far_rows = (far_rows + 63) / 64 * 64;
     fars = sink_blocks > 0 && after > 0 ? (after + far_rows - 1) / far_rows : 0;
   }
@@ -101,11 +103,12 @@ struct Place {
 // Workgroups: sequence, head, block of rows.  The blocks of one sequence and group of heads
 // read the same keys and values: where the groups fill the 8 XCDs evenly, each XCD (a
 // workgroup's number modulo 8) takes whole groups, so that its L2 holds them.  The last rows,
-// which see the most, come first.  (A kernel may number a group's items by itself: Place.)
+// which see the most, come first; in a grid of a round or two those of all groups do, and its
+// last workgroups are short (18 heads of 777 x 80, backward: 86 -> 65 us).  (A kernel may number a group's items by itself: Place.)
 struct Grid {
   int64_t first, total;
   int groups, per_group, per_head, blocks;  // per_head: heads of a group; blocks: of rows
-  int xcd;
+  int xcd, by_item;
   Grid(const Args& a, int heads, int blocks_) : first(0) {
     groups = a.batch * a.kv_heads;
     per_head = heads / a.kv_heads;
@@ -113,6 +116,7 @@ struct Grid {
     per_group = per_head * blocks;
     total = (int64_t)groups * per_group;
     xcd = groups % 8 == 0;
+    by_item = !xcd && total <= 512;
   }
   __device__ __forceinline__ Place place(int64_t id) const {
     Place p;
@@ -120,6 +124,9 @@ struct Grid {
       const int64_t k = id >> 3;
       p.group = (k / per_group) * 8 + (id & 7);
       p.item = (int)(k % per_group);
+    } else if (by_item) {
+      p.group = id % groups;
+      p.item = (int)(id / groups);
     } else {
       p.group = id / per_group;
       p.item = (int)(id - p.group * per_group);
