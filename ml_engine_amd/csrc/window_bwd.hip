@@ -486,8 +486,8 @@ void tile_backward(const Args& a, const BwdWork& wk, hipStream_t s) {
     mle::launch(prepare_kernel, (unsigned)std::min(tiles - f, kBlocks), 256, 0, s, a, wk, f);
   if (a.dim <= 64) {
     constexpr int NW = kKeyBlock / 32;
-    launch_both(narrow_kernel<64, NW>, Grid(a, a.kv_heads, wk.kv_items()), Grid(a, a.heads, (a.rows + 32 * NW - 1) / (32 * NW)),
-                64 * NW, s, a, wk);
+    launch_both(narrow_kernel<64, NW>, Grid(a, a.kv_heads, wk.kv_items(), 1024),
+                Grid(a, a.heads, (a.rows + 32 * NW - 1) / (32 * NW), 1024), 64 * NW, s, a, wk);
   } else {
     launch_wide(a, wk, s);
   }

@@ -429,7 +429,7 @@ __global__ __launch_bounds__(128 * NP, 2) void wide_kernel(Args a, BwdWork wk, G
 
 void launch_wide(const Args& a, const BwdWork& wk, hipStream_t s) {
   constexpr int NP = kKeyBlock / 32;
-  const Grid kv(a, a.kv_heads, wk.kv_items()), q(a, a.heads, (a.rows + 32 * NP - 1) / (32 * NP));
+  const Grid kv(a, a.kv_heads, wk.kv_items(), 1024), q(a, a.heads, (a.rows + 32 * NP - 1) / (32 * NP), 1024);
   if (a.dim <= 96)
     launch_both(wide_kernel<96, NP>, kv, q, 128 * NP, s, a, wk);
   else

@@ -246,13 +246,13 @@ void launch_dim(const Args& a, hipStream_t s) {
   // 1024 x 64, all keys: 40 against 46).
   const auto blocks = [&](int rows) { return (int64_t)a.batch * a.heads * ((a.rows + rows - 1) / rows); };
   if (a.window >= 512 && blocks(256) >= 256)
-    launch_blocks(tile_fwd_kernel<DP, 8, 1>, Grid(a, a.heads, (a.rows + 255) / 256), 512, s, a);
+    launch_blocks(tile_fwd_kernel<DP, 8, 1>, Grid(a, a.heads, (a.rows + 255) / 256, 8), 512, s, a);
   else if (blocks(64) <= 256 && blocks(64) > blocks(128))
-    launch_blocks(tile_fwd_kernel<DP, 4, 2>, Grid(a, a.heads, (a.rows + 63) / 64), 256, s, a);
+    launch_blocks(tile_fwd_kernel<DP, 4, 2>, Grid(a, a.heads, (a.rows + 63) / 64, 8), 256, s, a);
   else if (blocks(128) <= 256)
-    launch_blocks(tile_fwd_kernel<DP, 8, 2>, Grid(a, a.heads, (a.rows + 127) / 128), 512, s, a);
+    launch_blocks(tile_fwd_kernel<DP, 8, 2>, Grid(a, a.heads, (a.rows + 127) / 128, 8), 512, s, a);
   else
-    launch_blocks(tile_fwd_kernel<DP, 4, 1>, Grid(a, a.heads, (a.rows + 127) / 128), 256, s, a);
+    launch_blocks(tile_fwd_kernel<DP, 4, 1>, Grid(a, a.heads, (a.rows + 127) / 128, 8), 256, s, a);
 }
 
 }  // namespace

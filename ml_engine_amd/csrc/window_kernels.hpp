@@ -103,27 +103,32 @@ struct Place {
 // Workgroups: sequence, head, block of rows.  The blocks of one sequence and group of heads
 // read the same keys and values: where the groups fill the 8 XCDs evenly, each XCD (a
 // workgroup's number modulo 8) takes whole groups, so that its L2 holds them.  The last rows,
-// which see the most, come first; in a grid of a round or two those of all groups do, and its
-// last workgroups are short (18 heads of 777 x 80, backward: 86 -> 65 us).  (A kernel may number a group's items by itself: Place.)
+// which see the most, come first.  In a grid of a round or two (by_item) those of all groups do:
+// its last workgroups are short (18 heads of 777 x 80, backward: 86 -> 65 us), and long and
+// short ones share the CUs, where in turn they would each have their own (32 x 8 heads of 256
+// x 64: 28.5 + 81 -> 25 + 74 us).  With more than `mixed` of them to a group they mix anyway: 4 x 8
+// heads of 4096 x 64, 16 to a group forward, 161 us so against 170; backward 483 against 473.
+// (A kernel may number a group's items by itself: Place.)
 struct Grid {
   int64_t first, total;
   int groups, per_group, per_head, blocks;  // per_head: heads of a group; blocks: of rows
   int xcd, by_item;
-  Grid(const Args& a, int heads, int blocks_) : first(0) {
+  Grid(const Args& a, int heads, int blocks_, int mixed) : first(0) {
     groups = a.batch * a.kv_heads;
     per_head = heads / a.kv_heads;
     blocks = blocks_;
     per_group = per_head * blocks;
     total = (int64_t)groups * per_group;
     xcd = groups % 8 == 0;
-    by_item = !xcd && total <= 512;
+    by_item = xcd ? total <= 1024 && per_group <= mixed : total <= 512;
   }
   __device__ __forceinline__ Place place(int64_t id) const {
     Place p;
     if (xcd) {
       const int64_t k = id >> 3;
-      p.group = (k / per_group) * 8 + (id & 7);
-      p.item = (int)(k % per_group);
+      const int n = by_item ? groups >> 3 : per_group, hi = (int)(k / n), lo = (int)(k % n);
+      p.group = (int64_t)(by_item ? lo : hi) * 8 + (id & 7);
+      p.item = by_item ? hi : lo;
     } else if (by_item) {
       p.group = id % groups;
       p.item = (int)(id / groups);
