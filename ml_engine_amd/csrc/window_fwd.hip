@@ -10,7 +10,7 @@
 // Bound by vector instructions beside the products: splitting operands, masks, exponentials.
 // 2 x 16 heads of 4096 x 128 under a window of 1024 take 261-285 us (fp32 products at 215
 // TFLOP/s, matrix cores 33 % busy, vector units 41 %), 32 x 8 heads of 256 x 64 under one
-// of 128 28 us, where a workgroup's two to four tiles leave both idle most of the time.
+// of 128 25 us, where a workgroup's two to four tiles leave both idle most of the time.
 #include "window_tile.hpp"
 #include "window_kernels.hpp"
 
