@@ -24,7 +24,7 @@ def norm64(h):
 
 SHAPES = [(1, 1), (1, 32), (3, 31), (5, 33), (64, 256), (7, 330), (130, 512), (9, 1000), (33, 1024), (6, 1500), (40, 2048),
           (3, 2052), (5, 4096), (2, 6001), (3, 8192), (2, 8200), (3, 20001), (1500, 64), (4, 7), (6, 37), (5, 2049), (2, 8191),
-          (2500, 3)]
+          (2500, 3), (255, 100), (256, 2048), (257, 40)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)
@@ -116,7 +116,7 @@ def test_optional_outputs(hip):
     assert (outs[1][2] == 0).all() and (outs[2][1] == 0).all()
 
 
-@pytest.mark.parametrize("rows,cols", [(12, 300), (6, 4000), (4, 9000)])
+@pytest.mark.parametrize("rows,cols", [(12, 300), (6, 4000), (4, 9000), (250, 700)])
 def test_in_place(hip, rows, cols):
     """h over x, and dh over dy, give what buffers of their own give."""
     r = rng(4)
