@@ -180,30 +180,32 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile
   l += other_half(l);
   if constexpr (KW == 2) {
     // the second wave's sums to the first, both at the larger maximum and power of two
-    static_assert(NW / 2 * 64 * (16 * T::DB + 3) * sizeof(float) <= sizeof(lds), "room for a wave's sums");
-    float* at_lane = reinterpret_cast<float*>(lds) + (w / 2) * 64 * (16 * T::DB + 3) + lane;
+    static_assert(NW / 2 * 64 * (4 * T::DB + 1) * sizeof(f32x4) <= sizeof(lds), "room for a wave's sums");
+    f32x4* at_lane = reinterpret_cast<f32x4*>(lds) + (w / 2) * 64 * (4 * T::DB + 1) + lane;
     __syncthreads();  // the tiles have been read
     if (kw == 1) {
 #pragma unroll
       for (int d = 0; d < T::DB; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) at_lane[64 * (16 * d + r)] = o[d][r];
-      at_lane[64 * 16 * T::DB] = m;
-      at_lane[64 * (16 * T::DB + 1)] = l;
-      at_lane[64 * (16 * T::DB + 2)] = (float)ev;
+        for (int r = 0; r < 16; r += 4) at_lane[64 * (4 * d + r / 4)] = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+      at_lane[64 * 4 * T::DB] = f32x4{m, l, (float)ev, 0.f};
     }
     __syncthreads();
     if (kw == 1) return;
-    const float m1 = at_lane[64 * 16 * T::DB], l1 = at_lane[64 * (16 * T::DB + 1)], mj = fmaxf(m, m1);
-    const int ev1 = (int)at_lane[64 * (16 * T::DB + 2)], evj = max(ev, ev1);
+    const f32x4 other = at_lane[64 * 4 * T::DB];
+    const float m1 = other[0], l1 = other[1], mj = fmaxf(m, m1);
+    const int ev1 = (int)other[2], evj = max(ev, ev1);
     const float f0 = __builtin_amdgcn_exp2f(m - mj), f1 = __builtin_amdgcn_exp2f(m1 - mj);
     l = fmaf(l, f0, l1 * f1);
 #pragma unroll
     for (int d = 0; d < T::DB; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        o[d][r] = fmaf(__builtin_amdgcn_ldexpf(o[d][r], ev - evj), f0,
-                       __builtin_amdgcn_ldexpf(at_lane[64 * (16 * d + r)], ev1 - evj) * f1);
+      for (int r = 0; r < 16; r += 4) {
+        const f32x4 x = at_lane[64 * (4 * d + r / 4)];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          o[d][r + n] = fmaf(__builtin_amdgcn_ldexpf(o[d][r + n], ev - evj), f0, __builtin_amdgcn_ldexpf(x[n], ev1 - evj) * f1);
+      }
     m = mj, ev = evj;
   }
   float mark = l;  // not finite where a score or a sum is not

@@ -180,7 +180,14 @@ __device__ __forceinline__ float scale(int e) { return __builtin_bit_cast(float,
 
 // Eight values read as four from column col and four from col + 4 of n that are there (by now
 // or never), where four that reach past the end were read as the last four.
+// (FOURS: a way of its own for whole fours, which the widest kernels have no registers for.)
+template <bool FOURS>
 __device__ __forceinline__ void cut8(float (&x)[8], int n, int cut) {
+  if (FOURS && cut == 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = n > j ? x[j] : 0.f;
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < 8; k += 4) {
     const float v[4] = {x[k], x[k + 1], x[k + 2], x[k + 3]};
@@ -209,7 +216,7 @@ __device__ __forceinline__ float load_row(const float* __restrict__ p, int half,
   }
   if (dim < 16 * KS || !__all(there)) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) cut8(x[s], there ? dim - 16 * s - 8 * half : 0, dim & 3);
+    for (int s = 0; s < KS; ++s) cut8<(KS < 8)>(x[s], there ? dim - 16 * s - 8 * half : 0, dim & 3);
   }
   float m = 0.f;
 #pragma unroll
@@ -270,7 +277,7 @@ struct Share {
   __device__ __forceinline__ void clear(int r0, int end, int dim) {
     if (r0 + T::R <= end && dim == T::DP) return;
 #pragma unroll
-    for (int c = 0; c < N; ++c) cut8(x[c], r0 + row(c) < end ? dim - col(c) : 0, dim & 3);
+    for (int c = 0; c < N; ++c) cut8<(T::DP < 128)>(x[c], r0 + row(c) < end ? dim - col(c) : 0, dim & 3);
   }
   // The largest magnitude of the first (second) tensor's chunks.
   __device__ __forceinline__ float top(bool of_second) const {
