@@ -243,8 +243,8 @@ template <int DP>
 void launch_dim(const Args& a, hipStream_t s) {
   // 8 waves share a tile, 4 where the window is small: a workgroup walks over window + rows
   // keys, of which a wave computes window + 32.  Where that leaves CUs idle two waves share 32 rows'
-  // keys: 64 rows to a workgroup (6 heads of 777 x 80, window 200: 33 us against 40, 4 of 2048 x 64:
-  // 26 against 34), or 128 where 64 would be no more workgroups or too many (32 heads of
+  // keys: 64 rows to a workgroup (6 heads of 777 x 80, window 200: 30 us against 40, 4 of 2048 x 64:
+  // 25 against 34), or 128 where 64 would be no more workgroups or too many (32 heads of
   // 1024 x 64, all keys: 40 against 46).
   const auto blocks = [&](int rows) { return (int64_t)a.batch * a.heads * ((a.rows + rows - 1) / rows); };
   if (a.window >= 512 && blocks(256) >= 256)
