@@ -25,6 +25,14 @@ int check(const char* who, int batch, int rows, int keys, int heads, int kv_head
   return MLE_OK;
 }
 
+// Are these sizes that check() passes?  (The workspace queries answer 0 for others, and compute
+// with none of them.)
+bool takes(int batch, int rows, int keys, int heads, int kv_heads, int dim) {
+  return batch > 0 && batch <= (1 << 24) && rows > 0 && rows <= (1 << 30) && keys > 0 && keys <= (1 << 30) && heads > 0 &&
+         heads <= (1 << 16) && kv_heads > 0 && heads % kv_heads == 0 && dim > 0 && dim <= kMaxDim &&
+         (double)batch * heads * std::max(rows, keys) <= 1e12;
+}
+
 int check_ld(const char* who, const char* name, int64_t ld, int heads, int dim) {
   MLE_CHECK_ARG(ld >= (int64_t)heads * dim && ld <= ((int64_t)1 << 32), "%s: %s %lld for %d heads of %d", who, name,
                 (long long)ld, heads, dim);
@@ -70,7 +78,7 @@ int mle_window_attention_fwd(mle_stream stream, const float* q, int64_t ldq, con
 }
 
 size_t mle_window_attention_ws_bytes(int batch, int seq, int heads, int kv_heads, int head_dim, int window, int sinks) {
-  if (batch <= 0 || seq <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  if (!takes(batch, seq, seq, heads, kv_heads, head_dim)) return 0;
   Args a = make_args(nullptr, 0, nullptr, 0, nullptr, 0, 0, nullptr, batch, seq, seq, heads, kv_heads, head_dim, 1.f,
                      std::max(window, 1), std::max(sinks, 0));
   return BwdWork(a).place(a, nullptr);
@@ -111,7 +119,7 @@ int mle_window_attention_bwd(mle_stream stream, const float* q, int64_t ldq, con
 
 size_t mle_window_attention_step_ws_bytes(int batch, int tokens, int capacity, int heads, int kv_heads, int head_dim,
                                           int window, int sinks) {
-  if (batch <= 0 || tokens <= 0 || capacity <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0) return 0;
+  if (!takes(batch, tokens, capacity, heads, kv_heads, head_dim)) return 0;
   const Args a = make_args(nullptr, 0, nullptr, 0, nullptr, 0, 0, nullptr, batch, tokens, capacity, heads, kv_heads, head_dim,
                            1.f, std::max(window, 1), std::max(sinks, 0));
   return StepWork::few(tokens) ? StepWork(a).bytes(a) : 0;

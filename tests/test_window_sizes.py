@@ -1,0 +1,39 @@
+"""Sizes of the windowed attention that need no GPU: what the workspace queries take, and the
+host's arithmetic on the largest grids."""
+import subprocess
+import sys
+
+import pytest
+
+from ml_engine_amd import hip
+
+MOST = 2 ** 31 - 1
+ROOT = hip.LIB_DIR.parent.parent
+
+
+def query(name, *args):
+    """A query in a process of its own, which an arithmetic trap would end."""
+    code = f"import sys; sys.path.insert(0, {str(ROOT)!r}); from ml_engine_amd import hip; print(hip.lib().{name}{args})"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, (name, args, r.returncode, r.stderr[-300:])
+    return int(r.stdout)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("mle_window_attention_step_ws_bytes", (1, 1, 1000, 2, 4, 64, 500, 0)),        # fewer heads than heads of keys
+    ("mle_window_attention_step_ws_bytes", (1, 1, 1000, 6, 4, 64, 500, 0)),        # no whole groups
+    ("mle_window_attention_step_ws_bytes", (1, 31, 1000, MOST, 1, 64, 500, 0)),
+    ("mle_window_attention_step_ws_bytes", (MOST, 31, MOST, 1 << 16, 1, MOST, MOST, MOST)),
+    ("mle_window_attention_ws_bytes", (1, 300, 2, 4, 64, 500, 0)),
+    ("mle_window_attention_ws_bytes", (1, MOST, 2, 2, 64, 500, 0)),
+    ("mle_window_attention_ws_bytes", (1, 300, 2, 2, 129, 500, 0)),
+    ("mle_window_attention_ws_bytes", (MOST, MOST, MOST, 1, MOST, 500, MOST)),
+])
+def test_queries_of_sizes_that_the_calls_refuse(name, args):
+    assert query(name, *args) == 0
+
+
+def test_queries_of_the_largest_sizes():
+    """The largest that the calls take: a number per row and head at least, and no overflow."""
+    assert query("mle_window_attention_ws_bytes", 1, 1 << 30, 8, 8, 128, MOST, MOST) >= 8 * (8 << 30)
+    assert query("mle_window_attention_step_ws_bytes", 1, 31, 1 << 30, 8, 1, 128, MOST, 0) > 0
