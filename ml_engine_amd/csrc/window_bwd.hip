@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(Args a, BwdWork wk, int64_
 template <int DP, int NW>
 struct Shared {
   alignas(16) char lds[2][2][Tile<DP, 64>::BYTES];  // [buffer][Q, dout or K, V]
-  alignas(16) Rows<32> rows[4];
+  Rows<32> rows[4];
   alignas(16) Tops<NW> tops;
   int ex[NW];
 };

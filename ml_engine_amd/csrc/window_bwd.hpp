@@ -54,9 +54,10 @@ __device__ __forceinline__ void store_plain(const Args& a, float* part, int b, i
   }
 }
 
-// A row's part in the kv pass, by row of a tile.
+// A row's part in the kv pass, by row of a tile.  (Read four rows at a time from arrays of these.)
 template <int R>
-struct Rows {
+struct alignas(16) Rows {
+  static_assert(R % 4 == 0, "delta on 16 bytes");
   float lse[R];    // its log-sum less its exponent (log2 units); infinity: not there
   float delta[R];  // D in the units of dP
   int ex[R];

@@ -37,7 +37,7 @@ template <int DP, int NP>
 struct Shared {
   alignas(16) char lds[3][2][Tile<DP, 32>::BYTES];  // [buffer][Q, dout or K, V]
   alignas(16) Handed hand[2][NP];
-  alignas(16) Rows<32> rows[4];
+  Rows<32> rows[4];
   alignas(16) Tops<2 * NP> tops;
   int ex[2 * NP];
 };

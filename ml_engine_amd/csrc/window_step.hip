@@ -44,7 +44,7 @@ __device__ __forceinline__ int part_size(const Args& a) { return a.dim + 2; }
 template <int DU, bool FULL>
 __global__ __launch_bounds__(64 * kStepWaves, 2) void step_kernel(Args a, StepWork wk, int64_t first) {
   constexpr int KT = 4 * DU, PAD = 64 * DU + 4;
-  __shared__ float sum_o[kStepWaves][kRows][PAD];
+  __shared__ __attribute__((aligned(16))) float sum_o[kStepWaves][kRows][PAD];
   __shared__ float sum_m[kStepWaves][kRows], sum_l[kStepWaves][kRows];
   const int64_t id = first + blockIdx.x;
   const int split = (int)(id % wk.splits);

@@ -5,7 +5,7 @@ import sys
 
 import pytest
 
-from ml_engine_amd import hip
+from ml_engine_amd import build, hip
 
 MOST = 2 ** 31 - 1
 ROOT = hip.LIB_DIR.parent.parent
@@ -37,3 +37,22 @@ def test_queries_of_the_largest_sizes():
     """The largest that the calls take: a number per row and head at least, and no overflow."""
     assert query("mle_window_attention_ws_bytes", 1, 1 << 30, 8, 8, 128, MOST, MOST) >= 8 * (8 << 30)
     assert query("mle_window_attention_step_ws_bytes", 1, 31, 1 << 30, 8, 1, 128, MOST, 0) > 0
+
+
+def host_program(tmp_path, body, *includes):
+    """What a program of the kernels' headers' host side prints."""
+    src = tmp_path / "sizes.hip"
+    src.write_text("".join(f'#include "{hip.LIB_DIR.parent / "csrc" / i}"\n' for i in includes)
+                   + "#include <stdio.h>\nint main() {\n" + body + "\n}\n")
+    exe = tmp_path / "sizes"
+    subprocess.run([build.HIPCC, "--cuda-host-only", "-x", "hip", "-std=c++17", "-O1", "-w", f"-I{build.INCLUDE}", str(src),
+                    "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    return [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout.split()]
+
+
+def test_rows_of_a_tile_lie_at_whole_vectors(tmp_path):
+    """The backward reads four rows' log-sums and Ds at once from an array of these."""
+    size, align, lse, delta = host_program(
+        tmp_path, 'typedef wattn::Rows<32> R; printf("%zu %zu %zu %zu", sizeof(R), alignof(R), offsetof(R, lse), offsetof(R, delta));',
+        "window_bwd.hpp")
+    assert align >= 16 and size % 16 == 0 and lse % 16 == 0 and delta % 16 == 0
