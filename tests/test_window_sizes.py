@@ -56,3 +56,26 @@ def test_rows_of_a_tile_lie_at_whole_vectors(tmp_path):
         tmp_path, 'typedef wattn::Rows<32> R; printf("%zu %zu %zu %zu", sizeof(R), alignof(R), offsetof(R, lse), offsetof(R, delta));',
         "window_bwd.hpp")
     assert align >= 16 and size % 16 == 0 and lse % 16 == 0 and delta % 16 == 0
+
+
+def test_grids_of_more_than_32_bits(tmp_path):
+    """One-token sequences of many narrow heads: more groups than an int holds."""
+    got = host_program(tmp_path, """
+  wattn::Args a{};
+  a.batch = 1 << 24, a.kv_heads = 1 << 8, a.heads = 1 << 8, a.group = 1, a.rows = a.keys = 1, a.dim = 1, a.window = 1;
+  wattn::Grid g(a, a.heads, 1, 8);
+  printf("%lld %lld ", (long long)g.groups, (long long)g.total);
+  const int64_t ids[] = {0, 7, 8, (1ll << 32) - 1, (1ll << 31) + 5};
+  for (int64_t id : ids) {
+    const wattn::Place p = g.place(id);
+    printf("%lld %d ", (long long)p.group, p.item);
+  }
+  a.batch = (1 << 24) - 1, a.kv_heads = a.heads = 255;
+  wattn::Grid odd(a, a.heads, 3, 8);
+  const wattn::Place p = odd.place(odd.total - 1);
+  printf("%lld %lld %d", (long long)odd.groups, (long long)p.group, p.item);
+""", "window_kernels.hpp")
+    assert got[:2] == [1 << 32, 1 << 32]
+    assert got[2:12] == [x for i in (0, 7, 8, (1 << 32) - 1, (1 << 31) + 5) for x in (i, 0)]
+    n = ((1 << 24) - 1) * 255
+    assert got[12:] == [n, n - 1, 2]
