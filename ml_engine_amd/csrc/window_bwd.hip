@@ -138,7 +138,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
     odd |= !(top < INFINITY);
     ek = exponent(fmaxf(top, other_half(top)));
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) kf[s] = split8(x[s], scale(ek));
+    for (int s = 0; s < T::KS; ++s) kf[s] = split8<false>(x[s], scale(ek));
   }
   {
     float x[T::KS][8];
@@ -146,7 +146,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
     odd |= !(top < INFINITY);
     ev = exponent(fmaxf(top, other_half(top)));
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) vf[s] = split8(x[s], scale(ev));
+    for (int s = 0; s < T::KS; ++s) vf[s] = split8<false>(x[s], scale(ev));
   }
   const float cd = __builtin_amdgcn_ldexpf(1.f, ev + kUnit - 2 * kTop);
   __syncthreads();
@@ -339,7 +339,7 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
     top = fmaxf(top, other_half(top));
     odd |= !(top < INFINITY);
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) f[s] = split8(x[s], scale(exponent(top)));
+    for (int s = 0; s < T::KS; ++s) f[s] = split8<false>(x[s], scale(exponent(top)));
     return exponent(top);
   };
   const int64_t row = (int64_t)b * a.rows + (live ? i : 0);

@@ -98,7 +98,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
       odd |= !(top < INFINITY);
       eo = exponent(fmaxf(top, other_half(top)));
 #pragma unroll
-      for (int s = 0; s < T::KS; ++s) own[s] = split8(x[s], scale(eo));
+      for (int s = 0; s < T::KS; ++s) own[s] = split8<false>(x[s], scale(eo));
     }
     __syncthreads();
     int ex0 = m.ex[0];
@@ -307,7 +307,7 @@ __device__ __forceinline__ void q_pairs(const Args& a, const Block& blk, Shared<
       odd |= !(top < INFINITY);
       eo = exponent(top);
 #pragma unroll
-      for (int s = 0; s < T::KS; ++s) own[s] = split8(x[s], scale(eo));
+      for (int s = 0; s < T::KS; ++s) own[s] = split8<false>(x[s], scale(eo));
     }
     const int64_t st = ((int64_t)b * a.heads + h) * a.rows + (live ? i : 0);
     const float delta = live ? a.delta[st] : 0.f, lse = live ? a.lse_in[st] * kLog2e : 0.f;

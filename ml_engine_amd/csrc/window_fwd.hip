@@ -76,7 +76,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile
     const int ex = exponent(m);
     const float sc = a.scale < 0.f ? -scale(ex) : scale(ex);
 #pragma unroll
-    for (int s = 0; s < T::KS; ++s) q[s] = split8(x[s], sc);
+    for (int s = 0; s < T::KS; ++s) q[s] = split8<false>(x[s], sc);
     eq = ex;
   }
   int ek = 0, ev = -1000, ev_next = -1000;  // exponents: of the tile of K at hand, of V's operand so far

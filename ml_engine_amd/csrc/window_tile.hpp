@@ -2,11 +2,11 @@
 // cores with fp32 accuracy.
 //
 // Products.  An fp32 value x, scaled by a power of two so that its tile's largest is in
-// [2^14, 2^15), is held as two fp16 parts, hi its first 11 bits and lo the next 11: 22 bits of
-// every value down to 2^-18 of the largest, and 2^-40 of the largest below (the matrix
+// [2^14, 2^15), is held as two fp16 parts, hi its first 11 bits and lo the next 11 and a sign:
+// off by at most 2^-23 of x, or by 2^-39 of the tile's largest where that is more (the matrix
 // cores keep fp16's subnormals).  A product is hi hi + hi lo + lo hi, three
-// v_mfma_f32_32x32x16_f16, where three bf16 parts (split_core.hpp) take six.
-// What is not finite stays so in hi, and shows in the sums.
+// v_mfma_f32_32x32x16_f16, where three bf16 parts (split_core.hpp) take six; lo lo is at most
+// 2^-22 of it.  What is not finite stays so in hi, and shows in the sums.
 //
 // Layout.  A tile lies in LDS row by row, 128 or 256 bytes of fp16 to a row and plane,
 // the lo plane after the hi plane.  The 16-byte units of a row are permuted by an
@@ -64,31 +64,37 @@ __device__ __forceinline__ void mma3(const Frag& a, const Frag& b, f32x16& c) {
   c = mma(a.hi, b.hi, c);
 }
 
-// x in two parts: hi its first 11 bits, lo the next 11.  (Masked and subtracted: 5.1 ns a wave
-// and value; two v_fma_mix_f16 take 7.2.)
+// x in two parts: hi is x rounded to fp16, lo what hi as it is held leaves of it, rounded.  (A hi below
+// 2^-14 has fewer than 11 bits; what it drops is lo's too.)  FUSED: lo from hi by v_fma_mix_f32, four
+// instructions for two values, else by conversions, six.  Staged tiles take the first and rows from
+// the accumulators the second: 2 x 16 heads of 4096 x 128 under a window of 1024 take 253 us forward,
+// 261 with the first for both, 250 with the second; 6 heads of 777 x 80 28.9, 29.1 and 29.6.
+template <bool FUSED>
 __device__ __forceinline__ Frag split8(const float (&x)[8]) {
   f16x2 h[4], l[4];
+  float minus = -1.f;
+  if (FUSED) asm("" : "+s"(minus));  // (a product that the compiler keeps)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float a[2], b[2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      a[n] = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x[2 * j + n]) & 0xffffe000u);
-      b[n] = x[2 * j + n] - a[n];
-    }
-    h[j] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a[0], a[1]));
-    l[j] = f16x2{(_Float16)b[0], (_Float16)b[1]};
+    const float a = x[2 * j], b = x[2 * j + 1];
+    unsigned u = __builtin_bit_cast(unsigned, f16x2{(_Float16)a, (_Float16)b});
+    asm("" : "+v"(u));  // (one conversion for both values and both uses)
+    h[j] = __builtin_bit_cast(f16x2, u);
+    const float a0 = (float)h[j][0], b0 = (float)h[j][1];
+    l[j] = FUSED ? f16x2{(_Float16)fmaf(a0, minus, a), (_Float16)fmaf(b0, minus, b)} : f16x2{(_Float16)(a - a0), (_Float16)(b - b0)};
   }
   return Frag{__builtin_shufflevector(__builtin_shufflevector(h[0], h[1], 0, 1, 2, 3),
                                       __builtin_shufflevector(h[2], h[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7),
               __builtin_shufflevector(__builtin_shufflevector(l[0], l[1], 0, 1, 2, 3),
                                       __builtin_shufflevector(l[2], l[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7)};
 }
+// The same of x times a power of two.
+template <bool FUSED>
 __device__ __forceinline__ Frag split8(const float (&x)[8], float s) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = x[j] * s;
-  return split8(v);
+  return split8<FUSED>(v);
 }
 
 // Eight of a block's 16 rows as an operand.
@@ -96,13 +102,13 @@ __device__ __forceinline__ Frag split_rows(const f32x16& x, int s) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = x[8 * s + j];
-  return split8(v);
+  return split8<false>(v);
 }
 __device__ __forceinline__ Frag split_rows(const f32x16& x, int s, float scale) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = x[8 * s + j];
-  return split8(v, scale);
+  return split8<false>(v, scale);
 }
 
 // A lane's places in a tile: of frag_row's first step and of frag_col's first columns.  Later
@@ -294,7 +300,7 @@ struct Share {
       if (!has(c)) break;
       const bool s = second(c);
       const int r = row(c), u = col(c) / 8;
-      const Frag f = split8(x[c], scale_of(s, r));
+      const Frag f = split8<true>(x[c], scale_of(s, r));
       char* at = (s ? t1 : t0) + r * T::PITCH + ((u ^ swizzle<T::DP>(r)) << 4);
       *reinterpret_cast<f16x8*>(at) = f.hi;
       *reinterpret_cast<f16x8*>(at + T::PLANE) = f.lo;
