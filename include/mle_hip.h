@@ -423,9 +423,11 @@ int mle_attention_bwd(mle_stream stream, const float* q, const float* k, const f
  * over the visible keys, whatever the others hold.  Rows at or past a length have out 0 and
  * lse -infinity, and their gradients take no part; their k and v rows get gradients of 0.
  * lse [batch, heads, seq] is nullable where no backward follows; out is none of the inputs.
- * The products' operands are held in 22 bits (two fp16 parts and a power of two per tile of 32
- * or 64 positions, row or column): what is below 2^-18 of a tile's largest, hidden entries
- * among them, is held to 2^-40 of it.  Sums, statistics and exponentials are fp32.  Where a tile
+ * The products' operands are two fp16 parts and a power of two per tile of 32 or 64 positions,
+ * row or column: q, k, v and dout are off by at most 2^-23 of themselves or 2^-39 of the largest
+ * in their tile (of positions, hidden ones among them), P and dS (the backward) by 2^-23 of
+ * themselves or 2^-36 of the largest in their row or column; a product lacks at most 2^-22 of
+ * itself.  Sums, statistics and exponentials are fp32.  Where a tile
  * holds an infinity or a NaN, or lies far below an earlier one, rows are computed with fp32
  * products, key by key.  Results do not depend on timing.
  * MultiHeadAttention's softmax (mle_attention_fwd) is over columns; this is SOFTMAX type 0

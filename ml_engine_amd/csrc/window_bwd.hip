@@ -13,7 +13,7 @@
 // Scales.  A product sums over rows (kv) or keys (q) whose probabilities and gradients may be
 // of very unlike size, so the operands that are made here are held at powers of two of their
 // own column, a lane's: a key's P and dS (kv), a row's dS (q) have the largest seen so far
-// between 2^8 and 2^15, and a larger one rescales the lane's sums.  Rows of dout are at powers
+// between 2^12 and 2^15, and a larger one rescales the lane's sums.  Rows of dout are at powers
 // of two of their own too; P takes those up in its exponent.
 //
 // Here for heads of up to 64, a wave with 32 keys (rows) to itself: two workgroups of four waves
@@ -229,7 +229,7 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
       if (__any(mx + sj > 15.f)) {
         mx = fmaxf(mx, other_half(mx));
-        const float to = mx + sj > 15.f ? floorf(8.f - mx) : sj;
+        const float to = mx + sj > 15.f ? floorf(kHeld + 1 - mx) : sj;
         const int by = (int)(to - sj);
 #pragma unroll
         for (int d = 0; d < T::DB; ++d)

@@ -163,7 +163,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[r]);
         if (__any(mx + sj > 15.f)) {
           mx = fmaxf(mx, other_half(mx));
-          const float to = mx + sj > 15.f ? floorf(8.f - mx) : sj;
+          const float to = mx + sj > 15.f ? floorf(kHeld + 1 - mx) : sj;
           const int by = (int)(to - sj);
 #pragma unroll
           for (int d = 0; d < T::DB; ++d)

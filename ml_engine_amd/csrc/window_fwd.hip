@@ -4,8 +4,10 @@
 //
 // Scores come out as S^T = K Q^T, rows to lanes, so a row's statistics are a lane's
 // (two lanes hold 16 of every 32 keys of a row each), and P^T is the operand of
-// O^T += V^T P^T as it lies in the accumulators.  P is held at 2^8 for a row's maximum so
-// far; the sums are rescaled only when a score passes that by 2^7.
+// O^T += V^T P^T as it lies in the accumulators.  P is held at 2^12 for a row's maximum so
+// far, so that a weight is off by at most 2^-23 of it or 2^-37 of the row's largest; the sums are
+// rescaled only when a score passes that by 2^3 (at 2^8 and 2^7, small weights beside a large one
+// lost 2^-10 of themselves, and the times were the same to 1 %).
 //
 // Bound by vector instructions beside the products: splitting operands, masks, exponentials.
 // 2 x 16 heads of 4096 x 128 under a window of 1024 take 261-285 us (fp32 products at 215
@@ -19,7 +21,7 @@ using namespace mle;
 namespace wattn {
 namespace {
 
-constexpr float kHead = 8.f;
+constexpr float kHead = 12.f;  // log2
 
 template <int DP, int NW, int KW>
 __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile_fwd_kernel(Args a, Grid g) {

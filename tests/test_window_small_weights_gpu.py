@@ -91,6 +91,6 @@ def test_results_of_the_smallest_weights(hip, dim, heads):
     c.forward()
     c.backward()
     got, r = c.results(), bounds(c)
-    for name, at in (("dq", slice(ROW, ROW + 1)), ("dk", slice(0, 2)), ("dv", slice(0, 2))):
+    for name, at in (("out", slice(ROW, ROW + 1)), ("dq", slice(ROW, ROW + 1)), ("dk", slice(0, 2)), ("dv", slice(0, 2))):
         err = np.abs(got[name][0, at, :, 1:] - r[name][at, :, 1:])
         assert (err <= r["e_" + name][at, :, 1:]).all(), (name, float((err / r["e_" + name][at, :, 1:]).max()))
