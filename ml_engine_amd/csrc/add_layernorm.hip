@@ -7,7 +7,8 @@
 // One pass over a row: T lanes of a wave, or a workgroup of T threads, hold it
 // in registers, eight consecutive values to a thread and chunk.  The variance is
 // that of the centred values, so a mean far above the spread costs no bits; the
-// row's sums are in 64 bits.  The weight's and the bias's gradients are summed per
+// row's sums are in 64 bits.  The backward, which has the mean in 32 bits, takes what
+// that lacks from the row (rest_of).  The weight's and the bias's gradients are summed per
 // workgroup in registers and joined in order.  Bound by memory, each tensor passed once: 16384 x
 // 4096 take 204 us forward (5.3 TB/s) and 213 + 7.5 us backward (5.0 TB/s), 8192 x 512 with
 // three launches 35 us in all, 64 x 256 3.8 + 4.7 us.
@@ -22,6 +23,8 @@ namespace {
 constexpr int NT = 256;
 constexpr int kMaxParts = 512;          // partial weight gradients: workgroups of the backward
 constexpr int kFewRows = 256;           // up to which the backward is one launch
+constexpr int kRestRows = 8;            // of a workgroup of layernorm_rest_kernel
+constexpr int kWidest = 8192;           // columns of a row in registers
 constexpr int kRowsOfLaunch = 1 << 21;  // of a launch of one workgroup to a row: fewer than 2^32 threads
 
 struct LnArgs {
@@ -72,6 +75,17 @@ __device__ __forceinline__ double2 row_sums(double a, double b, double (*red)[2]
     b += red[i][1];
   }
   return make_double2(a, b);
+}
+
+// The backward's u = ((h - mean) - rest) rstd.  The mean's rounding moves u by at most 2^-24 |mean|
+// rstd; below 2^-22 that is left (rest 0, exactly), above it the rest of the mean is the mean of
+// h - mean, which costs such a row one sum more.
+__device__ __forceinline__ bool is_far(float mean, float rstd) { return fabsf(mean) * rstd > 4.f; }
+
+// A thread's share of that sum: n values of a chunk.
+__device__ __forceinline__ void add_rest(double& s, const float (&h)[8], int n, float mean) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += j < n ? (double)h[j] - (double)mean : 0.0;
 }
 
 __device__ __forceinline__ void load_sum8(const LnArgs& a, int64_t at, int n, float (&h)[8]) {
@@ -168,7 +182,7 @@ __device__ __forceinline__ void bwd_rows(const LnBwdArgs& a, int block, int bloc
     const bool live = row < a.rows;
     const int64_t base = (live ? row : a.rows - 1) * a.cols;
     const float rstd = live ? a.rstd[row] : 0.f, mean = live ? a.mean[row] : 0.f;
-    float u[C][8], g[C][8];
+    float u[C][8], g[C][8], rest = 0.f;
     double s1 = 0.0, s2 = 0.0;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -178,9 +192,20 @@ __device__ __forceinline__ void bwd_rows(const LnBwdArgs& a, int block, int bloc
       if (n == 0) continue;
       q8::load_row8(a.h + base + col, n, u[c]);
       q8::load_row8(a.dy + base + col, n, g[c]);  // (0 past the row's end, whatever u is there)
+    }
+    if (is_far(mean, rstd)) {  // (the same for all of a row's threads)
+      double s = 0.0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) add_rest(s, u[c], a.cols - (c * T + t) * 8, mean);
+      rest = (float)(row_sums<T>(s, 0.0, red).x / a.cols);
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * T + t) * 8, n = live ? min(max(a.cols - col, 0), 8) : 0;
+      if (n == 0) continue;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        u[c][j] = (u[c][j] - mean) * rstd;
+        u[c][j] = ((u[c][j] - mean) - rest) * rstd;
         dw[c][j] += g[c][j] * u[c][j];
         db[c][j] += g[c][j];
         g[c][j] *= w[c][j];
@@ -252,23 +277,56 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_small_kernel(LnBwdArgs a, fl
     return;
   }
   __shared__ float red[2][64][17];
-  const int c = threadIdx.x & 15, col = ((int)blockIdx.x - row_blocks) * 16 + c;
-  for (int g = threadIdx.x >> 4; g < 64; g += NT / 16) {
-    float u[4], d[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-#pragma clang fp contract(off)
-      const int r = 4 * g + k;
-      const bool there = r < a.rows && col < a.cols;
-      const int64_t at = there ? (int64_t)r * a.cols + col : 0;
-      const int row = there ? r : 0;
-      d[k] = there ? a.dy[at] : 0.f;
-      u[k] = there ? d[k] * ((a.h[at] - a.mean[row]) * a.rstd[row]) : 0.f;
-    }
-    red[0][g][c] = ((u[0] + u[1]) + u[2]) + u[3];
-    red[1][g][c] = ((d[0] + d[1]) + d[2]) + d[3];
+  __shared__ float rest[NT];
+  __shared__ unsigned long long far[NT / 64];  // rows of a wave's 64
+  static_assert(kFewRows <= NT, "a row to a thread");
+  {
+    const int row = threadIdx.x;
+    const unsigned long long bits = __ballot(row < a.rows && is_far(a.mean[row], a.rstd[row]));
+    if ((threadIdx.x & 63) == 0) far[threadIdx.x >> 6] = bits;
   }
+  const int c = threadIdx.x & 15, col = ((int)blockIdx.x - row_blocks) * 16 + c;
+  const auto sums = [&](bool with_rest) {
+    for (int g = threadIdx.x >> 4; g < 64; g += NT / 16) {
+      float u[4], d[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma clang fp contract(off)
+        const int r = 4 * g + k;
+        const bool there = r < a.rows && col < a.cols;
+        const int64_t at = there ? (int64_t)r * a.cols + col : 0;
+        const int row = there ? r : 0;
+        d[k] = there ? a.dy[at] : 0.f;
+        const float h = a.h[at] - a.mean[row];
+        u[k] = there ? d[k] * ((with_rest ? h - rest[row] : h) * a.rstd[row]) : 0.f;
+      }
+      red[0][g][c] = ((u[0] + u[1]) + u[2]) + u[3];
+      red[1][g][c] = ((d[0] + d[1]) + d[2]) + d[3];
+    }
+  };
+  sums(false);
   __syncthreads();
+  if (far[0] | far[1] | far[2] | far[3]) {  // once more with the rests of such rows, a row to a wave
+    float mine = 0.f;
+    for (unsigned long long left = far[threadIdx.x >> 6]; left; left &= left - 1) {
+      const int bit = __ffsll(left) - 1, lane = threadIdx.x & 63, r = (threadIdx.x & ~63) + bit;
+      const float mean = a.mean[r];
+      double s = 0.0;
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        const int at = (k * T + lane) * 8, n = min(max(a.cols - at, 0), 8);
+        float h[8] = {};
+        if (n > 0) q8::load_row8(a.h + (int64_t)r * a.cols + at, n, h);
+        add_rest(s, h, n, mean);
+      }
+      const float v = (float)(row_sums<T>(s, 0.0, nullptr).x / a.cols);
+      if (lane == bit) mine = v;
+    }
+    rest[threadIdx.x] = mine;
+    __syncthreads();
+    sums(true);
+    __syncthreads();
+  }
   if (threadIdx.x >= 64) return;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -278,34 +336,52 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_small_kernel(LnBwdArgs a, fl
   }
 }
 
+// The rest of a row's mean, 0 of a row that is not far; by a workgroup of 1024.
+__device__ __forceinline__ float rest_of(const LnBwdArgs& a, int64_t row, float mean, float rstd, double (*red)[2]) {
+  if (!is_far(mean, rstd)) return 0.f;
+  double s = 0.0;
+  for (int i = threadIdx.x; i < a.cols; i += 1024) s += (double)a.h[row * a.cols + i] - (double)mean;
+  return (float)(row_sums<1024>(s, 0.0, red).x / a.cols);
+}
+__global__ __launch_bounds__(1024) void layernorm_rest_kernel(LnBwdArgs a, float* __restrict__ rest) {
+  __shared__ double red[16][2];
+  const int64_t r0 = (int64_t)blockIdx.x * kRestRows;
+#pragma unroll
+  for (int k = 0; k < kRestRows; ++k) {
+    if (r0 + k >= a.rows) return;  // (the workgroup)
+    const float v = rest_of(a, r0 + k, a.mean[r0 + k], a.rstd[r0 + k], red);
+    if (threadIdx.x == 0) rest[r0 + k] = v;
+  }
+}
+
 // Rows wider than the register kernels take: h and dy read twice; the weight's and the
 // bias's gradients in a pass of their own (layernorm_dw_kernel).
 __global__ __launch_bounds__(1024) void layernorm_bwd_wide_kernel(LnBwdArgs a) {
   __shared__ double red[16][2];
   const int64_t base = (int64_t)blockIdx.x * a.cols;
-  const float rstd = a.rstd[blockIdx.x], mean = a.mean[blockIdx.x];
+  const float rstd = a.rstd[blockIdx.x], mean = a.mean[blockIdx.x], rest = rest_of(a, blockIdx.x, mean, rstd, red);
   double s1 = 0.0, s2 = 0.0;
   for (int i = threadIdx.x; i < a.cols; i += 1024) {
-    const float g = a.dy[base + i] * (a.w ? a.w[i] : 1.f), u = (a.h[base + i] - mean) * rstd;
+    const float g = a.dy[base + i] * (a.w ? a.w[i] : 1.f), u = ((a.h[base + i] - mean) - rest) * rstd;
     s1 += (double)g;
     s2 += (double)(g * u);
   }
   const double2 m = row_sums<1024>(s1, s2, red);
   const float m1 = (float)(m.x / a.cols), m2 = (float)(m.y / a.cols);
   for (int i = threadIdx.x; i < a.cols; i += 1024) {
-    const float g = a.dy[base + i] * (a.w ? a.w[i] : 1.f), u = (a.h[base + i] - mean) * rstd;
+    const float g = a.dy[base + i] * (a.w ? a.w[i] : 1.f), u = ((a.h[base + i] - mean) - rest) * rstd;
     const float v = (a.dres ? a.dres[base + i] : 0.f) + rstd * ((g - m1) - u * m2);
     a.dh[base + i] = (a.acc_dh ? a.dh[base + i] : 0.f) + v;
   }
 }
 // part[block y][.][col] = sums over rows y, y + gridDim.y, ...
-__global__ __launch_bounds__(NT) void layernorm_dw_kernel(LnBwdArgs a) {
+__global__ __launch_bounds__(NT) void layernorm_dw_kernel(LnBwdArgs a, const float* __restrict__ rest) {
   const int col = blockIdx.x * NT + threadIdx.x;
   if (col >= a.cols) return;
   float s = 0.f, b = 0.f;
   for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
     const float dy = a.dy[r * a.cols + col];
-    s += dy * ((a.h[r * a.cols + col] - a.mean[r]) * a.rstd[r]);
+    s += dy * (((a.h[r * a.cols + col] - a.mean[r]) - rest[r]) * a.rstd[r]);
     b += dy;
   }
   float* part = a.part + (int64_t)blockIdx.y * 2 * a.cols;
@@ -341,6 +417,8 @@ int parts_of(int rows, int cols) {
   return std::max(1, std::min(kMaxParts, (rows - 1) / rows_of_wg + 1));
 }
 
+size_t parts_floats(int rows, int cols) { return (size_t)parts_of(rows, cols) * 2 * cols; }
+
 int check(const char* who, int rows, int cols) {
   MLE_CHECK_ARG(rows >= 0 && cols > 0 && cols <= (1 << 30), "%s: bad shape %d x %d", who, rows, cols);
   return MLE_OK;
@@ -367,7 +445,7 @@ int mle_add_layernorm_fwd(mle_stream stream, int rows, int cols, const float* x,
     else if (cols <= 1024) mle::launch(layernorm_fwd_kernel<64, 2>, by4, NT, 0, s, a);
     else if (cols <= 2048) mle::launch(layernorm_fwd_kernel<64, 4>, by4, NT, 0, s, a);
     else if (cols <= 4096) mle::launch(layernorm_fwd_kernel<256, 2>, (unsigned)n, NT, 0, s, a);
-    else if (cols <= 8192) mle::launch(layernorm_fwd_kernel<256, 4>, (unsigned)n, NT, 0, s, a);
+    else if (cols <= kWidest) mle::launch(layernorm_fwd_kernel<256, 4>, (unsigned)n, NT, 0, s, a);
     else mle::launch(layernorm_fwd_kernel<1024, 0>, (unsigned)n, 1024, 0, s, a);
   }
   return check_launch("mle_add_layernorm_fwd");
@@ -375,7 +453,7 @@ int mle_add_layernorm_fwd(mle_stream stream, int rows, int cols, const float* x,
 
 size_t mle_add_layernorm_ws_bytes(int rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return (size_t)parts_of(rows, cols) * 2 * cols * sizeof(float);
+  return (parts_floats(rows, cols) + (cols > kWidest ? rows : 0)) * sizeof(float);  // (there, the rests of the means)
 }
 
 int mle_add_layernorm_bwd(mle_stream stream, int rows, int cols, const float* h, const float* w, const float* mean,
@@ -411,10 +489,15 @@ int mle_add_layernorm_bwd(mle_stream stream, int rows, int cols, const float* h,
   else if (cols <= 1024) mle::launch(layernorm_bwd_kernel<64, 2>, (unsigned)parts, NT, 0, s, a);
   else if (cols <= 2048) mle::launch(layernorm_bwd_kernel<64, 4>, (unsigned)parts, NT, 0, s, a);
   else if (cols <= 4096) mle::launch(layernorm_bwd_kernel<256, 2>, (unsigned)parts, NT, 0, s, a);
-  else if (cols <= 8192) mle::launch(layernorm_bwd_kernel<256, 4>, (unsigned)parts, NT, 0, s, a);
+  else if (cols <= kWidest) mle::launch(layernorm_bwd_kernel<256, 4>, (unsigned)parts, NT, 0, s, a);
   else {
     // the weight's sums first: dh may be dy's or h's buffer
-    if (sums) mle::launch(layernorm_dw_kernel, dim3((unsigned)((cols + NT - 1) / NT), (unsigned)parts), NT, 0, s, a);
+    if (sums) {
+      float* rest = static_cast<float*>(ws) + parts_floats(rows, cols);
+      mle::launch(layernorm_rest_kernel, (unsigned)((rows - 1) / kRestRows + 1), 1024, 0, s, a, rest);
+      mle::launch(layernorm_dw_kernel, dim3((unsigned)((cols + NT - 1) / NT), (unsigned)parts), NT, 0, s, a,
+                  static_cast<const float*>(rest));
+    }
     for (int64_t r0 = 0; r0 < rows; r0 += kRowsOfLaunch) {
       const int n = (int)std::min<int64_t>(rows - r0, kRowsOfLaunch);
       const int64_t at = r0 * cols;
