@@ -25,6 +25,7 @@ constexpr int kMaxParts = 512;          // partial weight gradients: workgroups 
 constexpr int kFewRows = 256;           // up to which the backward is one launch
 constexpr int kRestRows = 8;            // of a workgroup of layernorm_rest_kernel
 constexpr int kWidest = 8192;           // columns of a row in registers
+constexpr int kColsOfJoin = 1 << 25;    // of a launch of 64 threads to a column: fewer than 2^32 threads
 constexpr int kRowsOfLaunch = 1 << 21;  // of a launch of one workgroup to a row: fewer than 2^32 threads
 
 struct LnArgs {
@@ -390,15 +391,16 @@ __global__ __launch_bounds__(NT) void layernorm_dw_kernel(LnBwdArgs a, const flo
 }
 
 // dw (+)= and db (+)= the partial sums: 16 columns of one of them to a workgroup, 64
-// threads to a column, each adding every 64th part, and the threads' sums in order.
-__global__ __launch_bounds__(1024) void layernorm_join_kernel(const float* __restrict__ part, int parts, int cols,
+// threads to a column, each adding every 64th part, and the threads' sums in order.  From
+// column col0 on.
+__global__ __launch_bounds__(1024) void layernorm_join_kernel(const float* __restrict__ part, int parts, int cols, int col0,
                                                               float* __restrict__ dw, float* __restrict__ db,
                                                               int accumulate) {
   __shared__ float red[64][17];
   float* out = blockIdx.y ? db : dw;
   if (!out) return;
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + c;
+  const int col = col0 + (int)blockIdx.x * 16 + c;
   float s = 0.f;
   if (col < cols) {
 #pragma unroll 8
@@ -506,9 +508,9 @@ int mle_add_layernorm_bwd(mle_stream stream, int rows, int cols, const float* h,
       mle::launch(layernorm_bwd_wide_kernel, (unsigned)n, 1024, 0, s, b);
     }
   }
-  if (sums)
-    mle::launch(layernorm_join_kernel, dim3((unsigned)((cols + 15) / 16), 2), 1024, 0, s, static_cast<const float*>(ws), parts,
-                cols, dw, db, accumulate_dw);
+  for (int64_t c0 = 0; sums && c0 < cols; c0 += kColsOfJoin)
+    mle::launch(layernorm_join_kernel, dim3((unsigned)((std::min<int64_t>(cols - c0, kColsOfJoin) + 15) / 16), 2), 1024, 0, s,
+                static_cast<const float*>(ws), parts, cols, (int)c0, dw, db, accumulate_dw);
   return check_launch("mle_add_layernorm_bwd");
 }
 

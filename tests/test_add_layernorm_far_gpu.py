@@ -1,5 +1,5 @@
 """The layer norm's backward of rows whose mean lies far above their spread: what the differences
-within a row hold, dh, dw and db keep, at the sizes where it changes form."""
+within a row hold, dh, dw and db keep, at the sizes where it changes form.  And of the widest rows."""
 import numpy as np
 import pytest
 
@@ -63,3 +63,21 @@ def test_forms_agree(hip, rows, cols):
     for a, c in zip(one, two):
         assert np.array_equal(a, c)
     assert np.array_equal(one[1], run(hip, rows, cols, x, w, b, dy, dres, sums=False)[1])
+
+
+def test_more_columns_than_a_join_takes(hip):
+    """A row of 2^26 + 5 values: 64 threads to each column are more than a launch has."""
+    cols = (1 << 26) + 5
+    r = rng(3)
+    x, dy = (r.standard_normal((1, cols), dtype=np.float32) for _ in range(2))
+    gx, gdy, gm, gs, dw = hip.Buffer.from_array(x), hip.Buffer.from_array(dy), hip.Buffer.empty(1), hip.Buffer.empty(1), hip.Buffer.empty(cols)
+    db, ws = hip.Buffer.from_array(np.full(cols, 7, np.float32)), hip.Buffer(hip.lib().mle_add_layernorm_ws_bytes(1, cols))
+    hip.call("mle_add_layernorm_fwd", None, 1, cols, gx.ptr, None, None, None, EPS, None, None, gm.ptr, gs.ptr)
+    hip.call("mle_add_layernorm_bwd", None, 1, cols, gx.ptr, None, gm.ptr, gs.ptr, gdy.ptr, None, gdy.ptr, 0, dw.ptr, db.ptr, 0, ws.ptr,
+             ws.nbytes)
+    hip.sync()
+    h = x[0].astype(np.float64)
+    u = (h - h.mean()) / np.sqrt(h.var() + float(np.float32(EPS)))
+    # the mean's rounding, h - mean, rstd and two products
+    assert (np.abs(dw.numpy() - dy[0] * u) <= F32 * np.abs(dy[0]) * (6 * np.abs(u) + 1)).all()
+    assert np.array_equal(db.numpy(), dy[0])
