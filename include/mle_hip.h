@@ -420,12 +420,14 @@ int mle_attention_bwd(mle_stream stream, const float* q, const float* k, const f
  * window >= 1, sinks >= 0; window >= seq is plain causal attention.  lengths (device
  * int32 [batch], nullable: seq) are taken as at most seq and at least 0.
  *   S = scale q k^T,  P = exp(S - lse),  lse = log sum exp S,  out = P v
- * over the visible keys, whatever the others hold.  Rows at or past a length have out 0 and
+ * over the visible keys; what the others hold, infinities and NaN among it, reaches nothing, but for
+ * the bits that a tile's largest value takes from its neighbours (below).  Rows at or past a length have out 0 and
  * lse -infinity, and their gradients take no part; their k and v rows get gradients of 0.
  * lse [batch, heads, seq] is nullable where no backward follows; out is none of the inputs.
  * The products' operands are two fp16 parts and a power of two per tile of 32 or 64 positions,
  * row or column: q, k, v and dout are off by at most 2^-23 of themselves or 2^-39 of the largest
- * in their tile (of positions, hidden ones among them), P and dS (the backward) by 2^-23 of
+ * in their tile (the forward's tiles hold what some row of a workgroup's 64 to 256 sees, the
+ * backward's all positions up to the length), P and dS (the backward) by 2^-23 of
  * themselves or 2^-36 of the largest in their row or column; a product lacks at most 2^-22 of
  * itself.  Sums, statistics and exponentials are fp32.  Where a tile
  * holds an infinity or a NaN, or lies far below an earlier one, rows are computed with fp32

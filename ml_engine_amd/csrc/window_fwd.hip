@@ -57,11 +57,12 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW / KW == 2 ? 1 : 2) void tile
   Share<T, NT> kv;
   // Loads past the last tile are of the last once more and go unused: no branches around loads.
   auto row_of = [&](int t) { return tiles.row(min(t, count - 1)); };
-  auto fetch = [&](int t) {
-    kv.load(K, a.ldk, V, a.ldv, row_of(t), seq.len, a.dim);
-  };
+  // Keys that no row of the workgroup sees (after its last, and between the sinks and its first window)
+  // are zeros, so that what lies there, in a cache's places that were left for instance, takes no
+  // bits from the others of its tile.
+  auto fetch = [&](int t) { kv.load(K, a.ldk, V, a.ldv, row_of(t), last + 1, a.dim); };
   auto tell = [&](int t) {
-    kv.clear(row_of(t), seq.len, a.dim);
+    kv.clear(row_of(t), last + 1, a.dim, a.sinks, first - a.window + 1);
     tops.add(0, t, kv.top(false));
     tops.add(1, t, kv.top(true));
   };

@@ -278,12 +278,15 @@ struct Share {
       }
     }
   }
-  // Zeros from row `end` and column `dim` on; four values that reach past dim have been read as the
-  // last four.
-  __device__ __forceinline__ void clear(int r0, int end, int dim) {
-    if (r0 + T::R <= end && dim == T::DP) return;
+  // Zeros from row `end` and column `dim` on, and in rows h0 .. h1 - 1; four values that reach past
+  // dim have been read as the last four.
+  __device__ __forceinline__ void clear(int r0, int end, int dim, int h0 = 0, int h1 = 0) {
+    if (r0 + T::R <= end && dim == T::DP && (r0 >= h1 || r0 + T::R <= h0)) return;
 #pragma unroll
-    for (int c = 0; c < N; ++c) cut8<(T::DP < 128)>(x[c], r0 + row(c) < end ? dim - col(c) : 0, dim & 3);
+    for (int c = 0; c < N; ++c) {
+      const int r = r0 + row(c);
+      cut8<(T::DP < 128)>(x[c], (r < end) & ((r < h0) | (r >= h1)) ? dim - col(c) : 0, dim & 3);
+    }
   }
   // The largest magnitude of the first (second) tensor's chunks.
   __device__ __forceinline__ float top(bool of_second) const {
