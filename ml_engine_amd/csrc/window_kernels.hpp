@@ -77,11 +77,26 @@ struct StepWork {
     row_blocks = (a.group * a.rows + 15) / 16;
     const int64_t groups = (int64_t)a.batch * a.kv_heads * row_blocks;
     const int64_t keys = std::min<int64_t>(a.keys, (int64_t)a.sinks + a.window + a.rows - 1);
-    // enough workgroups for the chip's 256 CUs twice, 128 keys (a block to a wave) or more
-    // to each; one launch where a second would cost what it saves
     splits = 1;
-    if (groups < 200 && keys > 256)
-      splits = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + groups - 1) / groups, (keys + 127) / 128, 64}));
+    if (groups < 200) {
+      // enough workgroups for the chip's 256 CUs twice, 128 keys (a block to a wave) or more
+      // to each; one launch where a second would cost what it saves
+      if (keys > 256)
+        splits = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + groups - 1) / groups, (keys + 127) / 128, 64}));
+    } else if (row_blocks == 1) {
+      // Whole groups, but where CUs would wait for the longest or the last of them (8 heads of keys x
+      // 128, us whole and split; with more rows to a group splits only cost: 8 tokens of 32 x 32 heads
+      // over 2048 keys 172 and 194).  A window that takes in the whole cache leaves what is read to
+      // the lengths, which may be unlike: 32 of 1 to 8192: 261 and 211, one of 16384 among 31 of 500:
+      // 426 and 72, 64 of 2048 to 4096: 297 and 277; but 32 of 4100 each: 180 and 199, and below 2560 keys as
+      // much is lost (32 of 1 to 1024: 38 and 40).
+      if (keys == a.keys) splits = (int)std::max<int64_t>(1, std::min<int64_t>(keys / 1280, 8));
+      // Groups for a last round of half the CUs or less: 264 of 4100 keys 287 and 224, 384: 308 and 293, 520 of
+      // 2050: 239 and 217, 264 of 1024: 77 and 73; 720 of 2050: 275 and 286, 264 of 512: 44 and 46.
+      const int64_t last = groups % 256;
+      if (groups > 256 && groups < 1024 && last > 0 && last <= 128)
+        splits = std::max(splits, (int)std::max<int64_t>(1, std::min<int64_t>(keys / 512, 3)));
+    }
   }
   size_t bytes(const Args& a) const {
     return splits == 1 ? 0 : (size_t)a.batch * a.kv_heads * row_blocks * splits * 16 * (a.dim + 2) * sizeof(float);

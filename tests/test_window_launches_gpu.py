@@ -7,7 +7,7 @@ import pytest
 
 import wattn_ref as ref
 from conftest import rng
-from test_window_attention_gpu import Case
+from test_window_attention_gpu import Case, Step
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,26 @@ def test_forms(hip, form, dim):
             ref.check(got[name][i:i + 1, :, at], t, name, c.old[j][i:i + 1, :, at] if acc >> j & 1 else None)
         ref.check(got["out"][i:i + 1, :, q], t, "out")
         ref.check(got["lse"][i:i + 1, q], t, "lse")
+
+
+# batch, capacity, heads, heads of keys, dim, window, sinks, equal lengths
+STEPS = [
+    (33, 2700, 8, 8, 32, 9000, 0, 0),   # unlike lengths over whole caches: keys in parts
+    (26, 5200, 32, 8, 16, 5200, 0, 0),
+    (33, 1300, 8, 8, 48, 1100, 4, 1),   # a few groups past a round of the CUs
+    (66, 1700, 16, 8, 32, 1600, 0, 0),
+    (32, 1400, 8, 8, 64, 1100, 4, 0),   # whole groups
+    (30, 700, 8, 8, 40, 700, 0, 0),
+]
+
+
+@pytest.mark.parametrize("b,cap,h,kv,dim,w,s,equal", STEPS)
+def test_steps_of_many_groups(hip, b, cap, h, kv, dim, w, s, equal):
+    r = rng(cap)
+    lengths = np.full(b, cap) if equal else r.integers(0, cap + 1, b)
+    t = Step(hip, b, 1, cap, h, kv, dim, w, s, lengths)
+    t.run()
+    t.check()
+    one = t.out.get()
+    t.run()
+    assert np.array_equal(one, t.out.get())
