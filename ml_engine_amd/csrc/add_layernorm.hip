@@ -83,11 +83,26 @@ __device__ __forceinline__ double2 row_sums(double a, double b, double (*red)[2]
 // h - mean, which costs such a row one sum more.
 __device__ __forceinline__ bool is_far(float mean, float rstd) { return fabsf(mean) * rstd > 4.f; }
 
-// A thread's share of that sum: n values of a chunk.
-__device__ __forceinline__ void add_rest(double& s, const float (&h)[8], int n, float mean) {
+// That sum: eight consecutive differences in 32 bits (exact in rows far enough from zero, 3 roundings of
+// them in others), these in 64 and rounded to 2^-27 of the mean's power of two 2^k.  A far row's differences
+// add up to less than cols 2^(k - 1), so that up to 2^27 columns every sum of such is exact: the same
+// in any order, whatever the kernel's form.
+struct Rest {
+  float mean;
+  double grid;  // adding it leaves what is above 2^(k - 27)
+  double sum = 0.0;
+  __device__ __forceinline__ explicit Rest(float m) : mean(m) {
+    const int k = (int)((__builtin_bit_cast(unsigned, m) >> 23) & 255u) - 127;
+    grid = ldexp(1.5, k - 27 + 52);
+  }
+  // The first n of eight values (none where n is below 1).
+  __device__ __forceinline__ void add(const float (&h)[8], int n) {
+    float d[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s += j < n ? (double)h[j] - (double)mean : 0.0;
-}
+    for (int j = 0; j < 8; ++j) d[j] = j < n ? h[j] - mean : 0.f;
+    sum += ((double)(((d[0] + d[1]) + (d[2] + d[3])) + ((d[4] + d[5]) + (d[6] + d[7]))) + grid) - grid;
+  }
+};
 
 __device__ __forceinline__ void load_sum8(const LnArgs& a, int64_t at, int n, float (&h)[8]) {
   q8::load_row8(a.x + at, n, h);
@@ -195,10 +210,10 @@ __device__ __forceinline__ void bwd_rows(const LnBwdArgs& a, int block, int bloc
       q8::load_row8(a.dy + base + col, n, g[c]);  // (0 past the row's end, whatever u is there)
     }
     if (is_far(mean, rstd)) {  // (the same for all of a row's threads)
-      double s = 0.0;
+      Rest r(mean);
 #pragma unroll
-      for (int c = 0; c < C; ++c) add_rest(s, u[c], a.cols - (c * T + t) * 8, mean);
-      rest = (float)(row_sums<T>(s, 0.0, red).x / a.cols);
+      for (int c = 0; c < C; ++c) r.add(u[c], a.cols - (c * T + t) * 8);
+      rest = (float)(row_sums<T>(r.sum, 0.0, red).x / a.cols);
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -269,7 +284,9 @@ __device__ __forceinline__ float join64(const float (*red)[17]) {
 
 // Few rows, where launches are the time (256 x 512: 5.0 us against 7.2 in two, 64 x 256: 4.1 against
 // 6.1): both in one launch, the first `row_blocks` workgroups the rows and the others 16
-// columns of dw and db each, from dy and h once more; the same additions as in two launches.
+// columns of dw and db each, from dy and h once more; the same additions as in two launches.  Where
+// rows are far from zero each of these workgroups needs their rests, so all of h: 64 x 256 of only
+// such rows 7.8 us, 256 x 512 22, 256 x 2048 43 (and 6.0 of none).
 template <int T, int C>
 __global__ __launch_bounds__(NT) void layernorm_bwd_small_kernel(LnBwdArgs a, float* __restrict__ dw, float* __restrict__ db,
                                                                  int accumulate, int row_blocks) {
@@ -279,13 +296,10 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_small_kernel(LnBwdArgs a, fl
   }
   __shared__ float red[2][64][17];
   __shared__ float rest[NT];
-  __shared__ unsigned long long far[NT / 64];  // rows of a wave's 64
+  __shared__ int some[NT / 64];
   static_assert(kFewRows <= NT, "a row to a thread");
-  {
-    const int row = threadIdx.x;
-    const unsigned long long bits = __ballot(row < a.rows && is_far(a.mean[row], a.rstd[row]));
-    if ((threadIdx.x & 63) == 0) far[threadIdx.x >> 6] = bits;
-  }
+  const int any = __any((int)threadIdx.x < a.rows && is_far(a.mean[threadIdx.x], a.rstd[threadIdx.x]));
+  if ((threadIdx.x & 63) == 0) some[threadIdx.x >> 6] = any;
   const int c = threadIdx.x & 15, col = ((int)blockIdx.x - row_blocks) * 16 + c;
   const auto sums = [&](bool with_rest) {
     for (int g = threadIdx.x >> 4; g < 64; g += NT / 16) {
@@ -307,23 +321,28 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_small_kernel(LnBwdArgs a, fl
   };
   sums(false);
   __syncthreads();
-  if (far[0] | far[1] | far[2] | far[3]) {  // once more with the rests of such rows, a row to a wave
-    float mine = 0.f;
-    for (unsigned long long left = far[threadIdx.x >> 6]; left; left &= left - 1) {
-      const int bit = __ffsll(left) - 1, lane = threadIdx.x & 63, r = (threadIdx.x & ~63) + bit;
-      const float mean = a.mean[r];
-      double s = 0.0;
+  if (some[0] | some[1] | some[2] | some[3]) {  // once more with the rests of such rows: 16 lanes to four rows
+    const int lane = threadIdx.x & 15;
+    for (int r0 = threadIdx.x >> 4; r0 < a.rows; r0 += NT / 4) {
+      Rest v[4] = {Rest(a.mean[r0]), Rest(a.mean[min(r0 + 16, a.rows - 1)]), Rest(a.mean[min(r0 + 32, a.rows - 1)]),
+                   Rest(a.mean[min(r0 + 48, a.rows - 1)])};
+#pragma unroll 2
+      for (int at = 8 * lane; at < a.cols; at += 128) {
+        const int n = min(a.cols - at, 8);
+        float h[4][8];
 #pragma unroll
-      for (int k = 0; k < C; ++k) {
-        const int at = (k * T + lane) * 8, n = min(max(a.cols - at, 0), 8);
-        float h[8] = {};
-        if (n > 0) q8::load_row8(a.h + (int64_t)r * a.cols + at, n, h);
-        add_rest(s, h, n, mean);
+        for (int k = 0; k < 4; ++k) q8::load_row8(a.h + (int64_t)min(r0 + 16 * k, a.rows - 1) * a.cols + at, n, h[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k].add(h[k], n);
       }
-      const float v = (float)(row_sums<T>(s, 0.0, nullptr).x / a.cols);
-      if (lane == bit) mine = v;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) v[k].sum += __shfl_xor(v[k].sum, o, 64);
+        const int r = r0 + 16 * k;
+        if (lane == 0 && r < a.rows) rest[r] = is_far(v[k].mean, a.rstd[r]) ? (float)(v[k].sum / a.cols) : 0.f;
+      }
     }
-    rest[threadIdx.x] = mine;
     __syncthreads();
     sums(true);
     __syncthreads();
@@ -340,9 +359,14 @@ __global__ __launch_bounds__(NT) void layernorm_bwd_small_kernel(LnBwdArgs a, fl
 // The rest of a row's mean, 0 of a row that is not far; by a workgroup of 1024.
 __device__ __forceinline__ float rest_of(const LnBwdArgs& a, int64_t row, float mean, float rstd, double (*red)[2]) {
   if (!is_far(mean, rstd)) return 0.f;
-  double s = 0.0;
-  for (int i = threadIdx.x; i < a.cols; i += 1024) s += (double)a.h[row * a.cols + i] - (double)mean;
-  return (float)(row_sums<1024>(s, 0.0, red).x / a.cols);
+  Rest v(mean);
+  for (int at = 8 * threadIdx.x; at < a.cols; at += 8192) {
+    float h[8];
+    const int n = min(a.cols - at, 8);
+    q8::load_row8(a.h + row * a.cols + at, n, h);
+    v.add(h, n);
+  }
+  return (float)(row_sums<1024>(v.sum, 0.0, red).x / a.cols);
 }
 __global__ __launch_bounds__(1024) void layernorm_rest_kernel(LnBwdArgs a, float* __restrict__ rest) {
   __shared__ double red[16][2];
@@ -357,10 +381,11 @@ __global__ __launch_bounds__(1024) void layernorm_rest_kernel(LnBwdArgs a, float
 
 // Rows wider than the register kernels take: h and dy read twice; the weight's and the
 // bias's gradients in a pass of their own (layernorm_dw_kernel).
-__global__ __launch_bounds__(1024) void layernorm_bwd_wide_kernel(LnBwdArgs a) {
+__global__ __launch_bounds__(1024) void layernorm_bwd_wide_kernel(LnBwdArgs a, const float* __restrict__ rests) {
   __shared__ double red[16][2];
   const int64_t base = (int64_t)blockIdx.x * a.cols;
-  const float rstd = a.rstd[blockIdx.x], mean = a.mean[blockIdx.x], rest = rest_of(a, blockIdx.x, mean, rstd, red);
+  const float rstd = a.rstd[blockIdx.x], mean = a.mean[blockIdx.x];
+  const float rest = rests ? rests[blockIdx.x] : rest_of(a, blockIdx.x, mean, rstd, red);
   double s1 = 0.0, s2 = 0.0;
   for (int i = threadIdx.x; i < a.cols; i += 1024) {
     const float g = a.dy[base + i] * (a.w ? a.w[i] : 1.f), u = ((a.h[base + i] - mean) - rest) * rstd;
@@ -494,8 +519,8 @@ int mle_add_layernorm_bwd(mle_stream stream, int rows, int cols, const float* h,
   else if (cols <= kWidest) mle::launch(layernorm_bwd_kernel<256, 4>, (unsigned)parts, NT, 0, s, a);
   else {
     // the weight's sums first: dh may be dy's or h's buffer
+    float* rest = sums ? static_cast<float*>(ws) + parts_floats(rows, cols) : nullptr;
     if (sums) {
-      float* rest = static_cast<float*>(ws) + parts_floats(rows, cols);
       mle::launch(layernorm_rest_kernel, (unsigned)((rows - 1) / kRestRows + 1), 1024, 0, s, a, rest);
       mle::launch(layernorm_dw_kernel, dim3((unsigned)((cols + NT - 1) / NT), (unsigned)parts), NT, 0, s, a,
                   static_cast<const float*>(rest));
@@ -505,7 +530,7 @@ int mle_add_layernorm_bwd(mle_stream stream, int rows, int cols, const float* h,
       const int64_t at = r0 * cols;
       const LnBwdArgs b{n, cols, h + at, w, mean + r0, rstd + r0, dy + at, dres ? dres + at : dres, dh + at, accumulate_dh,
                         nullptr};
-      mle::launch(layernorm_bwd_wide_kernel, (unsigned)n, 1024, 0, s, b);
+      mle::launch(layernorm_bwd_wide_kernel, (unsigned)n, 1024, 0, s, b, static_cast<const float*>(rest ? rest + r0 : rest));
     }
   }
   for (int64_t c0 = 0; sums && c0 < cols; c0 += kColsOfJoin)
