@@ -238,16 +238,17 @@ __device__ __forceinline__ void kv_rows(const Args& a, const BwdWork& wk, const 
         sj = to;
         tj -= by;
       }
+      const float held = __builtin_amdgcn_ldexpf(1.f, (int)sj);  // (as a factor: in the exponent it would cost P's last bits)
       mx = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(s[r] + sj);
+        s[r] = __builtin_amdgcn_exp2f(s[r]) * held;
         x[r] = s[r] * fmaf(x[r], cd, -delta[r >> 2][r & 3]);
         mx = fmaxf(mx, fabsf(x[r]));
       }
       rescale(mx, tj, dk);
       const float ft = __builtin_amdgcn_ldexpf(1.f, tj);
-      const Frag pf[2] = {split_rows(s, 0), split_rows(s, 1)}, df[2] = {split_rows(x, 0, ft), split_rows(x, 1, ft)};
+      const Frag pf[2] = {split_rows<true>(s, 0, 1.f), split_rows<true>(s, 1, 1.f)}, df[2] = {split_rows<true>(x, 0, ft), split_rows<true>(x, 1, ft)};
       steps<4 * T::DB, AHEAD>([&](int i) { return frag_col<T>(i & 1 ? tq : tg, at, 2 * n + i / (2 * T::DB), (i >> 1) % T::DB); },
                               [&](int i, const Frag& f) {
                                 const int k = i / (2 * T::DB), d = (i >> 1) % T::DB;
@@ -407,7 +408,7 @@ __device__ __forceinline__ void q_rows(const Args& a, const Block& blk, Shared<D
       }
       rescale(mx, ti, dq);
       const float ft = __builtin_amdgcn_ldexpf(1.f, ti);
-      const Frag df[2] = {split_rows(x, 0, ft), split_rows(x, 1, ft)};
+      const Frag df[2] = {split_rows<true>(x, 0, ft), split_rows<true>(x, 1, ft)};
       steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<T>(tk, at, 2 * n + i / T::DB, i % T::DB); },
                               [&](int i, const Frag& f) { mma3(f, df[i / T::DB], dq[i % T::DB]); });
     }

@@ -171,10 +171,11 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
             for (int r = 0; r < 16; ++r) sum[d][r] = __builtin_amdgcn_ldexpf(sum[d][r], by);
           sj = to;
         }
+        const float held = __builtin_amdgcn_ldexpf(1.f, (int)sj);  // (as a factor: in the exponent it would cost P's last bits)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r] + sj);
+        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r]) * held;
         h.put(lane, x, sj);
-        op[0] = split_rows(x, 0), op[1] = split_rows(x, 1);
+        op[0] = split_rows<true>(x, 0, 1.f), op[1] = split_rows<true>(x, 1, 1.f);
       } else {
         f32x16 p;
         const float s = h.get(lane, p);
@@ -193,7 +194,7 @@ __device__ __forceinline__ void kv_pairs(const Args& a, const BwdWork& wk, const
         }
         rescale(mx, tj, sum);
         const float ft = __builtin_amdgcn_ldexpf(1.f, tj);
-        op[0] = split_rows(x, 0, ft), op[1] = split_rows(x, 1, ft);
+        op[0] = split_rows<true>(x, 0, ft), op[1] = split_rows<true>(x, 1, ft);
       }
       steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<T>(buf[!second], at, i / T::DB, i % T::DB); },
                               [&](int i, const Frag& f) { mma3(f, op[i / T::DB], sum[i % T::DB]); });
@@ -365,7 +366,7 @@ __device__ __forceinline__ void q_pairs(const Args& a, const Block& blk, Shared<
         }
         rescale(mx, ti, dq);
         const float ft = __builtin_amdgcn_ldexpf(1.f, ti);
-        const Frag op[2] = {split_rows(x, 0, ft), split_rows(x, 1, ft)};
+        const Frag op[2] = {split_rows<true>(x, 0, ft), split_rows<true>(x, 1, ft)};
         steps<2 * T::DB, AHEAD>([&](int i) { return frag_col<T>(buf[0], at, i / T::DB, i % T::DB); },
                                 [&](int i, const Frag& f) { mma3(f, op[i / T::DB], dq[i % T::DB]); });
       }

@@ -35,7 +35,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTop = 14;    // exponent of a tile's largest value
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
 
 // DP: columns, the head's dimension rounded up to 64, 96 or 128; R rows.
 template <int DP_, int R_>
@@ -64,19 +64,19 @@ __device__ __forceinline__ void mma3(const Frag& a, const Frag& b, f32x16& c) {
   c = mma(a.hi, b.hi, c);
 }
 
-// x in two parts: hi is x rounded to fp16, lo what hi as it is held leaves of it, rounded.  (A hi below
-// 2^-14 has fewer than 11 bits; what it drops is lo's too.)  FUSED: lo from hi by v_fma_mix_f32, four
-// instructions for two values, else by conversions, six.  Staged tiles take the first and rows from
-// the accumulators the second: 2 x 16 heads of 4096 x 128 under a window of 1024 take 253 us forward,
-// 261 with the first for both, 250 with the second; 6 heads of 777 x 80 28.9, 29.1 and 29.6.
+// x times a power of two s in two parts: hi is x s rounded to fp16, lo what hi as it is held leaves of it,
+// rounded.  (A hi below 2^-14 has fewer than 11 bits; what it drops is lo's too.)  FUSED: lo from hi by
+// v_fma_mix_f32, four instructions for two values, else by conversions, six.  Staged tiles take the
+// first, a wave's own rows the second, and so do rows from the accumulators in the forward: with the first
+// there too 2 x 16 heads of 4096 x 128 under a window of 1024 take 261 us forward instead of 253.
 template <bool FUSED>
-__device__ __forceinline__ Frag split8(const float (&x)[8]) {
+__device__ __forceinline__ Frag split8(const float (&x)[8], float s) {
   f16x2 h[4], l[4];
   float minus = -1.f;
   if (FUSED) asm("" : "+s"(minus));  // (a product that the compiler keeps)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = x[2 * j], b = x[2 * j + 1];
+    const float a = x[2 * j] * s, b = x[2 * j + 1] * s;
     unsigned u = __builtin_bit_cast(unsigned, f16x2{(_Float16)a, (_Float16)b});
     asm("" : "+v"(u));  // (one conversion for both values and both uses)
     h[j] = __builtin_bit_cast(f16x2, u);
@@ -88,27 +88,14 @@ __device__ __forceinline__ Frag split8(const float (&x)[8]) {
               __builtin_shufflevector(__builtin_shufflevector(l[0], l[1], 0, 1, 2, 3),
                                       __builtin_shufflevector(l[2], l[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7)};
 }
-// The same of x times a power of two.
-template <bool FUSED>
-__device__ __forceinline__ Frag split8(const float (&x)[8], float s) {
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = x[j] * s;
-  return split8<FUSED>(v);
-}
 
 // Eight of a block's 16 rows as an operand.
-__device__ __forceinline__ Frag split_rows(const f32x16& x, int s) {
-  float v[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = x[8 * s + j];
-  return split8<false>(v);
-}
+template <bool FUSED>
 __device__ __forceinline__ Frag split_rows(const f32x16& x, int s, float scale) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = x[8 * s + j];
-  return split8<false>(v, scale);
+  return split8<FUSED>(v, scale);
 }
 
 // A lane's places in a tile: of frag_row's first step and of frag_col's first columns.  Later

@@ -94,3 +94,15 @@ def test_results_of_the_smallest_weights(hip, dim, heads):
     for name, at in (("out", slice(ROW, ROW + 1)), ("dq", slice(ROW, ROW + 1)), ("dk", slice(0, 2)), ("dv", slice(0, 2))):
         err = np.abs(got[name][0, at, :, 1:] - r[name][at, :, 1:])
         assert (err <= r["e_" + name][at, :, 1:]).all(), (name, float((err / r["e_" + name][at, :, 1:]).max()))
+
+
+@pytest.mark.parametrize("dim,seq", [(64, 600), (128, 300), (80, 40), (64, 3000)])
+def test_log_sum_of_even_rows(hip, dim, seq):
+    """Queries of zeros: every sum is a whole number of equal weights, exact, so that lse is log(count) but for
+    its own rounding, 2^-24 of it, and that of the logarithm of a number's fraction, one step of 2^-23."""
+    def spoil(c):
+        c.q[:] = 0
+    c = Case(hip, 1, seq, 1, 1, dim, seq, 0, spoil=spoil)
+    c.forward()
+    want = np.log(np.arange(1, seq + 1))
+    assert (np.abs(c.lse.numpy()[0, 0] - want) <= U * want + 2 * U).all()
