@@ -20,8 +20,8 @@
 // to a CU, out of step.  Tiles of 32 rows in the kv pass, whose staging then fits beside the
 // sums (64-row tiles spilled, and every reload waited for the loads under way: 555 us against
 // 523 at 4 x 8 heads of 4096, window 1024); 64 keys in the q pass (528 with 32).  That
-// case takes 472 us now (fp32 products at 160 TFLOP/s), 32 x 8 heads of 256 under a window of 128
-// 73 us, prepare's 9 among them.
+// case takes 424 us now (fp32 products at 178 TFLOP/s), 32 x 8 heads of 256 under a window of 128
+// 72 us, prepare's 9 among them.
 #include "window_bwd.hpp"
 
 using namespace mle;

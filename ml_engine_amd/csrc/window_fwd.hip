@@ -10,9 +10,13 @@
 // lost 2^-10 of themselves, and the times were the same to 1 %).
 //
 // Bound by vector instructions beside the products: splitting operands, masks, exponentials.
-// 2 x 16 heads of 4096 x 128 under a window of 1024 take 261-285 us (fp32 products at 215
+// 2 x 16 heads of 4096 x 128 under a window of 1024 take 254 us (fp32 products at 237
 // TFLOP/s, matrix cores 33 % busy, vector units 41 %), 32 x 8 heads of 256 x 64 under one
-// of 128 25 us, where a workgroup's two to four tiles leave both idle most of the time.
+// of 128 24 us, where a workgroup's two to four tiles leave both idle most of the time.
+//
+// Of heads of 128 the form of 4 waves spills 5 vector registers and that of pairs and 8 waves 2; one
+// workgroup to a CU, which needs no spills, takes 129 us where two take 89 (8 x 16 heads of 1024
+// under a window of 128).
 #include "window_tile.hpp"
 #include "window_kernels.hpp"
 
