@@ -3,7 +3,7 @@
 // all of a SIMD's registers and then some; half of the work each, two waves of a SIMD fit, and
 // one's products run among the other's exponentials: 2 x 16 heads of 4096 x 128 under a window
 // of 1024 took 1405 us, preparation and joins among them, with a wave to 32 keys, and take 815 so
-// (fp32 products at 185 TFLOP/s, matrix cores 35 % busy, vector units 41 %).  Heads of 64 are better off without:
+// (fp32 products at 185 TFLOP/s, matrix cores 35 % busy, vector units 38 %).  Heads of 64 are better off without:
 // 577 us against 705 at 4 x 8 heads of 4096.
 #include "window_bwd.hpp"
 

@@ -11,7 +11,7 @@
 //
 // Bound by vector instructions beside the products: splitting operands, masks, exponentials.
 // 2 x 16 heads of 4096 x 128 under a window of 1024 take 254 us (fp32 products at 237
-// TFLOP/s, matrix cores 33 % busy, vector units 41 %), 32 x 8 heads of 256 x 64 under one
+// TFLOP/s, matrix cores 32 % busy, vector units 38 %), 32 x 8 heads of 256 x 64 under one
 // of 128 24 us, where a workgroup's two to four tiles leave both idle most of the time.
 //
 // Of heads of 128 the form of 4 waves spills 5 vector registers and that of pairs and 8 waves 2; one
